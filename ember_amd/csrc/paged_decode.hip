@@ -75,6 +75,7 @@
 
 #include "device.hpp"
 #include "kernels.hpp"
+#include "paged_device.hpp"
 
 namespace ember::hip {
 namespace {
@@ -111,22 +112,11 @@ struct DecodeParams {
     float eps;
 };
 
-// A load through the constant address space: with a wave-uniform address the
-// compiler emits s_load (scalar cache, lgkmcnt), which never waits for the
-// vector page loads in flight. Only for data the kernel does not write.
-template <class T>
-__device__ __forceinline__ T uniform_load(const T *p) {
-    return *(const __attribute__((address_space(4))) T *)(p);  // an address-space cast
-}
-
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
 // One page of K and V as this lane holds it: 4 x 8 dims of K and of V (which
 // keys and dims depends on the path: see the top of the file).
 template <typename T>
 struct PageRegs;
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 template <>
 struct PageRegs<f16> {  // V only: f16 pages stage K in LDS
     u32x4 v[4];
@@ -146,13 +136,6 @@ struct PageRegs<float> {
 // buffer_load_dwordx4 v, v_lane_off, s[desc] offen offset:imm nt, with no
 // per-page vector address arithmetic. A descriptor with no records (live =
 // false) makes the loads return 0 without touching memory.
-constexpr int kDescWord3 = 0x00020000;  // gfx9 raw buffer: 32-bit data format, no swizzle
-constexpr int kNonTemporal = 2;         // cache-policy bit nt of a gfx950 buffer load
-
-__device__ __forceinline__ u32x4 load_desc(__amdgpu_buffer_rsrc_t d, uint32_t off) {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, off, 0, kNonTemporal));
-}
-
 // One half of a page of one kv head (its 16 keys, or its 16 values) into
 // regs[4]: four loads per lane, load i at byte lane_off + step * i of the half.
 template <typename T, typename R>
@@ -234,11 +217,6 @@ __device__ __forceinline__ void unpack8(const float4 (&v)[2], float (&out)[8]) {
     out[7] = v[1].w;
 }
 
-// 2^x by the hardware instruction (v_exp_f32): exact powers of two at
-// integers, 0 at -inf; results below 2^-126 may flush to 0, which only drops
-// weights that cannot move an f32 sum.
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
 // The page's scores in a DPP row (16 lanes, c = lane % 16, each holding an
 // 8-dim partial dot product for the row's keys i = 0..3): reduced so that
 // the lanes of quad q = c / 4 hold key q's full score, with 11 instructions
@@ -277,48 +255,8 @@ __device__ __forceinline__ float quad_value(float v) {
     return dpp_mov<0x150 + 4 * Q>(v);
 }
 
-// f16 pages: max and sum over the four lane groups of a query column (lanes
-// c, c + 16, c + 32, c + 48). Groups 0 and 1, and 2 and 3, meet through
-// v_permlane16_swap, then the pairs through v_permlane32_swap. Both operations
-// are commutative, so every lane of the column gets the same bits; the sum is
-// (x0 + x1) + (x2 + x3).
-__device__ __forceinline__ float groups_max(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float groups_sum(float x) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// f16 pages: the A operand of the value products' dim tile TILE, dim
-// 8 c + TILE of this lane's keys 4 g .. 4 g + 3 (its four 8-dim slices of V,
-// one per key): two v_perm, each pairing one half of a word of two keys.
-template <int TILE>
-__device__ __forceinline__ f16x4 value_tile(const u32x4 (&v)[4]) {
-    constexpr uint32_t sel = (TILE & 1) ? 0x07060302u : 0x05040100u;  // high or low halves of (b, a)
-    constexpr int w = TILE / 2;
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const u32x2 pair = {__builtin_amdgcn_perm(v[1][w], v[0][w], sel),   // keys 4g, 4g + 1
-                        __builtin_amdgcn_perm(v[3][w], v[2][w], sel)};  // keys 4g + 2, 4g + 3
-    return __builtin_bit_cast(f16x4, pair);
-}
-
-__device__ __forceinline__ f16x8 as_f16x8(const u32x4 &x) { return __builtin_bit_cast(f16x8, x); }
-
 // Merges this lane's (m, l, acc) with the lane `mask` away; both lanes end
 // with the same values.
-// The running max of a row before any visible key: finite and far below any
-// score (|q.k| * scale of f16 vectors is below 1e12), so a row's first visible
-// key gives corr = 2^(kNoMax - max) = 0 exactly, as -inf would, while an empty
-// row keeps l = 0 and O = 0; the merges below treat it like -inf (weight 0
-// against any real max, and zeros when every part is empty).
-constexpr float kNoMax = -1.0e30f;
-
 __device__ __forceinline__ void merge_lanes(float &m, float &l, float (&acc)[8], int mask) {
     const float mo = __shfl_xor(m, mask, kWave), lo = __shfl_xor(l, mask, kWave);
     const float M = fmaxf(m, mo);
