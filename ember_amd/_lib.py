@@ -20,6 +20,9 @@ MAX_RUN = 8
 MAX_SPLIT_LEN = 1024
 STATIC_MAX_PARTIALS = 49152
 STATIC_MAX_COUNTERS = 16384
+STEP_MAX_SEQS = 4096
+STEP_MAX_REQUESTS = 65536
+STEP_SHORT, STEP_WIDE, STEP_LATE, STEP_INVALID = 1, 2, 4, 8
 OK = 0
 ERR_INVALID = -1
 DTYPE_F16 = 0
@@ -140,8 +143,39 @@ class ModelInfo(ctypes.Structure):
                 ("max_logit_rows", c_int32)]
 
 
+class StepTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("request", c_void_p), ("cached_len", c_void_p), ("new_len", c_void_p), ("request_tables", c_void_p),
+        ("free_blocks", c_void_p), ("free_cursor", c_void_p),
+        ("S", c_int32), ("R", c_int32), ("max_blocks", c_int32), ("n_free", c_int32), ("max_tokens", c_int32),
+        ("pad_block", c_int32),
+        ("query_start", c_void_p), ("context_len", c_void_p), ("positions", c_void_p), ("token_seq", c_void_p),
+        ("slots", c_void_p), ("block_tables", c_void_p), ("totals", c_void_p),
+    ]
+
+
+class RaggedBatch(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p), ("out", c_void_p), ("query_start", c_void_p),
+        ("positions", c_void_p), ("block_tables", c_void_p), ("q_stride", c_int64),
+        ("T", c_int32), ("S", c_int32), ("max_blocks", c_int32), ("n_heads", c_int32), ("n_kv", c_int32),
+        ("head_dim", c_int32), ("num_blocks", c_int32), ("dtype", c_int32), ("scale", c_float), ("max_query", c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class WindowAttnArgs(ctypes.Structure):
+    _fields_ = [("batch", RaggedBatch), ("window", c_int32), ("sinks", c_int32)]
+
+
+class PrefixAttnArgs(ctypes.Structure):
+    _fields_ = [("batch", RaggedBatch), ("group_start", c_void_p), ("prefix_len", c_void_p), ("n_groups", c_int32),
+                ("max_group", c_int32), ("max_prefix", c_int32), ("max_own", c_int32)]
+
+
 STRUCTS = [QkvArgs, AttnArgs, PrefillArgs, CopyArgs, KvConfig, StepBatchC, LayerIo, GemvArgs, NormArgs, EmbedArgs,
-           SampleParams, SampleArgs, ProbArgs, BackendOptions, ModelInfo]
+           SampleParams, SampleArgs, ProbArgs, BackendOptions, ModelInfo, StepTablesArgs, RaggedBatch, WindowAttnArgs,
+           PrefixAttnArgs]
 
 # name -> (restype, argtypes); every extern "C" symbol of include/ember_hip.h.
 PROTOTYPES = {
@@ -159,6 +193,11 @@ PROTOTYPES = {
     "ember_hip_embed": (c_int32, [POINTER(EmbedArgs), c_void_p]),
     "ember_hip_sample": (c_int32, [POINTER(SampleArgs), c_void_p]),
     "ember_hip_token_probs": (c_int32, [POINTER(ProbArgs), c_void_p]),
+    "ember_hip_step_tables": (c_int32, [POINTER(StepTablesArgs), c_void_p]),
+    "ember_hip_window_attn": (c_int32, [POINTER(WindowAttnArgs), c_void_p]),
+    "ember_hip_window_workspace_bytes": (c_int64, [POINTER(WindowAttnArgs)]),
+    "ember_hip_shared_prefix_attn": (c_int32, [POINTER(PrefixAttnArgs), c_void_p]),
+    "ember_hip_shared_prefix_workspace_bytes": (c_int64, [POINTER(PrefixAttnArgs)]),
     "ember_hip_last_error": (c_char_p, []),
     "ember_hip_abi_version": (c_int32, []),
     "ember_hip_sizeof": (c_int32, [c_int32]),

@@ -30,6 +30,8 @@ SOURCES = [
     CSRC / "gemm.hip",
     CSRC / "static_scratch.hip",
     CSRC / "sampling.hip",
+    CSRC / "step_tables.hip",
+    CSRC / "span_attn.hip",
     CSRC / "host" / "kvcache" / "block_manager.cpp",
     CSRC / "host" / "common" / "json.cpp",
     CSRC / "host" / "common" / "mmap_file.cpp",
@@ -86,6 +88,7 @@ EXTRA_FLAGS = {
     "linear.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
     "gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "kv_append.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=8"],
+    "span_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "prefill_attn.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
 }
 

@@ -43,6 +43,53 @@ int check_heads(const char *who, int head_dim, int n_heads, int n_kv) {
     return EMBER_OK;
 }
 
+// A ragged batch's sizes alone (what its workspace depends on).
+int check_batch_sizes(const char *who, const EmberRaggedBatch &b) {
+    if (int e = check_heads(who, b.head_dim, b.n_heads, b.n_kv)) return e;
+    if (!valid_dtype(b.dtype)) return set_error(EMBER_ERR_INVALID, "%s: unknown dtype %d", who, b.dtype);
+    if (b.T < 0 || b.S < 0 || b.max_blocks <= 0 || b.max_blocks > (1 << 26) || b.max_query < 1)
+        return set_error(EMBER_ERR_INVALID, "%s: bad sizes (T %d, S %d, max_blocks %d: 1..2^26, max_query %d)", who, b.T, b.S,
+                         b.max_blocks, b.max_query);
+    if (static_cast<long long>(b.T) * b.n_heads > 0x7fffffffLL)
+        return set_error(EMBER_ERR_INVALID, "%s: T x n_heads must fit 31 bits (got %d x %d)", who, b.T, b.n_heads);
+    return EMBER_OK;
+}
+
+int check_batch(const char *who, const EmberRaggedBatch &b) {
+    if (int e = check_batch_sizes(who, b)) return e;
+    if (b.num_blocks <= 0) return set_error(EMBER_ERR_INVALID, "%s: bad sizes (num_blocks %d)", who, b.num_blocks);
+    if (!(b.scale > 0.0f) || !std::isfinite(b.scale))  // the max is taken before scaling
+        return set_error(EMBER_ERR_INVALID, "%s: scale must be positive and finite", who);
+    const int per16 = b.dtype == EMBER_DTYPE_F16 ? 8 : 4;
+    if (b.q_stride < static_cast<int64_t>(b.n_heads) * kHeadDim || b.q_stride % per16 != 0)
+        return set_error(EMBER_ERR_INVALID, "%s: q_stride must be at least n_heads x 128 and a multiple of %d (got %lld)", who,
+                         per16, static_cast<long long>(b.q_stride));
+    if (b.workspace_bytes < 0 || reinterpret_cast<uintptr_t>(b.workspace) % 16 != 0)
+        return set_error(EMBER_ERR_INVALID, "%s: the workspace must be 16-byte aligned with a size >= 0", who);
+    if (b.T == 0 || b.S == 0) return EMBER_OK;
+    if (!b.q || !b.k_cache || !b.v_cache || !b.out || !b.query_start || !b.positions || !b.block_tables)
+        return set_error(EMBER_ERR_INVALID, "%s: a required pointer is null", who);
+    if ((reinterpret_cast<uintptr_t>(b.q) | reinterpret_cast<uintptr_t>(b.out) | reinterpret_cast<uintptr_t>(b.k_cache) |
+         reinterpret_cast<uintptr_t>(b.v_cache)) % 16 != 0)
+        return set_error(EMBER_ERR_INVALID, "%s: q, out and the pools must be 16-byte aligned", who);
+    return EMBER_OK;
+}
+
+int check_window(const char *who, const EmberWindowAttnArgs &a) {
+    if (a.window < 1 || a.sinks < 0)
+        return set_error(EMBER_ERR_INVALID, "%s: window must be at least 1 and sinks at least 0 (got %d, %d)", who, a.window,
+                         a.sinks);
+    return EMBER_OK;
+}
+
+int check_prefix(const char *who, const EmberPrefixAttnArgs &a) {
+    if (a.n_groups < 0 || a.n_groups > 4096 || a.max_group < 1 || a.max_prefix < 0 || a.max_own < 1)
+        return set_error(EMBER_ERR_INVALID,
+                         "%s: bad sizes (n_groups %d: 0..4096, max_group %d, max_prefix %d, max_own %d)", who, a.n_groups,
+                         a.max_group, a.max_prefix, a.max_own);
+    return EMBER_OK;
+}
+
 }  // namespace
 }  // namespace ember::hip
 
@@ -71,6 +118,10 @@ int32_t ember_hip_sizeof(int32_t which) {
         case 12: return sizeof(EmberProbArgs);
         case 13: return sizeof(EmberBackendOptions);
         case 14: return sizeof(EmberModelInfo);
+        case 15: return sizeof(EmberStepTablesArgs);
+        case 16: return sizeof(EmberRaggedBatch);
+        case 17: return sizeof(EmberWindowAttnArgs);
+        case 18: return sizeof(EmberPrefixAttnArgs);
         default: return -1;
     }
 }
@@ -285,6 +336,63 @@ int ember_hip_token_probs(const EmberProbArgs *a, void *stream) {
     if (!a->logits || !a->params || !a->rows || !a->tokens || !a->out)
         return set_error(EMBER_ERR_INVALID, "token_probs: a required pointer is null");
     return hip_status(launch_token_probs(*a, static_cast<hipStream_t>(stream)), "token_probs");
+}
+
+int ember_hip_step_tables(const EmberStepTablesArgs *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "step_tables: null arguments");
+    if (a->S < 0 || a->S > EMBER_STEP_MAX_SEQS || a->R < 0 || a->R > EMBER_STEP_MAX_REQUESTS || a->n_free < 0 ||
+        a->max_tokens < 0 || a->max_blocks < 1)
+        return set_error(EMBER_ERR_INVALID, "step_tables: bad sizes (S %d: 0..%d, R %d: 0..%d, n_free %d, max_tokens %d, max_blocks %d)",
+                         a->S, EMBER_STEP_MAX_SEQS, a->R, EMBER_STEP_MAX_REQUESTS, a->n_free, a->max_tokens, a->max_blocks);
+    if (static_cast<long long>(a->S + 1) * a->max_blocks * kPage > 0x7fffffffLL)
+        return set_error(EMBER_ERR_INVALID, "step_tables: (S + 1) x max_blocks x 16 must fit 31 bits (got S %d, max_blocks %d)", a->S,
+                         a->max_blocks);
+    if (!a->request && a->R < a->S)
+        return set_error(EMBER_ERR_INVALID, "step_tables: without request, R must be at least S (got %d, %d)", a->R, a->S);
+    if (a->pad_block < -1) return set_error(EMBER_ERR_INVALID, "step_tables: pad_block is a page or -1 (got %d)", a->pad_block);
+    if (!a->query_start || !a->block_tables || !a->totals || (a->S > 0 && (!a->cached_len || !a->new_len || !a->request_tables || !a->context_len)) ||
+        (a->max_tokens > 0 && (!a->positions || !a->token_seq || !a->slots)) || (a->n_free > 0 && !a->free_blocks))
+        return set_error(EMBER_ERR_INVALID, "step_tables: a required pointer is null");
+    if (a->free_cursor >= a->totals && a->free_cursor < a->totals + 4)
+        return set_error(EMBER_ERR_INVALID, "step_tables: free_cursor may not lie in the totals that this call writes");
+    return hip_status(launch_step_tables(*a, static_cast<hipStream_t>(stream)), "step_tables");
+}
+
+int ember_hip_window_attn(const EmberWindowAttnArgs *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "window_attn: null arguments");
+    if (int e = check_batch("window_attn", a->batch)) return e;
+    if (int e = check_window("window_attn", *a)) return e;
+    if (a->batch.T == 0 || a->batch.S == 0) return EMBER_OK;
+    return launch_window_attn(*a, static_cast<hipStream_t>(stream));
+}
+
+int64_t ember_hip_window_workspace_bytes(const EmberWindowAttnArgs *a) {
+    g_last_error.clear();
+    if (!a || check_batch_sizes("window_workspace_bytes", a->batch) || check_window("window_workspace_bytes", *a) ||
+        a->batch.T == 0 || a->batch.S == 0)
+        return 0;
+    return window_workspace_bytes(*a);
+}
+
+int ember_hip_shared_prefix_attn(const EmberPrefixAttnArgs *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "shared_prefix_attn: null arguments");
+    if (int e = check_batch("shared_prefix_attn", a->batch)) return e;
+    if (int e = check_prefix("shared_prefix_attn", *a)) return e;
+    if (a->batch.T == 0 || a->batch.S == 0) return EMBER_OK;
+    if (a->n_groups > 0 && (!a->group_start || !a->prefix_len))
+        return set_error(EMBER_ERR_INVALID, "shared_prefix_attn: a required pointer is null");
+    return launch_shared_prefix_attn(*a, static_cast<hipStream_t>(stream));
+}
+
+int64_t ember_hip_shared_prefix_workspace_bytes(const EmberPrefixAttnArgs *a) {
+    g_last_error.clear();
+    if (!a || check_batch_sizes("shared_prefix_workspace_bytes", a->batch) ||
+        check_prefix("shared_prefix_workspace_bytes", *a) || a->batch.T == 0 || a->batch.S == 0)
+        return 0;
+    return shared_prefix_workspace_bytes(*a);
 }
 
 int ember_hip_rmsnorm_rows(const EmberNormArgs *a, void *stream) {

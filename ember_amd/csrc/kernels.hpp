@@ -62,6 +62,13 @@ hipError_t launch_embed(const EmberEmbedArgs &a, hipStream_t stream);
 hipError_t launch_sample(const EmberSampleArgs &a, hipStream_t stream);
 hipError_t launch_token_probs(const EmberProbArgs &a, hipStream_t stream);
 
+hipError_t launch_step_tables(const EmberStepTablesArgs &a, hipStream_t stream);
+// Return EMBER_* / hipError_t codes: what fits one launch is known once the launch is planned.
+int launch_window_attn(const EmberWindowAttnArgs &a, hipStream_t stream);
+int launch_shared_prefix_attn(const EmberPrefixAttnArgs &a, hipStream_t stream);
+int64_t window_workspace_bytes(const EmberWindowAttnArgs &a);
+int64_t shared_prefix_workspace_bytes(const EmberPrefixAttnArgs &a);
+
 // Row capacities with a built decode kernel, ascending.
 constexpr int kDecodeRowInstances[] = {1, 2, 4, 8, 10, 16};
 

@@ -3,7 +3,9 @@
 Mirrors the reference's launcher seam (src/backend/cuda/kernels.cuh:74-120):
 ``qk_norm_rope_store`` (-> ember_hip_kv_append), ``paged_attention``
 (-> ember_hip_paged_decode), ``prefill_attention`` (-> ember_hip_prefill_attn),
-plus ``copy_pages`` (copy-on-write). Device tensors carry activations and pools;
+plus ``copy_pages`` (copy-on-write). ``step_tables``, ``window_attention`` and
+``shared_prefix_attention`` have no counterpart there: they take a step's integers
+from the device, with no host plan. Device tensors carry activations and pools;
 the step's integer arrays are given as host arrays, checked here (every index a
 kernel will follow is in range), then uploaded. Launches go to the current torch
 stream unless ``stream`` is given.
@@ -413,3 +415,189 @@ def rmsnorm_rows(x, w, out, eps: float, rows=None, stream=None):
         n.rows = r.data_ptr()
     check(_lib.lib().ember_hip_rmsnorm_rows(n, _stream_handle(stream)), "rmsnorm_rows")
     return keep
+
+
+def _on(t: torch.Tensor, stream):
+    """The stream handle for work on t's device, and that device made current if it is not (None, or its guard)."""
+    guard = None
+    if t.device.index != torch.cuda.current_device():
+        guard = torch.cuda.device(t.device)
+    if stream is None:
+        stream = torch.cuda.current_stream(t.device)
+    return (stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)), guard
+
+
+def _launch(fn, args, t: torch.Tensor, stream, what: str) -> None:
+    handle, guard = _on(t, stream)
+    if guard is None:
+        check(fn(args, handle), what)
+    else:
+        with guard:
+            check(fn(args, handle), what)
+
+
+def _same(t, name: str, device, dtype, shape=None) -> int:
+    """The address of a contiguous tensor that must be on `device` with this dtype (and shape)."""
+    if t.device != device or t.dtype != dtype or not t.is_contiguous():
+        raise EmberError(f"{name} must be a contiguous {dtype} tensor on {device}")
+    if shape is not None and t.shape != shape:
+        raise EmberError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
+    return t.data_ptr()
+
+
+class StepTables:
+    """A step's integers on the device, as step_tables writes them: query_start [S + 1], context_len [S],
+    positions / token_seq / slots [max_tokens], block_tables [S + 1, max_blocks], totals [4] (tokens, entries of
+    the free list taken by now, STEP_* bits, longest context)."""
+
+    def __init__(self, S: int, max_tokens: int, max_blocks: int, device="cuda"):
+        e = lambda *shape, dtype=torch.int32: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
+        self.S, self.max_tokens, self.max_blocks = S, max_tokens, max_blocks
+        self.query_start, self.context_len = e(S + 1), e(S)
+        self.positions, self.token_seq, self.slots = e(max_tokens), e(max_tokens), e(max_tokens, dtype=torch.int64)
+        self.block_tables, self.totals = e(S + 1, max_blocks), e(4)
+        self.device = self.totals.device
+        if self.device.type != "cuda":
+            raise EmberError("StepTables live on the device")
+
+
+def step_tables(out: StepTables, request_tables, cached_len, new_len, free_blocks, *, request=None, free_cursor=None,
+                pad_block: int = -1, stream=None) -> StepTables:
+    """The integers of a step from its requests' lengths, in one launch (ember_hip_step_tables).
+
+    request_tables [R, max_blocks]: each request's pages; the pages the step takes from free_blocks (from entry
+    free_cursor[0] on) are written behind them. cached_len [R]; new_len [S]; request [S] (None: rows 0..S-1).
+    All int32 on out's device. Nothing is checked on the host that would need the device's values: totals[2]
+    says which sequences got no tokens and why.
+    """
+    dev, i32 = out.device, torch.int32
+    a = _lib.StepTablesArgs()
+    if request_tables.dim() != 2 or request_tables.shape[1] != out.max_blocks:
+        raise EmberError(f"request_tables must be [R, {out.max_blocks}]")
+    R = request_tables.shape[0]
+    a.request_tables = _same(request_tables, "request_tables", dev, i32)
+    a.cached_len = _same(cached_len, "cached_len", dev, i32, (R,))
+    a.new_len = _same(new_len, "new_len", dev, i32, (out.S,))
+    if free_blocks.dim() != 1:
+        raise EmberError("free_blocks must be a list")
+    a.free_blocks = _same(free_blocks, "free_blocks", dev, i32)
+    if request is not None:
+        a.request = _same(request, "request", dev, i32, (out.S,))
+    if free_cursor is not None:
+        a.free_cursor = _same(free_cursor, "free_cursor", dev, i32, (1,))
+    a.S, a.R, a.max_blocks, a.n_free = out.S, R, out.max_blocks, free_blocks.shape[0]
+    a.max_tokens, a.pad_block = out.max_tokens, pad_block
+    a.query_start, a.context_len = out.query_start.data_ptr(), out.context_len.data_ptr()
+    a.positions, a.token_seq, a.slots = out.positions.data_ptr(), out.token_seq.data_ptr(), out.slots.data_ptr()
+    a.block_tables, a.totals = out.block_tables.data_ptr(), out.totals.data_ptr()
+    _launch(_lib.lib().ember_hip_step_tables, a, out.totals, stream, "step_tables")
+    return out
+
+
+def _batch_sizes(b, T, S, *, n_heads, n_kv, max_query, dtype, max_blocks) -> None:
+    b.T, b.S, b.n_heads, b.n_kv, b.head_dim = T, S, n_heads, n_kv, HEAD_DIM
+    b.max_blocks = 1 << 26 if max_blocks is None else max_blocks
+    b.max_query = max(1, T if max_query is None else max_query)
+    b.dtype = _lib.DTYPE_F16 if dtype == torch.float16 else _lib.DTYPE_F32
+
+
+def _ragged_batch(b, q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace) -> None:
+    """Fills an EmberRaggedBatch: q [T, n_heads, 128] (any token stride), pools [num_blocks, n_kv, 16, 128]."""
+    dev, i32 = q.device, torch.int32
+    code = _dtype_code(q)
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.stride(2) != 1 or q.stride(1) != HEAD_DIM or not q.is_cuda:
+        raise EmberError("q must be a device tensor [T, n_heads, 128] with each token's heads contiguous")
+    if k_pool.dim() != 4 or k_pool.shape[2] != BLOCK_SIZE or k_pool.shape[3] != HEAD_DIM:
+        raise EmberError("pools must be [num_blocks, n_kv, 16, 128]")
+    T, H = q.shape[0], q.shape[1]
+    b.q, b.q_stride = q.data_ptr(), q.stride(0) if T > 1 else H * HEAD_DIM
+    b.k_cache = _same(k_pool, "k_pool", dev, q.dtype)
+    b.v_cache = _same(v_pool, "v_pool", dev, q.dtype, k_pool.shape)
+    b.out = _same(out, "out", dev, q.dtype, q.shape)
+    b.query_start = _same(query_start, "query_start", dev, i32)
+    if query_start.dim() != 1 or query_start.shape[0] < 1:
+        raise EmberError("query_start must be [S + 1]")
+    S = query_start.shape[0] - 1
+    b.positions = _same(positions, "positions", dev, i32)
+    if positions.dim() != 1 or positions.shape[0] < T:
+        raise EmberError("positions must hold every token")
+    b.block_tables = _same(block_tables, "block_tables", dev, i32)
+    if block_tables.dim() != 2 or block_tables.shape[0] < S:
+        raise EmberError("block_tables must be [S, max_blocks] (more rows are not used)")
+    b.T, b.S, b.max_blocks, b.n_heads, b.n_kv, b.head_dim = T, S, block_tables.shape[1], H, k_pool.shape[1], HEAD_DIM
+    b.num_blocks, b.dtype = k_pool.shape[0], code
+    b.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale
+    b.max_query = max(1, T if max_query is None else max_query)
+    if workspace is not None:
+        if workspace.device != dev or not workspace.is_contiguous():
+            raise EmberError(f"workspace must be a contiguous tensor on {dev}")
+        b.workspace, b.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _workspace(n: int, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
+
+
+def window_workspace(T: int, S: int, *, n_heads, n_kv, window, sinks=0, max_query=None, dtype=torch.float16,
+                     max_blocks=None, device="cuda"):
+    """A workspace for window_attention of batches of these sizes, or None when such a call splits no keys."""
+    a = _lib.WindowAttnArgs()
+    _batch_sizes(a.batch, T, S, n_heads=n_heads, n_kv=n_kv, max_query=max_query, dtype=dtype, max_blocks=max_blocks)
+    a.window, a.sinks = window, sinks
+    return _workspace(int(_lib.lib().ember_hip_window_workspace_bytes(a)), device)
+
+
+def window_attention(q, k_pool, v_pool, out, query_start, positions, block_tables, *, window: int, sinks: int = 0,
+                     max_query=None, scale=None, workspace=None, stream=None):
+    """Attention of each token to itself, the window - 1 tokens before it and its sequence's first `sinks` tokens
+    (ember_hip_window_attn); returns out.
+
+    q [T, n_heads, 128] (a part of wider rows is fine), out the same, contiguous; pools [num_blocks, n_kv, 16, 128];
+    query_start [S + 1], positions [T] and block_tables [S, max_blocks] int32 on the device, as step_tables writes
+    them. Pages that no token of the step attends to are not read and may have been freed. Rows of q past
+    query_start[S] are left alone. max_query: the most tokens of one sequence (None: T); workspace: of
+    window_workspace, not shared by calls that overlap in time (None: no splits).
+    """
+    a = _lib.WindowAttnArgs()
+    _ragged_batch(a.batch, q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
+    a.window, a.sinks = window, sinks
+    _launch(_lib.lib().ember_hip_window_attn, a, q, stream, "window_attn")
+    return out
+
+
+def _prefix_sizes(a, T, n_groups, max_group, max_prefix, max_own) -> None:
+    far = min(a.batch.max_blocks * BLOCK_SIZE, 0x7FFFFFFF)
+    a.n_groups = n_groups
+    a.max_group = max(1, T if max_group is None else max_group)
+    a.max_prefix = far if max_prefix is None else max_prefix
+    a.max_own = max(1, far if max_own is None else max_own)
+
+
+def shared_prefix_workspace(T: int, S: int, n_groups: int, *, n_heads, n_kv, max_query=None, max_group=None,
+                            max_prefix=None, max_own=None, dtype=torch.float16, max_blocks=None, device="cuda"):
+    """A workspace for shared_prefix_attention of batches of these sizes."""
+    a = _lib.PrefixAttnArgs()
+    _batch_sizes(a.batch, T, S, n_heads=n_heads, n_kv=n_kv, max_query=max_query, dtype=dtype, max_blocks=max_blocks)
+    _prefix_sizes(a, T, n_groups, max_group, max_prefix, max_own)
+    return _workspace(int(_lib.lib().ember_hip_shared_prefix_workspace_bytes(a)), device)
+
+
+def shared_prefix_attention(q, k_pool, v_pool, out, query_start, positions, block_tables, group_start, prefix_len, *,
+                            max_query=None, max_group=None, max_prefix=None, max_own=None, scale=None, workspace=None,
+                            stream=None):
+    """Causal attention of groups of sequences that share a cached prefix, read once for the group
+    (ember_hip_shared_prefix_attn); returns out.
+
+    As window_attention, and: group_start [n_groups + 1], group g being sequences group_start[g] ..
+    group_start[g + 1] - 1; prefix_len [n_groups], the tokens they share, read through the table of the group's
+    first sequence. max_query, max_group (new tokens of one sequence and of one group), max_prefix and max_own
+    (tokens of a prefix and behind it) shape the launch; a step beyond them is computed too, only slower.
+    """
+    a = _lib.PrefixAttnArgs()
+    _ragged_batch(a.batch, q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
+    n_groups = prefix_len.shape[0]
+    a.group_start = _same(group_start, "group_start", q.device, torch.int32, (n_groups + 1,))
+    a.prefix_len = _same(prefix_len, "prefix_len", q.device, torch.int32, (n_groups,))
+    _prefix_sizes(a, q.shape[0], n_groups, max_group, max_prefix, max_own)
+    _launch(_lib.lib().ember_hip_shared_prefix_attn, a, q, stream, "shared_prefix_attn")
+    return out

@@ -347,6 +347,117 @@ typedef struct EmberProbArgs {
  * (kernels.cuh:132-133; k_sampling.cu:172-186). */
 int ember_hip_token_probs(const EmberProbArgs *args, void *stream);
 
+/* ---- 1b. steps planned on the GPU, windows and shared prefixes -------------
+ * No counterpart in the reference, whose host packs every step's integers
+ * (src/backend/cuda/cuda_backend.cu:153-205) and whose attention reads each
+ * sequence's whole context. The tables of a step are made from the requests'
+ * lengths on the device; both attentions take them as they are, with no host
+ * plan: the sizes they ask for (max_query and the like) shape the launch, and
+ * a step that exceeds them is computed all the same, only slower. */
+
+#define EMBER_STEP_MAX_SEQS 4096      /* sequences of one ember_hip_step_tables call */
+#define EMBER_STEP_MAX_REQUESTS 65536 /* rows of its request tables */
+
+/* totals[2] of ember_hip_step_tables: why some sequence got no tokens. */
+#define EMBER_STEP_SHORT 1   /* the free list had no pages left for it */
+#define EMBER_STEP_WIDE 2    /* its context would pass max_blocks pages */
+#define EMBER_STEP_LATE 4    /* the sequences up to it have more than max_tokens new tokens */
+#define EMBER_STEP_INVALID 8 /* its request is outside the tables or named twice, or a length is negative or too long */
+
+typedef struct EmberStepTablesArgs {
+    const int32_t *request;     /* [S] each sequence's row of the request tables, none twice; NULL = rows 0..S-1 */
+    const int32_t *cached_len;  /* [R] tokens of each request whose K/V its pages hold */
+    const int32_t *new_len;     /* [S] tokens the step adds to each sequence (0 is allowed) */
+    int32_t *request_tables;    /* [R, max_blocks] each request's pages; those the step takes are written behind them */
+    const int32_t *free_blocks; /* [n_free] pages that may be taken, in this order */
+    const int32_t *free_cursor; /* [1] how many of them are taken already, or NULL = 0. Not totals + 1 of this call */
+    int32_t S, R, max_blocks, n_free;
+    int32_t max_tokens;         /* rows of positions, token_seq and slots */
+    int32_t pad_block;          /* the page that padding tokens write to, or -1 */
+    int32_t *query_start;       /* [S + 1] */
+    int32_t *context_len;       /* [S] tokens after the step */
+    int32_t *positions;         /* [max_tokens]; rows past the step's tokens: 0 */
+    int32_t *token_seq;         /* [max_tokens]; rows past the step's tokens: S */
+    int64_t *slots;             /* [max_tokens] page * 16 + slot; rows past the step's tokens: pad_block * 16 (-1) */
+    int32_t *block_tables;      /* [S + 1, max_blocks]; entries past a sequence's pages: -1; row S: pad_block, then -1 */
+    int32_t *totals;            /* [4] tokens, entries of free_blocks taken by now, EMBER_STEP_* bits, longest context */
+} EmberStepTablesArgs;
+
+/* The integers of a step from its requests' lengths, in one launch:
+ *   have = ceil(cached / 16), need = ceil((cached + new) / 16) - have,
+ *   query_start = the running sum of new_len, table row = the request's `have`
+ *   pages, then its `need` next entries of free_blocks (sequences in order),
+ *   position = cached + i, slot = table[position / 16] * 16 + position % 16.
+ * A sequence whose tokens cannot all be placed gets none of them (its row and
+ * context stay as they were) and sets a bit of totals[2]; EMBER_STEP_INVALID
+ * ones get an empty row and context 0. Rows past the step's tokens are padding
+ * that the append and decode kernels may run over: they belong to row S.
+ * The inputs are left as they are but for request_tables, so a repeated call
+ * gives the same tables; the next step passes totals + 1 (of a buffer that it
+ * does not write) as free_cursor. S * max_blocks * 16 must fit 31 bits. */
+int ember_hip_step_tables(const EmberStepTablesArgs *args, void *stream);
+
+/* A ragged batch over the paged cache: the tokens of sequence s are rows
+ * query_start[s] .. query_start[s + 1] - 1 of q, at positions that count up by
+ * one; their K/V are in the pages already. Rows of no sequence are left as
+ * they are, and so is everything past T. Any number of query heads per kv
+ * head; head_dim 128. K and V of visible keys are finite (the append kernels
+ * clamp them); other slots may hold anything, NaN included. A table entry
+ * outside the pool reads as a page of zeros. A token at a negative position
+ * gets zeros; one past its table reads up to the table's end. */
+typedef struct EmberRaggedBatch {
+    const void *q;               /* [T, n_heads, 128], q_stride elements between tokens */
+    const void *k_cache, *v_cache; /* [num_blocks][n_kv][16][128] */
+    void *out;                   /* [T, n_heads, 128], contiguous */
+    const int32_t *query_start;  /* [S + 1] ascending, within 0..T */
+    const int32_t *positions;    /* [T] */
+    const int32_t *block_tables; /* [S, max_blocks] */
+    int64_t q_stride;            /* at least n_heads * 128; q and its rows 16-byte aligned */
+    int32_t T, S, max_blocks, n_heads, n_kv, head_dim, num_blocks, dtype;
+    float scale;                 /* positive */
+    int32_t max_query;           /* tokens of the longest sequence's run; more are computed, slower */
+    /* Scratch for splitting the keys over work-groups, 16-byte aligned, no
+     * initial contents, nothing kept between launches. With NULL or fewer bytes
+     * than ember_hip_*_workspace_bytes says there are fewer splits, and the call
+     * is slower. Launches that overlap in time must not share one. */
+    void *workspace;
+    int64_t workspace_bytes;
+} EmberRaggedBatch;
+
+typedef struct EmberWindowAttnArgs {
+    EmberRaggedBatch batch;
+    int32_t window;              /* a token sees itself and the window - 1 tokens before it (at least 1) */
+    int32_t sinks;               /* and the sequence's first `sinks` tokens (0: none) */
+} EmberWindowAttnArgs;
+
+/* out[i] = softmax over keys j <= p_i with p_i - j < window or j < sinks of
+ * scale q_i . k_j, times V, for every token of every sequence. Only the pages
+ * that hold such keys are read: the table entries of others are not followed,
+ * so a serving program may free those pages. */
+int ember_hip_window_attn(const EmberWindowAttnArgs *args, void *stream);
+/* Bytes of workspace ember_hip_window_attn uses for these sizes (only the
+ * sizes, dtype, window and sinks of args are read; 0: it would not split).
+ * Enough for any smaller max_blocks too. */
+int64_t ember_hip_window_workspace_bytes(const EmberWindowAttnArgs *args);
+
+typedef struct EmberPrefixAttnArgs {
+    EmberRaggedBatch batch;
+    const int32_t *group_start;  /* [n_groups + 1] ascending: group g is sequences group_start[g] .. group_start[g + 1] - 1 */
+    const int32_t *prefix_len;   /* [n_groups] tokens that the group's sequences share (any number, not only whole pages) */
+    int32_t n_groups;
+    int32_t max_group;           /* new tokens of the largest group, */
+    int32_t max_prefix, max_own; /* the longest prefix, and the most keys of a sequence behind it: more are computed, slower */
+} EmberPrefixAttnArgs;
+
+/* Causal attention (keys 0..p_i of each token) of sequences that share a
+ * cached prefix: keys below prefix_len[g] are read once for the whole group,
+ * through the table of the group's first sequence, those behind it through
+ * each sequence's own. A token inside the prefix sees the prefix up to itself.
+ * Sequences of no group share nothing. With groups, two partials of every
+ * (token, head) need workspace in any case: 1040 bytes * T * n_heads. */
+int ember_hip_shared_prefix_attn(const EmberPrefixAttnArgs *args, void *stream);
+int64_t ember_hip_shared_prefix_workspace_bytes(const EmberPrefixAttnArgs *args);
+
 /* Description of the last failure on this thread ("" if none). */
 const char *ember_hip_last_error(void);
 int ember_hip_abi_version(void);
@@ -354,7 +465,9 @@ int ember_hip_abi_version(void);
  * 0 EmberQkvArgs, 1 EmberAttnArgs, 2 EmberPrefillArgs, 3 EmberCopyArgs,
  * 4 EmberKvConfig, 5 EmberStepBatch, 6 EmberLayerIo, 7 EmberGemvArgs,
  * 8 EmberNormArgs, 9 EmberEmbedArgs, 10 EmberSampleParams, 11 EmberSampleArgs,
- * 12 EmberProbArgs, 13 EmberBackendOptions, 14 EmberModelInfo; -1 otherwise. */
+ * 12 EmberProbArgs, 13 EmberBackendOptions, 14 EmberModelInfo,
+ * 15 EmberStepTablesArgs, 16 EmberRaggedBatch, 17 EmberWindowAttnArgs,
+ * 18 EmberPrefixAttnArgs; -1 otherwise. */
 int32_t ember_hip_sizeof(int32_t which);
 
 /* ---- 2. KV block manager ------------------------------------------------- */

@@ -1,0 +1,109 @@
+"""Step tables, windowed and shared-prefix attention: what the C ABI refuses before any launch, and the workspaces."""
+import pytest
+
+from ember_amd import _lib
+from ember_amd import kernels as K
+
+
+def _tables():
+    a = _lib.StepTablesArgs()
+    for f in ("cached_len", "new_len", "request_tables", "free_blocks", "query_start", "context_len", "positions", "token_seq",
+              "slots", "block_tables", "totals"):
+        setattr(a, f, 4096)  # never followed: every call here is refused
+    a.S, a.R, a.max_blocks, a.n_free, a.max_tokens, a.pad_block = 2, 3, 4, 5, 6, 0
+    return a
+
+
+@pytest.mark.parametrize("field,value,text", [
+    ("S", -1, "bad sizes"), ("S", _lib.STEP_MAX_SEQS + 1, "bad sizes"), ("R", -1, "bad sizes"), ("R", _lib.STEP_MAX_REQUESTS + 1, "bad sizes"),
+    ("R", 1, "R must be at least S"), ("n_free", -1, "bad sizes"), ("max_tokens", -1, "bad sizes"), ("max_blocks", 0, "bad sizes"),
+    ("max_blocks", 1 << 26, "31 bits"), ("pad_block", -2, "pad_block"), ("free_cursor", 4096 + 4, "free_cursor"),
+    *((f, None, "null") for f in ("cached_len", "new_len", "request_tables", "free_blocks", "query_start", "context_len", "positions",
+                                  "token_seq", "slots", "block_tables", "totals"))])
+def test_step_tables_refusals(field, value, text):
+    a = _tables()
+    setattr(a, field, value)
+    assert _lib.lib().ember_hip_step_tables(a, None) == _lib.ERR_INVALID
+    assert text in _lib.last_error()
+
+
+def _batch(a):
+    b = a.batch
+    for f in ("q", "k_cache", "v_cache", "out", "query_start", "positions", "block_tables"):
+        setattr(b, f, 4096)
+    b.T, b.S, b.max_blocks, b.n_heads, b.n_kv, b.head_dim, b.num_blocks = 4, 2, 8, 16, 8, 128, 32
+    b.q_stride, b.scale, b.max_query, b.dtype = 2048, 0.1, 2, _lib.DTYPE_F16
+    return a
+
+
+def _window():
+    a = _batch(_lib.WindowAttnArgs())
+    a.window, a.sinks = 16, 4
+    return a
+
+
+def _prefix():
+    a = _batch(_lib.PrefixAttnArgs())
+    a.group_start, a.prefix_len, a.n_groups, a.max_group, a.max_prefix, a.max_own = 4096, 4096, 1, 4, 16, 16
+    return a
+
+
+BATCH = [("T", -1, "bad sizes"), ("S", -1, "bad sizes"), ("max_blocks", 0, "bad sizes"), ("max_blocks", 1 << 27, "bad sizes"),
+         ("max_query", 0, "bad sizes"), ("n_heads", 15, "do not group"), ("n_kv", 0, "do not group"), ("head_dim", 64, "head_dim"),
+         ("num_blocks", 0, "bad sizes"), ("dtype", 2, "dtype"), ("scale", 0.0, "scale"), ("scale", -1.0, "scale"),
+         ("scale", float("nan"), "scale"), ("scale", float("inf"), "scale"), ("q_stride", 2040, "q_stride"), ("q_stride", 2052, "q_stride"),
+         ("T", 1 << 28, "31 bits"), ("workspace", 8, "workspace"), ("workspace_bytes", -1, "workspace"), ("q", 4104, "aligned"),
+         ("out", 4104, "aligned"), ("k_cache", 4104, "aligned"), ("v_cache", 4104, "aligned"),
+         *((f, None, "null") for f in ("q", "k_cache", "v_cache", "out", "query_start", "positions", "block_tables"))]
+
+
+@pytest.mark.parametrize("make,entry", [(_window, "ember_hip_window_attn"), (_prefix, "ember_hip_shared_prefix_attn")],
+                         ids=["window", "prefix"])
+@pytest.mark.parametrize("field,value,text", BATCH)
+def test_batch_refusals(make, entry, field, value, text):
+    a = make()
+    setattr(a.batch, field, value)
+    assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
+    assert text in _lib.last_error()
+
+
+@pytest.mark.parametrize("make,entry,field,value,text", [
+    (_window, "ember_hip_window_attn", "window", 0, "window"), (_window, "ember_hip_window_attn", "sinks", -1, "sinks"),
+    (_prefix, "ember_hip_shared_prefix_attn", "n_groups", -1, "bad sizes"), (_prefix, "ember_hip_shared_prefix_attn", "n_groups", 4097, "bad sizes"),
+    (_prefix, "ember_hip_shared_prefix_attn", "max_group", 0, "bad sizes"), (_prefix, "ember_hip_shared_prefix_attn", "max_prefix", -1, "bad sizes"),
+    (_prefix, "ember_hip_shared_prefix_attn", "max_own", 0, "bad sizes"), (_prefix, "ember_hip_shared_prefix_attn", "group_start", None, "null"),
+    (_prefix, "ember_hip_shared_prefix_attn", "prefix_len", None, "null"), (_prefix, "ember_hip_shared_prefix_attn", "n_groups", 1, "bytes of workspace")])
+def test_span_refusals(make, entry, field, value, text):
+    a = make()
+    setattr(a, field, value)
+    assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
+    assert text in _lib.last_error()
+
+
+def test_null_and_empty_calls():
+    lib = _lib.lib()
+    for entry in ("ember_hip_step_tables", "ember_hip_window_attn", "ember_hip_shared_prefix_attn"):
+        assert getattr(lib, entry)(None, None) == _lib.ERR_INVALID
+    for entry in ("ember_hip_window_workspace_bytes", "ember_hip_shared_prefix_workspace_bytes"):
+        assert getattr(lib, entry)(None) == 0
+    for make, entry in ((_window, "ember_hip_window_attn"), (_prefix, "ember_hip_shared_prefix_attn")):
+        for field in ("T", "S"):
+            a = make()
+            setattr(a.batch, field, 0)
+            assert getattr(lib, entry)(a, None) == _lib.OK  # nothing to do, nothing launched
+
+
+def test_workspace_covers_smaller_tables():
+    """A workspace sized without a table width holds the partials of any table width."""
+    size = _lib.lib().ember_hip_window_workspace_bytes
+    for S in (1, 3, 40):
+        for window in (20, 500, 5000):
+            for q in (1, 9, 200):
+                a = _window()
+                a.window, a.batch.S, a.batch.T, a.batch.max_query, a.batch.max_blocks = window, S, S * q, q, 1 << 26
+                most = size(a)
+                for blocks in (1, 7, 33, 64, 130, 400, 1000):
+                    a.batch.max_blocks = blocks
+                    assert size(a) <= most
+    assert K.window_workspace(64, 64, n_heads=16, n_kv=8, window=100000, max_query=1, device="cpu") is not None
+    assert K.window_workspace(1, 1, n_heads=16, n_kv=8, window=10, max_query=1, device="cpu") is None
