@@ -11,10 +11,10 @@
 //   own      rows of one sequence, base = its group's prefix length.
 // The pages that hold such keys are at most two runs of the table (the first
 // tokens' and the rest), numbered through as virtual pages, so no other entry
-// of the table is followed and a split is a run of virtual pages. Rows that
-// are split (over a long axis, or into prefix and own keys) leave partials
-// (running max, sum, unnormalised output) in slots of the workspace, which a
-// merge launch joins in slot order: no atomics, the same bits every time.
+// of the table is followed and a split is a run of virtual pages. Partials
+// (running max, sum, unnormalised output) of rows that are split, over a long
+// axis or into prefix and own keys, go to slots of the workspace, and a merge
+// launch joins them in slot order: no atomics, the same bits every time.
 //
 // Two forms. Few rows (16 at most: decode, verify) are bound by the read of
 // the pages: span_walk_kernel gives each wave pages of its own, straight from
@@ -32,10 +32,10 @@
 namespace ember::hip {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
 constexpr int kWalkRows = 16;              // query rows of a walk work-group: one MFMA column each
-constexpr int kTileRows = 32 * kWaves;     // query rows of a tile work-group: 32 a wave
+constexpr int kTileWaves = 4;              // a tile's waves in one key group: 32 query rows each
+constexpr int kTileRows = 32 * kTileWaves;
+constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kBlockPages = 4;             // pages of a tile's key block
 constexpr int kBlockKeys = kBlockPages * kPage;
 constexpr int kNoWindow = INT_MAX;
@@ -66,30 +66,34 @@ struct Rows {
     int t0, rows;     // first token, (token, head) rows
     int seq;          // the table's row
     int base, limit;  // keys base .. limit - 1
+    int pos;          // the first token's position, if there is one token (rows == G)
 };
 
-// The prefix length of sequence s's group; 0 if it is in none. 64 starts are looked at together, so up to 4096
-// groups cost two loads one after the other.
-__device__ __forceinline__ int own_base(const SpanParams &p, int s, int lane, bool &grouped) {
+// The group of sequence s by 64-ary search (one step for up to 63 groups): whether it is in one, and its prefix length.
+__device__ __forceinline__ bool group_of(const SpanParams &p, int s, int lane, int &prefix) {
     int lo = 0, n = p.n_groups;  // the group, if there is one, is among lo .. lo + n - 1
+    prefix = 0;
     while (n > 0) {
-        const int step = (n + kWave - 1) / kWave;
-        const int at = lo + lane * step;
-        const bool starts = lane * step < n && p.group_start[at] <= s;
-        const int c = __popcll(__builtin_amdgcn_ballot_w64(starts));  // starts are ascending: lanes 0 .. c - 1
-        if (c == 0) break;
-        const int from = uniform(lo + (c - 1) * step);
+        const int step = (n + kWave - 2) / (kWave - 1);  // lanes 0 .. 62 look at a start each, the one behind them at the end
+        const int at = min(lo + lane * step, p.n_groups);
+        const int start = p.group_start[at], len = p.prefix_len[min(at, p.n_groups - 1)];
+        const int c = __popcll(__builtin_amdgcn_ballot_w64(lane * step < n && start <= s));  // starts ascend: lanes 0 .. c - 1
+        if (c == 0) return false;
         if (step == 1) {
-            grouped = s < uniform_load(p.group_start + from + 1);
-            return grouped ? max(0, uniform_load(p.prefix_len + from)) : 0;
+            prefix = max(0, __builtin_amdgcn_readlane(len, c - 1));
+            const bool in = s < __builtin_amdgcn_readlane(start, c);
+            prefix = in ? prefix : 0;
+            return in;
         }
+        const int from = lo + (c - 1) * step;
         n = min(step, lo + n - from);
         lo = from;
     }
-    grouped = false;
-    return 0;
+    return false;
 }
 
+// What one trip to memory can tell of a work item. A sequence of a pure decode step has its token at row `unit`: its
+// position is requested beside query_start and used if query_start says so.
 __device__ __forceinline__ Rows rows_of(const SpanParams &p, const Phase &ph, int unit, int lane, bool &grouped) {
     Rows r;
     int s0 = unit, s1 = unit + 1;
@@ -97,16 +101,20 @@ __device__ __forceinline__ Rows rows_of(const SpanParams &p, const Phase &ph, in
     r.limit = INT_MAX;
     grouped = true;
     if (ph.kind == kPrefixRows) {
-        s0 = clamped(uniform_load(p.group_start + unit), p.S);
-        s1 = clamped(uniform_load(p.group_start + unit + 1), p.S);
+        s0 = uniform_load(p.group_start + unit);
+        s1 = uniform_load(p.group_start + unit + 1);
         r.limit = max(0, uniform_load(p.prefix_len + unit));
-    } else if (ph.kind == kOwnRows) {
-        r.base = own_base(p, unit, lane, grouped);
+        s0 = clamped(s0, p.S);
+        s1 = max(clamped(s1, p.S), s0);
     }
-    r.t0 = clamped(uniform_load(p.query_start + s0), p.T);
-    r.rows = max(0, clamped(uniform_load(p.query_start + s1), p.T) - r.t0) * p.G;
+    int guess = uniform_load(p.positions + min(unit, p.T - 1));
+    const int t0 = uniform_load(p.query_start + s0), t1 = uniform_load(p.query_start + s1);
+    if (ph.kind == kOwnRows) grouped = group_of(p, unit, lane, r.base);
+    r.t0 = clamped(t0, p.T);
+    r.rows = max(0, clamped(t1, p.T) - r.t0) * p.G;
     r.seq = min(s0, p.S - 1);
-    if (s1 <= s0) r.rows = 0;
+    if (r.rows == p.G && r.t0 != unit) guess = uniform_load(p.positions + r.t0);
+    r.pos = guess;
     return r;
 }
 
@@ -141,31 +149,40 @@ __device__ __forceinline__ bool visible(int j, int base, int top, int pos, int w
 
 // ---- few rows: a page per wave ----
 
-// Lane l = 16 g + c serves query column c, the item's row c (columns past the last repeat it). The f16 form is
-// the decode kernel's: S^T = K Q^T on v_mfma_f32_16x16x32_f16 with the keys staged in the wave's LDS by direct
-// loads, O^T += V^T P^T on v_mfma_f32_16x16x16_f16 with V in registers. f32 pages use v_mfma_f32_16x16x4_f32 the
-// same way: step s of the scores takes dim 16 (s / 4) + 4 g + s % 4 from lane group g, so a lane loads key c in
-// 16-byte pieces; step v of the values takes key 4 g + v, which the lane's own scores belong to.
-template <typename T>
+// Lane l = 16 g + c serves query column c, the item's row c (columns past the last repeat it). f16 pages: S^T = K Q^T
+// on v_mfma_f32_16x16x32_f16 (step s takes dims 32 s + 8 g .. + 7), O^T += V^T P^T on v_mfma_f32_16x16x16_f16. f32
+// pages use v_mfma_f32_16x16x4_f32 the same way: step s of the scores takes dim 16 (s / 4) + 4 g + s % 4 from lane
+// group g, so a lane loads key c in 16-byte pieces; step v of the values takes key 4 g + v, which the lane's own
+// scores belong to. Keys of the f16 form pass through LDS (direct loads of four whole rows an instruction, swizzled)
+// where a CU runs 16 waves, each with half a page in flight. DEEP keeps two whole pages in registers instead, for 8
+// waves a CU.
+template <typename T, bool DEEP>
 struct WalkPage;
 template <>
-struct WalkPage<f16> {
+struct WalkPage<f16, false> {
     u32x4 v[4];  // keys 4 g + i, dims 8 c .. 8 c + 7
 };
 template <>
-struct WalkPage<float> {
+struct WalkPage<f16, true> {
+    u32x4 k[4];  // key c, dims 32 i + 8 g .. + 7
+    u32x4 v[4];
+};
+template <>
+struct WalkPage<float, false> {
     u32x4 k[8];     // key c, dims 16 i + 4 g .. + 3
     u32x4 v[4][2];  // keys 4 g + i, dims 8 c .. 8 c + 7
 };
 
-template <typename T>
-__device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, const int id) {
-    constexpr int D = kHeadDim;
-    constexpr bool F16 = sizeof(T) == 2;
-    constexpr int RP = D + 4;            // floats of a row's partial in LDS: 16 rows' pieces of one dim on distinct banks
-    constexpr int RW = kWalkRows * RP;   // floats of a wave's region (its first 4 KiB also stage f16 keys)
-    __shared__ __align__(16) float red[kWaves * RW];
-    __shared__ float red_m[kWalkRows][kWaves], red_l[kWalkRows][kWaves];
+constexpr int kWalkRowPitch = kHeadDim + 4;               // floats of a row's partial: 16 rows' pieces of one dim on distinct banks
+constexpr int kWalkWave = kWalkRows * kWalkRowPitch;      // floats of a wave's region (f16: its first 4 KiB also stage keys)
+constexpr int walk_lds_floats(int W) { return W * (kWalkWave + 2 * kWalkRows); }
+
+template <typename T, int W, bool DEEP>  // W waves
+__device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, const int id, float *red) {
+    constexpr int D = kHeadDim, kThreads = W * kWave, RP = kWalkRowPitch, RW = kWalkWave;
+    constexpr bool F16 = sizeof(T) == 2, STAGED = F16 && !DEEP;
+    constexpr int KQ = F16 ? 4 : 8;  // 16-byte pieces of a row of q or K in a lane
+    float *const red_m = red + W * RW, *const red_l = red_m + W * kWalkRows;  // [row][wave]
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int g = lane >> 4, c = lane & 15;
     const int kvh = id % p.n_kv;
@@ -180,98 +197,137 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
     const int64_t head_off = static_cast<int64_t>(kvh) * (kPage * D), block_stride = static_cast<int64_t>(p.n_kv) * (kPage * D);
     const T *const kbase = static_cast<const T *>(p.k) + head_off, *const vbase = static_cast<const T *>(p.v) + head_off;
     const int window = ph.kind == kWindowRows ? p.window : kNoWindow, sinks = ph.kind == kWindowRows ? p.sinks : 0;
+    const int table_top = p.max_blocks * kPage - 1;
+    const bool partial = p.slots > 1;
+    // Without a window the pages start at the base: their ids are requested before the positions are known.
+    const int early_page = r.base / kPage + split * ph.pages + wave + lane * W;
+    int early = -1;
+    if (ph.kind != kWindowRows && early_page < p.max_blocks) early = table[early_page];
 
     for (int row0 = tile0 * kWalkRows; row0 < r.rows; row0 += ph.tiles * kWalkRows) {
         const int nrows = min(kWalkRows, r.rows - row0);
         const int my_row = row0 + min(c, nrows - 1);
         const int my_tok = r.t0 + my_row / p.G, my_head = kvh * p.G + my_row % p.G;
-        const int my_pos = max(p.positions[my_tok], -1);
-        // The row's q as the scores' B operand; used after the first pages are on their way.
-        u32x4 qf[F16 ? 4 : 8];
+        auto top_of = [&](int pos) { return min(min(pos, r.limit - 1), table_top); };
+        int my_pos, min_pos, max_pos, min_top, max_top;
+        if (r.rows == p.G) {
+            my_pos = min_pos = max_pos = max(r.pos, -1);
+            min_top = max_top = top_of(my_pos);
+        } else {
+            my_pos = max(p.positions[my_tok], -1);
+            min_pos = max_pos = my_pos;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                min_pos = min(min_pos, __shfl_xor(min_pos, o, kWave));
+                max_pos = max(max_pos, __shfl_xor(max_pos, o, kWave));
+            }
+            min_pos = uniform(min_pos), max_pos = uniform(max_pos);
+            min_top = top_of(min_pos), max_top = top_of(max_pos);
+        }
+        const int my_top = top_of(my_pos);
+        u32x4 qf[KQ];  // the row's q as the scores' B operand
         {
             const T *qp = static_cast<const T *>(p.q) + my_tok * p.q_stride + my_head * D;
 #pragma unroll
-            for (int i = 0; i < (F16 ? 4 : 8); i++)
-                qf[i] = *reinterpret_cast<const u32x4 *>(qp + (F16 ? 32 * i + 8 * g : 16 * i + 4 * g));
+            for (int i = 0; i < KQ; i++) qf[i] = *reinterpret_cast<const u32x4 *>(qp + (F16 ? 32 * i + 8 * g : 16 * i + 4 * g));
         }
-        const int my_top = min(min(my_pos, r.limit - 1), p.max_blocks * kPage - 1);
-        int min_pos = my_pos, max_pos = my_pos, min_top = my_top, max_top = my_top;
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            min_pos = min(min_pos, __shfl_xor(min_pos, o, kWave));
-            max_pos = max(max_pos, __shfl_xor(max_pos, o, kWave));
-            min_top = min(min_top, __shfl_xor(min_top, o, kWave));
-            max_top = max(max_top, __shfl_xor(max_top, o, kWave));
-        }
-        min_pos = uniform(min_pos), max_pos = uniform(max_pos), min_top = uniform(min_top), max_top = uniform(max_top);
         const Span sp = span_of(r, window, sinks, min_pos, max_top);
         const int v0 = min(split * ph.pages, sp.pages);
         const int v1 = split == ph.splits - 1 ? sp.pages : min(v0 + ph.pages, sp.pages);
+        if (partial && v0 >= v1) {  // nothing to read: the slot is empty
+            if (tid < nrows) {
+                const int64_t at = static_cast<int64_t>(r.t0 + (row0 + tid) / p.G) * p.n_heads + kvh * p.G + (row0 + tid) % p.G;
+                float2 *const ml = reinterpret_cast<float2 *>(p.part_ml) + at * p.slots;
+                ml[ph.slot0 + split] = make_float2(kNoMax, 0.0f);
+                if (!grouped && split == 0)
+                    for (int i = 0; i < ph.slot0; i++) ml[i] = make_float2(kNoMax, 0.0f);
+            }
+            continue;
+        }
 
         float mc = kNoMax, lc = 0.0f;
         f32x4 o[8];  // o[t][v]: dim 32 g + 8 v + t of column c
 #pragma unroll
         for (int t = 0; t < 8; t++) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         uint32_t *const kstage = reinterpret_cast<uint32_t *>(&red[wave * RW]);
-        uint32_t k_dma[4], k_rd[4];  // f16: the swizzled stage (slot 16 k + (q ^ k): chunk q of key k), bytes and dwords
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            k_dma[i] = 1024u * i + 256u * g + 16u * ((c ^ (4 * i + g)) & 15);
-            k_rd[i] = 64u * c + 4u * (((4 * i + g) ^ c) & 15);
-        }
-        // The block ids of up to 64 virtual pages, one a lane; wave w takes pages w, w + 4, ...
-        for (int cv = v0; cv < v1; cv += kWave) {
-            const int chunk = min(kWave, v1 - cv);
-            const int n = chunk > wave ? (chunk - 1 - wave) / kWaves + 1 : 0;
-            const int ids = lane < chunk ? table[sp.page(cv + lane)] : -1;
+        // The swizzled stage: slot 16 k + (q ^ k) holds chunk q of key k. Load i writes keys 4 i .. + 3 (lane l the 16
+        // bytes at 16 l), step i reads chunk 4 i + g of key c; both differ between i by an exclusive or and a constant.
+        const uint32_t k_dma = 256u * g + 16u * (c ^ g), k_rd = 256u * c + 16u * (c ^ g);  // bytes
+        const uint32_t v_off = F16 ? 1024u * g + 16u * c : 2048u * g + 32u * c, k_off = (F16 ? 256u : 512u) * c + 16u * g;
+        // Wave w takes pages w, w + W, ...; the block ids of up to 64 of them at a time, one a lane.
+        for (int cv = v0 + wave; cv < v1; cv += W * kWave) {
+            const int n = min(kWave, (v1 - cv + W - 1) / W);
+            int ids = early;
+            if (ph.kind == kWindowRows || cv != v0 + wave) ids = lane < n ? table[sp.page(cv + lane * W)] : -1;
+            using Page = WalkPage<T, DEEP>;
             auto desc_of = [&](const T *base, int j) {
-                const int blk = __builtin_amdgcn_readlane(ids, min(wave + j * kWaves, chunk - 1));
+                const int blk = __builtin_amdgcn_readlane(ids, min(j, n - 1));
                 const bool live = j < n && blk >= 0 && blk < p.num_blocks;  // dead: no records, the loads give zeros
                 return __builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(base) + (live ? blk : 0) * block_stride, 0,
                                                          live ? kPage * D * static_cast<int>(sizeof(T)) : 0, kDescWord3);
             };
-            WalkPage<T> A;
-            auto fetch_keys = [&](int j) {
+            // A lane's offsets are made opaque where they are used: their constant parts then go into the loads, where
+            // the compiler would hold each sum in a register of its own across the loop.
+            auto here = [](uint32_t x) {
+                asm volatile("" : "+v"(x));
+                return x;
+            };
+            auto fetch_keys = [&](Page &A, int j) {
                 const __amdgpu_buffer_rsrc_t d = desc_of(kbase, j);
-                if constexpr (F16) {
+                const uint32_t off = here(STAGED ? k_dma : k_off);
+                if constexpr (STAGED) {
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                            d, (__attribute__((address_space(3))) void *)(kstage + 256 * i), 16, k_dma[i], 0, 0, kNonTemporal);
+                            d, (__attribute__((address_space(3))) void *)(kstage + 256 * i), 16, (off ^ (64u * i)) + 1024u * i, 0, 0,
+                            kNonTemporal);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) A.k[i] = load_desc(d, 512u * c + 64u * i + 16u * g);
+                    for (int i = 0; i < KQ; i++) A.k[i] = load_desc(d, off + 64u * i);
                 }
             };
-            auto fetch_values = [&](int j) {
+            auto fetch_values = [&](Page &A, int j) {
                 const __amdgpu_buffer_rsrc_t d = desc_of(vbase, j);
+                const uint32_t off = here(v_off);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     if constexpr (F16) {
-                        A.v[i] = load_desc(d, 1024u * g + 256u * i + 16u * c);
+                        A.v[i] = load_desc(d, off + 256u * i);
                     } else {
-                        A.v[i][0] = load_desc(d, 2048u * g + 512u * i + 32u * c);
-                        A.v[i][1] = load_desc(d, 2048u * g + 512u * i + 32u * c + 16u);
+                        A.v[i][0] = load_desc(d, off + 512u * i);
+                        A.v[i][1] = load_desc(d, off + 512u * i + 16u);
                     }
                 }
             };
-            fetch_keys(0);
-            fetch_values(0);
-            for (int j = 0; j < n; j++) {
-                const int page = sp.page(cv + wave + j * kWaves);
+            // Page j: its scores and the online softmax, then its values; `next` is called between, once its keys
+            // have been read.
+            auto consume = [&](Page &A, int j, auto next) {
+                const int page = sp.page(cv + j * W);
                 f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // s[v]: raw score of key 4 g + v
                 if constexpr (F16) {
                     u32x4 kf[4];
+                    if constexpr (STAGED) {  // at most the page's four value loads, issued after them, are out: its keys are here
+                        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    const uint32_t off = here(k_rd);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) kf[i] = *reinterpret_cast<const u32x4 *>(kstage + k_rd[i]);
+                    for (int i = 0; i < 4; i++) {
+                        if constexpr (STAGED) kf[i] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(kstage) + (off ^ (64u * i)));
+                        else kf[i] = A.k[i];
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(kf[i]), as_f16x8(qf[i]), s, 0, 0, 0);
                 } else {
+                    f32x4 s2 = s;  // two chains: each product waits for the one before it
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
+                    for (int i = 0; i < KQ; i++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
+                        for (int e = 0; e < 4; e += 2) {
                             s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(A.k[i][e]), __uint_as_float(qf[i][e]), s, 0, 0, 0);
+                            s2 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(A.k[i][e + 1]), __uint_as_float(qf[i][e + 1]), s2, 0, 0, 0);
+                        }
+                    s = s + s2;
                 }
                 uint32_t dead = 0;  // bit v: no row sees key 4 g + v, whose values may then be anything
                 if (!whole_page(page, r, window, sinks, max_pos, min_top)) {
@@ -293,7 +349,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
 #pragma unroll
                 for (int v = 0; v < 4; v++) w[v] = exp2_hw(__builtin_fmaf(s[v], p.scale_log2, -mn));
                 // f16: the weights are rounded to f16, the products' operand, and summed as rounded, so that the
-                // rounding of a weight (2^-12 of it at most) moves numerator and denominator alike.
+                // rounding of a weight (2^-11 of it at most) moves numerator and denominator alike.
                 f16x4 wh;
                 if constexpr (F16) {
 #pragma unroll
@@ -305,9 +361,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 }
 #pragma unroll
                 for (int t = 0; t < 8; t++) o[t] = o[t] * corr;
-                __builtin_amdgcn_sched_barrier(0);
-                fetch_keys(j + 1);
-                __builtin_amdgcn_sched_barrier(0);
+                next();
                 if (__builtin_amdgcn_ballot_w64(dead != 0)) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
@@ -336,13 +390,48 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                         for (int t = 0; t < 8; t++)
                             o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(A.v[v][t / 4][t % 4]), w[v], o[t], 0, 0, 0);
                 }
+            };
+            if constexpr (DEEP) {
+                Page A, B;
+                fetch_keys(A, 0);
+                fetch_values(A, 0);
+                fetch_keys(B, 1);
+                fetch_values(B, 1);
+                auto nothing = [] {};
+                for (int j = 0; j < n; j += 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    consume(A, j, nothing);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch_keys(A, j + 2);
+                    fetch_values(A, j + 2);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j + 1 < n) consume(B, j + 1, nothing);
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch_keys(B, j + 3);
+                    fetch_values(B, j + 3);
+                }
+            } else {
+                // Keys and values are requested in this order and nothing moves across: the wait for staged keys counts.
+                Page A;
                 __builtin_amdgcn_sched_barrier(0);
-                fetch_values(j + 1);
+                fetch_keys(A, 0);
                 __builtin_amdgcn_sched_barrier(0);
+                fetch_values(A, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                for (int j = 0; j < n; j++) {
+                    consume(A, j, [&] {
+                        __builtin_amdgcn_sched_barrier(0);
+                        fetch_keys(A, j + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch_values(A, j + 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                // The fetch past the last page still writes zeros into the stage, where the next chunk's keys or the
+                // wave's partial go.
+                if constexpr (STAGED) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
-            // The fetch past the last page still writes zeros into the stage, where the next chunk's keys or the
-            // wave's partial go.
-            __builtin_amdgcn_s_waitcnt(0);
         }
 
         // The column's sum over its lane groups, the wave's partial into LDS, and the waves' merge in order.
@@ -355,51 +444,52 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 *reinterpret_cast<float4 *>(dst + 4) = make_float4(o[4][v], o[5][v], o[6][v], o[7][v]);
             }
             if (g == 0) {
-                red_m[c][wave] = mc;
-                red_l[c][wave] = lc;
+                red_m[c * W + wave] = mc;
+                red_l[c * W + wave] = lc;
             }
         }
         __syncthreads();
-        for (int idx = tid; idx < nrows * D; idx += kThreads) {
-            const int row = idx / D, d = idx % D;
-            float M = kNoMax;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) M = fmaxf(M, red_m[row][w]);
-            float L = 0.0f, O = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                const float f = exp2_hw(red_m[row][w] - M);
-                L = L + red_l[row][w] * f;
-                O = O + red[w * RW + row * RP + d] * f;
+        for (int i = tid; i < nrows * (D / 2); i += kThreads) {
+            const int row = i / (D / 2), d = 2 * (i % (D / 2));
+            float M = kNoMax, L = 0.0f;
+#pragma unroll 4
+            for (int w = 0; w < W; w++) M = fmaxf(M, red_m[row * W + w]);
+            float2 O = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+            for (int w = 0; w < W; w++) {
+                const float f = exp2_hw(red_m[row * W + w] - M);
+                const float2 x = *reinterpret_cast<const float2 *>(&red[w * RW + row * RP + d]);
+                L = L + red_l[row * W + w] * f;
+                O.x = O.x + x.x * f;
+                O.y = O.y + x.y * f;
             }
-            const int tok = r.t0 + (row0 + row) / p.G, head = kvh * p.G + (row0 + row) % p.G;
-            const int64_t at = static_cast<int64_t>(tok) * p.n_heads + head;
-            if (p.slots == 1) {
-                static_cast<T *>(p.out)[at * D + d] = from_f32<T>(L > 0.0f ? O / L : 0.0f);
-            } else {
+            const int64_t at = static_cast<int64_t>(r.t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
+            if (partial) {
                 const int64_t slot = at * p.slots + ph.slot0 + split;
-                p.part_acc[slot * D + d] = O;
+                float2 *const ml = reinterpret_cast<float2 *>(p.part_ml);
+                *reinterpret_cast<float2 *>(p.part_acc + slot * D + d) = O;
                 if (d == 0) {
-                    p.part_ml[slot * 2] = M;
-                    p.part_ml[slot * 2 + 1] = L;
-                    // rows of no group: their prefix slots hold nothing
-                    if (!grouped && split == 0)
-                        for (int i = 0; i < ph.slot0; i++) {
-                            p.part_ml[(at * p.slots + i) * 2] = kNoMax;
-                            p.part_ml[(at * p.slots + i) * 2 + 1] = 0.0f;
-                        }
+                    ml[slot] = make_float2(M, L);
+                    if (!grouped && split == 0)  // a row of no group: its prefix slots hold nothing
+                        for (int k = 0; k < ph.slot0; k++) ml[at * p.slots + k] = make_float2(kNoMax, 0.0f);
                 }
+            } else {
+                T *const dst = static_cast<T *>(p.out) + at * D + d;
+                dst[0] = from_f32<T>(L > 0.0f ? O.x / L : 0.0f);
+                dst[1] = from_f32<T>(L > 0.0f ? O.y / L : 0.0f);
             }
         }
         __syncthreads();  // the regions are the next row tile's stages
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) span_walk_kernel(SpanParams p, Phase a, Phase b, int a_groups) {
+// Two phases in one launch (b.units may be 0). A CU holds 16 waves of the f16 form and 8 of the f32 form.
+template <typename T, int W>
+__global__ void __launch_bounds__(W *kWave, (sizeof(T) == 2 ? 4 : 2)) span_walk_kernel(SpanParams p, Phase a, Phase b, int a_groups) {
+    __shared__ __align__(16) float red[walk_lds_floats(W)];
     const int id = static_cast<int>(blockIdx.x);
     const bool second = id >= a_groups;
-    walk_item<T>(p, second ? b : a, second ? id - a_groups : id);
+    walk_item<T, W, false>(p, second ? b : a, second ? id - a_groups : id, red);
 }
 
 // ---- many rows: key blocks shared in LDS (f16) ----
@@ -418,14 +508,22 @@ typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
 // How far (base 2) a score may pass the reference max before the reference moves: weights stay below 2^8, which
 // f16 holds, and most blocks rescale nothing.
 constexpr float kLazy = 8.0f;
+constexpr int kAhead = 4;  // value operands in flight ahead of their products
 
-__global__ void __launch_bounds__(kThreads, 2) span_tile_kernel(SpanParams p, Phase ph) {
+// KG key groups of 4 waves, the same rows each: group g takes blocks g, g + KG, ... through buffers of its own, and
+// the last ones hand their partials to group 0 through LDS.
+constexpr int kBuffer = kBlockKeys * kRow;
+constexpr int tile_lds_bytes(int KG) { return KG * 4 * kBuffer * static_cast<int>(sizeof(f16)) + 64; }
+
+template <int KG>
+__device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, const int id, unsigned char *lds) {
     constexpr int D = kHeadDim;
-    __shared__ __align__(16) f16 k_lds[2][kBlockKeys * kRow], v_lds[2][kBlockKeys * kRow];
-    __shared__ int ext[kWaves][4];
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
+    f16 *const k_all = reinterpret_cast<f16 *>(lds), *const v_all = k_all + KG * 2 * kBuffer;
+    int *const ext = reinterpret_cast<int *>(v_all + KG * 2 * kBuffer);  // [wave][2]
+    const int group = KG == 1 ? 0 : uniform(static_cast<int>(threadIdx.x) / kTileThreads);
+    const int tid = static_cast<int>(threadIdx.x) % kTileThreads, lane = tid % kWave, wave = uniform(tid / kWave);
+    f16 *const k_lds = k_all + group * 2 * kBuffer, *const v_lds = v_all + group * 2 * kBuffer;  // two buffers each
     const int h = lane >> 5, c = lane & 31;
-    const int id = static_cast<int>(blockIdx.x);
     const int kvh = id % p.n_kv;
     int rest = id / p.n_kv;
     const int split = rest % ph.splits;
@@ -460,17 +558,20 @@ __global__ void __launch_bounds__(kThreads, 2) span_tile_kernel(SpanParams p, Ph
             hi_top = max(hi_top, __shfl_xor(hi_top, o, kWave));
         }
         lo_pos = uniform(lo_pos), hi_pos = uniform(hi_pos), lo_top = uniform(lo_top), hi_top = uniform(hi_top);
-        if (lane == 0) ext[wave][0] = lo_pos, ext[wave][1] = hi_top;
+        if (group == 0 && lane == 0) ext[2 * wave] = lo_pos, ext[2 * wave + 1] = hi_top;
         __syncthreads();
         int min_pos = lo_pos, max_top = hi_top;  // of the tile
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) min_pos = min(min_pos, ext[w][0]), max_top = max(max_top, ext[w][1]);
+        for (int w = 0; w < kTileWaves; w++) min_pos = min(min_pos, ext[2 * w]), max_top = max(max_top, ext[2 * w + 1]);
         min_pos = uniform(min_pos), max_top = uniform(max_top);
         const Span sp = span_of(r, window, sinks, min_pos, max_top);
         const int v0 = min(split * ph.pages, sp.pages);
         const int v1 = split == ph.splits - 1 ? sp.pages : min(v0 + ph.pages, sp.pages);
-        const int blocks = (v1 - v0 + kBlockPages - 1) / kBlockPages;
+        const int blocks = (v1 - v0 + kBlockPages - 1) / kBlockPages;  // this group's: group, group + KG, ...
+        const bool partial = p.slots > 1;
 
+        // This lane's part of a value operand: key 4 h + r / 4, dims 16 (l / 16 % 2) + 4 (r % 4) .. + 3 of its 16-lane block.
+        const int v_at = (4 * h + lane % 16 / 4) * kRow + 16 * (lane / 16 % 2) + 4 * (lane % 4);
         float m = -INFINITY, l = 0.0f;
         f32x16 o[4];
 #pragma unroll
@@ -478,73 +579,118 @@ __global__ void __launch_bounds__(kThreads, 2) span_tile_kernel(SpanParams p, Ph
 #pragma unroll
             for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
 
-        // A block's pages into registers: each page one 16-byte piece a thread, of key tid / 16. Keys that no row of
-        // the tile sees may hold anything: their values become zeros, so that a zero weight meets no NaN.
+        // Keys that this lane's row sees: n from `from` on, and those below `sink_end`.
+        const int from = max(r.base, window == kNoWindow ? 0 : max(my_pos - window + 1, 0));
+        const uint32_t n_from = max(my_top - from + 1, 0);
+        const int sink_end = min(sinks, my_top + 1);
+        // Virtual pages whole0 .. whole1 - 1: every row of the wave sees every key of them.
+        const int whole_key = max(r.base, window == kNoWindow ? 0 : hi_pos - window + 1);
+        const int whole0 = sp.head + (max(whole_key, 0) + kPage - 1) / kPage - (sp.skip + sp.head);
+        const int whole1 = (lo_top + 1) / kPage - sp.skip;
+        // Keys that some row of the tile sees, likewise. Others may hold anything: their values are read as zeros
+        // (an offset past the page's records), so that a zero weight meets no NaN.
+        const uint32_t n_live = max(max_top - sp.lo + 1, 0);
+        const int sink_live = min(sinks, max_top + 1);
+
+        // A block's pages into registers: each page one 16-byte piece a thread, of key tid / 16. Where the pages of
+        // 64 virtual pages are, and their bytes (0: not in the pool, the loads give zeros), one page a lane.
         u32x4 kr[kBlockPages], vr[kBlockPages];
-        int ids = -1, next_ids = v0 + lane < v1 ? table[sp.page(v0 + lane)] : -1;  // 64 virtual pages, one a lane
+        // Step b of this group reads virtual pages first_page(b) .. + 3.
+        auto first_page = [&](int b) { return v0 + (b * KG + group) * kBlockPages; };
+        auto id_of = [&](int b0) {  // lane 4 i + j: page j of step b0 + i
+            const int v = first_page(b0 + lane / kBlockPages) + lane % kBlockPages;
+            return v < v1 ? table[sp.page(v)] : -1;
+        };
+        int next_ids = id_of(0);
+        int64_t at64 = 0;
+        int bytes64 = 0;
         auto fetch = [&](int b) {
             if (b % (kWave / kBlockPages) == 0) {
-                ids = next_ids;
-                const int v = v0 + b * kBlockPages + kWave + lane;
-                next_ids = v < v1 ? table[sp.page(v)] : -1;
+                const bool live = next_ids >= 0 && next_ids < p.num_blocks;
+                at64 = (live ? next_ids : 0) * block_stride * static_cast<int64_t>(sizeof(f16));
+                bytes64 = live ? kPage * D * 2 : 0;
+                next_ids = id_of(b + kWave / kBlockPages);
             }
 #pragma unroll
             for (int j = 0; j < kBlockPages; j++) {
-                const int v = v0 + b * kBlockPages + j;
-                const int blk = __builtin_amdgcn_readlane(ids, (b * kBlockPages + j) % kWave);
-                const bool live = v < v1 && blk >= 0 && blk < p.num_blocks;
-                const int64_t at = (live ? blk : 0) * block_stride;
-                const int bytes = live ? kPage * D * 2 : 0;
-                const __amdgpu_buffer_rsrc_t kd = __builtin_amdgcn_make_buffer_rsrc(const_cast<f16 *>(kbase) + at, 0, bytes, kDescWord3);
-                const __amdgpu_buffer_rsrc_t vd = __builtin_amdgcn_make_buffer_rsrc(const_cast<f16 *>(vbase) + at, 0, bytes, kDescWord3);
+                const int n = (b * kBlockPages + j) % kWave;
+                const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(
+                                       __builtin_amdgcn_readlane(static_cast<int>(at64 >> 32), n))) << 32 |
+                                   static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at64), n)));
+                const int bytes = __builtin_amdgcn_readlane(bytes64, n);
+                const int key = sp.page(first_page(b) + j) * kPage + tid / 16;
+                const bool live = (static_cast<uint32_t>(key - sp.lo) < n_live) | (key < sink_live);
+                const __amdgpu_buffer_rsrc_t kd = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<char *>(reinterpret_cast<const char *>(kbase) + at), 0, bytes, kDescWord3);
+                const __amdgpu_buffer_rsrc_t vd = __builtin_amdgcn_make_buffer_rsrc(
+                    const_cast<char *>(reinterpret_cast<const char *>(vbase) + at), 0, bytes, kDescWord3);
                 kr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kd, 16 * tid, 0, 0));
-                vr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vd, 16 * tid, 0, 0));
+                vr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vd, live ? 16 * tid : kPage * D * 2, 0, 0));
             }
         };
         auto stage = [&](int b) {
 #pragma unroll
             for (int j = 0; j < kBlockPages; j++) {
-                const int key = sp.page(v0 + b * kBlockPages + j) * kPage + tid / 16;
-                const bool dead = key < r.base || key > max_top || (key < sp.lo && key >= sinks);
                 const int at = (j * kPage + tid / 16) * kRow + tid % 16 * 8;
-                *reinterpret_cast<u32x4 *>(&k_lds[b & 1][at]) = kr[j];
-                *reinterpret_cast<u32x4 *>(&v_lds[b & 1][at]) = dead ? u32x4{0, 0, 0, 0} : vr[j];
+                *reinterpret_cast<u32x4 *>(&k_lds[(b & 1) * kBuffer + at]) = kr[j];
+                *reinterpret_cast<u32x4 *>(&v_lds[(b & 1) * kBuffer + at]) = vr[j];
             }
         };
-        if (blocks > 0) {
+        const int steps = (blocks + KG - 1) / KG;
+        if (steps > 0) {
             fetch(0);
             stage(0);
         }
         __syncthreads();
-        for (int b = 0; b < blocks; b++) {
-            if (b + 1 < blocks) fetch(b + 1);
-            const f16 *const kl = k_lds[b & 1], *const vl = v_lds[b & 1];
+        for (int b = 0; b < steps; b++) {
+            if (b + 1 < steps) fetch(b + 1);
+            const f16 *const kl = k_lds + (b & 1) * kBuffer + c * kRow + 8 * h, *const vl = v_lds + (b & 1) * kBuffer + v_at;
+            // Scores: the operands of a 32-key half are all requested before its first product, and each is
+            // replaced by the other half's as soon as its product is issued.
             f32x16 s[2];
+            f16x8 ka[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) ka[i] = *reinterpret_cast<const f16x8 *>(kl + 16 * i);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int t = 0; t < 2; t++) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const f16x8 a = *reinterpret_cast<const f16x8 *>(&kl[(32 * t + c) * kRow + 16 * i + 8 * h]);
-                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qf[i], s[t], 0, 0, 0);
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i], qf[i], s[t], 0, 0, 0);
+                    if (t == 0) ka[i] = *reinterpret_cast<const f16x8 *>(kl + 32 * kRow + 16 * i);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            // The first values, in flight during the softmax: operand n = 4 j + t is dim tile t of keys 16 j .. + 15.
+            auto value = [&](int n) {
+                const f16 *const at = vl + n / 4 * 16 * kRow + n % 4 * 32;
+                const f16x4 lo4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)at));
+                const f16x4 hi4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)(at + 8 * kRow)));
+                return f16x8{lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
+            };
+            f16x8 va[kAhead];
 #pragma unroll
-            for (int j = 0; j < kBlockPages; j++) {
-                const int v = v0 + b * kBlockPages + j;
-                const int page = sp.page(v);
-                if (v < v1 && whole_page(page, r, window, sinks, hi_pos, lo_top)) continue;
+            for (int n = 0; n < kAhead; n++) va[n] = value(n);
+            __builtin_amdgcn_sched_barrier(0);
+            // (a run is whole blocks for every group, so pages past it lie past every row's keys)
+            const int vb = first_page(b);
+            if (!(vb >= whole0 && vb + kBlockPages <= whole1)) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int key = page * kPage + 8 * (i / 4) + 4 * h + i % 4;
-                    const bool see = v < v1 && visible(key, r.base, my_top, my_pos, window, sinks);
-                    s[j / 2][8 * (j % 2) + i] = see ? s[j / 2][8 * (j % 2) + i] : -INFINITY;
+                for (int j = 0; j < kBlockPages; j++) {
+                    const int key0 = sp.page(vb + j) * kPage + 4 * h;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int key = key0 + 8 * (i / 4) + i % 4;
+                        const bool see = (static_cast<uint32_t>(key - from) < n_from) | (key < sink_end);
+                        s[j / 2][8 * (j % 2) + i] = see ? s[j / 2][8 * (j % 2) + i] : -INFINITY;
+                    }
                 }
             }
-            float top = s[0][0];
+            float top = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-            for (int i = 1; i < 32; i++) top = fmaxf(top, s[i / 16][i % 16]);
+            for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
             top = top * p.scale_log2;
             if (__builtin_amdgcn_ballot_w64(top > m + kLazy)) {
                 const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
@@ -557,8 +703,8 @@ __global__ void __launch_bounds__(kThreads, 2) span_tile_kernel(SpanParams p, Ph
                 for (int t = 0; t < 4; t++) o[t] = o[t] * corr;
             }
             const float neg = m == -INFINITY ? 0.0f : -m;
-            f16x8 w[4];
             const f16x2 ones = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+            f16x8 w[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
@@ -568,74 +714,131 @@ __global__ void __launch_bounds__(kThreads, 2) span_tile_kernel(SpanParams p, Ph
                 for (int i = 0; i < 4; i++) l = __builtin_amdgcn_fdot2(f16x2{w[j][2 * i], w[j][2 * i + 1]}, ones, l, false);
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const int r16 = lane & 15;
-                    const f16 *const at = &vl[(16 * j + 4 * h + r16 / 4) * kRow + 32 * t + 16 * (lane >> 4 & 1) + 4 * (r16 % 4)];
-                    const f16x4 lo4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)at));
-                    const f16x4 hi4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)(at + 8 * kRow)));
-                    const f16x8 a = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, w[j], o[t], 0, 0, 0);
-                }
-            if (b + 1 < blocks) stage(b + 1);
+            for (int n = 0; n < 16; n++) {
+                o[n % 4] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[n % kAhead], w[n / 4], o[n % 4], 0, 0, 0);
+                if (n + kAhead < 16) va[n % kAhead] = value(n + kAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (b + 1 < steps) stage(b + 1);
             __syncthreads();
         }
 
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-        l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-        if (mine) {
+        if constexpr (KG == 2) {  // group 1's partial, through the buffers (every wave is past its last block)
+            f32x4 *const hand = reinterpret_cast<f32x4 *>(k_all) + tid;
+            static_assert(17 * kTileThreads * sizeof(f32x4) <= KG * 2 * kBuffer * sizeof(f16));
+            if (group == 1) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    hand[i * kTileThreads] = f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+                hand[16 * kTileThreads] = f32x4{m, l, 0.0f, 0.0f};
+            }
+            __syncthreads();
+            if (group == 0) {
+                const f32x4 ml = hand[16 * kTileThreads];
+                const float top = fmaxf(m, ml[0]);
+                const float f0 = m == -INFINITY ? 0.0f : exp2_hw(m - top), f1 = ml[0] == -INFINITY ? 0.0f : exp2_hw(ml[0] - top);
+                m = top;
+                l = l * f0 + ml[1] * f1;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const f32x4 x = hand[i * kTileThreads];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[i / 4][4 * (i % 4) + e] = o[i / 4][4 * (i % 4) + e] * f0 + x[e] * f1;
+                }
+            }
+            __syncthreads();  // the buffers are the next row tile's
+        }
+        if (group == 0 && mine) {
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+            l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
             const int64_t at = static_cast<int64_t>(my_tok) * p.n_heads + my_head;
-            if (p.slots == 1) {
+            if (partial) {
+                const int64_t slot = at * p.slots + ph.slot0 + split;
+                float *const dst = p.part_acc + slot * D + 4 * h;
+                if (blocks > 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++)  // dims 32 (i / 4) + 8 (i % 4) + 4 h .. + 3
+                        *reinterpret_cast<float4 *>(dst + 8 * i) = make_float4(o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
+                                                                               o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]);
+                }
+                if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + slot * 2) = make_float2(l > 0.0f ? m : kNoMax, l);
+            } else {
                 f16 *const dst = static_cast<f16 *>(p.out) + at * D + 4 * h;
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {  // dims 32 (i / 4) + 8 (i % 4) + 4 h .. + 3
-                    f16x4 x;
+                for (int i = 0; i < 16; i++) {
+                    f16x4 y;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] = static_cast<f16>(o[i / 4][4 * (i % 4) + e] * inv);
-                    *reinterpret_cast<f16x4 *>(dst + 8 * i) = x;
-                }
-            } else {
-                const int64_t slot = at * p.slots + ph.slot0 + split;
-                float *const dst = p.part_acc + slot * D + 4 * h;
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    *reinterpret_cast<float4 *>(dst + 8 * i) = make_float4(o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
-                                                                           o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]);
-                if (h == 0) {
-                    p.part_ml[slot * 2] = l > 0.0f ? m : kNoMax;
-                    p.part_ml[slot * 2 + 1] = l;
+                    for (int e = 0; e < 4; e++) y[e] = static_cast<f16>(o[i / 4][4 * (i % 4) + e] * inv);
+                    *reinterpret_cast<f16x4 *>(dst + 8 * i) = y;
                 }
             }
         }
     }
 }
 
+template <int KG>
+__global__ void __launch_bounds__(KG *kTileThreads, 2) span_tile_kernel(SpanParams p, Phase ph) {
+    __shared__ __align__(16) unsigned char lds[tile_lds_bytes(KG)];
+    tile_item<KG>(p, ph, static_cast<int>(blockIdx.x), lds);
+}
+
+// Tiles of a prefix beside walks of the own keys: the tiles are bound by their products, the walks by the memory, and
+// a CU runs one work-group of each.
+__global__ void __launch_bounds__(kTileThreads, 2) span_mixed_kernel(SpanParams p, Phase tiles, Phase walks, int tile_groups) {
+    static_assert(tile_lds_bytes(1) >= walk_lds_floats(kTileWaves) * 4);
+    __shared__ __align__(16) unsigned char lds[tile_lds_bytes(1)];
+    const int id = static_cast<int>(blockIdx.x);
+    if (id < tile_groups) tile_item<1>(p, tiles, id, lds);
+    else walk_item<f16, kTileWaves, true>(p, walks, id - tile_groups, reinterpret_cast<float *>(lds));
+}
+
 // ---- the slots' merge: a wave per (token, head), two dims a lane ----
 
+constexpr int kMergeWaves = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) span_merge_kernel(SpanParams p) {
-    constexpr int D = kHeadDim;
+__global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanParams p) {
+    constexpr int D = kHeadDim, C = 8;  // slots whose partials are requested together
     const int lane = static_cast<int>(threadIdx.x) % kWave;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kWaves + uniform(static_cast<int>(threadIdx.x) / kWave);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kMergeWaves + uniform(static_cast<int>(threadIdx.x) / kWave);
     const int64_t tok = at / p.n_heads;
-    if (tok < clamped(uniform_load(p.query_start), p.T) || tok >= clamped(uniform_load(p.query_start + p.S), p.T)) return;
-    const float *const ml = p.part_ml + at * p.slots * 2;
+    const int first = uniform_load(p.query_start), last = uniform_load(p.query_start + p.S);
+    if (tok < clamped(first, p.T) || tok >= clamped(last, p.T)) return;
+    const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + at * p.slots;
     const float *const acc = p.part_acc + at * p.slots * D + 2 * lane;
-    float M = kNoMax;
-    for (int s = lane; s < p.slots; s += kWave) M = fmaxf(M, ml[2 * s]);
+    float M = kNoMax, L = 0.0f, x = 0.0f, y = 0.0f;
+    for (int s0 = 0; s0 < p.slots; s0 += kWave) {  // a lane holds a slot's (max, sum)
+        const float2 mine = s0 + lane < p.slots ? ml[s0 + lane] : make_float2(kNoMax, 0.0f);
+        float top = mine.x;
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, kWave));
-    float L = 0.0f, x = 0.0f, y = 0.0f;
-    for (int s = 0; s < p.slots; s++) {
-        const float ls = ml[2 * s + 1];
-        if (!(ls > 0.0f)) continue;  // an empty slot's accumulators are not written
-        const float f = exp2_hw(ml[2 * s] - M);
-        const float2 a = *reinterpret_cast<const float2 *>(acc + static_cast<int64_t>(s) * D);
-        L = L + ls * f;
-        x = x + a.x * f;
-        y = y + a.y * f;
+        for (int o = 1; o < kWave; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
+        top = fmaxf(M, top);
+        const float corr = exp2_hw(M - top);
+        M = top;
+        L = L * corr, x = x * corr, y = y * corr;
+        const float f = mine.y > 0.0f ? exp2_hw(mine.x - top) : 0.0f;
+        const float l = mine.y * f;
+        // Only slots that hold something are read (an empty one's partial is not written), C at a time.
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(mine.y > 0.0f); left != 0;) {
+            float2 a[C];
+            int slot[C];
+            uint64_t rest = left;
+#pragma unroll
+            for (int i = 0; i < C; i++) {
+                slot[i] = rest ? __builtin_ctzll(rest) : -1;
+                a[i] = *reinterpret_cast<const float2 *>(acc + static_cast<int64_t>(s0 + max(slot[i], __builtin_ctzll(left))) * D);
+                rest = rest & (rest - 1);
+            }
+            left = rest;
+#pragma unroll
+            for (int i = 0; i < C; i++) {
+                const float w = slot[i] < 0 ? 0.0f : __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), max(slot[i], 0)));
+                L = L + (slot[i] < 0 ? 0.0f : __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), max(slot[i], 0))));
+                x = x + a[i].x * w;
+                y = y + a[i].y * w;
+            }
+        }
     }
     T *const dst = static_cast<T *>(p.out) + at * D + 2 * lane;
     dst[0] = from_f32<T>(L > 0.0f ? x / L : 0.0f);
@@ -644,53 +847,65 @@ __global__ void __launch_bounds__(kThreads) span_merge_kernel(SpanParams p) {
 
 // ---- host: phases and launches ----
 
-// Cuts `pages` virtual pages into runs, for `items` work-groups per run: enough for `want` work-groups in all, each
-// run at least `least` pages. Returns the runs that were allowed, which only grow with `pages` (the splits, equal
-// runs of whole pages, need not): the workspace is sized by them.
-int cut(Phase &ph, int64_t items, int pages, int want, int least) {
-    const int64_t most = std::max(1, pages / least);
-    const int64_t runs = std::clamp<int64_t>(want / std::max<int64_t>(1, items), 1, most);
-    ph.pages = std::max<int>(1, static_cast<int>((pages + runs - 1) / runs));
+// Cuts `pages` virtual pages into runs of a multiple of `unit`, `items` work-groups a run: as many as make `want`
+// work-groups in all, each at least `least` pages. Returns the runs that were allowed, which only grow with `pages`
+// (the splits, equal runs of whole units, need not): the workspace is sized by them.
+int cut(Phase &ph, int64_t items, int pages, int want, int least, int unit) {
+    const int64_t runs = std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(1, items), pages / least));
+    ph.pages = std::max<int>(1, static_cast<int>((pages + runs * unit - 1) / (runs * unit))) * unit;
     ph.splits = std::max(1, (pages + ph.pages - 1) / ph.pages);
     return static_cast<int>(runs);
 }
 
 struct Launch {
     Phase first{}, second{};  // second.units == 0: none
-    bool first_tiled = false;
+    bool tiled = false;       // the first phase is tiles
     int slots = 1, most_slots = 1;  // slots, and those that the workspace is sized for
 };
 
 int64_t groups_of(const Phase &ph, int n_kv) { return static_cast<int64_t>(ph.units) * ph.tiles * ph.splits * n_kv; }
 
 int64_t partial_bytes(const EmberRaggedBatch &b, int slots) {
-    return slots == 1 ? 0 : static_cast<int64_t>(b.T) * b.n_heads * slots * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float));
+    return slots <= 1 ? 0 : static_cast<int64_t>(b.T) * b.n_heads * slots * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 int tiles_for(int64_t tokens, int G, int rows) { return static_cast<int>(std::max<int64_t>(1, (tokens * G + rows - 1) / rows)); }
 
-// Work-groups wanted in a launch (two tile work-groups fill a CU's LDS and registers, four walk ones do) and the
-// least pages worth a work-group of their own.
-constexpr int kTileGroups = 512, kWalkGroups = 1024, kTileLeast = 16, kWalkLeast = 8;
+Phase rows_phase(int kind, int units, int64_t tokens, int G, bool tiled, int slot0) {
+    return Phase{kind, units, tiles_for(tokens, G, tiled ? kTileRows : kWalkRows), 1, 1, slot0};
+}
 
 // `spread` halves the work-groups asked for, step by step, until the workspace holds the partials.
+int cut_phase(Phase &ph, int n_kv, int pages, int want, int least, bool tiled, int spread) {
+    return cut(ph, static_cast<int64_t>(ph.units) * ph.tiles * n_kv, pages, want >> spread, least,
+               tiled ? 2 * kBlockPages : 1);  // a run of whole blocks for both of a tile's key groups
+}
+constexpr int kLeastSpread = 10;  // no splits
+
+// A window's launch wants a CU's worth of waves on each of the 256 CUs. A work-group of 16 walking waves (or 8 tile
+// waves) fills one alone; only when there are fewer work-groups than CUs, and a split still leaves each wave kWalkLeast
+// / 16 pages (each tile group kTileLeast / 2), are the keys cut, since that costs a merge launch.
+constexpr int kCus = 256, kWalkLeast = 128, kTileLeast = 32;
+
 Launch plan_window(const EmberWindowAttnArgs &a, int spread) {
     const EmberRaggedBatch &b = a.batch;
     const int G = b.n_heads / b.n_kv;
     const int64_t most = std::min(b.max_query, b.T);
     Launch l;
-    l.first_tiled = b.dtype == EMBER_DTYPE_F16 && most * G > kWalkRows;
-    const int rows = l.first_tiled ? kTileRows : kWalkRows;
-    l.first = Phase{kWindowRows, b.S, tiles_for(most, G, rows), 1, 1, 0};
+    l.tiled = b.dtype == EMBER_DTYPE_F16 && most * G > kWalkRows;
+    l.first = rows_phase(kWindowRows, b.S, most, G, l.tiled, 0);
     // a tile's keys: the first tokens' pages, and the windows of its tokens
-    const int64_t tokens = std::min<int64_t>(most, (rows + G - 1) / G + 1);
+    const int64_t tokens = std::min<int64_t>(most, ((l.tiled ? kTileRows : kWalkRows) + G - 1) / G + 1);
     const int64_t near = (std::min<int64_t>(a.window, static_cast<int64_t>(b.max_blocks) * kPage) + tokens + kPage - 1) / kPage + 1;
     const int pages = static_cast<int>(std::min<int64_t>(b.max_blocks, near + (static_cast<int64_t>(a.sinks) + kPage - 1) / kPage));
-    l.most_slots = cut(l.first, static_cast<int64_t>(b.S) * l.first.tiles * b.n_kv, pages,
-                       (l.first_tiled ? kTileGroups : kWalkGroups) >> spread, l.first_tiled ? kTileLeast : kWalkLeast);
+    l.most_slots = cut_phase(l.first, b.n_kv, pages, kCus, l.tiled ? kTileLeast : kWalkLeast, l.tiled, spread);
     l.slots = l.first.splits;
     return l;
 }
+
+// A prefix's launch has a merge behind it in any case, so its phases are cut finely: tiles of kTileWant work-groups in
+// all, walks of two pages a wave or more.
+constexpr int kTileWant = 256, kWalkWant = 1024, kWalkFine = 8;
 
 Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     const EmberRaggedBatch &b = a.batch;
@@ -698,21 +913,18 @@ Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     const int64_t in_group = std::min(a.max_group, b.T), in_seq = std::min(b.max_query, b.T);
     auto pages_of = [&](int keys) { return std::min(b.max_blocks, keys / kPage + 2); };
     Launch l;
-    l.first_tiled = b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
+    l.tiled = b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
+    l.most_slots = 0;
     if (a.n_groups > 0) {
-        l.first = Phase{kPrefixRows, a.n_groups, tiles_for(in_group, G, l.first_tiled ? kTileRows : kWalkRows), 1, 1, 0};
-        l.most_slots = cut(l.first, static_cast<int64_t>(a.n_groups) * l.first.tiles * b.n_kv, pages_of(a.max_prefix),
-                           (l.first_tiled ? kTileGroups : kWalkGroups) >> spread, l.first_tiled ? kTileLeast : kWalkLeast);
-    } else {
-        l.most_slots = 0;
+        l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, l.tiled, 0);
+        l.most_slots = cut_phase(l.first, b.n_kv, pages_of(a.max_prefix), l.tiled ? kTileWant : kWalkWant,
+                                 l.tiled ? kTileLeast : kWalkFine, l.tiled, spread);
     }
-    l.second = Phase{kOwnRows, b.S, tiles_for(in_seq, G, kWalkRows), 1, 1, l.first.splits};
-    l.most_slots += cut(l.second, static_cast<int64_t>(b.S) * l.second.tiles * b.n_kv, pages_of(a.max_own),
-                        kWalkGroups >> spread, kWalkLeast);
+    l.second = rows_phase(kOwnRows, b.S, in_seq, G, false, l.first.splits);
+    l.most_slots += cut_phase(l.second, b.n_kv, pages_of(a.max_own), kWalkWant, kWalkFine, false, spread);
     l.slots = l.first.splits + l.second.splits;
     return l;
 }
-constexpr int kLeastSpread = 10;  // 1024 >> 10 = 1: no splits
 
 SpanParams params_of(const EmberRaggedBatch &b, int slots) {
     SpanParams p{};
@@ -721,30 +933,42 @@ SpanParams params_of(const EmberRaggedBatch &b, int slots) {
     p.q_stride = b.q_stride;
     p.T = b.T, p.S = b.S, p.max_blocks = b.max_blocks, p.n_heads = b.n_heads, p.n_kv = b.n_kv;
     p.G = b.n_heads / b.n_kv, p.num_blocks = b.num_blocks, p.slots = slots;
-    p.part_acc = static_cast<float *>(b.workspace);
-    if (p.part_acc) p.part_ml = p.part_acc + static_cast<int64_t>(b.T) * b.n_heads * slots * kHeadDim;
+    if (slots > 1) {
+        p.part_acc = static_cast<float *>(b.workspace);
+        p.part_ml = p.part_acc + static_cast<int64_t>(b.T) * b.n_heads * slots * kHeadDim;
+    }
     p.window = kNoWindow;
     p.scale_log2 = b.scale * kLog2e;
     return p;
 }
 
+template <typename T, int W>
+void launch_walk(const SpanParams &p, const Launch &l, unsigned first, unsigned second, hipStream_t stream) {
+    hipLaunchKernelGGL((span_walk_kernel<T, W>), dim3(first + second), dim3(W * kWave), 0, stream, p, l.first, l.second,
+                       static_cast<int>(first));
+}
+
 template <typename T>
 hipError_t run(const SpanParams &p, const Launch &l, hipStream_t stream) {
-    const int64_t first = groups_of(l.first, p.n_kv), second = l.second.units ? groups_of(l.second, p.n_kv) : 0;
-    if (l.first_tiled) {
-        if constexpr (sizeof(T) == 2) {
-            if (first) hipLaunchKernelGGL(span_tile_kernel, dim3(static_cast<unsigned>(first)), dim3(kThreads), 0, stream, p, l.first);
-            if (second)
-                hipLaunchKernelGGL(span_walk_kernel<T>, dim3(static_cast<unsigned>(second)), dim3(kThreads), 0, stream, p,
-                                   l.second, l.second, static_cast<int>(second));
-        }
-    } else if (first + second) {
-        hipLaunchKernelGGL(span_walk_kernel<T>, dim3(static_cast<unsigned>(first + second)), dim3(kThreads), 0, stream, p,
-                           l.first, l.second, static_cast<int>(first));
+    const unsigned first = static_cast<unsigned>(groups_of(l.first, p.n_kv)), second = static_cast<unsigned>(groups_of(l.second, p.n_kv));
+    bool done = first + second == 0;
+    if constexpr (sizeof(T) == 2) {
+        if (l.tiled && second)
+            hipLaunchKernelGGL(span_mixed_kernel, dim3(first + second), dim3(kTileThreads), 0, stream, p, l.first, l.second, static_cast<int>(first));
+        else if (l.tiled && first <= kCus)
+            hipLaunchKernelGGL(span_tile_kernel<2>, dim3(first), dim3(2 * kTileThreads), 0, stream, p, l.first);
+        else if (l.tiled)
+            hipLaunchKernelGGL(span_tile_kernel<1>, dim3(first), dim3(kTileThreads), 0, stream, p, l.first);
+        else if (!second && first <= kCus)  // a window's work-groups are as wide as their share of the chip
+            launch_walk<T, 16>(p, l, first, second, stream);
+        done = done || l.tiled || (!second && first <= kCus);
     }
+    if (!done && !second && first <= 2 * kCus) launch_walk<T, 8>(p, l, first, second, stream);
+    else if (!done) launch_walk<T, 4>(p, l, first, second, stream);
     if (l.slots > 1) {
         const int64_t rows = static_cast<int64_t>(p.T) * p.n_heads;
-        hipLaunchKernelGGL(span_merge_kernel<T>, dim3(static_cast<unsigned>((rows + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, p);
+        hipLaunchKernelGGL(span_merge_kernel<T>, dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)),
+                           dim3(kMergeWaves * kWave), 0, stream, p);
     }
     return hipGetLastError();
 }
