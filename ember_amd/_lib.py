@@ -164,13 +164,13 @@ class RaggedBatch(ctypes.Structure):
     ]
 
 
-class WindowAttnArgs(ctypes.Structure):
-    _fields_ = [("batch", RaggedBatch), ("window", c_int32), ("sinks", c_int32)]
+class WindowAttnArgs(ctypes.Structure):  # the batch's fields, then its own (the same layout, filled in one call)
+    _fields_ = RaggedBatch._fields_ + [("window", c_int32), ("sinks", c_int32)]
 
 
 class PrefixAttnArgs(ctypes.Structure):
-    _fields_ = [("batch", RaggedBatch), ("group_start", c_void_p), ("prefix_len", c_void_p), ("n_groups", c_int32),
-                ("max_group", c_int32), ("max_prefix", c_int32), ("max_own", c_int32)]
+    _fields_ = RaggedBatch._fields_ + [("group_start", c_void_p), ("prefix_len", c_void_p), ("n_groups", c_int32),
+                                       ("max_group", c_int32), ("max_prefix", c_int32), ("max_own", c_int32)]
 
 
 STRUCTS = [QkvArgs, AttnArgs, PrefillArgs, CopyArgs, KvConfig, StepBatchC, LayerIo, GemvArgs, NormArgs, EmbedArgs,

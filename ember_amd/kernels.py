@@ -417,32 +417,29 @@ def rmsnorm_rows(x, w, out, eps: float, rows=None, stream=None):
     return keep
 
 
-def _on(t: torch.Tensor, stream):
-    """The stream handle for work on t's device, and that device made current if it is not (None, or its guard)."""
-    guard = None
-    if t.device.index != torch.cuda.current_device():
-        guard = torch.cuda.device(t.device)
+# The calls below run once per layer or step around kernels of a few microseconds, so what they check, they check with
+# few Python operations.
+
+def _launch(fn, args, dev: int, stream, what: str) -> None:
+    """fn(args, stream) on device `dev`: on `stream`, or on torch's current stream of that device."""
     if stream is None:
-        stream = torch.cuda.current_stream(t.device)
-    return (stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)), guard
-
-
-def _launch(fn, args, t: torch.Tensor, stream, what: str) -> None:
-    handle, guard = _on(t, stream)
-    if guard is None:
-        check(fn(args, handle), what)
+        handle = torch._C._cuda_getCurrentRawStream(dev)
     else:
-        with guard:
-            check(fn(args, handle), what)
+        handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+    if dev == torch.cuda.current_device():
+        code = fn(args, handle)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(args, handle)
+    if code:
+        check(code, what)
 
 
-def _same(t, name: str, device, dtype, shape=None) -> int:
-    """The address of a contiguous tensor that must be on `device` with this dtype (and shape)."""
-    if t.device != device or t.dtype != dtype or not t.is_contiguous():
-        raise EmberError(f"{name} must be a contiguous {dtype} tensor on {device}")
-    if shape is not None and t.shape != shape:
-        raise EmberError(f"{name} must have shape {tuple(shape)} (got {tuple(t.shape)})")
-    return t.data_ptr()
+def _refuse(tensors: dict, dev: int, dtype) -> None:
+    """Names the first of these tensors that is not a contiguous `dtype` tensor on device `dev`."""
+    for name, t in tensors.items():
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+            raise EmberError(f"{name} must be a contiguous {dtype} tensor on cuda:{dev}")
 
 
 class StepTables:
@@ -456,9 +453,13 @@ class StepTables:
         self.query_start, self.context_len = e(S + 1), e(S)
         self.positions, self.token_seq, self.slots = e(max_tokens), e(max_tokens), e(max_tokens, dtype=torch.int64)
         self.block_tables, self.totals = e(S + 1, max_blocks), e(4)
-        self.device = self.totals.device
-        if self.device.type != "cuda":
+        if not self.totals.is_cuda:
             raise EmberError("StepTables live on the device")
+        a = self._args = _lib.StepTablesArgs()  # what no call changes
+        a.S, a.max_tokens, a.max_blocks = S, max_tokens, max_blocks
+        a.query_start, a.context_len = self.query_start.data_ptr(), self.context_len.data_ptr()
+        a.positions, a.token_seq, a.slots = self.positions.data_ptr(), self.token_seq.data_ptr(), self.slots.data_ptr()
+        a.block_tables, a.totals = self.block_tables.data_ptr(), self.totals.data_ptr()
 
 
 def step_tables(out: StepTables, request_tables, cached_len, new_len, free_blocks, *, request=None, free_cursor=None,
@@ -470,68 +471,72 @@ def step_tables(out: StepTables, request_tables, cached_len, new_len, free_block
     All int32 on out's device. Nothing is checked on the host that would need the device's values: totals[2]
     says which sequences got no tokens and why.
     """
-    dev, i32 = out.device, torch.int32
-    a = _lib.StepTablesArgs()
-    if request_tables.dim() != 2 or request_tables.shape[1] != out.max_blocks:
-        raise EmberError(f"request_tables must be [R, {out.max_blocks}]")
-    R = request_tables.shape[0]
-    a.request_tables = _same(request_tables, "request_tables", dev, i32)
-    a.cached_len = _same(cached_len, "cached_len", dev, i32, (R,))
-    a.new_len = _same(new_len, "new_len", dev, i32, (out.S,))
-    if free_blocks.dim() != 1:
-        raise EmberError("free_blocks must be a list")
-    a.free_blocks = _same(free_blocks, "free_blocks", dev, i32)
+    dev, i32 = out.totals.get_device(), torch.int32
+    for t in (request_tables, cached_len, new_len, free_blocks):
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            _refuse(dict(request_tables=request_tables, cached_len=cached_len, new_len=new_len, free_blocks=free_blocks), dev, i32)
+    R = len(request_tables)
+    if request_tables.shape != (R, out.max_blocks) or cached_len.shape != (R,) or new_len.shape != (out.S,) \
+            or free_blocks.dim() != 1:
+        raise EmberError(f"request_tables, cached_len, new_len and free_blocks must be [R, {out.max_blocks}], [R], "
+                         f"[{out.S}] and a list")
+    a = out._args
+    a.request_tables, a.cached_len = request_tables.data_ptr(), cached_len.data_ptr()
+    a.new_len, a.free_blocks = new_len.data_ptr(), free_blocks.data_ptr()
+    a.request = a.free_cursor = None
     if request is not None:
-        a.request = _same(request, "request", dev, i32, (out.S,))
+        _refuse(dict(request=request), dev, i32)
+        if request.shape != new_len.shape:
+            raise EmberError("request must name a row for each new_len")
+        a.request = request.data_ptr()
     if free_cursor is not None:
-        a.free_cursor = _same(free_cursor, "free_cursor", dev, i32, (1,))
-    a.S, a.R, a.max_blocks, a.n_free = out.S, R, out.max_blocks, free_blocks.shape[0]
-    a.max_tokens, a.pad_block = out.max_tokens, pad_block
-    a.query_start, a.context_len = out.query_start.data_ptr(), out.context_len.data_ptr()
-    a.positions, a.token_seq, a.slots = out.positions.data_ptr(), out.token_seq.data_ptr(), out.slots.data_ptr()
-    a.block_tables, a.totals = out.block_tables.data_ptr(), out.totals.data_ptr()
-    _launch(_lib.lib().ember_hip_step_tables, a, out.totals, stream, "step_tables")
+        _refuse(dict(free_cursor=free_cursor), dev, i32)
+        if free_cursor.numel() != 1:
+            raise EmberError("free_cursor must be one number")
+        a.free_cursor = free_cursor.data_ptr()
+    a.R, a.n_free, a.pad_block = R, len(free_blocks), pad_block
+    _launch(_lib.lib().ember_hip_step_tables, a, dev, stream, "step_tables")
     return out
 
 
-def _batch_sizes(b, T, S, *, n_heads, n_kv, max_query, dtype, max_blocks) -> None:
-    b.T, b.S, b.n_heads, b.n_kv, b.head_dim = T, S, n_heads, n_kv, HEAD_DIM
-    b.max_blocks = 1 << 26 if max_blocks is None else max_blocks
-    b.max_query = max(1, T if max_query is None else max_query)
-    b.dtype = _lib.DTYPE_F16 if dtype == torch.float16 else _lib.DTYPE_F32
-
-
-def _ragged_batch(b, q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace) -> None:
-    """Fills an EmberRaggedBatch: q [T, n_heads, 128] (any token stride), pools [num_blocks, n_kv, 16, 128]."""
-    dev, i32 = q.device, torch.int32
-    code = _dtype_code(q)
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.stride(2) != 1 or q.stride(1) != HEAD_DIM or not q.is_cuda:
-        raise EmberError("q must be a device tensor [T, n_heads, 128] with each token's heads contiguous")
-    if k_pool.dim() != 4 or k_pool.shape[2] != BLOCK_SIZE or k_pool.shape[3] != HEAD_DIM:
-        raise EmberError("pools must be [num_blocks, n_kv, 16, 128]")
-    T, H = q.shape[0], q.shape[1]
-    b.q, b.q_stride = q.data_ptr(), q.stride(0) if T > 1 else H * HEAD_DIM
-    b.k_cache = _same(k_pool, "k_pool", dev, q.dtype)
-    b.v_cache = _same(v_pool, "v_pool", dev, q.dtype, k_pool.shape)
-    b.out = _same(out, "out", dev, q.dtype, q.shape)
-    b.query_start = _same(query_start, "query_start", dev, i32)
-    if query_start.dim() != 1 or query_start.shape[0] < 1:
-        raise EmberError("query_start must be [S + 1]")
-    S = query_start.shape[0] - 1
-    b.positions = _same(positions, "positions", dev, i32)
-    if positions.dim() != 1 or positions.shape[0] < T:
-        raise EmberError("positions must hold every token")
-    b.block_tables = _same(block_tables, "block_tables", dev, i32)
-    if block_tables.dim() != 2 or block_tables.shape[0] < S:
-        raise EmberError("block_tables must be [S, max_blocks] (more rows are not used)")
-    b.T, b.S, b.max_blocks, b.n_heads, b.n_kv, b.head_dim = T, S, block_tables.shape[1], H, k_pool.shape[1], HEAD_DIM
-    b.num_blocks, b.dtype = k_pool.shape[0], code
-    b.scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else scale
-    b.max_query = max(1, T if max_query is None else max_query)
+def _ragged_batch(q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace):
+    """Checks a ragged batch and returns its device and the fields of an EmberRaggedBatch, in order: q [T, n_heads, 128]
+    (any token stride), pools [num_blocks, n_kv, 16, 128]."""
+    dev, dtype, i32 = q.get_device(), q.dtype, torch.int32
+    if dev < 0 or not (dtype is torch.float16 or dtype is torch.float32):
+        raise EmberError(f"q must be an f16 or f32 device tensor (got {dtype} on {q.device})")
+    for t in (k_pool, v_pool, out):
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+            _refuse(dict(k_pool=k_pool, v_pool=v_pool, out=out), dev, dtype)
+    for t in (query_start, positions, block_tables):
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            _refuse(dict(query_start=query_start, positions=positions, block_tables=block_tables), dev, i32)
+    shape, pool, stride = q.shape, k_pool.shape, q.stride()
+    if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1 or stride[1] != HEAD_DIM:
+        raise EmberError("q must be [T, n_heads, 128] with each token's heads contiguous")
+    if len(pool) != 4 or pool[2] != BLOCK_SIZE or pool[3] != HEAD_DIM or v_pool.shape != pool or out.shape != shape:
+        raise EmberError("pools must be [num_blocks, n_kv, 16, 128] alike, and out shaped like q")
+    T, H, _ = shape
+    S = query_start.numel() - 1
+    table = block_tables.shape
+    if S < 0 or positions.numel() < T or len(table) != 2 or table[0] < S:
+        raise EmberError("query_start must be [S + 1], positions hold every token, block_tables be [S, max_blocks] (or more rows)")
+    ws = ws_bytes = 0
     if workspace is not None:
-        if workspace.device != dev or not workspace.is_contiguous():
-            raise EmberError(f"workspace must be a contiguous tensor on {dev}")
-        b.workspace, b.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            raise EmberError(f"workspace must be a contiguous tensor on cuda:{dev}")
+        ws, ws_bytes = workspace.data_ptr(), workspace.nbytes
+    return dev, (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), query_start.data_ptr(),
+                 positions.data_ptr(), block_tables.data_ptr(), stride[0] if T > 1 else H * HEAD_DIM, T, S, table[1], H,
+                 pool[1], HEAD_DIM, pool[0], _lib.DTYPE_F16 if dtype is torch.float16 else _lib.DTYPE_F32,
+                 HEAD_DIM ** -0.5 if scale is None else scale, (T or 1) if max_query is None else max_query, ws, ws_bytes)
+
+
+def _batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks):
+    """The fields of an EmberRaggedBatch of which only the sizes count."""
+    return (0, 0, 0, 0, 0, 0, 0, n_heads * HEAD_DIM, T, S, 1 << 26 if max_blocks is None else max_blocks, n_heads, n_kv,
+            HEAD_DIM, 1, _lib.DTYPE_F16 if dtype == torch.float16 else _lib.DTYPE_F32, 1.0,
+            (T or 1) if max_query is None else max_query, 0, 0)
 
 
 def _workspace(n: int, device):
@@ -541,9 +546,7 @@ def _workspace(n: int, device):
 def window_workspace(T: int, S: int, *, n_heads, n_kv, window, sinks=0, max_query=None, dtype=torch.float16,
                      max_blocks=None, device="cuda"):
     """A workspace for window_attention of batches of these sizes, or None when such a call splits no keys."""
-    a = _lib.WindowAttnArgs()
-    _batch_sizes(a.batch, T, S, n_heads=n_heads, n_kv=n_kv, max_query=max_query, dtype=dtype, max_blocks=max_blocks)
-    a.window, a.sinks = window, sinks
+    a = _lib.WindowAttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks), window, sinks)
     return _workspace(int(_lib.lib().ember_hip_window_workspace_bytes(a)), device)
 
 
@@ -558,27 +561,22 @@ def window_attention(q, k_pool, v_pool, out, query_start, positions, block_table
     query_start[S] are left alone. max_query: the most tokens of one sequence (None: T); workspace: of
     window_workspace, not shared by calls that overlap in time (None: no splits).
     """
-    a = _lib.WindowAttnArgs()
-    _ragged_batch(a.batch, q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
-    a.window, a.sinks = window, sinks
-    _launch(_lib.lib().ember_hip_window_attn, a, q, stream, "window_attn")
+    dev, batch = _ragged_batch(q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
+    _launch(_lib.lib().ember_hip_window_attn, _lib.WindowAttnArgs(*batch, window, sinks), dev, stream, "window_attn")
     return out
 
 
-def _prefix_sizes(a, T, n_groups, max_group, max_prefix, max_own) -> None:
-    far = min(a.batch.max_blocks * BLOCK_SIZE, 0x7FFFFFFF)
-    a.n_groups = n_groups
-    a.max_group = max(1, T if max_group is None else max_group)
-    a.max_prefix = far if max_prefix is None else max_prefix
-    a.max_own = max(1, far if max_own is None else max_own)
+def _prefix_sizes(T, n_groups, max_group, max_prefix, max_own, max_blocks):
+    far = min(max_blocks * BLOCK_SIZE, 0x7FFFFFFF)
+    return (n_groups, (T or 1) if max_group is None else max_group, far if max_prefix is None else max_prefix,
+            far if max_own is None else max_own)
 
 
 def shared_prefix_workspace(T: int, S: int, n_groups: int, *, n_heads, n_kv, max_query=None, max_group=None,
                             max_prefix=None, max_own=None, dtype=torch.float16, max_blocks=None, device="cuda"):
     """A workspace for shared_prefix_attention of batches of these sizes."""
-    a = _lib.PrefixAttnArgs()
-    _batch_sizes(a.batch, T, S, n_heads=n_heads, n_kv=n_kv, max_query=max_query, dtype=dtype, max_blocks=max_blocks)
-    _prefix_sizes(a, T, n_groups, max_group, max_prefix, max_own)
+    batch = _batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks)
+    a = _lib.PrefixAttnArgs(*batch, 0, 0, *_prefix_sizes(T, n_groups, max_group, max_prefix, max_own, batch[10]))
     return _workspace(int(_lib.lib().ember_hip_shared_prefix_workspace_bytes(a)), device)
 
 
@@ -593,11 +591,14 @@ def shared_prefix_attention(q, k_pool, v_pool, out, query_start, positions, bloc
     first sequence. max_query, max_group (new tokens of one sequence and of one group), max_prefix and max_own
     (tokens of a prefix and behind it) shape the launch; a step beyond them is computed too, only slower.
     """
-    a = _lib.PrefixAttnArgs()
-    _ragged_batch(a.batch, q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
-    n_groups = prefix_len.shape[0]
-    a.group_start = _same(group_start, "group_start", q.device, torch.int32, (n_groups + 1,))
-    a.prefix_len = _same(prefix_len, "prefix_len", q.device, torch.int32, (n_groups,))
-    _prefix_sizes(a, q.shape[0], n_groups, max_group, max_prefix, max_own)
-    _launch(_lib.lib().ember_hip_shared_prefix_attn, a, q, stream, "shared_prefix_attn")
+    dev, batch = _ragged_batch(q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
+    for t in (group_start, prefix_len):
+        if t.dtype is not torch.int32 or t.get_device() != dev or not t.is_contiguous():
+            _refuse(dict(group_start=group_start, prefix_len=prefix_len), dev, torch.int32)
+    n_groups = prefix_len.numel()
+    if group_start.numel() != n_groups + 1:
+        raise EmberError("group_start must be [n_groups + 1], for as many groups as prefix_len has")
+    a = _lib.PrefixAttnArgs(*batch, group_start.data_ptr(), prefix_len.data_ptr(),
+                            *_prefix_sizes(batch[8], n_groups, max_group, max_prefix, max_own, batch[10]))
+    _launch(_lib.lib().ember_hip_shared_prefix_attn, a, dev, stream, "shared_prefix_attn")
     return out

@@ -28,7 +28,7 @@ def test_step_tables_refusals(field, value, text):
 
 
 def _batch(a):
-    b = a.batch
+    b = a  # the batch's fields come first
     for f in ("q", "k_cache", "v_cache", "out", "query_start", "positions", "block_tables"):
         setattr(b, f, 4096)
     b.T, b.S, b.max_blocks, b.n_heads, b.n_kv, b.head_dim, b.num_blocks = 4, 2, 8, 16, 8, 128, 32
@@ -62,7 +62,7 @@ BATCH = [("T", -1, "bad sizes"), ("S", -1, "bad sizes"), ("max_blocks", 0, "bad 
 @pytest.mark.parametrize("field,value,text", BATCH)
 def test_batch_refusals(make, entry, field, value, text):
     a = make()
-    setattr(a.batch, field, value)
+    setattr(a, field, value)
     assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
     assert text in _lib.last_error()
 
@@ -89,7 +89,7 @@ def test_null_and_empty_calls():
     for make, entry in ((_window, "ember_hip_window_attn"), (_prefix, "ember_hip_shared_prefix_attn")):
         for field in ("T", "S"):
             a = make()
-            setattr(a.batch, field, 0)
+            setattr(a, field, 0)
             assert getattr(lib, entry)(a, None) == _lib.OK  # nothing to do, nothing launched
 
 
@@ -100,10 +100,10 @@ def test_workspace_covers_smaller_tables():
         for window in (20, 500, 5000):
             for q in (1, 9, 200):
                 a = _window()
-                a.window, a.batch.S, a.batch.T, a.batch.max_query, a.batch.max_blocks = window, S, S * q, q, 1 << 26
+                a.window, a.S, a.T, a.max_query, a.max_blocks = window, S, S * q, q, 1 << 26
                 most = size(a)
                 for blocks in (1, 7, 33, 64, 130, 400, 1000):
-                    a.batch.max_blocks = blocks
+                    a.max_blocks = blocks
                     assert size(a) <= most
-    assert K.window_workspace(64, 64, n_heads=16, n_kv=8, window=100000, max_query=1, device="cpu") is not None
+    assert K.window_workspace(4, 4, n_heads=16, n_kv=8, window=100000, max_query=1, device="cpu") is not None
     assert K.window_workspace(1, 1, n_heads=16, n_kv=8, window=10, max_query=1, device="cpu") is None
