@@ -187,10 +187,13 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
     const int g = lane >> 4, c = lane & 15;
     const int kvh = id % p.n_kv;
     int rest = id / p.n_kv;
-    const int split = rest % ph.splits;
-    rest /= ph.splits;
-    const int tile0 = rest % ph.tiles, unit = rest / ph.tiles;
+    const int tile0 = rest % ph.tiles;
+    rest /= ph.tiles;
+    const int split = rest % ph.splits, unit = rest / ph.splits;
 
+    // Up to its pages a work-group runs at raised wave priority: the CU's streaming waves otherwise win the issue
+    // arbitration, and its few dependent loads wait behind theirs.
+    __builtin_amdgcn_s_setprio(3);
     bool grouped;
     const Rows r = rows_of(p, ph, unit, lane, grouped);
     const int32_t *const table = p.tables + static_cast<int64_t>(r.seq) * p.max_blocks;
@@ -397,6 +400,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 fetch_values(A, 0);
                 fetch_keys(B, 1);
                 fetch_values(B, 1);
+                __builtin_amdgcn_s_setprio(0);
                 auto nothing = [] {};
                 for (int j = 0; j < n; j += 2) {
                     __builtin_amdgcn_sched_barrier(0);
@@ -418,6 +422,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 __builtin_amdgcn_sched_barrier(0);
                 fetch_values(A, 0);
                 __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(0);
                 for (int j = 0; j < n; j++) {
                     consume(A, j, [&] {
                         __builtin_amdgcn_sched_barrier(0);
@@ -485,7 +490,8 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
 
 // Two phases in one launch (b.units may be 0). A CU holds 16 waves of the f16 form and 8 of the f32 form.
 template <typename T, int W>
-__global__ void __launch_bounds__(W *kWave, (sizeof(T) == 2 ? 4 : 2)) span_walk_kernel(SpanParams p, Phase a, Phase b, int a_groups) {
+__global__ void __launch_bounds__(W *kWave, (sizeof(T) == 2 ? 4 : 2))
+    span_walk_kernel(SpanParams p, Phase a, Phase b, int a_groups) {
     __shared__ __align__(16) float red[walk_lds_floats(W)];
     const int id = static_cast<int>(blockIdx.x);
     const bool second = id >= a_groups;
@@ -526,10 +532,13 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
     const int h = lane >> 5, c = lane & 31;
     const int kvh = id % p.n_kv;
     int rest = id / p.n_kv;
-    const int split = rest % ph.splits;
-    rest /= ph.splits;
-    const int tile0 = rest % ph.tiles, unit = rest / ph.tiles;
+    const int tile0 = rest % ph.tiles;
+    rest /= ph.tiles;
+    const int split = rest % ph.splits, unit = rest / ph.splits;
 
+    // Up to its pages a work-group runs at raised wave priority: the CU's streaming waves otherwise win the issue
+    // arbitration, and its few dependent loads wait behind theirs.
+    __builtin_amdgcn_s_setprio(3);
     bool grouped;
     const Rows r = rows_of(p, ph, unit, lane, grouped);
     const int32_t *const table = p.tables + static_cast<int64_t>(r.seq) * p.max_blocks;
@@ -639,6 +648,7 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         const int steps = (blocks + KG - 1) / KG;
         if (steps > 0) {
             fetch(0);
+            __builtin_amdgcn_s_setprio(0);
             stage(0);
         }
         __syncthreads();
@@ -785,11 +795,11 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) span_tile_kernel(SpanPara
 
 // Tiles of a prefix beside walks of the own keys: the tiles are bound by their products, the walks by the memory, and
 // a CU runs one work-group of each.
-__global__ void __launch_bounds__(kTileThreads, 2) span_mixed_kernel(SpanParams p, Phase tiles, Phase walks, int tile_groups) {
+__global__ void __launch_bounds__(kTileThreads, 2) span_mixed_kernel(SpanParams p, Phase first, Phase walks, int tile_groups) {
     static_assert(tile_lds_bytes(1) >= walk_lds_floats(kTileWaves) * 4);
     __shared__ __align__(16) unsigned char lds[tile_lds_bytes(1)];
     const int id = static_cast<int>(blockIdx.x);
-    if (id < tile_groups) tile_item<1>(p, tiles, id, lds);
+    if (id < tile_groups) tile_item<1>(p, first, id, lds);
     else walk_item<f16, kTileWaves, true>(p, walks, id - tile_groups, reinterpret_cast<float *>(lds));
 }
 
@@ -944,8 +954,8 @@ SpanParams params_of(const EmberRaggedBatch &b, int slots) {
 
 template <typename T, int W>
 void launch_walk(const SpanParams &p, const Launch &l, unsigned first, unsigned second, hipStream_t stream) {
-    hipLaunchKernelGGL((span_walk_kernel<T, W>), dim3(first + second), dim3(W * kWave), 0, stream, p, l.first, l.second,
-                       static_cast<int>(first));
+    hipLaunchKernelGGL((span_walk_kernel<T, W>), dim3(first + second), dim3(W * kWave), 0, stream, p, l.first,
+                       l.second, static_cast<int>(first));
 }
 
 template <typename T>
@@ -954,7 +964,8 @@ hipError_t run(const SpanParams &p, const Launch &l, hipStream_t stream) {
     bool done = first + second == 0;
     if constexpr (sizeof(T) == 2) {
         if (l.tiled && second)
-            hipLaunchKernelGGL(span_mixed_kernel, dim3(first + second), dim3(kTileThreads), 0, stream, p, l.first, l.second, static_cast<int>(first));
+            hipLaunchKernelGGL(span_mixed_kernel, dim3(first + second), dim3(kTileThreads), 0, stream, p, l.first, l.second,
+                               static_cast<int>(first));
         else if (l.tiled && first <= kCus)
             hipLaunchKernelGGL(span_tile_kernel<2>, dim3(first), dim3(2 * kTileThreads), 0, stream, p, l.first);
         else if (l.tiled)
