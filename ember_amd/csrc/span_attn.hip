@@ -153,34 +153,29 @@ __device__ __forceinline__ bool visible(int j, int base, int top, int pos, int w
 // on v_mfma_f32_16x16x32_f16 (step s takes dims 32 s + 8 g .. + 7), O^T += V^T P^T on v_mfma_f32_16x16x16_f16. f32
 // pages use v_mfma_f32_16x16x4_f32 the same way: step s of the scores takes dim 16 (s / 4) + 4 g + s % 4 from lane
 // group g, so a lane loads key c in 16-byte pieces; step v of the values takes key 4 g + v, which the lane's own
-// scores belong to. Keys of the f16 form pass through LDS (direct loads of four whole rows an instruction, swizzled)
-// where a CU runs 16 waves, each with half a page in flight. DEEP keeps two whole pages in registers instead, for 8
-// waves a CU.
-template <typename T, bool DEEP>
+// scores belong to. Keys of the f16 form pass through LDS (direct loads of four whole rows an instruction, swizzled).
+// Where a CU runs 16 waves, each has half a page in flight; DEEP keeps two whole pages instead, for 8 waves a CU.
+template <typename T>
 struct WalkPage;
 template <>
-struct WalkPage<f16, false> {
+struct WalkPage<f16> {
     u32x4 v[4];  // keys 4 g + i, dims 8 c .. 8 c + 7
 };
 template <>
-struct WalkPage<f16, true> {
-    u32x4 k[4];  // key c, dims 32 i + 8 g .. + 7
-    u32x4 v[4];
-};
-template <>
-struct WalkPage<float, false> {
+struct WalkPage<float> {
     u32x4 k[8];     // key c, dims 16 i + 4 g .. + 3
     u32x4 v[4][2];  // keys 4 g + i, dims 8 c .. 8 c + 7
 };
 
 constexpr int kWalkRowPitch = kHeadDim + 4;               // floats of a row's partial: 16 rows' pieces of one dim on distinct banks
-constexpr int kWalkWave = kWalkRows * kWalkRowPitch;      // floats of a wave's region (f16: its first 4 KiB also stage keys)
+constexpr int kWalkWave = kWalkRows * kWalkRowPitch;      // floats of a wave's region (f16: it also stages keys, 4 KiB a page)
+constexpr int kStageWords = kPage * kHeadDim / 2;
 constexpr int walk_lds_floats(int W) { return W * (kWalkWave + 2 * kWalkRows); }
 
 template <typename T, int W, bool DEEP>  // W waves
 __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, const int id, float *red) {
     constexpr int D = kHeadDim, kThreads = W * kWave, RP = kWalkRowPitch, RW = kWalkWave;
-    constexpr bool F16 = sizeof(T) == 2, STAGED = F16 && !DEEP;
+    constexpr bool F16 = sizeof(T) == 2;
     constexpr int KQ = F16 ? 4 : 8;  // 16-byte pieces of a row of q or K in a lane
     float *const red_m = red + W * RW, *const red_l = red_m + W * kWalkRows;  // [row][wave]
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
@@ -262,7 +257,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
             const int n = min(kWave, (v1 - cv + W - 1) / W);
             int ids = early;
             if (ph.kind == kWindowRows || cv != v0 + wave) ids = lane < n ? table[sp.page(cv + lane * W)] : -1;
-            using Page = WalkPage<T, DEEP>;
+            using Page = WalkPage<T>;
             auto desc_of = [&](const T *base, int j) {
                 const int blk = __builtin_amdgcn_readlane(ids, min(j, n - 1));
                 const bool live = j < n && blk >= 0 && blk < p.num_blocks;  // dead: no records, the loads give zeros
@@ -275,14 +270,15 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 asm volatile("" : "+v"(x));
                 return x;
             };
-            auto fetch_keys = [&](Page &A, int j) {
+            auto fetch_keys = [&](Page &A, int j, int buffer) {
                 const __amdgpu_buffer_rsrc_t d = desc_of(kbase, j);
-                const uint32_t off = here(STAGED ? k_dma : k_off);
-                if constexpr (STAGED) {
+                const uint32_t off = here(F16 ? k_dma : k_off);
+                if constexpr (F16) {
+                    uint32_t *const to = kstage + buffer * kStageWords;
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                            d, (__attribute__((address_space(3))) void *)(kstage + 256 * i), 16, (off ^ (64u * i)) + 1024u * i, 0, 0,
+                            d, (__attribute__((address_space(3))) void *)(to + 256 * i), 16, (off ^ (64u * i)) + 1024u * i, 0, 0,
                             kNonTemporal);
                 } else {
 #pragma unroll
@@ -304,21 +300,20 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
             };
             // Page j: its scores and the online softmax, then its values; `next` is called between, once its keys
             // have been read.
-            auto consume = [&](Page &A, int j, auto next) {
+            auto consume = [&](Page &A, int j, int buffer, auto next) {
                 const int page = sp.page(cv + j * W);
                 f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};  // s[v]: raw score of key 4 g + v
                 if constexpr (F16) {
+                    // Loads end in order, and only so many are out behind the page's keys: its values, and DEEP the next
+                    // page's keys and values.
+                    if constexpr (DEEP) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+                    else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+                    __builtin_amdgcn_sched_barrier(0);
                     u32x4 kf[4];
-                    if constexpr (STAGED) {  // at most the page's four value loads, issued after them, are out: its keys are here
-                        asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
                     const uint32_t off = here(k_rd);
+                    const char *const from = reinterpret_cast<const char *>(kstage + buffer * kStageWords);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if constexpr (STAGED) kf[i] = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(kstage) + (off ^ (64u * i)));
-                        else kf[i] = A.k[i];
-                    }
+                    for (int i = 0; i < 4; i++) kf[i] = *reinterpret_cast<const u32x4 *>(from + (off ^ (64u * i)));
 #pragma unroll
                     for (int i = 0; i < 4; i++) s = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(kf[i]), as_f16x8(qf[i]), s, 0, 0, 0);
                 } else {
@@ -394,49 +389,45 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                             o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(A.v[v][t / 4][t % 4]), w[v], o[t], 0, 0, 0);
                 }
             };
+            // Keys and values are requested in the order that the waits count on: nothing moves across the fences.
+            auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+            auto fetch = [&](Page &A, int j, int buffer) {
+                fence();
+                fetch_keys(A, j, buffer);
+                fence();
+                fetch_values(A, j);
+                fence();
+            };
             if constexpr (DEEP) {
+                static_assert(2 * kStageWords <= kWalkWave);
                 Page A, B;
-                fetch_keys(A, 0);
-                fetch_values(A, 0);
-                fetch_keys(B, 1);
-                fetch_values(B, 1);
+                fetch(A, 0, 0);
+                fetch(B, 1, 1);
                 __builtin_amdgcn_s_setprio(0);
-                auto nothing = [] {};
                 for (int j = 0; j < n; j += 2) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    consume(A, j, nothing);
-                    __builtin_amdgcn_sched_barrier(0);
-                    fetch_keys(A, j + 2);
-                    fetch_values(A, j + 2);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (j + 1 < n) consume(B, j + 1, nothing);
-                    __builtin_amdgcn_sched_barrier(0);
-                    fetch_keys(B, j + 3);
-                    fetch_values(B, j + 3);
+                    consume(A, j, 0, fence);
+                    fetch(A, j + 2, 0);
+                    if (j + 1 < n) consume(B, j + 1, 1, fence);
+                    fetch(B, j + 3, 1);
                 }
             } else {
-                // Keys and values are requested in this order and nothing moves across: the wait for staged keys counts.
                 Page A;
-                __builtin_amdgcn_sched_barrier(0);
-                fetch_keys(A, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                fetch_values(A, 0);
-                __builtin_amdgcn_sched_barrier(0);
+                fetch(A, 0, 0);
                 __builtin_amdgcn_s_setprio(0);
                 for (int j = 0; j < n; j++) {
-                    consume(A, j, [&] {
-                        __builtin_amdgcn_sched_barrier(0);
-                        fetch_keys(A, j + 1);
-                        __builtin_amdgcn_sched_barrier(0);
+                    consume(A, j, 0, [&] {
+                        fence();
+                        fetch_keys(A, j + 1, 0);
+                        fence();
                     });
-                    __builtin_amdgcn_sched_barrier(0);
+                    fence();
                     fetch_values(A, j + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+                    fence();
                 }
-                // The fetch past the last page still writes zeros into the stage, where the next chunk's keys or the
-                // wave's partial go.
-                if constexpr (STAGED) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             }
+            // The fetches past the last page still write zeros into the stage, where the next chunk's keys or the
+            // wave's partial go.
+            if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
 
         // The column's sum over its lane groups, the wave's partial into LDS, and the waves' merge in order.
@@ -892,30 +883,50 @@ int cut_phase(Phase &ph, int n_kv, int pages, int want, int least, bool tiled, i
 }
 constexpr int kLeastSpread = 10;  // no splits
 
-// A window's launch wants a CU's worth of waves on each of the 256 CUs. A work-group of 16 walking waves (or 8 tile
-// waves) fills one alone; only when there are fewer work-groups than CUs, and a split still leaves each wave kWalkLeast
-// / 16 pages (each tile group kTileLeast / 2), are the keys cut, since that costs a merge launch.
-constexpr int kCus = 256, kWalkLeast = 128, kTileLeast = 32;
+// A window's work-group fills a CU (16 walking waves, 8 of f32 pages or of a tile), and with fewer work-groups than CUs
+// the keys may be cut, at the price of the merge launch: the runs that take least by what a wave's page (a tile's pair
+// of blocks) takes when the memory is not the bound, and a merge. One sequence, 8 kv heads, f16, measured: 2000 keys
+// uncut 13.2 us, 4000 keys 25.6 us, of which 5 us are no page's; f32 3.3 us a page.
+constexpr int kCus = 256;
+constexpr double kMergeUs = 4.0;
+
+int best_runs(int pages, int pages_a_step, double step_us, int most) {
+    int best = 1;
+    double least = 1e30;
+    for (int runs = 1; runs <= most; runs++) {
+        const int steps = (pages + runs * pages_a_step - 1) / (runs * pages_a_step);
+        const double us = steps * step_us + (runs > 1 ? kMergeUs + 0.02 * runs : 0.0);
+        if (us < least) least = us, best = runs;
+    }
+    return best;
+}
 
 Launch plan_window(const EmberWindowAttnArgs &a, int spread) {
     const EmberRaggedBatch &b = a.batch;
     const int G = b.n_heads / b.n_kv;
     const int64_t most = std::min(b.max_query, b.T);
+    const bool f16_pages = b.dtype == EMBER_DTYPE_F16;
     Launch l;
-    l.tiled = b.dtype == EMBER_DTYPE_F16 && most * G > kWalkRows;
+    l.tiled = f16_pages && most * G > kWalkRows;
     l.first = rows_phase(kWindowRows, b.S, most, G, l.tiled, 0);
     // a tile's keys: the first tokens' pages, and the windows of its tokens
     const int64_t tokens = std::min<int64_t>(most, ((l.tiled ? kTileRows : kWalkRows) + G - 1) / G + 1);
     const int64_t near = (std::min<int64_t>(a.window, static_cast<int64_t>(b.max_blocks) * kPage) + tokens + kPage - 1) / kPage + 1;
     const int pages = static_cast<int>(std::min<int64_t>(b.max_blocks, near + (static_cast<int64_t>(a.sinks) + kPage - 1) / kPage));
-    l.most_slots = cut_phase(l.first, b.n_kv, pages, kCus, l.tiled ? kTileLeast : kWalkLeast, l.tiled, spread);
+    const int64_t items = static_cast<int64_t>(b.S) * l.first.tiles * b.n_kv;
+    const int pages_a_step = l.tiled ? 2 * kBlockPages : f16_pages ? 16 : 8;
+    l.most_slots = static_cast<int>(std::clamp<int64_t>((kCus >> spread) / items, 1, (pages + pages_a_step - 1) / pages_a_step));
+    const int runs = best_runs(pages, pages_a_step, l.tiled ? 1.85 : f16_pages ? 1.2 : 3.3, l.most_slots);
+    const int unit = l.tiled ? 2 * kBlockPages : 1;
+    l.first.pages = (pages + runs * unit - 1) / (runs * unit) * unit;
+    l.first.splits = std::max(1, (pages + l.first.pages - 1) / l.first.pages);
     l.slots = l.first.splits;
     return l;
 }
 
 // A prefix's launch has a merge behind it in any case, so its phases are cut finely: tiles of kTileWant work-groups in
 // all, walks of two pages a wave or more.
-constexpr int kTileWant = 256, kWalkWant = 1024, kWalkFine = 8;
+constexpr int kTileWant = 256, kTileLeast = 32, kWalkWant = 1024, kWalkFine = 8;
 
 Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     const EmberRaggedBatch &b = a.batch;
@@ -925,13 +936,14 @@ Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     Launch l;
     l.tiled = b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
     l.most_slots = 0;
+    const int fine = b.dtype == EMBER_DTYPE_F16 ? kWalkFine : kWalkFine / 2;  // f32 pages are twice the bytes and the time
     if (a.n_groups > 0) {
         l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, l.tiled, 0);
         l.most_slots = cut_phase(l.first, b.n_kv, pages_of(a.max_prefix), l.tiled ? kTileWant : kWalkWant,
-                                 l.tiled ? kTileLeast : kWalkFine, l.tiled, spread);
+                                 l.tiled ? kTileLeast : fine, l.tiled, spread);
     }
     l.second = rows_phase(kOwnRows, b.S, in_seq, G, false, l.first.splits);
-    l.most_slots += cut_phase(l.second, b.n_kv, pages_of(a.max_own), kWalkWant, kWalkFine, false, spread);
+    l.most_slots += cut_phase(l.second, b.n_kv, pages_of(a.max_own), kWalkWant, fine, false, spread);
     l.slots = l.first.splits + l.second.splits;
     return l;
 }
