@@ -88,7 +88,7 @@ EXTRA_FLAGS = {
     "linear.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
     "gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "kv_append.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=8"],
-    "span_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
+    "span_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "prefill_attn.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
 }
 

@@ -90,6 +90,33 @@ int check_prefix(const char *who, const EmberPrefixAttnArgs &a) {
     return EMBER_OK;
 }
 
+// Every work-group reads the inputs while others write the outputs: in place is not possible.
+int check_step_aliases(const EmberStepTablesArgs &a) {
+    struct Range {
+        const char *name;
+        const void *at;
+        int64_t bytes;
+    };
+    const int64_t i32 = sizeof(int32_t), table = static_cast<int64_t>(a.max_blocks) * i32;
+    const Range in[] = {{"request", a.request, a.S * i32},          {"cached_len", a.cached_len, a.R * i32},
+                        {"new_len", a.new_len, a.S * i32},          {"free_blocks", a.free_blocks, a.n_free * i32},
+                        {"request_tables", a.request_tables, a.R * table}};
+    const Range out[] = {{"query_start", a.query_start, (a.S + 1) * i32},
+                         {"context_len", a.context_len, a.S * i32},
+                         {"positions", a.positions, a.max_tokens * i32},
+                         {"token_seq", a.token_seq, a.max_tokens * i32},
+                         {"slots", a.slots, a.max_tokens * 2 * i32},
+                         {"block_tables", a.block_tables, (a.S + 1) * table},
+                         {"totals", a.totals, 4 * i32}};
+    for (const Range &x : in)
+        for (const Range &y : out) {
+            const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at), y0 = reinterpret_cast<uintptr_t>(y.at);
+            if (x0 && y0 && x0 < y0 + y.bytes && y0 < x0 + x.bytes)
+                return set_error(EMBER_ERR_INVALID, "step_tables: %s overlaps %s, which this call writes", x.name, y.name);
+        }
+    return EMBER_OK;
+}
+
 }  // namespace
 }  // namespace ember::hip
 
@@ -356,6 +383,7 @@ int ember_hip_step_tables(const EmberStepTablesArgs *a, void *stream) {
         return set_error(EMBER_ERR_INVALID, "step_tables: a required pointer is null");
     if (a->free_cursor >= a->totals && a->free_cursor < a->totals + 4)
         return set_error(EMBER_ERR_INVALID, "step_tables: free_cursor may not lie in the totals that this call writes");
+    if (int e = check_step_aliases(*a)) return e;
     return hip_status(launch_step_tables(*a, static_cast<hipStream_t>(stream)), "step_tables");
 }
 

@@ -61,6 +61,10 @@ struct SpanParams {
 
 __device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
 
+// Whether a sum of weights holds anything: also when it is NaN (of a NaN in q, say), which a comparison would take for
+// an empty row's 0 and so turn the row into zeros.
+__device__ __forceinline__ bool filled(float l) { return __float_as_uint(l) != 0; }
+
 // The rows of one work item and the bounds of the keys they see.
 struct Rows {
     int t0, rows;     // first token, (token, head) rows
@@ -471,8 +475,8 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 }
             } else {
                 T *const dst = static_cast<T *>(p.out) + at * D + d;
-                dst[0] = from_f32<T>(L > 0.0f ? O.x / L : 0.0f);
-                dst[1] = from_f32<T>(L > 0.0f ? O.y / L : 0.0f);
+                dst[0] = from_f32<T>(filled(L) ? O.x / L : 0.0f);
+                dst[1] = from_f32<T>(filled(L) ? O.y / L : 0.0f);
             }
         }
         __syncthreads();  // the regions are the next row tile's stages
@@ -762,10 +766,10 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
                         *reinterpret_cast<float4 *>(dst + 8 * i) = make_float4(o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
                                                                                o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]);
                 }
-                if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + slot * 2) = make_float2(l > 0.0f ? m : kNoMax, l);
+                if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + slot * 2) = make_float2(filled(l) ? m : kNoMax, l);
             } else {
                 f16 *const dst = static_cast<f16 *>(p.out) + at * D + 4 * h;
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                const float inv = filled(l) ? 1.0f / l : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     f16x4 y;
@@ -818,10 +822,10 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
         const float corr = exp2_hw(M - top);
         M = top;
         L = L * corr, x = x * corr, y = y * corr;
-        const float f = mine.y > 0.0f ? exp2_hw(mine.x - top) : 0.0f;
+        const float f = filled(mine.y) ? exp2_hw(mine.x - top) : 0.0f;
         const float l = mine.y * f;
         // Only slots that hold something are read (an empty one's partial is not written), C at a time.
-        for (uint64_t left = __builtin_amdgcn_ballot_w64(mine.y > 0.0f); left != 0;) {
+        for (uint64_t left = __builtin_amdgcn_ballot_w64(filled(mine.y)); left != 0;) {
             float2 a[C];
             int slot[C];
             uint64_t rest = left;
@@ -842,8 +846,8 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
         }
     }
     T *const dst = static_cast<T *>(p.out) + at * D + 2 * lane;
-    dst[0] = from_f32<T>(L > 0.0f ? x / L : 0.0f);
-    dst[1] = from_f32<T>(L > 0.0f ? y / L : 0.0f);
+    dst[0] = from_f32<T>(filled(L) ? x / L : 0.0f);
+    dst[1] = from_f32<T>(filled(L) ? y / L : 0.0f);
 }
 
 // ---- host: phases and launches ----

@@ -394,7 +394,8 @@ typedef struct EmberStepTablesArgs {
  * that the append and decode kernels may run over: they belong to row S.
  * The inputs are left as they are but for request_tables, so a repeated call
  * gives the same tables; the next step passes totals + 1 (of a buffer that it
- * does not write) as free_cursor. S * max_blocks * 16 must fit 31 bits. */
+ * does not write) as free_cursor. No input may overlap an output.
+ * (S + 1) * max_blocks * 16 must fit 31 bits. */
 int ember_hip_step_tables(const EmberStepTablesArgs *args, void *stream);
 
 /* A ragged batch over the paged cache: the tokens of sequence s are rows
@@ -402,7 +403,8 @@ int ember_hip_step_tables(const EmberStepTablesArgs *args, void *stream);
  * one; their K/V are in the pages already. Rows of no sequence are left as
  * they are, and so is everything past T. Any number of query heads per kv
  * head; head_dim 128. K and V of visible keys are finite (the append kernels
- * clamp them); other slots may hold anything, NaN included. A table entry
+ * clamp them); other slots may hold anything, NaN included. A NaN in a row of
+ * q makes that (token, head) NaN and no other. A table entry
  * outside the pool reads as a page of zeros. A token at a negative position
  * gets zeros; one past its table reads up to the table's end. */
 typedef struct EmberRaggedBatch {

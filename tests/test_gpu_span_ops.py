@@ -134,6 +134,10 @@ def test_step_tables_python_refusals(device):
         K.step_tables(out, *good, request=i(3))
     with pytest.raises(EmberError):
         K.step_tables(out, *good, free_cursor=out.totals[1:2])
+    with pytest.raises(EmberError, match="cached_len overlaps context_len"):
+        K.step_tables(out, i(2, 4), out.context_len, i(2), i(5))
+    with pytest.raises(EmberError, match="request_tables overlaps block_tables"):
+        K.step_tables(out, out.block_tables, i(3), i(2), i(5))
     with pytest.raises(EmberError):
         K.step_tables(out, *good, pad_block=-2)
     with pytest.raises(EmberError):
@@ -318,6 +322,32 @@ def test_window_blocks_outside_the_pool_read_as_zeros(rng, device):
         b.check(sees)
 
 
+@pytest.mark.parametrize("f16,heads,kv,cached,new,window", [
+    (True, 4, 2, [100, 31, 40], [1, 1, 1], 64), (True, 8, 1, [100, 31], [3, 1], 64), (False, 4, 2, [100, 31], [3, 1], 64),
+    (True, 4, 1, [0, 90], [80, 70], 100), (True, 16, 16, [50] * 10, [200] * 10, 60), (True, 2, 1, [3000], [1], 2500)],
+    ids=["decode", "verify", "f32", "tiles", "many tiles", "split"])
+def test_window_nan_in_q_stays_in_its_row_and_is_not_hidden(rng, device, f16, heads, kv, cached, new, window):
+    b, sees = window_batch(rng, device, cached, np.array(new), heads, kv, f16, window, 3)
+    kw = dict(window=window, sinks=3, max_query=max(new), workspace=window_ws(b, heads, kv, window, 3, device, max(new)))
+    K.window_attention(*b.args(), **kw)
+    b.check(sees)
+    _nan_rows(b, heads, lambda: K.window_attention(*b.args(), **kw))
+
+
+def _nan_rows(b, heads, call):
+    clean = b.out.clone()
+    rows = [(0, 0), (b.T - 1, heads - 1)]
+    for t, h in rows:
+        b.dev["q"][t, h, 5 + h] = float("nan")
+        clean[t, h] = 0
+    b.out.fill_(123.0)
+    call()
+    for t, h in rows:
+        assert torch.isnan(b.out[t, h]).all()
+        b.out[t, h] = 0
+    assert torch.equal(b.out, clean)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 def test_window_q_inside_wider_rows_and_another_stream(rng, device, new):
     H, KV = 16, 8
@@ -437,6 +467,19 @@ def test_prefix_tokens_inside_it_and_sequences_of_no_group(rng, device):
     K.shared_prefix_attention(t(q), t(k), t(v), out, dint(start, device), dint(pos, device), dint(tables, device),
                               dint([0], device), dint([], device), workspace=ws, max_query=6)
     assert (np.abs(out.double().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("f16,heads,kv,groups", [(True, 4, 2, [3, 2]), (True, 16, 1, [9, 4]), (False, 4, 2, [3, 2])],
+                         ids=["walks", "tiles", "f32"])
+def test_prefix_nan_in_q_stays_in_its_row_and_is_not_hidden(rng, device, f16, heads, kv, groups):
+    n = sum(groups)
+    b = prefix_batch(rng, device, groups, [333, 90], rng.integers(1, 70, n), np.ones(n, int), heads, kv, f16)
+    kw = dict(max_query=1, max_group=max(groups), max_prefix=333, max_own=70)
+    ws = prefix_ws(b, heads, kv, device, **kw)
+    call = lambda: K.shared_prefix_attention(*b.args(), b.group_start, b.prefix, workspace=ws, **kw)  # noqa: E731
+    call()
+    b.check(causal)
+    _nan_rows(b, heads, call)
 
 
 def test_prefix_many_groups(rng, device):

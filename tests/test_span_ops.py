@@ -27,6 +27,22 @@ def test_step_tables_refusals(field, value, text):
     assert text in _lib.last_error()
 
 
+@pytest.mark.parametrize("field,at,other", [
+    ("cached_len", 0x20000, "context_len"), ("request", 0x20000 + 4, "context_len"), ("new_len", 0x10000 + 8, "query_start"),
+    ("request_tables", 0x60000 + 16, "block_tables"), ("free_blocks", 0x70000 - 4 * 4, "totals"), ("cached_len", 0x50000 + 44, "slots"),
+    ("new_len", 0x30000 + 20, "positions"), ("request", 0x40000, "token_seq")])
+def test_step_tables_refuse_to_work_in_place(field, at, other):
+    """Inputs that overlap outputs, by one entry and more (S 2, R 3, 4 pages a row, 6 token rows); no pointer is followed."""
+    a = _tables()
+    for i, f in enumerate(("query_start", "context_len", "positions", "token_seq", "slots", "block_tables", "totals")):
+        setattr(a, f, 0x10000 * (i + 1))
+    for i, f in enumerate(("request", "cached_len", "new_len", "free_blocks", "request_tables")):
+        setattr(a, f, 0x100000 + 0x10000 * i)
+    setattr(a, field, at)
+    assert _lib.lib().ember_hip_step_tables(a, None) == _lib.ERR_INVALID
+    assert f"{field} overlaps {other}" in _lib.last_error()
+
+
 def _batch(a):
     b = a  # the batch's fields come first
     for f in ("q", "k_cache", "v_cache", "out", "query_start", "positions", "block_tables"):
