@@ -852,16 +852,6 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
 
 // ---- host: phases and launches ----
 
-// Cuts `pages` virtual pages into runs of a multiple of `unit`, `items` work-groups a run: as many as make `want`
-// work-groups in all, each at least `least` pages. Returns the runs that were allowed, which only grow with `pages`
-// (the splits, equal runs of whole units, need not): the workspace is sized by them.
-int cut(Phase &ph, int64_t items, int pages, int want, int least, int unit) {
-    const int64_t runs = std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(1, items), pages / least));
-    ph.pages = std::max<int>(1, static_cast<int>((pages + runs * unit - 1) / (runs * unit))) * unit;
-    ph.splits = std::max(1, (pages + ph.pages - 1) / ph.pages);
-    return static_cast<int>(runs);
-}
-
 struct Launch {
     Phase first{}, second{};  // second.units == 0: none
     bool tiled = false;       // the first phase is tiles
@@ -881,11 +871,13 @@ Phase rows_phase(int kind, int units, int64_t tokens, int G, bool tiled, int slo
 }
 
 // `spread` halves the work-groups asked for, step by step, until the workspace holds the partials.
-int cut_phase(Phase &ph, int n_kv, int pages, int want, int least, bool tiled, int spread) {
-    return cut(ph, static_cast<int64_t>(ph.units) * ph.tiles * n_kv, pages, want >> spread, least,
-               tiled ? 2 * kBlockPages : 1);  // a run of whole blocks for both of a tile's key groups
-}
 constexpr int kLeastSpread = 10;  // no splits
+
+// Cuts `pages` virtual pages into `runs` equal runs of a multiple of `unit`, or fewer where those reach the end sooner.
+void set_runs(Phase &ph, int pages, int runs, int unit) {
+    ph.pages = std::max(1, (pages + runs * unit - 1) / (runs * unit)) * unit;
+    ph.splits = std::max(1, (pages + ph.pages - 1) / ph.pages);
+}
 
 // A window's work-group fills a CU (16 walking waves, 8 of f32 pages or of a tile), and with fewer work-groups than CUs
 // the keys may be cut, at the price of the merge launch: the runs that take least by what a wave's page (a tile's pair
@@ -921,16 +913,61 @@ Launch plan_window(const EmberWindowAttnArgs &a, int spread) {
     const int pages_a_step = l.tiled ? 2 * kBlockPages : f16_pages ? 16 : 8;
     l.most_slots = static_cast<int>(std::clamp<int64_t>((kCus >> spread) / items, 1, (pages + pages_a_step - 1) / pages_a_step));
     const int runs = best_runs(pages, pages_a_step, l.tiled ? 1.85 : f16_pages ? 1.2 : 3.3, l.most_slots);
-    const int unit = l.tiled ? 2 * kBlockPages : 1;
-    l.first.pages = (pages + runs * unit - 1) / (runs * unit) * unit;
-    l.first.splits = std::max(1, (pages + l.first.pages - 1) / l.first.pages);
+    set_runs(l.first, pages, runs, l.tiled ? 2 * kBlockPages : 1);
     l.slots = l.first.splits;
     return l;
 }
 
-// A prefix's launch has a merge behind it in any case, so its phases are cut finely: tiles of kTileWant work-groups in
-// all, walks of two pages a wave or more.
-constexpr int kTileWant = 256, kTileLeast = 32, kWalkWant = 1024, kWalkFine = 8;
+// A prefix's launch has a merge behind it in any case, so its walks are cut finely: two pages a wave or more.
+constexpr int kWalkWant = 1024, kWalkFine = 8;
+
+// Returns the runs that were allowed, which only grow with `pages` (the splits need not): the workspace is sized by them.
+int cut_phase(Phase &ph, int n_kv, int pages, int least, int spread) {
+    const int64_t items = static_cast<int64_t>(ph.units) * ph.tiles * n_kv;
+    const int runs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((kWalkWant >> spread) / std::max<int64_t>(1, items), pages / least)));
+    set_runs(ph, pages, runs, 1);
+    return runs;
+}
+
+// Tiles of the prefix beside walks of the own keys: the splits that take least by what was measured of the mixed
+// launch (f16). A tile's pair of blocks 3 us, plus 0.4 of the time that the own keys' walks keep the memory busy beside
+// it; four pages of a walk (one a wave) 1.25 us and 4 us before them; a slot of every (token, head) 1040 bytes written
+// and read at 2.7 TB/s. The own keys are taken to be half of the longest sequence's on average, at 5.5 TB/s, where the
+// caller names a longest, and none otherwise. 64 sequences on 8000 shared tokens, 32 heads, own keys up to 1500: 7, 9
+// and 13 splits 54.9, 54.5 and 60.4 us, 3 splits 86.5 us; 105 sequences on 3529 tokens, 12 heads, own keys up to 224:
+// 3, 4 and 6 splits 43.4, 34.2 and 28.6 us.
+constexpr int kTileUnit = 2 * kBlockPages;  // pages
+constexpr int kMostRuns = 64;
+constexpr double kTilePairUs = 3.0, kTileBeside = 0.4, kWalkStepUs = 1.25, kWalkStartUs = 4.0;
+constexpr double kSlotBytesPerUs = 2.7e6, kOwnBytesPerUs = 5.5e6;
+
+void cut_mixed(Launch &l, const EmberRaggedBatch &b, int prefix_pages, int own_pages, bool own_known, int spread) {
+    const int64_t tiles = static_cast<int64_t>(l.first.units) * l.first.tiles * b.n_kv;
+    const int64_t walks = static_cast<int64_t>(l.second.units) * l.second.tiles * b.n_kv;
+    const double slot_us = static_cast<double>(b.T) * b.n_heads * (2 * (kHeadDim + 2) * sizeof(float)) / kSlotBytesPerUs;
+    const double page_bytes = 2.0 * kPage * kHeadDim * sizeof(uint16_t);
+    const double own_us = own_known ? 0.5 * walks * own_pages * page_bytes / kOwnBytesPerUs : 0.0;
+    // Work-groups: tiles one a CU, walks two.
+    const int most_tiles = static_cast<int>(std::clamp<int64_t>((kCus >> spread) / tiles, 1, std::min(kMostRuns, (prefix_pages + kTileUnit - 1) / kTileUnit)));
+    const int most_walks = static_cast<int>(std::clamp<int64_t>((2 * kCus >> spread) / walks, 1, std::min(kMostRuns, (own_pages + kTileWaves - 1) / kTileWaves)));
+    auto least = [&](int most, auto us) {
+        int best = 1;
+        double best_us = us(1);
+        for (int n = 2; n <= most; n++)
+            if (const double x = us(n); x < best_us) best = n, best_us = x;
+        return best;
+    };
+    auto steps = [](int pages, int runs, int unit) { return (pages + runs * unit - 1) / (runs * unit); };
+    auto walk_us = [&](int n) { return std::max(own_us, kWalkStartUs + kWalkStepUs * steps(own_pages, n, kTileWaves)); };
+    const int own_runs = least(most_walks, [&](int n) { return walk_us(n) + n * slot_us; });
+    const double beside_us = kWalkStartUs + walk_us(own_runs);
+    const int runs = least(most_tiles, [&](int n) {
+        return std::max(beside_us, kTilePairUs * steps(prefix_pages, n, kTileUnit) + kTileBeside * own_us) + n * slot_us;
+    });
+    set_runs(l.first, prefix_pages, runs, kTileUnit);
+    set_runs(l.second, own_pages, own_runs, 1);
+    l.most_slots = most_tiles + most_walks;
+}
 
 Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     const EmberRaggedBatch &b = a.batch;
@@ -938,16 +975,18 @@ Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     const int64_t in_group = std::min(a.max_group, b.T), in_seq = std::min(b.max_query, b.T);
     auto pages_of = [&](int keys) { return std::min(b.max_blocks, keys / kPage + 2); };
     Launch l;
-    l.tiled = b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
+    l.tiled = a.n_groups > 0 && b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
     l.most_slots = 0;
-    const int fine = b.dtype == EMBER_DTYPE_F16 ? kWalkFine : kWalkFine / 2;  // f32 pages are twice the bytes and the time
-    if (a.n_groups > 0) {
-        l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, l.tiled, 0);
-        l.most_slots = cut_phase(l.first, b.n_kv, pages_of(a.max_prefix), l.tiled ? kTileWant : kWalkWant,
-                                 l.tiled ? kTileLeast : fine, l.tiled, spread);
+    if (a.n_groups > 0) l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, l.tiled, 0);
+    l.second = rows_phase(kOwnRows, b.S, in_seq, G, false, 0);
+    if (l.tiled) {
+        cut_mixed(l, b, pages_of(a.max_prefix), pages_of(a.max_own), a.max_own / kPage < b.max_blocks, spread);
+    } else {
+        const int fine = b.dtype == EMBER_DTYPE_F16 ? kWalkFine : kWalkFine / 2;  // f32 pages are twice the bytes and the time
+        if (a.n_groups > 0) l.most_slots = cut_phase(l.first, b.n_kv, pages_of(a.max_prefix), fine, spread);
+        l.most_slots += cut_phase(l.second, b.n_kv, pages_of(a.max_own), fine, spread);
     }
-    l.second = rows_phase(kOwnRows, b.S, in_seq, G, false, l.first.splits);
-    l.most_slots += cut_phase(l.second, b.n_kv, pages_of(a.max_own), kWalkWant, fine, false, spread);
+    l.second.slot0 = l.first.splits;
     l.slots = l.first.splits + l.second.splits;
     return l;
 }
