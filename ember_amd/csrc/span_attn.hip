@@ -38,6 +38,7 @@ constexpr int kTileRows = 32 * kTileWaves;
 constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kBlockPages = 4;             // pages of a tile's key block
 constexpr int kBlockKeys = kBlockPages * kPage;
+static_assert(kBlockPages == kTileWaves);  // a wave loads one of them
 constexpr int kNoWindow = INT_MAX;
 
 enum Kind : int { kWindowRows, kPrefixRows, kOwnRows };
@@ -502,7 +503,9 @@ __global__ void __launch_bounds__(W *kWave, (sizeof(T) == 2 ? 4 : 2))
 //   O^T += V^T P^T  the lane's scores, as weights in f16, are the B operand as they stand (the order of the keys
 //                 inside one product is free); the A operand, the same keys of dim c, comes from the transposing
 //                 LDS read: lane r of a 16-lane block reads four dims of key r / 4, lane i receives dim i of 4 keys.
-constexpr int kRow = kHeadDim + 16;  // LDS row of a key, halves: 72 dwords, so 8 rows start 8 banks apart
+// LDS rows, halves. Keys: 68 dwords, so that 16 rows' pieces of 16 bytes, read at once, lie on the 64 banks side by side.
+// Values: 80 dwords, so that the four rows and two dim blocks of a transposing read of 32 lanes do.
+constexpr int kKeyRow = kHeadDim + 8, kValueRow = kHeadDim + 32;
 typedef __fp16 tr16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
 
@@ -513,17 +516,17 @@ constexpr int kAhead = 4;  // value operands in flight ahead of their products
 
 // KG key groups of 4 waves, the same rows each: group g takes blocks g, g + KG, ... through buffers of its own, and
 // the last ones hand their partials to group 0 through LDS.
-constexpr int kBuffer = kBlockKeys * kRow;
-constexpr int tile_lds_bytes(int KG) { return KG * 4 * kBuffer * static_cast<int>(sizeof(f16)) + 64; }
+constexpr int kKeyBuffer = kBlockKeys * kKeyRow, kValueBuffer = kBlockKeys * kValueRow;
+constexpr int tile_lds_bytes(int KG) { return KG * 2 * (kKeyBuffer + kValueBuffer) * static_cast<int>(sizeof(f16)) + 64; }
 
 template <int KG>
 __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, const int id, unsigned char *lds) {
     constexpr int D = kHeadDim;
-    f16 *const k_all = reinterpret_cast<f16 *>(lds), *const v_all = k_all + KG * 2 * kBuffer;
-    int *const ext = reinterpret_cast<int *>(v_all + KG * 2 * kBuffer);  // [wave][2]
+    f16 *const k_all = reinterpret_cast<f16 *>(lds), *const v_all = k_all + KG * 2 * kKeyBuffer;
+    int *const ext = reinterpret_cast<int *>(v_all + KG * 2 * kValueBuffer);  // [wave][2]
     const int group = KG == 1 ? 0 : uniform(static_cast<int>(threadIdx.x) / kTileThreads);
     const int tid = static_cast<int>(threadIdx.x) % kTileThreads, lane = tid % kWave, wave = uniform(tid / kWave);
-    f16 *const k_lds = k_all + group * 2 * kBuffer, *const v_lds = v_all + group * 2 * kBuffer;  // two buffers each
+    f16 *const k_lds = k_all + group * 2 * kKeyBuffer, *const v_lds = v_all + group * 2 * kValueBuffer;  // two buffers each
     const int h = lane >> 5, c = lane & 31;
     const int kvh = id % p.n_kv;
     int rest = id / p.n_kv;
@@ -575,7 +578,7 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         const bool partial = p.slots > 1;
 
         // This lane's part of a value operand: key 4 h + r / 4, dims 16 (l / 16 % 2) + 4 (r % 4) .. + 3 of its 16-lane block.
-        const int v_at = (4 * h + lane % 16 / 4) * kRow + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+        const int v_at = (4 * h + lane % 16 / 4) * kValueRow + 16 * (lane / 16 % 2) + 4 * (lane % 4);
         float m = -INFINITY, l = 0.0f;
         f32x16 o[4];
 #pragma unroll
@@ -596,48 +599,55 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         const uint32_t n_live = max(max_top - sp.lo + 1, 0);
         const int sink_live = min(sinks, max_top + 1);
 
-        // A block's pages into registers: each page one 16-byte piece a thread, of key tid / 16. Where the pages of
-        // 64 virtual pages are, and their bytes (0: not in the pool, the loads give zeros), one page a lane.
-        u32x4 kr[kBlockPages], vr[kBlockPages];
+        // A block's pages into registers, a page a wave: 16 bytes of keys 4 i + l / 16 a lane. The ids of 64 steps' pages
+        // are held one a lane; one outside the pool has no records, and its loads give zeros.
+        u32x4 kr[4], vr[4];
         // Step b of this group reads virtual pages first_page(b) .. + 3.
         auto first_page = [&](int b) { return v0 + (b * KG + group) * kBlockPages; };
-        auto id_of = [&](int b0) {  // lane 4 i + j: page j of step b0 + i
-            const int v = first_page(b0 + lane / kBlockPages) + lane % kBlockPages;
+        auto id_of = [&](int b) {
+            const int v = first_page(b) + wave;
             return v < v1 ? table[sp.page(v)] : -1;
         };
-        int next_ids = id_of(0);
-        int64_t at64 = 0;
-        int bytes64 = 0;
+        int ids = -1, next_ids = id_of(lane);
+        // Lane offsets are made opaque: their constant parts then go into the accesses, where the compiler would hold
+        // each sum in a register of its own across the loop.
+        auto here = [](int x) {
+            asm volatile("" : "+v"(x));
+            return x;
+        };
         auto fetch = [&](int b) {
-            if (b % (kWave / kBlockPages) == 0) {
-                const bool live = next_ids >= 0 && next_ids < p.num_blocks;
-                at64 = (live ? next_ids : 0) * block_stride * static_cast<int64_t>(sizeof(f16));
-                bytes64 = live ? kPage * D * 2 : 0;
-                next_ids = id_of(b + kWave / kBlockPages);
+            if (b % kWave == 0) {
+                ids = next_ids;
+                next_ids = id_of(b + kWave + lane);
             }
+            const int blk = __builtin_amdgcn_readlane(ids, b % kWave);
+            const bool live = blk >= 0 && blk < p.num_blocks;
+            const int64_t at = (live ? blk : 0) * block_stride;
+            const int bytes = live ? kPage * D * static_cast<int>(sizeof(f16)) : 0;
+            const __amdgpu_buffer_rsrc_t kd = __builtin_amdgcn_make_buffer_rsrc(const_cast<f16 *>(kbase) + at, 0, bytes, kDescWord3);
+            const __amdgpu_buffer_rsrc_t vd = __builtin_amdgcn_make_buffer_rsrc(const_cast<f16 *>(vbase) + at, 0, bytes, kDescWord3);
+            auto load = [](__amdgpu_buffer_rsrc_t d, int off) {
+                return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, off, 0, 0));
+            };
+            constexpr int kPast = kPage * D * static_cast<int>(sizeof(f16));
+            const int at_lane = here(lane), off = 16 * at_lane, key0 = sp.page(first_page(b) + wave) * kPage + at_lane / 16;
 #pragma unroll
-            for (int j = 0; j < kBlockPages; j++) {
-                const int n = (b * kBlockPages + j) % kWave;
-                const int64_t at = static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(
-                                       __builtin_amdgcn_readlane(static_cast<int>(at64 >> 32), n))) << 32 |
-                                   static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at64), n)));
-                const int bytes = __builtin_amdgcn_readlane(bytes64, n);
-                const int key = sp.page(first_page(b) + j) * kPage + tid / 16;
-                const bool live = (static_cast<uint32_t>(key - sp.lo) < n_live) | (key < sink_live);
-                const __amdgpu_buffer_rsrc_t kd = __builtin_amdgcn_make_buffer_rsrc(
-                    const_cast<char *>(reinterpret_cast<const char *>(kbase) + at), 0, bytes, kDescWord3);
-                const __amdgpu_buffer_rsrc_t vd = __builtin_amdgcn_make_buffer_rsrc(
-                    const_cast<char *>(reinterpret_cast<const char *>(vbase) + at), 0, bytes, kDescWord3);
-                kr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kd, 16 * tid, 0, 0));
-                vr[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vd, live ? 16 * tid : kPage * D * 2, 0, 0));
+            for (int i = 0; i < 4; i++) kr[i] = load(kd, off + 1024 * i);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = key0 + 4 * i;
+                const bool seen = (static_cast<uint32_t>(key - sp.lo) < n_live) | (key < sink_live);
+                vr[i] = load(vd, seen ? off + 1024 * i : kPast);
             }
         };
         auto stage = [&](int b) {
+            const int at_lane = here(lane), key = kPage * wave + at_lane / 16, dim = at_lane % 16 * 8;
+            f16 *const kp = k_lds + (b & 1) * kKeyBuffer + key * kKeyRow + dim;
+            f16 *const vp = v_lds + (b & 1) * kValueBuffer + key * kValueRow + dim;
 #pragma unroll
-            for (int j = 0; j < kBlockPages; j++) {
-                const int at = (j * kPage + tid / 16) * kRow + tid % 16 * 8;
-                *reinterpret_cast<u32x4 *>(&k_lds[(b & 1) * kBuffer + at]) = kr[j];
-                *reinterpret_cast<u32x4 *>(&v_lds[(b & 1) * kBuffer + at]) = vr[j];
+            for (int i = 0; i < 4; i++) {
+                *reinterpret_cast<u32x4 *>(kp + 4 * i * kKeyRow) = kr[i];
+                *reinterpret_cast<u32x4 *>(vp + 4 * i * kValueRow) = vr[i];
             }
         };
         const int steps = (blocks + KG - 1) / KG;
@@ -649,7 +659,8 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         __syncthreads();
         for (int b = 0; b < steps; b++) {
             if (b + 1 < steps) fetch(b + 1);
-            const f16 *const kl = k_lds + (b & 1) * kBuffer + c * kRow + 8 * h, *const vl = v_lds + (b & 1) * kBuffer + v_at;
+            const f16 *const kl = k_lds + (b & 1) * kKeyBuffer + c * kKeyRow + 8 * h;
+            const f16 *const vl = v_lds + (b & 1) * kValueBuffer + v_at;
             // Scores: the operands of a 32-key half are all requested before its first product, and each is
             // replaced by the other half's as soon as its product is issued.
             f32x16 s[2];
@@ -664,15 +675,15 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i], qf[i], s[t], 0, 0, 0);
-                    if (t == 0) ka[i] = *reinterpret_cast<const f16x8 *>(kl + 32 * kRow + 16 * i);
+                    if (t == 0) ka[i] = *reinterpret_cast<const f16x8 *>(kl + 32 * kKeyRow + 16 * i);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             // The first values, in flight during the softmax: operand n = 4 j + t is dim tile t of keys 16 j .. + 15.
             auto value = [&](int n) {
-                const f16 *const at = vl + n / 4 * 16 * kRow + n % 4 * 32;
+                const f16 *const at = vl + n / 4 * 16 * kValueRow + n % 4 * 32;
                 const f16x4 lo4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)at));
-                const f16x4 hi4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)(at + 8 * kRow)));
+                const f16x4 hi4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)(at + 8 * kValueRow)));
                 return f16x8{lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
             };
             f16x8 va[kAhead];
@@ -730,7 +741,7 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
 
         if constexpr (KG == 2) {  // group 1's partial, through the buffers (every wave is past its last block)
             f32x4 *const hand = reinterpret_cast<f32x4 *>(k_all) + tid;
-            static_assert(17 * kTileThreads * sizeof(f32x4) <= KG * 2 * kBuffer * sizeof(f16));
+            static_assert(17 * kTileThreads * sizeof(f32x4) <= KG * 2 * kKeyBuffer * sizeof(f16));
             if (group == 1) {
 #pragma unroll
                 for (int i = 0; i < 16; i++)
