@@ -20,7 +20,15 @@
 // the pages: span_walk_kernel gives each wave pages of its own, straight from
 // HBM. Many rows (prompt chunks, a group's rows before a long prefix) are bound by
 // the products: span_tile_kernel shares 64-key blocks in LDS between waves of
-// 32 rows each.
+// 32 rows each. span_mixed_kernel runs both in one launch.
+//
+// Measured (kernel time, one MI355X; each kernel's own figures stand beside it):
+//   walk   32 decodes, windows of 4096 tokens, 16 / 8 heads   75.6 us, 6.4 TB/s
+//          64 verify runs of up to 5 tokens, windows of 1000  43.2 us, 6.1 TB/s
+//          1 decode, a window of 512                           8.0 us: a chain of four trips to memory
+//   tile   2000 tokens, windows of 4096                       86 us, 780 TFLOP/s
+//   mixed  64 decodes behind 8000 shared tokens               52 us, and 5.4 us the merge
+//          256 decodes in 16 groups                          108 us (4.7 TB/s), and 5.6 us the merge
 #include <algorithm>
 #include <climits>
 
@@ -160,6 +168,11 @@ __device__ __forceinline__ bool visible(int j, int base, int top, int pos, int w
 // group g, so a lane loads key c in 16-byte pieces; step v of the values takes key 4 g + v, which the lane's own
 // scores belong to. Keys of the f16 form pass through LDS (direct loads of four whole rows an instruction, swizzled).
 // Where a CU runs 16 waves, each has half a page in flight; DEEP keeps two whole pages instead, for 8 waves a CU.
+//
+// Bound by HBM where the launch fills the chip (6.4 TB/s), else by latency: query_start and positions, the table, the
+// pages, the merge of the waves are trips that wait for one another, 8 us for one page a wave. Hence a page per wave
+// (a work-group per kv head reads 16 pages at once), W = 16 waves up to one work-group a CU, 8 up to two, 4 beyond,
+// no scratch (any spill costs a launch 7 to 10 us), and lane offsets that go into the loads' immediates.
 template <typename T>
 struct WalkPage;
 template <>
@@ -511,9 +524,17 @@ typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
 
 // How far (base 2) a score may pass the reference max before the reference moves: weights stay below 2^8, which
 // f16 holds, and most blocks rescale nothing.
+// The weights are rounded to f16, the products' operand (2^-11 of each at most), and summed as rounded, so numerator
+// and denominator move alike.
 constexpr float kLazy = 8.0f;
 constexpr int kAhead = 4;  // value operands in flight ahead of their products
 
+// Bound by the two waves of a SIMD taking turns: at 2000 tokens behind 12,000 (windows of 4096) the matrix unit is
+// busy 34% of the cycles, the VALU 35%, LDS 26%, HBM hardly at all. 128 rows share a block's 32 KiB, and a page a wave
+// is loaded a block ahead through registers. Tried: loads straight to LDS with three key buffers, and the groups half a
+// step apart (4 us less, for twice the code), weights of the next keys between the products of the last (2 us more),
+// 8 value operands ahead in place of 4 (no change).
+//
 // KG key groups of 4 waves, the same rows each: group g takes blocks g, g + KG, ... through buffers of its own, and
 // the last ones hand their partials to group 0 through LDS.
 constexpr int kKeyBuffer = kBlockKeys * kKeyRow, kValueBuffer = kBlockKeys * kValueRow;
@@ -800,7 +821,9 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) span_tile_kernel(SpanPara
 }
 
 // Tiles of a prefix beside walks of the own keys: the tiles are bound by their products, the walks by the memory, and
-// a CU runs one work-group of each.
+// a CU runs one work-group of each. 64 sequences on 8000 shared tokens (32 / 8 heads, 13 splits): tiles alone 31 us,
+// walks alone 45, together 62, each with its launch and merge. The tiles come first: interleaved with the walks by 8
+// work-groups they end later (68 us), and with raised priority for the walks too (65 us).
 __global__ void __launch_bounds__(kTileThreads, 2) span_mixed_kernel(SpanParams p, Phase first, Phase walks, int tile_groups) {
     static_assert(tile_lds_bytes(1) >= walk_lds_floats(kTileWaves) * 4);
     __shared__ __align__(16) unsigned char lds[tile_lds_bytes(1)];
@@ -810,6 +833,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) span_mixed_kernel(SpanParams 
 }
 
 // ---- the slots' merge: a wave per (token, head), two dims a lane ----
+//
+// 520 bytes a slot read, 3 to 5.5 us with the launch. A last-arriver's merge inside the launch before it (a count and
+// device-scope stores) took longer than this launch.
 
 constexpr int kMergeWaves = 4;
 

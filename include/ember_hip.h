@@ -8,7 +8,8 @@
  *      the CUDA launchers of the reference's kernel seam
  *      (src/backend/cuda/kernels.cuh:74-120) field for field, plus a few
  *      documented additions (pool size for bounds guards, element type, query
- *      runs).
+ *      runs). 1b: launchers without a counterpart there, for steps planned on
+ *      the GPU, windowed attention and shared prefixes.
  *   2. The KV block manager (src/kvcache/block_manager.hpp:25-67) behind an
  *      opaque handle, plus two additive calls (share, copy_on_write) that the
  *      reference does not have.
