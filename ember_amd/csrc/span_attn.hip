@@ -613,7 +613,7 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         const int sink_end = min(sinks, my_top + 1);
         // Virtual pages whole0 .. whole1 - 1: every row of the wave sees every key of them.
         const int whole_key = max(r.base, window == kNoWindow ? 0 : hi_pos - window + 1);
-        const int whole0 = sp.head + (max(whole_key, 0) + kPage - 1) / kPage - (sp.skip + sp.head);
+        const int whole0 = static_cast<int>((static_cast<uint32_t>(max(whole_key, 0)) + kPage - 1) / kPage) - sp.skip;
         const int whole1 = (lo_top + 1) / kPage - sp.skip;
         // Keys that some row of the tile sees, likewise. Others may hold anything: their values are read as zeros
         // (an offset past the page's records), so that a zero weight meets no NaN.

@@ -494,6 +494,8 @@ def step_tables(out: StepTables, request_tables, cached_len, new_len, free_block
         if free_cursor.numel() != 1:
             raise EmberError("free_cursor must be one number")
         a.free_cursor = free_cursor.data_ptr()
+    if not -1 <= pad_block <= 0x7FFFFFFF:
+        raise EmberError(f"pad_block is a page or -1 (got {pad_block})")
     a.R, a.n_free, a.pad_block = R, len(free_blocks), pad_block
     _launch(_lib.lib().ember_hip_step_tables, a, dev, stream, "step_tables")
     return out
@@ -543,9 +545,15 @@ def _workspace(n: int, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
 
 
+def _check_window(window: int, sinks: int) -> None:
+    if not (0 < window <= 0x7FFFFFFF and 0 <= sinks <= 0x7FFFFFFF):
+        raise EmberError(f"window must be 1 .. 2^31 - 1 and sinks 0 .. 2^31 - 1 (got {window}, {sinks})")
+
+
 def window_workspace(T: int, S: int, *, n_heads, n_kv, window, sinks=0, max_query=None, dtype=torch.float16,
                      max_blocks=None, device="cuda"):
     """A workspace for window_attention of batches of these sizes, or None when such a call splits no keys."""
+    _check_window(window, sinks)
     a = _lib.WindowAttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks), window, sinks)
     return _workspace(int(_lib.lib().ember_hip_window_workspace_bytes(a)), device)
 
@@ -561,6 +569,7 @@ def window_attention(q, k_pool, v_pool, out, query_start, positions, block_table
     query_start[S] are left alone. max_query: the most tokens of one sequence (None: T); workspace: of
     window_workspace, not shared by calls that overlap in time (None: no splits).
     """
+    _check_window(window, sinks)
     dev, batch = _ragged_batch(q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace)
     _launch(_lib.lib().ember_hip_window_attn, _lib.WindowAttnArgs(*batch, window, sinks), dev, stream, "window_attn")
     return out

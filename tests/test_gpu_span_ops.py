@@ -311,6 +311,30 @@ def test_window_rows_without_keys_and_positions_outside_the_table(rng, device):
         assert (b.out[0] == 0).all() and (b.out[2] == 0).all() and (b.out[1] != 0).any()
 
 
+@pytest.mark.parametrize("window", [1, 7, 2 ** 31 - 2, 2 ** 31 - 1])
+def test_window_positions_up_to_the_last_int(rng, device, window):
+    """Positions far past the table: the first tokens, and what a window as wide leaves of the table."""
+    b, _ = window_batch(rng, device, [100, 100, 100], [1, 1, 1], 4, 2, True, 200, 0, pad_rows=0)
+    sees = lambda s, p, j: (j <= p) & ((p - j < window) | (j < 5))  # noqa: E731
+    b.pos = np.array([2 ** 31 - 1, 2 ** 31 - 9, 2 ** 31 - 20])
+    b.dev["pos"] = dint(b.pos, device)
+    k, v = (rng.standard_normal(b.k.shape).astype(np.float16) for _ in range(2))
+    b.k, b.v, b.dev["k"], b.dev["v"] = k, v, torch.from_numpy(k).to(device), torch.from_numpy(v).to(device)
+    b.tables = rng.integers(0, k.shape[0], b.tables.shape)
+    b.dev["table"] = dint(b.tables, device)
+    for hint in (1, 100):  # the walk and the tile form
+        b.out.fill_(123.0)
+        K.window_attention(*b.args(), window=window, sinks=5, max_query=hint)
+        b.check(sees)
+
+
+def test_window_long_tiles_take_page_ids_more_than_once(rng, device):
+    """More than 64 blocks in a key group, whose ids are held 64 at a time; the window starts inside a page."""
+    b, sees = window_batch(rng, device, [12000], [40], 4, 1, True, 10001, 3)
+    K.window_attention(*b.args(), window=10001, sinks=3)
+    b.check(sees)
+
+
 def test_window_blocks_outside_the_pool_read_as_zeros(rng, device):
     b, sees = window_batch(rng, device, [100, 100], [1, 1], 4, 2, True, 200, 0)
     b.tables[0, 2], b.tables[0, 4], b.tables[1, 0], b.tables[1, 6] = b.k.shape[0], -5, 2 ** 31 - 1, -2 ** 31
@@ -501,6 +525,15 @@ def test_prefix_long_one_in_many_splits(rng, device):
         b.check(causal)
 
 
+def test_prefix_and_own_keys_of_thousands_of_tokens_unsplit(rng, device):
+    """A tile's and a walk's page ids taken more than once, where the workspace allows no splits."""
+    own = np.concatenate([[9000, 4200], rng.integers(1, 40, 10)])
+    b = prefix_batch(rng, device, [12], [9000], own, np.ones(12, int), 4, 2, True)
+    least = torch.empty(2 * b.q.shape[0] * 4 * 130 * 4, dtype=torch.uint8, device=device)
+    K.shared_prefix_attention(*b.args(), b.group_start, b.prefix, workspace=least, max_query=1, max_group=12)
+    b.check(causal)
+
+
 def test_small_workspaces(rng, device):
     """Fewer splits where the workspace has room for fewer; an error where not even two partials fit."""
     b = prefix_batch(rng, device, [6], [700], rng.integers(1, 40, 6), np.ones(6, int), 16, 8, True)
@@ -542,6 +575,15 @@ def test_attention_python_refusals(rng, device):
     for bad in ((dint([0], device), pl), (gs.long(), pl), (gs, pl.cpu())):
         with pytest.raises(EmberError):
             K.shared_prefix_attention(*good, *bad)
+
+
+def test_window_sizes_beyond_32_bits_are_refused(rng, device):
+    b, _ = window_batch(rng, device, [40], [1], 4, 2, True, 30, 0)
+    for window, sinks in ((2 ** 32 + 5, 0), (2 ** 31, 0), (5, 2 ** 32 + 1), (0, 0), (5, -1)):
+        with pytest.raises(EmberError):
+            K.window_attention(*b.args(), window=window, sinks=sinks)
+        with pytest.raises(EmberError):
+            K.window_workspace(1, 1, n_heads=4, n_kv=2, window=window, sinks=sinks, device=device)
 
 
 def test_empty_batches(rng, device):
