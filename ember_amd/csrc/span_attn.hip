@@ -893,6 +893,7 @@ struct Launch {
     Phase first{}, second{};  // second.units == 0: none
     bool tiled = false;       // the first phase is tiles
     int slots = 1, most_slots = 1;  // slots, and those that the workspace is sized for
+    int pages = 0;                  // of a window's row tile, at most
 };
 
 int64_t groups_of(const Phase &ph, int n_kv) { return static_cast<int64_t>(ph.units) * ph.tiles * ph.splits * n_kv; }
@@ -946,6 +947,7 @@ Launch plan_window(const EmberWindowAttnArgs &a, int spread) {
     const int64_t tokens = std::min<int64_t>(most, ((l.tiled ? kTileRows : kWalkRows) + G - 1) / G + 1);
     const int64_t near = (std::min<int64_t>(a.window, static_cast<int64_t>(b.max_blocks) * kPage) + tokens + kPage - 1) / kPage + 1;
     const int pages = static_cast<int>(std::min<int64_t>(b.max_blocks, near + (static_cast<int64_t>(a.sinks) + kPage - 1) / kPage));
+    l.pages = pages;
     const int64_t items = static_cast<int64_t>(b.S) * l.first.tiles * b.n_kv;
     const int pages_a_step = l.tiled ? 2 * kBlockPages : f16_pages ? 16 : 8;
     l.most_slots = static_cast<int>(std::clamp<int64_t>((kCus >> spread) / items, 1, (pages + pages_a_step - 1) / pages_a_step));
@@ -1094,7 +1096,14 @@ int fit(const char *who, const EmberRaggedBatch &b, Plan plan, Launch &l) {
 
 }  // namespace
 
-int64_t window_workspace_bytes(const EmberWindowAttnArgs &a) { return partial_bytes(a.batch, plan_window(a, 0).most_slots); }
+// A window's workspace holds the partials of these sizes and of smaller batches, which split more: fewer work-groups than
+// CUs, so at most kCus tiles of rows in all.
+int64_t window_workspace_bytes(const EmberWindowAttnArgs &a) {
+    const Launch l = plan_window(a, 0);
+    const int64_t slots = std::clamp<int64_t>(kCus / a.batch.n_kv, 1, (l.pages + kTileUnit - 1) / kTileUnit);
+    const int64_t rows = slots > 1 ? std::min<int64_t>(static_cast<int64_t>(a.batch.T) * a.batch.n_heads * slots, kCus * kTileRows) : 0;
+    return std::max(partial_bytes(a.batch, l.most_slots), rows * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float)));
+}
 int64_t shared_prefix_workspace_bytes(const EmberPrefixAttnArgs &a) { return partial_bytes(a.batch, plan_prefix(a, 0).most_slots); }
 
 int launch_window_attn(const EmberWindowAttnArgs &a, hipStream_t stream) {

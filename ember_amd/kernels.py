@@ -552,7 +552,8 @@ def _check_window(window: int, sinks: int) -> None:
 
 def window_workspace(T: int, S: int, *, n_heads, n_kv, window, sinks=0, max_query=None, dtype=torch.float16,
                      max_blocks=None, device="cuda"):
-    """A workspace for window_attention of batches of these sizes, or None when such a call splits no keys."""
+    """A workspace for window_attention of batches of these sizes and smaller ones, or None when no such call splits
+    its keys."""
     _check_window(window, sinks)
     a = _lib.WindowAttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks), window, sinks)
     return _workspace(int(_lib.lib().ember_hip_window_workspace_bytes(a)), device)

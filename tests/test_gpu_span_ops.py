@@ -550,6 +550,18 @@ def test_small_workspaces(rng, device):
     w.check(sees)
 
 
+def test_window_workspace_of_a_large_batch_splits_small_ones_as_their_own_does(rng, device):
+    b, sees = window_batch(rng, device, [4000], [1], 16, 8, True, 3900, 4, pad_rows=0)
+    outs = []
+    for S in (1, 64):
+        ws = K.window_workspace(S, S, n_heads=16, n_kv=8, window=3900, sinks=4, max_query=1, device=device)
+        b.out.fill_(123.0)
+        K.window_attention(*b.args(), window=3900, sinks=4, max_query=1, workspace=ws)
+        b.check(sees)
+        outs.append(b.out.clone())
+    assert torch.equal(*outs)
+
+
 def test_attention_python_refusals(rng, device):
     b, _ = window_batch(rng, device, [10, 20], [1, 1], 4, 2, True, 8, 0)
     good = b.args()

@@ -123,3 +123,20 @@ def test_workspace_covers_smaller_tables():
                     assert size(a) <= most
     assert K.window_workspace(4, 4, n_heads=16, n_kv=8, window=100000, max_query=1, device="cpu") is not None
     assert K.window_workspace(1, 1, n_heads=16, n_kv=8, window=10, max_query=1, device="cpu") is None
+
+
+def test_a_window_workspace_covers_smaller_batches():
+    """Fewer sequences split more: what one of them needs alone, a larger batch's workspace holds."""
+    size = _lib.lib().ember_hip_window_workspace_bytes
+
+    def bytes_for(S, q, **kw):
+        a = _window()
+        a.window, a.S, a.T, a.max_query, a.max_blocks = 4096, S, S * q, q, 1 << 26
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return size(a)
+    for kw in (dict(), dict(dtype=_lib.DTYPE_F32), dict(n_heads=8, n_kv=1, q_stride=1024)):
+        for q in (1, 4, 300):
+            sizes = [bytes_for(S, q, **kw) for S in (1, 2, 5, 16, 33, 100, 400)]
+            assert sizes == sorted(sizes) and sizes[0] > 0
+            assert bytes_for(7, 1, **kw) <= bytes_for(7, q, **kw)
