@@ -141,8 +141,10 @@ struct Span {
 
 __device__ __forceinline__ Span span_of(const Rows &r, int window, int sinks, int min_pos, int max_top) {
     Span s;
+    // A window that starts behind the last key has none: it starts there at most (the end of a page, if there are first
+    // tokens), so that no page number is further than the table's end and a tile's blocks behind it.
     s.lo = max(r.base, window == kNoWindow ? 0 : min_pos - window + 1);
-    s.lo = max(s.lo, 0);
+    s.lo = min(max(s.lo, 0), max_top + 1);
     const int first = s.lo / kPage;
     s.head = min((max(min(sinks, max_top + 1), 0) + kPage - 1) / kPage, first);
     s.skip = first - s.head;
