@@ -47,7 +47,7 @@ constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kBlockPages = 4;             // pages of a tile's key block
 constexpr int kBlockKeys = kBlockPages * kPage;
 static_assert(kBlockPages == kTileWaves);  // a wave loads one of them
-constexpr int kNoWindow = INT_MAX;
+constexpr uint32_t kNoWindow = 1u << 31;  // past any distance of two positions
 
 enum Kind : int { kWindowRows, kPrefixRows, kOwnRows };
 
@@ -64,7 +64,8 @@ struct SpanParams {
     const int32_t *query_start, *positions, *tables, *group_start, *prefix_len;
     float *part_acc, *part_ml;  // [T, n_heads, slots][128], [T, n_heads, slots][2]
     int64_t q_stride;
-    int T, S, max_blocks, n_heads, n_kv, G, num_blocks, n_groups, window, sinks, slots;
+    int T, S, max_blocks, n_heads, n_kv, G, num_blocks, n_groups, sinks, slots;
+    uint32_t window;
     float scale_log2;
 };
 
@@ -139,12 +140,16 @@ struct Span {
     __device__ __forceinline__ int page(int v) const { return v < head ? v : v + skip; }
 };
 
-__device__ __forceinline__ Span span_of(const Rows &r, int window, int sinks, int min_pos, int max_top) {
+// The first key that a window reaches from a position.
+__device__ __forceinline__ int window_start(int pos, uint32_t window) {
+    return window == kNoWindow ? 0 : pos - static_cast<int>(window) + 1;
+}
+
+__device__ __forceinline__ Span span_of(const Rows &r, uint32_t window, int sinks, int min_pos, int max_top) {
     Span s;
     // A window that starts behind the last key has none: it starts there at most (the end of a page, if there are first
     // tokens), so that no page number is further than the table's end and a tile's blocks behind it.
-    s.lo = max(r.base, window == kNoWindow ? 0 : min_pos - window + 1);
-    s.lo = min(max(s.lo, 0), max_top + 1);
+    s.lo = min(max(max(r.base, window_start(min_pos, window)), 0), max_top + 1);
     const int first = s.lo / kPage;
     s.head = min((max(min(sinks, max_top + 1), 0) + kPage - 1) / kPage, first);
     s.skip = first - s.head;
@@ -153,13 +158,13 @@ __device__ __forceinline__ Span span_of(const Rows &r, int window, int sinks, in
 }
 
 // Whether every key of a page is visible to every row (positions min_pos .. max_pos, highest keys at least min_top).
-__device__ __forceinline__ bool whole_page(int page, const Rows &r, int window, int sinks, int max_pos, int min_top) {
+__device__ __forceinline__ bool whole_page(int page, const Rows &r, uint32_t window, int sinks, int max_pos, int min_top) {
     const int j0 = page * kPage;
-    return j0 >= r.base && j0 + kPage - 1 <= min_top && (max_pos - j0 < window || j0 + kPage <= sinks);
+    return j0 >= r.base && j0 + kPage - 1 <= min_top && (static_cast<uint32_t>(max_pos - j0) < window || j0 + kPage <= sinks);
 }
 
-__device__ __forceinline__ bool visible(int j, int base, int top, int pos, int window, int sinks) {
-    return j >= base && j <= top && (pos - j < window || j < sinks);
+__device__ __forceinline__ bool visible(int j, int base, int top, int pos, uint32_t window, int sinks) {
+    return j >= base && j <= top && (static_cast<uint32_t>(pos - j) < window || j < sinks);
 }
 
 // ---- few rows: a page per wave ----
@@ -214,7 +219,8 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
     const int32_t *const table = p.tables + static_cast<int64_t>(r.seq) * p.max_blocks;
     const int64_t head_off = static_cast<int64_t>(kvh) * (kPage * D), block_stride = static_cast<int64_t>(p.n_kv) * (kPage * D);
     const T *const kbase = static_cast<const T *>(p.k) + head_off, *const vbase = static_cast<const T *>(p.v) + head_off;
-    const int window = ph.kind == kWindowRows ? p.window : kNoWindow, sinks = ph.kind == kWindowRows ? p.sinks : 0;
+    const uint32_t window = ph.kind == kWindowRows ? p.window : kNoWindow;
+    const int sinks = ph.kind == kWindowRows ? p.sinks : 0;
     const int table_top = p.max_blocks * kPage - 1;
     const bool partial = p.slots > 1;
     // Without a window the pages start at the base: their ids are requested before the positions are known.
@@ -565,7 +571,8 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
     const int32_t *const table = p.tables + static_cast<int64_t>(r.seq) * p.max_blocks;
     const int64_t head_off = static_cast<int64_t>(kvh) * (kPage * D), block_stride = static_cast<int64_t>(p.n_kv) * (kPage * D);
     const f16 *const kbase = static_cast<const f16 *>(p.k) + head_off, *const vbase = static_cast<const f16 *>(p.v) + head_off;
-    const int window = ph.kind == kWindowRows ? p.window : kNoWindow, sinks = ph.kind == kWindowRows ? p.sinks : 0;
+    const uint32_t window = ph.kind == kWindowRows ? p.window : kNoWindow;
+    const int sinks = ph.kind == kWindowRows ? p.sinks : 0;
 
     for (int row0 = tile0 * kTileRows; row0 < r.rows; row0 += ph.tiles * kTileRows) {
         const int my_row = min(row0 + 32 * wave + c, r.rows - 1);  // rows past the last repeat it
@@ -610,11 +617,11 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
             for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
 
         // Keys that this lane's row sees: n from `from` on, and those below `sink_end`.
-        const int from = max(r.base, window == kNoWindow ? 0 : max(my_pos - window + 1, 0));
+        const int from = max(r.base, max(window_start(my_pos, window), 0));
         const uint32_t n_from = max(my_top - from + 1, 0);
         const int sink_end = min(sinks, my_top + 1);
         // Virtual pages whole0 .. whole1 - 1: every row of the wave sees every key of them.
-        const int whole_key = max(r.base, window == kNoWindow ? 0 : hi_pos - window + 1);
+        const int whole_key = max(r.base, window_start(hi_pos, window));
         const int whole0 = static_cast<int>((static_cast<uint32_t>(max(whole_key, 0)) + kPage - 1) / kPage) - sp.skip;
         const int whole1 = (lo_top + 1) / kPage - sp.skip;
         // Keys that some row of the tile sees, likewise. Others may hold anything: their values are read as zeros
@@ -1112,7 +1119,7 @@ int launch_window_attn(const EmberWindowAttnArgs &a, hipStream_t stream) {
     Launch l;
     if (int e = fit("window_attn", a.batch, [&](int spread) { return plan_window(a, spread); }, l)) return e;
     SpanParams p = params_of(a.batch, l.slots);
-    p.window = a.window, p.sinks = a.sinks;
+    p.window = static_cast<uint32_t>(a.window), p.sinks = a.sinks;
     return hip_status(a.batch.dtype == EMBER_DTYPE_F16 ? run<f16>(p, l, stream) : run<float>(p, l, stream), "window_attn");
 }
 

@@ -70,3 +70,34 @@ def test_window_page_ids_outside_the_pool_in_both_forms(rng, device, n, tiles):
     assert tile_form(b, n) == tiles
     K.window_attention(*b.args(), window=200, max_query=n)
     b.check(sees)
+
+
+@FORMS
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+def test_window_of_every_position_but_the_first(rng, device, n, tiles, f16):
+    """Window 2^31 - 1: only a token at position 2^31 - 1 is too far from key 0."""
+    b, _ = window_batch(rng, device, [100] * 2, [n] * 2, H, KV, f16, 200, 0, pad_rows=0)
+    with_any_pages(b, rng, device)
+    b.tables[:, 1:] = -1  # key 0's page is what shows
+    b.dev["table"] = dint(b.tables, device)
+    at_positions(b, device, [2 ** 31 - n, 2 ** 31 - 1 - n], n)
+    assert tile_form(b, n) == (tiles and f16)
+    K.window_attention(*b.args(), window=2 ** 31 - 1, max_query=n)
+    b.check(lambda s, p, j: p - j < 2 ** 31 - 1)
+
+
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("n", [1, 12])
+def test_prefix_calls_at_the_last_position_see_the_whole_table(rng, device, f16, n):
+    """Causal rows have no window: a token at position 2^31 - 1 sees key 0, in a group and in none."""
+    b, _ = window_batch(rng, device, [100] * 3, [n] * 3, H, KV, f16, 200, 0, pad_rows=0)
+    with_any_pages(b, rng, device)
+    b.tables[1, :1] = b.tables[0, :1]
+    b.dev["table"] = dint(b.tables, device)
+    at_positions(b, device, [2 ** 31 - n] * 3, n)
+    for group in ([0, 2], [0, 1]):  # sequences 2, and 1 and 2, are in none
+        hints = dict(max_query=n, max_group=2 * n)
+        ws = K.shared_prefix_workspace(3 * n, 3, 1, n_heads=H, n_kv=KV, dtype=b.out.dtype, device=device, **hints)
+        b.out.fill_(123.0)
+        K.shared_prefix_attention(*b.args(), dint(group, device), dint([16], device), workspace=ws, **hints)
+        b.check(lambda s, p, j: j <= p)
