@@ -30,6 +30,7 @@
 //   mixed  64 decodes behind 8000 shared tokens               52 us, and 5.4 us the merge
 //          256 decodes in 16 groups                          108 us (4.7 TB/s), and 5.6 us the merge
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 
 #include "capi_errors.hpp"
@@ -70,6 +71,15 @@ struct SpanParams {
 };
 
 __device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
+
+// The running max of a row before any visible key: finite, so that a difference of two is a number, and below any score.
+constexpr float kNoKeys = -FLT_MAX;
+
+// The exponent of a weight is one fused s * scale - max, the max rounded: what the rounding leaves of the top score,
+// half an ulp at most, moves all weights of the row alike and cancels. From 2^22 on it is not small beside f16's or f32's
+// exponents: there s * scale is rounded first, as the max was, and the top weight is 1 at any size.
+// (each row by itself: its bits do not depend on the other rows of its wave)
+constexpr float kFar = 4194304.0f;
 
 // Whether a sum of weights holds anything: also when it is NaN (of a NaN in q, say), which a comparison would take for
 // an empty row's 0 and so turn the row into zeros.
@@ -262,14 +272,14 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
             if (tid < nrows) {
                 const int64_t at = static_cast<int64_t>(r.t0 + (row0 + tid) / p.G) * p.n_heads + kvh * p.G + (row0 + tid) % p.G;
                 float2 *const ml = reinterpret_cast<float2 *>(p.part_ml) + at * p.slots;
-                ml[ph.slot0 + split] = make_float2(kNoMax, 0.0f);
+                ml[ph.slot0 + split] = make_float2(kNoKeys, 0.0f);
                 if (!grouped && split == 0)
-                    for (int i = 0; i < ph.slot0; i++) ml[i] = make_float2(kNoMax, 0.0f);
+                    for (int i = 0; i < ph.slot0; i++) ml[i] = make_float2(kNoKeys, 0.0f);
             }
             continue;
         }
 
-        float mc = kNoMax, lc = 0.0f;
+        float mc = kNoKeys, lc = 0.0f;
         f32x4 o[8];  // o[t][v]: dim 32 g + 8 v + t of column c
 #pragma unroll
         for (int t = 0; t < 8; t++) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -369,9 +379,15 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 const float mn = fmaxf(mc, groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * p.scale_log2);
                 const float corr = exp2_hw(mc - mn);
                 mc = mn;
+                float mul = p.scale_log2, add = -mn;
+                if (const bool far = fabsf(mn) >= kFar; __builtin_amdgcn_ballot_w64(far)) {
+#pragma unroll
+                    for (int v = 0; v < 4; v++) s[v] = far ? s[v] * mul + add : __builtin_fmaf(s[v], mul, add);
+                    mul = 1.0f, add = 0.0f;
+                }
                 float w[4];
 #pragma unroll
-                for (int v = 0; v < 4; v++) w[v] = exp2_hw(__builtin_fmaf(s[v], p.scale_log2, -mn));
+                for (int v = 0; v < 4; v++) w[v] = exp2_hw(__builtin_fmaf(s[v], mul, add));
                 // f16: the weights are rounded to f16, the products' operand, and summed as rounded, so that the
                 // rounding of a weight (2^-11 of it at most) moves numerator and denominator alike.
                 f16x4 wh;
@@ -473,7 +489,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
         __syncthreads();
         for (int i = tid; i < nrows * (D / 2); i += kThreads) {
             const int row = i / (D / 2), d = 2 * (i % (D / 2));
-            float M = kNoMax, L = 0.0f;
+            float M = kNoKeys, L = 0.0f;
 #pragma unroll 4
             for (int w = 0; w < W; w++) M = fmaxf(M, red_m[row * W + w]);
             float2 O = make_float2(0.0f, 0.0f);
@@ -493,7 +509,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 if (d == 0) {
                     ml[slot] = make_float2(M, L);
                     if (!grouped && split == 0)  // a row of no group: its prefix slots hold nothing
-                        for (int k = 0; k < ph.slot0; k++) ml[at * p.slots + k] = make_float2(kNoMax, 0.0f);
+                        for (int k = 0; k < ph.slot0; k++) ml[at * p.slots + k] = make_float2(kNoKeys, 0.0f);
                 }
             } else {
                 T *const dst = static_cast<T *>(p.out) + at * D + d;
@@ -738,24 +754,31 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
 #pragma unroll
             for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
             top = top * p.scale_log2;
-            if (__builtin_amdgcn_ballot_w64(top > m + kLazy)) {
+            if (__builtin_amdgcn_ballot_w64(top - m > kLazy)) {
                 const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 const float row_top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-                const bool grow = row_top > m + kLazy;
+                const bool grow = row_top - m > kLazy;
                 const float corr = grow ? exp2_hw(m - row_top) : 1.0f;  // 0 from a row that had seen nothing
                 m = grow ? row_top : m;
                 l = l * corr;
 #pragma unroll
                 for (int t = 0; t < 4; t++) o[t] = o[t] * corr;
             }
-            const float neg = m == -INFINITY ? 0.0f : -m;
+            float mul = p.scale_log2, neg = m == -INFINITY ? 0.0f : -m;
+            if (const bool far = fabsf(neg) >= kFar; __builtin_amdgcn_ballot_w64(far)) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[t][i] = far ? s[t][i] * mul + neg : __builtin_fmaf(s[t][i], mul, neg);
+                mul = 1.0f, neg = 0.0f;
+            }
             const f16x2 ones = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
             f16x8 w[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
-                    w[j][i] = static_cast<f16>(exp2_hw(__builtin_fmaf(s[j / 2][8 * (j % 2) + i], p.scale_log2, neg)));
+                    w[j][i] = static_cast<f16>(exp2_hw(__builtin_fmaf(s[j / 2][8 * (j % 2) + i], mul, neg)));
 #pragma unroll
                 for (int i = 0; i < 4; i++) l = __builtin_amdgcn_fdot2(f16x2{w[j][2 * i], w[j][2 * i + 1]}, ones, l, false);
             }
@@ -807,7 +830,7 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
                         *reinterpret_cast<float4 *>(dst + 8 * i) = make_float4(o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1],
                                                                                o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]);
                 }
-                if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + slot * 2) = make_float2(filled(l) ? m : kNoMax, l);
+                if (h == 0) *reinterpret_cast<float2 *>(p.part_ml + slot * 2) = make_float2(filled(l) ? m : kNoKeys, l);
             } else {
                 f16 *const dst = static_cast<f16 *>(p.out) + at * D + 4 * h;
                 const float inv = filled(l) ? 1.0f / l : 0.0f;
@@ -858,9 +881,9 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
     if (tok < clamped(first, p.T) || tok >= clamped(last, p.T)) return;
     const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + at * p.slots;
     const float *const acc = p.part_acc + at * p.slots * D + 2 * lane;
-    float M = kNoMax, L = 0.0f, x = 0.0f, y = 0.0f;
+    float M = kNoKeys, L = 0.0f, x = 0.0f, y = 0.0f;
     for (int s0 = 0; s0 < p.slots; s0 += kWave) {  // a lane holds a slot's (max, sum)
-        const float2 mine = s0 + lane < p.slots ? ml[s0 + lane] : make_float2(kNoMax, 0.0f);
+        const float2 mine = s0 + lane < p.slots ? ml[s0 + lane] : make_float2(kNoKeys, 0.0f);
         float top = mine.x;
 #pragma unroll
         for (int o = 1; o < kWave; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));

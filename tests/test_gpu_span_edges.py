@@ -1,11 +1,12 @@
-"""The span attentions at their edges: positions and windows at the ends of 32 bits, in the walk and in the tile form."""
+"""The span attentions at their edges: positions and windows at the ends of 32 bits, and scores of any size,
+in the walk and in the tile form."""
 import numpy as np
 import pytest
 import torch
 
 from ember_amd import kernels as K
-from span_reference import PAGE
-from test_gpu_span_ops import dint, window_batch
+from span_reference import D, PAGE
+from test_gpu_span_ops import dint, prefix_batch, prefix_ws, window_batch
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +102,65 @@ def test_prefix_calls_at_the_last_position_see_the_whole_table(rng, device, f16,
         b.out.fill_(123.0)
         K.shared_prefix_attention(*b.args(), dint(group, device), dint([16], device), workspace=ws, **hints)
         b.check(lambda s, p, j: j <= p)
+
+
+def largest_score_takes_all(b, sees):
+    """Scores so large that the top one's weight is 1 (their gaps exceed what f32 sums lose): its value is the output.
+    The only rounding is that of weights and sums, each exact here, and of the output: half a step."""
+    torch.cuda.synchronize()
+    got = b.out.double().cpu().numpy()
+    group = b.q.shape[1] // b.k.shape[1]
+    for s in range(len(b.start) - 1):
+        for t in range(b.start[s], b.start[s + 1]):
+            j = np.arange(b.pos[t] + 1)
+            j = j[sees(s, b.pos[t], j)]
+            for h in range(b.q.shape[1]):
+                k, v = (x[b.tables[s, j // PAGE], h // group, j % PAGE].astype(np.float64) for x in (b.k, b.v))
+                e = k @ b.q[t, h].astype(np.float64)
+                lost = 130 * 2.0 ** -24 * (np.abs(k) @ np.abs(b.q[t, h].astype(np.float64))).max()
+                top = np.sort(e)[::-1]
+                if len(e) > 1 and (top[0] - top[1]) * D ** -0.5 < 200 + 2 * lost:
+                    continue  # too near a tie for f32
+                want = v[e.argmax()]
+                step = 2.0 ** -11 if b.f16 else 2.0 ** -21
+                assert (np.abs(got[t, h] - want) <= step * np.abs(want)).all(), (t, h, got[t, h][:4], want[:4])
+
+
+def large(b, device, size, rng):
+    """q and keys of this size, random signs and mantissas."""
+    for name, x in (("q", b.q), ("k", b.k)):
+        x[...] = (size * rng.uniform(0.3, 1, x.shape) * rng.choice([-1, 1], x.shape)).astype(x.dtype)
+        b.dev[name] = torch.from_numpy(x).to(device)
+
+
+@pytest.mark.parametrize("f16,size", [(True, 3e4), (True, 500.0), (False, 1e5), (False, 3e17)])
+@pytest.mark.parametrize("n", [1, 6, 12, 70])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (50, 0), (400, 3)])
+def test_window_scores_of_any_size(rng, device, f16, size, n, window, sinks):
+    """Scores of 1e4 to 1e36, positive and negative: weights and sums stay finite, and no row turns into zeros."""
+    b, sees = window_batch(rng, device, [0, 300, 40], [n] * 3, H, KV, f16, 10 ** 6, 0)
+    large(b, device, size, rng)
+    for ws in (None, K.window_workspace(b.q.shape[0], 3, n_heads=H, n_kv=KV, window=window, sinks=sinks, max_query=n,
+                                        dtype=b.out.dtype, device=device)):
+        b.out.fill_(123.0)
+        K.window_attention(*b.args(), window=window, sinks=sinks, max_query=n, workspace=ws)
+        largest_score_takes_all(b, lambda s, p, j: (j <= p) & ((p - j < window) | (j < sinks)))
+
+
+@pytest.mark.parametrize("f16,size", [(True, 3e4), (False, 1e5), (False, 3e17)])
+@pytest.mark.parametrize("groups,prefix", [([3, 1], [37, 1]), ([12], [333])])
+def test_prefix_scores_of_any_size(rng, device, f16, size, groups, prefix):
+    """The same before and behind a shared prefix, whose partials are merged."""
+    S = sum(groups)
+    b = prefix_batch(rng, device, groups, prefix, rng.integers(1, 90, S), np.ones(S, int), H, KV, f16)
+    first = np.concatenate([[0], np.cumsum(groups)])
+    large(b, device, size, rng)
+    for g, n in enumerate(prefix):  # a partly shared page's copies hold the same keys again
+        for s in range(first[g] + 1, first[g + 1]):
+            if n % PAGE:
+                a, c = b.tables[first[g], n // PAGE], b.tables[s, n // PAGE]
+                b.k[c, :, :n % PAGE] = b.k[a, :, :n % PAGE]
+    b.dev["k"] = torch.from_numpy(b.k).to(device)
+    hints = dict(max_query=1, max_group=max(groups), max_prefix=max(prefix), max_own=90)
+    K.shared_prefix_attention(*b.args(), b.group_start, b.prefix, workspace=prefix_ws(b, H, KV, device, **hints), **hints)
+    largest_score_takes_all(b, lambda s, p, j: j <= p)
