@@ -81,6 +81,12 @@ constexpr float kNoKeys = -FLT_MAX;
 // (each row by itself: its bits do not depend on the other rows of its wave)
 constexpr float kFar = 4194304.0f;
 
+// f16 weights are 2^(score - reference), the reference up to 15 below the max (65504 is f16's end): a long tail of weights
+// that f16 could not hold beside a largest weight of 1 counts. Sums and outputs are in the same units, so nothing else
+// changes. A far max takes no such step, which its rounding would swallow.
+constexpr float kMostExponent = 15.0f;
+__device__ __forceinline__ float below(float top, float step) { return fabsf(top) < kFar ? top - step : top; }
+
 // Whether a sum of weights holds anything: also when it is NaN (of a NaN in q, say), which a comparison would take for
 // an empty row's 0 and so turn the row into zeros.
 __device__ __forceinline__ bool filled(float l) { return __float_as_uint(l) != 0; }
@@ -376,7 +382,8 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 }
                 // Online softmax in base 2, the scale in the exponent. mc starts finite, so a row that has seen
                 // nothing yet keeps weight sums of 0 and corrections of 1.
-                const float mn = fmaxf(mc, groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * p.scale_log2);
+                const float top = groups_max(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))) * p.scale_log2;
+                const float mn = fmaxf(mc, F16 ? below(top, kMostExponent) : top);
                 const float corr = exp2_hw(mc - mn);
                 mc = mn;
                 float mul = p.scale_log2, add = -mn;
@@ -389,7 +396,8 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
 #pragma unroll
                 for (int v = 0; v < 4; v++) w[v] = exp2_hw(__builtin_fmaf(s[v], mul, add));
                 // f16: the weights are rounded to f16, the products' operand, and summed as rounded, so that the
-                // rounding of a weight (2^-11 of it at most) moves numerator and denominator alike.
+                // rounding of a weight moves numerator and denominator alike: 2^-11 of it at most down to 2^-29 of
+                // the largest, 2^-40 of the largest below.
                 f16x4 wh;
                 if constexpr (F16) {
 #pragma unroll
@@ -546,10 +554,10 @@ constexpr int kKeyRow = kHeadDim + 8, kValueRow = kHeadDim + 32;
 typedef __fp16 tr16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
 
-// How far (base 2) a score may pass the reference max before the reference moves: weights stay below 2^8, which
-// f16 holds, and most blocks rescale nothing.
-// The weights are rounded to f16, the products' operand (2^-11 of each at most), and summed as rounded, so numerator
-// and denominator move alike.
+// How far (base 2) a row's max may grow before the reference moves, so that most blocks rescale nothing: it is set
+// kMostExponent - kLazy below the max, and weights stay below 2^kMostExponent.
+// The weights are rounded to f16, the products' operand, and summed as rounded, so numerator and denominator move alike:
+// 2^-11 of each at most down to 2^-21 of the largest, 2^-32 of the largest below.
 constexpr float kLazy = 8.0f;
 constexpr int kAhead = 4;  // value operands in flight ahead of their products
 
@@ -754,12 +762,13 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
 #pragma unroll
             for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
             top = top * p.scale_log2;
-            if (__builtin_amdgcn_ballot_w64(top - m > kLazy)) {
+            if (__builtin_amdgcn_ballot_w64(top - m > kMostExponent)) {
                 const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
                 const float row_top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
-                const bool grow = row_top - m > kLazy;
-                const float corr = grow ? exp2_hw(m - row_top) : 1.0f;  // 0 from a row that had seen nothing
-                m = grow ? row_top : m;
+                const bool grow = row_top - m > kMostExponent;
+                const float reference = below(row_top, kMostExponent - kLazy);
+                const float corr = grow ? exp2_hw(m - reference) : 1.0f;  // 0 from a row that had seen nothing
+                m = grow ? reference : m;
                 l = l * corr;
 #pragma unroll
                 for (int t = 0; t < 4; t++) o[t] = o[t] * corr;

@@ -1,5 +1,7 @@
-"""The span attentions at their edges: positions and windows at the ends of 32 bits, and scores of any size,
-in the walk and in the tile form."""
+"""The span attentions at their edges: positions and windows at the ends of 32 bits, scores of any size,
+and long tails of small weights, in the walk and in the tile form."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -164,3 +166,48 @@ def test_prefix_scores_of_any_size(rng, device, f16, size, groups, prefix):
     hints = dict(max_query=1, max_group=max(groups), max_prefix=max(prefix), max_own=90)
     K.shared_prefix_attention(*b.args(), b.group_start, b.prefix, workspace=prefix_ws(b, H, KV, device, **hints), **hints)
     largest_score_takes_all(b, lambda s, p, j: j <= p)
+
+
+def tail_batch(rng, device, n, keys, depth):
+    """n tokens of one sequence behind `keys` keys: key 0 has score 0 and value 0, all others score -depth (base 2, with
+    scale ln 2) and value 1: the output is x / (1 + x), x = (keys seen - 1) 2^-depth."""
+    b, _ = window_batch(rng, device, [keys], [n], H, KV, True, 10 ** 6, 0)
+    b.q[...], b.k[...], b.v[...] = 0, 0, 1
+    b.q[..., 0], b.k[..., 0] = 1, -depth
+    b.k[b.tables[0, 0], :, 0, 0], b.v[b.tables[0, 0], :, 0] = 0, 0
+    for name in "qkv":
+        b.dev[name] = torch.from_numpy(getattr(b, name)).to(device)
+    return b
+
+
+def check_tail(b, depth):
+    """A weight is rounded by 2^-11 of itself, or by 2^-32 of the largest where f16 ends; exponents (error 2^-22 of
+    depth + 2^7, in f32) and sums of up to 2^14 terms in f32 (2^-10 of x at the very most); the output by half a step."""
+    torch.cuda.synchronize()
+    got = b.out[:b.T].double().cpu().numpy()
+    seen = b.pos.astype(np.float64)  # keys 1 .. position
+    x = seen * 2.0 ** -depth
+    want = (x / (1 + x))[:, None, None]
+    tol = want * (2.0 ** -11 + 2.0 ** -11 + (depth + 128) * 2.0 ** -22 + 2.0 ** -10) + seen[:, None, None] * 2.0 ** -32 + 2.0 ** -25
+    assert (np.abs(got - want) <= tol).all(), (got.min(), got.max(), want.min())
+
+
+@pytest.mark.parametrize("n", [1, 6, 12, 70])
+@pytest.mark.parametrize("depth", [10, 17, 23, 25, 26])
+def test_window_long_tails_of_small_weights_count(rng, device, n, depth):
+    """8000 keys of 2^-23 to 2^-26 of the largest weight: less than f16 holds of 1, and up to a thousandth of the row."""
+    b = tail_batch(rng, device, n, 8000, depth)
+    for ws in (None, K.window_workspace(b.q.shape[0], 1, n_heads=H, n_kv=KV, window=10 ** 6, max_query=n, device=device)):
+        b.out.fill_(123.0)
+        K.window_attention(*b.args(), window=10 ** 6, max_query=n, scale=math.log(2.0), workspace=ws)
+        check_tail(b, depth)
+
+
+@pytest.mark.parametrize("n", [1, 12])
+@pytest.mark.parametrize("prefix", [16, 6016])
+def test_prefix_long_tails_of_small_weights_count(rng, device, n, prefix):
+    b = tail_batch(rng, device, n, 8000, 25)
+    hints = dict(max_query=n, max_group=n, max_prefix=prefix, max_own=8100 - prefix)
+    ws = K.shared_prefix_workspace(b.q.shape[0], 1, 1, n_heads=H, n_kv=KV, device=device, **hints)
+    K.shared_prefix_attention(*b.args(), dint([0, 1], device), dint([prefix], device), scale=math.log(2.0), workspace=ws, **hints)
+    check_tail(b, 25)
