@@ -881,10 +881,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) span_mixed_kernel(SpanParams 
 constexpr int kMergeWaves = 4;
 
 template <typename T>
-__global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanParams p) {
+__global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanParams p, int64_t first_row) {
     constexpr int D = kHeadDim, C = 8;  // slots whose partials are requested together
     const int lane = static_cast<int>(threadIdx.x) % kWave;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kMergeWaves + uniform(static_cast<int>(threadIdx.x) / kWave);
+    const int64_t at = first_row + static_cast<int64_t>(blockIdx.x) * kMergeWaves + uniform(static_cast<int>(threadIdx.x) / kWave);
     const int64_t tok = at / p.n_heads;
     const int first = uniform_load(p.query_start), last = uniform_load(p.query_start + p.S);
     if (tok < clamped(first, p.T) || tok >= clamped(last, p.T)) return;
@@ -945,8 +945,18 @@ int64_t partial_bytes(const EmberRaggedBatch &b, int slots) {
 
 int tiles_for(int64_t tokens, int G, int rows) { return static_cast<int>(std::max<int64_t>(1, (tokens * G + rows - 1) / rows)); }
 
-Phase rows_phase(int kind, int units, int64_t tokens, int G, bool tiled, int slot0) {
-    return Phase{kind, units, tiles_for(tokens, G, tiled ? kTileRows : kWalkRows), 1, 1, slot0};
+// `tokens` of every unit are the caller's longest run, or all of the step's: with many units most of the work-groups would
+// find no rows, at about 1 us for 300 of them. Beyond kMostGroups a unit's row tiles share its work-groups, which also
+// keeps a launch within HIP's 2^32 threads for any number of tokens. The share is odd: with an even one, 1000
+// decodes take 2 to 3 times as long, as if the few work-groups that have rows went to the same part of each XCD. Measured, us, at most
+// 2^15, 2^16, 2^17 work-groups and without a bound: 1000 decodes without max_query, window 1724, 1748, 1763 and 4870, shared
+// prefix 232, 275, 384 and 2012; 40 chunks of 512 tokens among 1000 sequences, shared prefix 1668, 1396, 1283 and 2124.
+constexpr int64_t kMostGroups = 1 << 16;
+constexpr int64_t kMostLaunch = UINT32_MAX / kTileThreads;  // work-groups of the launches that can be large: 256 threads
+
+Phase rows_phase(int kind, int units, int64_t tokens, int G, int n_kv, bool tiled, int slot0) {
+    const int64_t shared = (std::max<int64_t>(1, kMostGroups / (static_cast<int64_t>(units) * n_kv)) - 1) | 1;
+    return Phase{kind, units, static_cast<int>(std::min<int64_t>(tiles_for(tokens, G, tiled ? kTileRows : kWalkRows), shared)), 1, 1, slot0};
 }
 
 // `spread` halves the work-groups asked for, step by step, until the workspace holds the partials.
@@ -983,7 +993,7 @@ Launch plan_window(const EmberWindowAttnArgs &a, int spread) {
     const bool f16_pages = b.dtype == EMBER_DTYPE_F16;
     Launch l;
     l.tiled = f16_pages && most * G > kWalkRows;
-    l.first = rows_phase(kWindowRows, b.S, most, G, l.tiled, 0);
+    l.first = rows_phase(kWindowRows, b.S, most, G, b.n_kv, l.tiled, 0);
     // a tile's keys: the first tokens' pages, and the windows of its tokens
     const int64_t tokens = std::min<int64_t>(most, ((l.tiled ? kTileRows : kWalkRows) + G - 1) / G + 1);
     const int64_t near = (std::min<int64_t>(a.window, static_cast<int64_t>(b.max_blocks) * kPage) + tokens + kPage - 1) / kPage + 1;
@@ -1057,8 +1067,8 @@ Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     Launch l;
     l.tiled = a.n_groups > 0 && b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
     l.most_slots = 0;
-    if (a.n_groups > 0) l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, l.tiled, 0);
-    l.second = rows_phase(kOwnRows, b.S, in_seq, G, false, 0);
+    if (a.n_groups > 0) l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, b.n_kv, l.tiled, 0);
+    l.second = rows_phase(kOwnRows, b.S, in_seq, G, b.n_kv, false, 0);
     if (l.tiled) {
         cut_mixed(l, b, pages_of(a.max_prefix), pages_of(a.max_own), a.max_own / kPage < b.max_blocks, spread);
     } else {
@@ -1112,9 +1122,12 @@ hipError_t run(const SpanParams &p, const Launch &l, hipStream_t stream) {
     if (!done && !second && first <= 2 * kCus) launch_walk<T, 8>(p, l, first, second, stream);
     else if (!done) launch_walk<T, 4>(p, l, first, second, stream);
     if (l.slots > 1) {
+        constexpr int64_t most = int64_t{1} << 25;  // rows of one launch
+        static_assert(most % kMergeWaves == 0 && most * kWave <= UINT32_MAX);
         const int64_t rows = static_cast<int64_t>(p.T) * p.n_heads;
-        hipLaunchKernelGGL(span_merge_kernel<T>, dim3(static_cast<unsigned>((rows + kMergeWaves - 1) / kMergeWaves)),
-                           dim3(kMergeWaves * kWave), 0, stream, p);
+        for (int64_t first_row = 0; first_row < rows; first_row += most)
+            hipLaunchKernelGGL(span_merge_kernel<T>, dim3(static_cast<unsigned>((std::min(most, rows - first_row) + kMergeWaves - 1) / kMergeWaves)),
+                               dim3(kMergeWaves * kWave), 0, stream, p, first_row);
     }
     return hipGetLastError();
 }
@@ -1130,8 +1143,8 @@ int fit(const char *who, const EmberRaggedBatch &b, Plan plan, Launch &l) {
             return set_error(EMBER_ERR_INVALID, "%s: needs %lld bytes of workspace at least (got %lld)", who,
                              static_cast<long long>(partial_bytes(b, l.slots)), static_cast<long long>(room));
     }
-    if (groups_of(l.first, b.n_kv) + groups_of(l.second, b.n_kv) > INT_MAX)
-        return set_error(EMBER_ERR_INVALID, "%s: too many work-groups for one launch", who);
+    if (groups_of(l.first, b.n_kv) + groups_of(l.second, b.n_kv) > kMostLaunch)
+        return set_error(EMBER_ERR_INVALID, "%s: too many work-groups for one launch (S %d x n_kv %d)", who, b.S, b.n_kv);
     return EMBER_OK;
 }
 

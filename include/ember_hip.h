@@ -354,7 +354,9 @@ int ember_hip_token_probs(const EmberProbArgs *args, void *stream);
  * sequence's whole context. The tables of a step are made from the requests'
  * lengths on the device; both attentions take them as they are, with no host
  * plan: the sizes they ask for (max_query and the like) shape the launch, and
- * a step that exceeds them is computed all the same, only slower. */
+ * a step that exceeds them, or comes without them, is computed all the same,
+ * only slower. S * n_kv (and n_groups * n_kv) must leave a launch below 2^24
+ * work-groups of 256 threads; larger ones are refused. */
 
 #define EMBER_STEP_MAX_SEQS 4096      /* sequences of one ember_hip_step_tables call */
 #define EMBER_STEP_MAX_REQUESTS 65536 /* rows of its request tables */

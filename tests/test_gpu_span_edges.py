@@ -1,5 +1,5 @@
 """The span attentions at their edges: positions and windows at the ends of 32 bits, scores of any size,
-and long tails of small weights, in the walk and in the tile form."""
+long tails of small weights (in the walk and in the tile form), and steps of more work-groups than a launch holds."""
 import math
 
 import numpy as np
@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from ember_amd import kernels as K
-from span_reference import D, PAGE
+from span_reference import D, PAGE, attention_reference
 from test_gpu_span_ops import dint, prefix_batch, prefix_ws, window_batch
 
 pytestmark = pytest.mark.gpu
@@ -211,3 +211,71 @@ def test_prefix_long_tails_of_small_weights_count(rng, device, n, prefix):
     ws = K.shared_prefix_workspace(b.q.shape[0], 1, 1, n_heads=H, n_kv=KV, device=device, **hints)
     K.shared_prefix_attention(*b.args(), dint([0, 1], device), dint([prefix], device), scale=math.log(2.0), workspace=ws, **hints)
     check_tail(b, 25)
+
+
+def pages_and_tables(rng, device, S, W, dt, blocks=300):
+    k, v = (rng.standard_normal((blocks, 8, PAGE, D)).astype(dt) for _ in range(2))
+    return k, v, torch.from_numpy(k).to(device), torch.from_numpy(v).to(device), rng.integers(0, blocks, (S, W))
+
+
+def test_prefix_4096_decodes_without_hints(rng, device):
+    """max_query is all 4096 tokens then: 512 row tiles for each of 4096 sequences and 8 kv heads, 2^32 threads if each
+    had a work-group."""
+    S = 4096
+    k, v, dk, dv, tables = pages_and_tables(rng, device, S, 3, np.float16)
+    tables[:2000, 0] = tables[0, 0]
+    pos = rng.integers(16, 48, S)
+    q = rng.standard_normal((S, 16, D)).astype(np.float16)
+    out = torch.empty((S, 16, D), dtype=torch.float16, device=device)
+    ws = K.shared_prefix_workspace(S, S, 1, n_heads=16, n_kv=8, device=device)
+    K.shared_prefix_attention(torch.from_numpy(q).to(device), dk, dv, out, dint(np.arange(S + 1), device), dint(pos, device),
+                              dint(tables, device), dint([0, 2000], device), dint([16], device), workspace=ws)
+    some = np.unique(np.concatenate([[0, 1, 1999, 2000, S - 1], rng.integers(0, S, 40)]))
+    want, bound = attention_reference(q[some], k, v, tables[some], np.arange(len(some) + 1), pos[some], lambda s, p, j: j <= p, True)
+    assert (np.abs(out.double().cpu().numpy()[some] - want) <= bound).all()
+    assert not torch.isnan(out).any()
+
+
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+def test_window_2048_verify_runs_without_hints(rng, device, f16):
+    S, n = 2048, 4
+    dt = np.float16 if f16 else np.float32
+    k, v, dk, dv, tables = pages_and_tables(rng, device, S, 4, dt)
+    pos = (rng.integers(0, 60, S)[:, None] + np.arange(n)).reshape(-1)
+    q = rng.standard_normal((S * n, 16, D)).astype(dt)
+    out = torch.full((S * n, 16, D), float("nan"), dtype=dk.dtype, device=device)
+    K.window_attention(torch.from_numpy(q).to(device), dk, dv, out, dint(np.arange(S + 1) * n, device), dint(pos, device),
+                       dint(tables, device), window=20, sinks=3)
+    some = np.unique(np.concatenate([[0, S - 1], rng.integers(0, S, 12)]))
+    rows = (some[:, None] * n + np.arange(n)).reshape(-1)
+    want, bound = attention_reference(q[rows], k, v, tables[some], np.arange(len(some) + 1) * n, pos[rows],
+                                      lambda s, p, j: (j <= p) & ((p - j < 20) | (j < 3)), f16)
+    assert (np.abs(out.double().cpu().numpy()[rows] - want) <= bound).all()
+    assert not torch.isnan(out).any()
+
+
+def test_prefix_partials_of_more_rows_than_one_merge_launch_holds(rng, device):
+    """Tokens around row 2^25 and behind row 2^26 of (token, head), the others of no sequence; most of the 105 GB are
+    never touched."""
+    T = 2 ** 22 + 8
+    need = T * 16 * (2 * D * 2 + 2 * (D + 2) * 4)
+    if torch.cuda.mem_get_info()[0] < need + (8 << 30):
+        pytest.skip(f"needs {need >> 30} GB of free GPU memory")
+    k, v, dk, dv, tables = pages_and_tables(rng, device, 3, 4, np.float16)
+    tables[1, 0] = tables[0, 0]
+    q, out = (torch.empty((T, 16, D), dtype=torch.float16, device=device) for _ in range(2))
+    pos = torch.zeros(T, dtype=torch.int32, device=device)
+    ws = torch.empty(T * 16 * 2 * (D + 2) * 4, dtype=torch.uint8, device=device)
+    for at in (2 ** 21 - 2, T - 5):
+        host = rng.standard_normal((5, 16, D)).astype(np.float16)
+        where = np.array([40, 41, 20, 50, 51])
+        q[at:at + 5], pos[at:at + 5] = torch.from_numpy(host).to(device), dint(where, device)
+        out[at - 2:at + 5] = 123.0
+        K.shared_prefix_attention(q, dk, dv, out, dint([at, at + 2, at + 3, at + 5], device), pos, dint(tables, device),
+                                  dint([0, 2], device), dint([16], device), max_query=2, max_group=3, max_prefix=16, max_own=64,
+                                  workspace=ws)
+        want, bound = attention_reference(host, k, v, tables, [0, 2, 3, 5], where, lambda s, p, j: j <= p, True)
+        assert (np.abs(out[at:at + 5].double().cpu().numpy() - want) <= bound).all()
+        assert (out[at - 2:at] == 123.0).all()
+    del q, out, ws
+    torch.cuda.empty_cache()

@@ -140,3 +140,13 @@ def test_a_window_workspace_covers_smaller_batches():
             sizes = [bytes_for(S, q, **kw) for S in (1, 2, 5, 16, 33, 100, 400)]
             assert sizes == sorted(sizes) and sizes[0] > 0
             assert bytes_for(7, 1, **kw) <= bytes_for(7, q, **kw)
+
+
+@pytest.mark.parametrize("make,entry", [(_window, "ember_hip_window_attn"), (_prefix, "ember_hip_shared_prefix_attn")],
+                         ids=["window", "prefix"])
+def test_more_sequences_than_one_launch_holds_are_refused(make, entry):
+    """2^24 work-groups of 256 threads are 2^32 threads; no pointer is followed."""
+    a = make()
+    a.S, a.max_query, a.workspace, a.workspace_bytes = 1 << 21, 1, 4096, 1 << 40
+    assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
+    assert "too many work-groups" in _lib.last_error()
