@@ -63,9 +63,9 @@ struct SpanParams {
     const void *q, *k, *v;
     void *out;
     const int32_t *query_start, *positions, *tables, *group_start, *prefix_len;
-    float *part_acc, *part_ml;  // [T, n_heads, slots][128], [T, n_heads, slots][2]
+    float *part_acc, *part_ml;  // [part_tokens, n_heads, slots][128], [part_tokens, n_heads, slots][2]
     int64_t q_stride;
-    int T, S, max_blocks, n_heads, n_kv, G, num_blocks, n_groups, sinks, slots;
+    int T, S, max_blocks, n_heads, n_kv, G, num_blocks, n_groups, sinks, slots, part_tokens;
     uint32_t window;
     float scale_log2;
 };
@@ -97,6 +97,7 @@ struct Rows {
     int seq;          // the table's row
     int base, limit;  // keys base .. limit - 1
     int pos;          // the first token's position, if there is one token (rows == G)
+    bool partial;     // whether the step is split (else the first split does all)
 };
 
 // The group of sequence s by 64-ary search (one step for up to 63 groups): whether it is in one, and its prefix length.
@@ -140,8 +141,15 @@ __device__ __forceinline__ Rows rows_of(const SpanParams &p, const Phase &ph, in
     int guess = uniform_load(p.positions + min(unit, p.T - 1));
     const int t0 = uniform_load(p.query_start + s0), t1 = uniform_load(p.query_start + s1);
     if (ph.kind == kOwnRows) grouped = group_of(p, unit, lane, r.base);
-    r.t0 = clamped(t0, p.T);
-    r.rows = max(0, clamped(t1, p.T) - r.t0) * p.G;
+    // A step of more tokens than the workspace has rows for (more than the sizes named) is not split.
+    int most = p.T;
+    r.partial = p.slots > 1;
+    if (r.partial && p.part_tokens < p.T) {
+        r.partial = uniform_load(p.query_start + p.S) <= p.part_tokens;
+        most = r.partial ? p.part_tokens : p.T;
+    }
+    r.t0 = clamped(t0, most);
+    r.rows = max(0, clamped(t1, most) - r.t0) * p.G;
     r.seq = min(s0, p.S - 1);
     if (r.rows == p.G && r.t0 != unit) guess = uniform_load(p.positions + r.t0);
     r.pos = guess;
@@ -238,7 +246,8 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
     const uint32_t window = ph.kind == kWindowRows ? p.window : kNoWindow;
     const int sinks = ph.kind == kWindowRows ? p.sinks : 0;
     const int table_top = p.max_blocks * kPage - 1;
-    const bool partial = p.slots > 1;
+    const bool partial = r.partial;
+    if (!partial && split > 0) return;
     // Without a window the pages start at the base: their ids are requested before the positions are known.
     const int early_page = r.base / kPage + split * ph.pages + wave + lane * W;
     int early = -1;
@@ -273,7 +282,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
         }
         const Span sp = span_of(r, window, sinks, min_pos, max_top);
         const int v0 = min(split * ph.pages, sp.pages);
-        const int v1 = split == ph.splits - 1 ? sp.pages : min(v0 + ph.pages, sp.pages);
+        const int v1 = split == ph.splits - 1 || !partial ? sp.pages : min(v0 + ph.pages, sp.pages);
         if (partial && v0 >= v1) {  // nothing to read: the slot is empty
             if (tid < nrows) {
                 const int64_t at = static_cast<int64_t>(r.t0 + (row0 + tid) / p.G) * p.n_heads + kvh * p.G + (row0 + tid) % p.G;
@@ -592,6 +601,8 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
     __builtin_amdgcn_s_setprio(3);
     bool grouped;
     const Rows r = rows_of(p, ph, unit, lane, grouped);
+    const bool partial = r.partial;
+    if (!partial && split > 0) return;
     const int32_t *const table = p.tables + static_cast<int64_t>(r.seq) * p.max_blocks;
     const int64_t head_off = static_cast<int64_t>(kvh) * (kPage * D), block_stride = static_cast<int64_t>(p.n_kv) * (kPage * D);
     const f16 *const kbase = static_cast<const f16 *>(p.k) + head_off, *const vbase = static_cast<const f16 *>(p.v) + head_off;
@@ -627,9 +638,8 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         min_pos = uniform(min_pos), max_top = uniform(max_top);
         const Span sp = span_of(r, window, sinks, min_pos, max_top);
         const int v0 = min(split * ph.pages, sp.pages);
-        const int v1 = split == ph.splits - 1 ? sp.pages : min(v0 + ph.pages, sp.pages);
+        const int v1 = split == ph.splits - 1 || !partial ? sp.pages : min(v0 + ph.pages, sp.pages);
         const int blocks = (v1 - v0 + kBlockPages - 1) / kBlockPages;  // this group's: group, group + KG, ...
-        const bool partial = p.slots > 1;
 
         // This lane's part of a value operand: key 4 h + r / 4, dims 16 (l / 16 % 2) + 4 (r % 4) .. + 3 of its 16-lane block.
         const int v_at = (4 * h + lane % 16 / 4) * kValueRow + 16 * (lane / 16 % 2) + 4 * (lane % 4);
@@ -887,6 +897,7 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
     const int64_t at = first_row + static_cast<int64_t>(blockIdx.x) * kMergeWaves + uniform(static_cast<int>(threadIdx.x) / kWave);
     const int64_t tok = at / p.n_heads;
     const int first = uniform_load(p.query_start), last = uniform_load(p.query_start + p.S);
+    if (last > p.part_tokens && p.part_tokens < p.T) return;  // not split
     if (tok < clamped(first, p.T) || tok >= clamped(last, p.T)) return;
     const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + at * p.slots;
     const float *const acc = p.part_acc + at * p.slots * D + 2 * lane;
@@ -935,12 +946,13 @@ struct Launch {
     bool tiled = false;       // the first phase is tiles
     int slots = 1, most_slots = 1;  // slots, and those that the workspace is sized for
     int pages = 0;                  // of a window's row tile, at most
+    int tokens = 0;                 // that the workspace has room for
 };
 
 int64_t groups_of(const Phase &ph, int n_kv) { return static_cast<int64_t>(ph.units) * ph.tiles * ph.splits * n_kv; }
 
-int64_t partial_bytes(const EmberRaggedBatch &b, int slots) {
-    return slots <= 1 ? 0 : static_cast<int64_t>(b.T) * b.n_heads * slots * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float));
+int64_t partial_bytes(const EmberRaggedBatch &b, int tokens, int slots) {
+    return slots <= 1 ? 0 : static_cast<int64_t>(tokens) * b.n_heads * slots * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 int tiles_for(int64_t tokens, int G, int rows) { return static_cast<int>(std::max<int64_t>(1, (tokens * G + rows - 1) / rows)); }
@@ -992,6 +1004,7 @@ Launch plan_window(const EmberWindowAttnArgs &a, int spread) {
     const int64_t most = std::min(b.max_query, b.T);
     const bool f16_pages = b.dtype == EMBER_DTYPE_F16;
     Launch l;
+    l.tokens = static_cast<int>(std::min<int64_t>(b.T, b.S * most));  // rows of padding need no partials
     l.tiled = f16_pages && most * G > kWalkRows;
     l.first = rows_phase(kWindowRows, b.S, most, G, b.n_kv, l.tiled, 0);
     // a tile's keys: the first tokens' pages, and the windows of its tokens
@@ -1065,6 +1078,7 @@ Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     const int64_t in_group = std::min(a.max_group, b.T), in_seq = std::min(b.max_query, b.T);
     auto pages_of = [&](int keys) { return std::min(b.max_blocks, keys / kPage + 2); };
     Launch l;
+    l.tokens = b.T;
     l.tiled = a.n_groups > 0 && b.dtype == EMBER_DTYPE_F16 && in_group * G > kWalkRows;
     l.most_slots = 0;
     if (a.n_groups > 0) l.first = rows_phase(kPrefixRows, a.n_groups, in_group, G, b.n_kv, l.tiled, 0);
@@ -1081,16 +1095,16 @@ Launch plan_prefix(const EmberPrefixAttnArgs &a, int spread) {
     return l;
 }
 
-SpanParams params_of(const EmberRaggedBatch &b, int slots) {
+SpanParams params_of(const EmberRaggedBatch &b, const Launch &l) {
     SpanParams p{};
     p.q = b.q, p.k = b.k_cache, p.v = b.v_cache, p.out = b.out;
     p.query_start = b.query_start, p.positions = b.positions, p.tables = b.block_tables;
     p.q_stride = b.q_stride;
     p.T = b.T, p.S = b.S, p.max_blocks = b.max_blocks, p.n_heads = b.n_heads, p.n_kv = b.n_kv;
-    p.G = b.n_heads / b.n_kv, p.num_blocks = b.num_blocks, p.slots = slots;
-    if (slots > 1) {
+    p.G = b.n_heads / b.n_kv, p.num_blocks = b.num_blocks, p.slots = l.slots, p.part_tokens = l.tokens;
+    if (l.slots > 1) {
         p.part_acc = static_cast<float *>(b.workspace);
-        p.part_ml = p.part_acc + static_cast<int64_t>(b.T) * b.n_heads * slots * kHeadDim;
+        p.part_ml = p.part_acc + static_cast<int64_t>(l.tokens) * b.n_heads * l.slots * kHeadDim;
     }
     p.window = kNoWindow;
     p.scale_log2 = b.scale * kLog2e;
@@ -1124,7 +1138,7 @@ hipError_t run(const SpanParams &p, const Launch &l, hipStream_t stream) {
     if (l.slots > 1) {
         constexpr int64_t most = int64_t{1} << 25;  // rows of one launch
         static_assert(most % kMergeWaves == 0 && most * kWave <= UINT32_MAX);
-        const int64_t rows = static_cast<int64_t>(p.T) * p.n_heads;
+        const int64_t rows = static_cast<int64_t>(p.part_tokens) * p.n_heads;
         for (int64_t first_row = 0; first_row < rows; first_row += most)
             hipLaunchKernelGGL(span_merge_kernel<T>, dim3(static_cast<unsigned>((std::min(most, rows - first_row) + kMergeWaves - 1) / kMergeWaves)),
                                dim3(kMergeWaves * kWave), 0, stream, p, first_row);
@@ -1138,10 +1152,10 @@ int fit(const char *who, const EmberRaggedBatch &b, Plan plan, Launch &l) {
     const int64_t room = b.workspace ? b.workspace_bytes : 0;
     for (int spread = 0; spread <= kLeastSpread; spread++) {
         l = plan(spread);
-        if (partial_bytes(b, l.slots) <= room) break;
+        if (partial_bytes(b, l.tokens, l.slots) <= room) break;
         if (spread == kLeastSpread)
             return set_error(EMBER_ERR_INVALID, "%s: needs %lld bytes of workspace at least (got %lld)", who,
-                             static_cast<long long>(partial_bytes(b, l.slots)), static_cast<long long>(room));
+                             static_cast<long long>(partial_bytes(b, l.tokens, l.slots)), static_cast<long long>(room));
     }
     if (groups_of(l.first, b.n_kv) + groups_of(l.second, b.n_kv) > kMostLaunch)
         return set_error(EMBER_ERR_INVALID, "%s: too many work-groups for one launch (S %d x n_kv %d)", who, b.S, b.n_kv);
@@ -1151,19 +1165,21 @@ int fit(const char *who, const EmberRaggedBatch &b, Plan plan, Launch &l) {
 }  // namespace
 
 // A window's workspace holds the partials of these sizes and of smaller batches, which split more: fewer work-groups than
-// CUs, so at most kCus tiles of rows in all.
+// CUs, so at most kCus tiles of rows in all (of S x max_query tokens; rows of padding behind them have no partials).
 int64_t window_workspace_bytes(const EmberWindowAttnArgs &a) {
     const Launch l = plan_window(a, 0);
     const int64_t slots = std::clamp<int64_t>(kCus / a.batch.n_kv, 1, (l.pages + kTileUnit - 1) / kTileUnit);
-    const int64_t rows = slots > 1 ? std::min<int64_t>(static_cast<int64_t>(a.batch.T) * a.batch.n_heads * slots, kCus * kTileRows) : 0;
-    return std::max(partial_bytes(a.batch, l.most_slots), rows * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float)));
+    const int64_t rows = slots > 1 ? std::min<int64_t>(static_cast<int64_t>(l.tokens) * a.batch.n_heads * slots, kCus * kTileRows) : 0;
+    return std::max(partial_bytes(a.batch, l.tokens, l.most_slots), rows * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float)));
 }
-int64_t shared_prefix_workspace_bytes(const EmberPrefixAttnArgs &a) { return partial_bytes(a.batch, plan_prefix(a, 0).most_slots); }
+int64_t shared_prefix_workspace_bytes(const EmberPrefixAttnArgs &a) {
+    return partial_bytes(a.batch, a.batch.T, plan_prefix(a, 0).most_slots);
+}
 
 int launch_window_attn(const EmberWindowAttnArgs &a, hipStream_t stream) {
     Launch l;
     if (int e = fit("window_attn", a.batch, [&](int spread) { return plan_window(a, spread); }, l)) return e;
-    SpanParams p = params_of(a.batch, l.slots);
+    SpanParams p = params_of(a.batch, l);
     p.window = static_cast<uint32_t>(a.window), p.sinks = a.sinks;
     return hip_status(a.batch.dtype == EMBER_DTYPE_F16 ? run<f16>(p, l, stream) : run<float>(p, l, stream), "window_attn");
 }
@@ -1171,7 +1187,7 @@ int launch_window_attn(const EmberWindowAttnArgs &a, hipStream_t stream) {
 int launch_shared_prefix_attn(const EmberPrefixAttnArgs &a, hipStream_t stream) {
     Launch l;
     if (int e = fit("shared_prefix_attn", a.batch, [&](int spread) { return plan_prefix(a, spread); }, l)) return e;
-    SpanParams p = params_of(a.batch, l.slots);
+    SpanParams p = params_of(a.batch, l);
     p.group_start = a.group_start, p.prefix_len = a.prefix_len, p.n_groups = a.n_groups;
     return hip_status(a.batch.dtype == EMBER_DTYPE_F16 ? run<f16>(p, l, stream) : run<float>(p, l, stream), "shared_prefix_attn");
 }

@@ -1,5 +1,6 @@
 """The span attentions at their edges: positions and windows at the ends of 32 bits, scores of any size,
-long tails of small weights (in the walk and in the tile form), and steps of more work-groups than a launch holds."""
+long tails of small weights (in the walk and in the tile form), steps of more work-groups
+than a launch holds, and padded ones."""
 import math
 
 import numpy as np
@@ -279,3 +280,37 @@ def test_prefix_partials_of_more_rows_than_one_merge_launch_holds(rng, device):
         assert (out[at - 2:at] == 123.0).all()
     del q, out, ws
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("n", [1, 12])
+def test_window_padded_steps_split_as_their_tokens_do(rng, device, f16, n):
+    """Rows of padding behind the tokens take no room in the workspace and change no bit."""
+    b, sees = window_batch(rng, device, [4000], [n], H, KV, f16, 3900, 4, pad_rows=500)
+    q, k, v, out, *batch = b.args()
+    outs = []
+    for rows in (n, n + 500):
+        ws = K.window_workspace(rows, 1, n_heads=H, n_kv=KV, window=3900, sinks=4, max_query=n, dtype=out.dtype, device=device)
+        assert ws.nbytes == window_bytes(n, f16)
+        out.fill_(123.0)
+        K.window_attention(q[:rows], k, v, out[:rows], *batch, window=3900, sinks=4, max_query=n, workspace=ws)
+        b.check(sees)
+        outs.append(out.clone())
+    assert torch.equal(*outs)
+
+
+def window_bytes(n, f16):
+    return K.window_workspace(n, 1, n_heads=H, n_kv=KV, window=3900, sinks=4, max_query=n, device="cpu",
+                              dtype=torch.float16 if f16 else torch.float32).nbytes
+
+
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+@pytest.mark.parametrize("n,hint", [(2, 1), (40, 12), (40, 1)])
+def test_window_steps_of_more_tokens_than_named_stay_inside_their_workspace(rng, device, f16, n, hint):
+    """One sequence of n tokens, named as `hint`: not split, right, and nothing is written behind the workspace."""
+    b, sees = window_batch(rng, device, [4000], [n], H, KV, f16, 3900, 4)
+    size = window_bytes(hint, f16)
+    room = torch.full((size + 4096,), 77, dtype=torch.uint8, device=device)
+    K.window_attention(*b.args(), window=3900, sinks=4, max_query=hint, workspace=room[:size])
+    b.check(sees)
+    assert (room == 77).all()  # not split: nothing is written at all

@@ -150,3 +150,23 @@ def test_more_sequences_than_one_launch_holds_are_refused(make, entry):
     a.S, a.max_query, a.workspace, a.workspace_bytes = 1 << 21, 1, 4096, 1 << 40
     assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
     assert "too many work-groups" in _lib.last_error()
+
+
+def test_a_window_workspace_covers_padded_batches():
+    """The same with rows of padding: T stays, or shrinks less than the sequences and their tokens do."""
+    size = _lib.lib().ember_hip_window_workspace_bytes
+    for kw in (dict(), dict(dtype=_lib.DTYPE_F32), dict(n_heads=8, n_kv=1, q_stride=1024)):
+        for T, S, q in ((512, 512, 1), (512, 64, 8), (64, 64, 1), (2048, 4, 512), (300, 1, 300)):
+            def bytes_for(t, s, m, blocks=1 << 26):
+                a = _window()
+                a.window, a.T, a.S, a.max_query, a.max_blocks = 4096, t, s, m, blocks
+                for k, v in kw.items():
+                    setattr(a, k, v)
+                return size(a)
+            most = bytes_for(T, S, q)
+            for t in (T, T // 2 + 1, 1):
+                for s in {S, S // 2 + 1, 4, 1}:
+                    for m in {q, q // 3 + 1, 2, 1}:
+                        for blocks in (1 << 26, 100, 3):
+                            if s <= S and m <= q:
+                                assert bytes_for(t, s, m, blocks) <= most, (kw, T, S, q, t, s, m, blocks)
