@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <iterator>
 #include <string>
 
 #include "capi_errors.hpp"
@@ -90,7 +91,7 @@ int check_prefix(const char *who, const EmberPrefixAttnArgs &a) {
     return EMBER_OK;
 }
 
-// Every work-group reads the inputs while others write the outputs: in place is not possible.
+// Every work-group reads the inputs while others write the outputs: in place is not possible. The request tables are both.
 int check_step_aliases(const EmberStepTablesArgs &a) {
     struct Range {
         const char *name;
@@ -98,22 +99,30 @@ int check_step_aliases(const EmberStepTablesArgs &a) {
         int64_t bytes;
     };
     const int64_t i32 = sizeof(int32_t), table = static_cast<int64_t>(a.max_blocks) * i32;
+    const Range request_tables = {"request_tables", a.request_tables, a.R * table};
     const Range in[] = {{"request", a.request, a.S * i32},          {"cached_len", a.cached_len, a.R * i32},
                         {"new_len", a.new_len, a.S * i32},          {"free_blocks", a.free_blocks, a.n_free * i32},
-                        {"request_tables", a.request_tables, a.R * table}};
+                        {"free_cursor", a.free_cursor, i32},        request_tables};
     const Range out[] = {{"query_start", a.query_start, (a.S + 1) * i32},
                          {"context_len", a.context_len, a.S * i32},
                          {"positions", a.positions, a.max_tokens * i32},
                          {"token_seq", a.token_seq, a.max_tokens * i32},
                          {"slots", a.slots, a.max_tokens * 2 * i32},
                          {"block_tables", a.block_tables, (a.S + 1) * table},
-                         {"totals", a.totals, 4 * i32}};
+                         {"totals", a.totals, 4 * i32},
+                         request_tables};
+    auto overlap = [](const Range &x, const Range &y) {
+        const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at), y0 = reinterpret_cast<uintptr_t>(y.at);
+        return x0 && y0 && x.bytes > 0 && y.bytes > 0 && x0 < y0 + y.bytes && y0 < x0 + x.bytes;
+    };
     for (const Range &x : in)
-        for (const Range &y : out) {
-            const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at), y0 = reinterpret_cast<uintptr_t>(y.at);
-            if (x0 && y0 && x0 < y0 + y.bytes && y0 < x0 + x.bytes)
+        for (const Range &y : out)
+            if (x.name != y.name && overlap(x, y))
                 return set_error(EMBER_ERR_INVALID, "step_tables: %s overlaps %s, which this call writes", x.name, y.name);
-        }
+    for (const Range &x : out)
+        for (const Range *y = &x + 1; y != std::end(out); y++)
+            if (overlap(x, *y))
+                return set_error(EMBER_ERR_INVALID, "step_tables: %s overlaps %s, which this call writes", x.name, y->name);
     return EMBER_OK;
 }
 

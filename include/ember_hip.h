@@ -397,7 +397,8 @@ typedef struct EmberStepTablesArgs {
  * that the append and decode kernels may run over: they belong to row S.
  * The inputs are left as they are but for request_tables, so a repeated call
  * gives the same tables; the next step passes totals + 1 (of a buffer that it
- * does not write) as free_cursor. No input may overlap an output.
+ * does not write) as free_cursor. No input may overlap an output, nor two
+ * outputs each other (request_tables is both).
  * (S + 1) * max_blocks * 16 must fit 31 bits. */
 int ember_hip_step_tables(const EmberStepTablesArgs *args, void *stream);
 

@@ -170,3 +170,29 @@ def test_a_window_workspace_covers_padded_batches():
                         for blocks in (1 << 26, 100, 3):
                             if s <= S and m <= q:
                                 assert bytes_for(t, s, m, blocks) <= most, (kw, T, S, q, t, s, m, blocks)
+
+
+APART = {f: 0x10000 * (i + 1) for i, f in enumerate(
+    ("query_start", "context_len", "positions", "token_seq", "slots", "block_tables", "totals", "request", "cached_len", "new_len",
+     "free_blocks", "free_cursor", "request_tables"))}
+
+
+@pytest.mark.parametrize("field,at,text", [
+    # the request tables are written, beside every other input (3 rows of 4 pages)
+    ("request", APART["request_tables"] + 44, "request overlaps request_tables"), ("cached_len", APART["request_tables"] - 8, "cached_len overlaps request_tables"),
+    ("new_len", APART["request_tables"] + 16, "new_len overlaps request_tables"), ("free_blocks", APART["request_tables"] + 20, "free_blocks overlaps request_tables"),
+    ("free_cursor", APART["request_tables"] + 40, "free_cursor overlaps request_tables"),
+    # the cursor in any output
+    ("free_cursor", APART["query_start"] + 8, "free_cursor overlaps query_start"), ("free_cursor", APART["context_len"], "free_cursor overlaps context_len"),
+    ("free_cursor", APART["positions"] + 20, "free_cursor overlaps positions"), ("free_cursor", APART["slots"] + 44, "free_cursor overlaps slots"),
+    ("free_cursor", APART["block_tables"], "free_cursor overlaps block_tables"), ("free_cursor", APART["totals"] + 4, "free_cursor"),
+    # two outputs
+    ("positions", APART["token_seq"] + 20, "positions overlaps token_seq"), ("context_len", APART["query_start"] + 8, "query_start overlaps context_len"),
+    ("request_tables", APART["slots"] + 40, "request_tables overlaps slots"), ("totals", APART["block_tables"] + 44, "block_tables overlaps totals")])
+def test_step_tables_refuse_what_another_work_group_would_write(field, at, text):
+    a = _tables()
+    for f, x in APART.items():
+        setattr(a, f, x)
+    setattr(a, field, at)
+    assert _lib.lib().ember_hip_step_tables(a, None) == _lib.ERR_INVALID
+    assert text in _lib.last_error()
