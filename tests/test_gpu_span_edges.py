@@ -1,15 +1,16 @@
 """The span attentions at their edges: positions and windows at the ends of 32 bits, scores of any size,
 long tails of small weights (in the walk and in the tile form), steps of more work-groups
-than a launch holds, and padded ones."""
+than a launch holds, and padded ones. Step tables of wide and unaligned rows, and the lengths between steps."""
 import math
 
 import numpy as np
 import pytest
 import torch
 
+from ember_amd import _lib
 from ember_amd import kernels as K
-from span_reference import D, PAGE, attention_reference
-from test_gpu_span_ops import dint, prefix_batch, prefix_ws, window_batch
+from span_reference import D, PAGE, attention_reference, step_tables_reference
+from test_gpu_span_ops import FIELDS, dint, prefix_batch, prefix_ws, random_tables, window_batch
 
 pytestmark = pytest.mark.gpu
 
@@ -314,3 +315,32 @@ def test_window_steps_of_more_tokens_than_named_stay_inside_their_workspace(rng,
     K.window_attention(*b.args(), window=3900, sinks=4, max_query=hint, workspace=room[:size])
     b.check(sees)
     assert (room == 77).all()  # not split: nothing is written at all
+
+
+# ---- step tables ----
+
+def tables_at(rng, device, W, shift):
+    """Step tables whose request rows (or whose own rows) start `shift` entries behind a 16-byte boundary."""
+    request, cached, new, tables, free = random_tables(rng, 9, 12, W, W * PAGE - 300, 200)
+    want = step_tables_reference(request, cached, new, tables, free, 0, int(new.sum()) + 3, 5)
+    flat = torch.full((12 * W + 8,), -77, dtype=torch.int32, device=device)
+    rows = flat[shift:shift + 12 * W].view(12, W)
+    rows.copy_(dint(tables, device))
+    out = K.StepTables(9, int(new.sum()) + 3, W, device)
+    K.step_tables(out, rows, dint(cached, device), dint(new, device), dint(free, device), request=dint(request, device), pad_block=5)
+    torch.cuda.synchronize()
+    for f in FIELDS:
+        assert np.array_equal(getattr(out, f).cpu().numpy(), want[f]), f
+    assert np.array_equal(rows.cpu().numpy(), want["request_tables"])
+    assert (flat[:shift] == -77).all() and (flat[shift + 12 * W:] == -77).all()
+
+
+@pytest.mark.parametrize("W", [1024, 1028, 2048, 2052, 3100])
+def test_step_tables_rows_of_several_segments_four_entries_at_a_time(rng, device, W):
+    tables_at(rng, device, W, 0)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3, 4])
+@pytest.mark.parametrize("W", [24, 1028, 1029])
+def test_step_tables_rows_off_a_16_byte_boundary(rng, device, W, shift):
+    tables_at(rng, device, W, shift)
