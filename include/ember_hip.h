@@ -378,7 +378,7 @@ typedef struct EmberStepTablesArgs {
     int32_t max_tokens;         /* rows of positions, token_seq and slots */
     int32_t pad_block;          /* the page that padding tokens write to, or -1 */
     int32_t *query_start;       /* [S + 1] */
-    int32_t *context_len;       /* [S] tokens after the step */
+    int32_t *context_len;       /* [S] tokens after the step (0 of an EMBER_STEP_INVALID one: the cached length stands) */
     int32_t *positions;         /* [max_tokens]; rows past the step's tokens: 0 */
     int32_t *token_seq;         /* [max_tokens]; rows past the step's tokens: S */
     int64_t *slots;             /* [max_tokens] page * 16 + slot; rows past the step's tokens: pad_block * 16 (-1) */

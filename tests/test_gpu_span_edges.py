@@ -344,3 +344,19 @@ def test_step_tables_rows_of_several_segments_four_entries_at_a_time(rng, device
 @pytest.mark.parametrize("W", [24, 1028, 1029])
 def test_step_tables_rows_off_a_16_byte_boundary(rng, device, W, shift):
     tables_at(rng, device, W, shift)
+
+
+def test_step_lengths_survive_an_invalid_step(rng, device):
+    """The lengths' update between steps, max(length, context), keeps those of requests that an invalid step left out
+    (a negative new_len, a request named twice): their context_len is 0."""
+    request = np.array([3, 1, 4, 4, 0])
+    cached, new = np.array([40, 17, 5, 64, 90, 33]), np.array([2, -1, 1, 1, 3])
+    tables = np.full((6, 8), -1)
+    for r, c in enumerate(cached):
+        tables[r, :-(-c // PAGE)] = 10 * r + np.arange(-(-c // PAGE))
+    out, lengths, rows = K.StepTables(5, 16, 8, device), dint(cached, device), dint(request, device)
+    K.step_tables(out, dint(tables, device), lengths, dint(new, device), dint(np.arange(100, 120), device), request=rows)
+    at = rows.long()
+    lengths.index_copy_(0, at, torch.maximum(lengths[at], out.context_len))
+    assert out.context_len.tolist() == [66, 0, 0, 0, 43] and out.totals.tolist()[2] == _lib.STEP_INVALID
+    assert lengths.tolist() == [43, 17, 5, 66, 90, 33]
