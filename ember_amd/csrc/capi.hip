@@ -59,8 +59,8 @@ int check_batch_sizes(const char *who, const EmberRaggedBatch &b) {
 int check_batch(const char *who, const EmberRaggedBatch &b) {
     if (int e = check_batch_sizes(who, b)) return e;
     if (b.num_blocks <= 0) return set_error(EMBER_ERR_INVALID, "%s: bad sizes (num_blocks %d)", who, b.num_blocks);
-    if (!(b.scale > 0.0f) || !std::isfinite(b.scale))  // the max is taken before scaling
-        return set_error(EMBER_ERR_INVALID, "%s: scale must be positive and finite", who);
+    if (!(b.scale > 0.0f) || !std::isfinite(b.scale * kLog2e))  // the max is taken before scaling, in base 2
+        return set_error(EMBER_ERR_INVALID, "%s: scale must be positive and finite, also in base 2 (below 2.3e38)", who);
     const int per16 = b.dtype == EMBER_DTYPE_F16 ? 8 : 4;
     if (b.q_stride < static_cast<int64_t>(b.n_heads) * kHeadDim || b.q_stride % per16 != 0)
         return set_error(EMBER_ERR_INVALID, "%s: q_stride must be at least n_heads x 128 and a multiple of %d (got %lld)", who,

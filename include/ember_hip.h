@@ -420,7 +420,7 @@ typedef struct EmberRaggedBatch {
     const int32_t *block_tables; /* [S, max_blocks] */
     int64_t q_stride;            /* at least n_heads * 128; q and its rows 16-byte aligned */
     int32_t T, S, max_blocks, n_heads, n_kv, head_dim, num_blocks, dtype;
-    float scale;                 /* positive */
+    float scale;                 /* positive, below 2.3e38 */
     int32_t max_query;           /* tokens of the longest sequence's run; more are computed, slower */
     /* Scratch for splitting the keys over work-groups, 16-byte aligned, no
      * initial contents, nothing kept between launches. With NULL or fewer bytes

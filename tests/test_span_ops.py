@@ -196,3 +196,12 @@ def test_step_tables_refuse_what_another_work_group_would_write(field, at, text)
     setattr(a, field, at)
     assert _lib.lib().ember_hip_step_tables(a, None) == _lib.ERR_INVALID
     assert text in _lib.last_error()
+
+
+@pytest.mark.parametrize("make,entry", [(_window, "ember_hip_window_attn"), (_prefix, "ember_hip_shared_prefix_attn")],
+                         ids=["window", "prefix"])
+def test_scales_that_are_infinite_in_base_2_are_refused(make, entry):
+    a = make()
+    a.scale = 3e38
+    assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
+    assert "scale" in _lib.last_error()
