@@ -98,6 +98,7 @@ struct Rows {
     int base, limit;  // keys base .. limit - 1
     int pos;          // the first token's position, if there is one token (rows == G)
     bool partial;     // whether the step is split (else the first split does all)
+    int part0;        // the token of the workspace's first row
 };
 
 // The group of sequence s by 64-ary search (one step for up to 63 groups): whether it is in one, and its prefix length.
@@ -142,14 +143,16 @@ __device__ __forceinline__ Rows rows_of(const SpanParams &p, const Phase &ph, in
     const int t0 = uniform_load(p.query_start + s0), t1 = uniform_load(p.query_start + s1);
     if (ph.kind == kOwnRows) grouped = group_of(p, unit, lane, r.base);
     // A step of more tokens than the workspace has rows for (more than the sizes named) is not split.
-    int most = p.T;
+    int least = 0, most = p.T;
     r.partial = p.slots > 1;
+    r.part0 = 0;
     if (r.partial && p.part_tokens < p.T) {
-        r.partial = uniform_load(p.query_start + p.S) <= p.part_tokens;
-        most = r.partial ? p.part_tokens : p.T;
+        r.part0 = clamped(uniform_load(p.query_start), p.T);
+        r.partial = clamped(uniform_load(p.query_start + p.S), p.T) - r.part0 <= p.part_tokens;
+        if (r.partial) least = r.part0, most = min(r.part0 + p.part_tokens, p.T);
     }
-    r.t0 = clamped(t0, most);
-    r.rows = max(0, clamped(t1, most) - r.t0) * p.G;
+    r.t0 = min(max(t0, least), most);
+    r.rows = max(0, min(t1, most) - r.t0) * p.G;
     r.seq = min(s0, p.S - 1);
     if (r.rows == p.G && r.t0 != unit) guess = uniform_load(p.positions + r.t0);
     r.pos = guess;
@@ -285,7 +288,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
         const int v1 = split == ph.splits - 1 || !partial ? sp.pages : min(v0 + ph.pages, sp.pages);
         if (partial && v0 >= v1) {  // nothing to read: the slot is empty
             if (tid < nrows) {
-                const int64_t at = static_cast<int64_t>(r.t0 + (row0 + tid) / p.G) * p.n_heads + kvh * p.G + (row0 + tid) % p.G;
+                const int64_t at = static_cast<int64_t>(r.t0 - r.part0 + (row0 + tid) / p.G) * p.n_heads + kvh * p.G + (row0 + tid) % p.G;
                 float2 *const ml = reinterpret_cast<float2 *>(p.part_ml) + at * p.slots;
                 ml[ph.slot0 + split] = make_float2(kNoKeys, 0.0f);
                 if (!grouped && split == 0)
@@ -518,7 +521,7 @@ __device__ __forceinline__ void walk_item(const SpanParams &p, const Phase &ph, 
                 O.x = O.x + x.x * f;
                 O.y = O.y + x.y * f;
             }
-            const int64_t at = static_cast<int64_t>(r.t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
+            const int64_t at = static_cast<int64_t>(r.t0 - (partial ? r.part0 : 0) + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
             if (partial) {
                 const int64_t slot = at * p.slots + ph.slot0 + split;
                 float2 *const ml = reinterpret_cast<float2 *>(p.part_ml);
@@ -839,7 +842,7 @@ __device__ __forceinline__ void tile_item(const SpanParams &p, const Phase &ph, 
         if (group == 0 && mine) {
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
             l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-            const int64_t at = static_cast<int64_t>(my_tok) * p.n_heads + my_head;
+            const int64_t at = static_cast<int64_t>(my_tok - (partial ? r.part0 : 0)) * p.n_heads + my_head;
             if (partial) {
                 const int64_t slot = at * p.slots + ph.slot0 + split;
                 float *const dst = p.part_acc + slot * D + 4 * h;
@@ -895,10 +898,10 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
     constexpr int D = kHeadDim, C = 8;  // slots whose partials are requested together
     const int lane = static_cast<int>(threadIdx.x) % kWave;
     const int64_t at = first_row + static_cast<int64_t>(blockIdx.x) * kMergeWaves + uniform(static_cast<int>(threadIdx.x) / kWave);
-    const int64_t tok = at / p.n_heads;
-    const int first = uniform_load(p.query_start), last = uniform_load(p.query_start + p.S);
-    if (last > p.part_tokens && p.part_tokens < p.T) return;  // not split
-    if (tok < clamped(first, p.T) || tok >= clamped(last, p.T)) return;
+    const int first = clamped(uniform_load(p.query_start), p.T), last = clamped(uniform_load(p.query_start + p.S), p.T);
+    const int part0 = p.part_tokens < p.T ? first : 0;
+    const int64_t tok = at / p.n_heads + part0;
+    if (last - part0 > p.part_tokens || tok < first || tok >= last) return;  // not split, or of no sequence
     const float2 *const ml = reinterpret_cast<const float2 *>(p.part_ml) + at * p.slots;
     const float *const acc = p.part_acc + at * p.slots * D + 2 * lane;
     float M = kNoKeys, L = 0.0f, x = 0.0f, y = 0.0f;
@@ -934,7 +937,7 @@ __global__ void __launch_bounds__(kMergeWaves *kWave) span_merge_kernel(SpanPara
             }
         }
     }
-    T *const dst = static_cast<T *>(p.out) + at * D + 2 * lane;
+    T *const dst = static_cast<T *>(p.out) + (at + static_cast<int64_t>(part0) * p.n_heads) * D + 2 * lane;
     dst[0] = from_f32<T>(filled(L) ? x / L : 0.0f);
     dst[1] = from_f32<T>(filled(L) ? y / L : 0.0f);
 }

@@ -443,8 +443,8 @@ typedef struct EmberWindowAttnArgs {
 int ember_hip_window_attn(const EmberWindowAttnArgs *args, void *stream);
 /* Bytes of workspace ember_hip_window_attn uses for these sizes (only the
  * sizes, dtype, window and sinks of args are read; 0: it would not split).
- * Enough for smaller T, S, max_query and max_blocks too. A step whose
- * tokens reach past row S * max_query is not split. */
+ * Enough for smaller T, S, max_query and max_blocks too. A step of more
+ * than S * max_query tokens is not split. */
 int64_t ember_hip_window_workspace_bytes(const EmberWindowAttnArgs *args);
 
 typedef struct EmberPrefixAttnArgs {

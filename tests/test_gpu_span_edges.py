@@ -360,3 +360,25 @@ def test_step_lengths_survive_an_invalid_step(rng, device):
     lengths.index_copy_(0, at, torch.maximum(lengths[at], out.context_len))
     assert out.context_len.tolist() == [66, 0, 0, 0, 43] and out.totals.tolist()[2] == _lib.STEP_INVALID
     assert lengths.tolist() == [43, 17, 5, 66, 90, 33]
+
+
+@pytest.mark.parametrize("f16", [True, False], ids=["f16", "f32"])
+def test_window_parts_of_a_step_split_as_steps_of_their_own_do(rng, device, f16):
+    """A step's decodes and its chunk in two calls over slices of query_start and the tables, each with the workspace of
+    its own tokens: the same bits as when the tokens are a step of their own."""
+    cached, new = [4000, 3000, 3500], [1, 1, 40]
+    b, sees = window_batch(rng, device, cached, new, H, KV, f16, 3900, 4, pad_rows=20)
+    q, k, v, out, start, pos, tables = b.args()
+    for s0, s1, n in ((0, 2, 1), (2, 3, 40)):
+        a, e = int(b.start[s0]), int(b.start[s1])
+        size = dict(n_heads=H, n_kv=KV, window=3900, sinks=4, max_query=n, dtype=out.dtype, device=device)
+        ws = K.window_workspace(e - a, s1 - s0, **size)
+        assert ws is not None
+        ws.fill_(255)  # NaN: only what the call has written may count
+        kw = dict(window=3900, sinks=4, max_query=n, workspace=ws)
+        K.window_attention(q, k, v, out, start[s0:s1 + 1], pos, tables[s0:s1], **kw)
+        alone = torch.empty((e - a, H, D), dtype=out.dtype, device=device)
+        K.window_attention(q[a:e], k, v, alone, dint(b.start[s0:s1 + 1] - a, device), pos[a:e], tables[s0:s1], **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(out[a:e], alone)
+    b.check(sees)
