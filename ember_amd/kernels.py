@@ -541,7 +541,13 @@ def _batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks):
             (T or 1) if max_query is None else max_query, 0, 0)
 
 
-def _workspace(n: int, device):
+def _workspace(size, args, dtype, device):
+    """A workspace of size(args) bytes, or None for 0 of them."""
+    if not (dtype is torch.float16 or dtype is torch.float32):
+        raise EmberError(f"dtype must be f16 or f32 (got {dtype})")
+    n = int(size(args))
+    if n == 0 and _lib.last_error():  # sizes that no call takes
+        raise EmberError(_lib.last_error())
     return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
 
 
@@ -556,7 +562,7 @@ def window_workspace(T: int, S: int, *, n_heads, n_kv, window, sinks=0, max_quer
     its keys."""
     _check_window(window, sinks)
     a = _lib.WindowAttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks), window, sinks)
-    return _workspace(int(_lib.lib().ember_hip_window_workspace_bytes(a)), device)
+    return _workspace(_lib.lib().ember_hip_window_workspace_bytes, a, dtype, device)
 
 
 def window_attention(q, k_pool, v_pool, out, query_start, positions, block_tables, *, window: int, sinks: int = 0,
@@ -587,7 +593,7 @@ def shared_prefix_workspace(T: int, S: int, n_groups: int, *, n_heads, n_kv, max
     """A workspace for shared_prefix_attention of batches of these sizes."""
     batch = _batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks)
     a = _lib.PrefixAttnArgs(*batch, 0, 0, *_prefix_sizes(T, n_groups, max_group, max_prefix, max_own, batch[10]))
-    return _workspace(int(_lib.lib().ember_hip_shared_prefix_workspace_bytes(a)), device)
+    return _workspace(_lib.lib().ember_hip_shared_prefix_workspace_bytes, a, dtype, device)
 
 
 def shared_prefix_attention(q, k_pool, v_pool, out, query_start, positions, block_tables, group_start, prefix_len, *,

@@ -1,5 +1,6 @@
 """Step tables, windowed and shared-prefix attention: what the C ABI refuses before any launch, and the workspaces."""
 import pytest
+import torch
 
 from ember_amd import _lib
 from ember_amd import kernels as K
@@ -205,3 +206,15 @@ def test_scales_that_are_infinite_in_base_2_are_refused(make, entry):
     a.scale = 3e38
     assert getattr(_lib.lib(), entry)(a, None) == _lib.ERR_INVALID
     assert "scale" in _lib.last_error()
+
+
+@pytest.mark.parametrize("bad", [dict(n_heads=15), dict(n_kv=0), dict(T=-1), dict(S=-2), dict(max_query=0), dict(max_blocks=0),
+                                 dict(dtype=torch.bfloat16), dict(dtype=torch.int32)])
+@pytest.mark.parametrize("make", [K.window_workspace, K.shared_prefix_workspace], ids=["window", "prefix"])
+def test_workspaces_of_sizes_that_no_call_takes_are_refused(make, bad):
+    kw = dict(T=64, S=8, n_heads=16, n_kv=8, max_query=8, device="cpu")
+    kw.update(dict(window=4096) if make is K.window_workspace else dict(n_groups=2))
+    assert make(**kw) is not None
+    with pytest.raises(K.EmberError):
+        make(**{**kw, **bad})
+    assert make(**{**kw, "T": 0}) is None
