@@ -22,13 +22,13 @@
 // the products: span_tile_kernel shares 64-key blocks in LDS between waves of
 // 32 rows each. span_mixed_kernel runs both in one launch.
 //
-// Measured (kernel time, one MI355X; each kernel's own figures stand beside it):
-//   walk   32 decodes, windows of 4096 tokens, 16 / 8 heads   75.6 us, 6.4 TB/s
-//          64 verify runs of up to 5 tokens, windows of 1000  43.2 us, 6.1 TB/s
-//          1 decode, a window of 512                           8.0 us: a chain of four trips to memory
-//   tile   2000 tokens, windows of 4096                       86 us, 780 TFLOP/s
-//   mixed  64 decodes behind 8000 shared tokens               52 us, and 5.4 us the merge
-//          256 decodes in 16 groups                          108 us (4.7 TB/s), and 5.6 us the merge
+// Measured (us a call among others, one MI355X; each kernel's own figures stand beside it):
+//   walk   32 decodes, windows of 4096 tokens, 16 / 8 heads   75.4, 6.4 TB/s
+//          64 verify runs of up to 5 tokens, windows of 1000  43.5, 6.1 TB/s
+//          1 decode, a window of 512                           7.7: a chain of four trips to memory
+//   tile   2000 tokens, windows of 4096                       86 to 89 (by the clock that a box settles at), 760 to 780 TFLOP/s
+//   mixed  64 decodes behind 8000 shared tokens               55, of which the merge takes 5
+//          256 decodes in 16 groups                          110 (4.7 TB/s), of which the merge takes 5
 #include <algorithm>
 #include <cfloat>
 #include <climits>

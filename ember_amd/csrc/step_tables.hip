@@ -13,7 +13,7 @@
 // follow, of what the accepted sequences have.
 //
 // Bound by latency: 9 work-groups for 32 sequences take 6.2 us (lengths, scan,
-// table entries wait for one another), 251 for 1000 sequences 9.9 us, of which
+// table entries wait for one another), 501 for 1000 sequences 9.9 us, of which
 // the tables' 12.6 MB are 2 us. Tokens on work-groups of their own gained nothing.
 //
 // A request named twice would take two runs of pages for one row: a bitmap of

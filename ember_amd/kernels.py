@@ -558,8 +558,8 @@ def _check_window(window: int, sinks: int) -> None:
 
 def window_workspace(T: int, S: int, *, n_heads, n_kv, window, sinks=0, max_query=None, dtype=torch.float16,
                      max_blocks=None, device="cuda"):
-    """A workspace for window_attention of batches of these sizes and smaller ones, or None when no such call splits
-    its keys."""
+    """A workspace for window_attention of batches of these sizes and smaller ones (padded or not), or None when no such
+    call splits its keys."""
     _check_window(window, sinks)
     a = _lib.WindowAttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks), window, sinks)
     return _workspace(_lib.lib().ember_hip_window_workspace_bytes, a, dtype, device)
@@ -599,7 +599,7 @@ def shared_prefix_workspace(T: int, S: int, n_groups: int, *, n_heads, n_kv, max
 def shared_prefix_attention(q, k_pool, v_pool, out, query_start, positions, block_tables, group_start, prefix_len, *,
                             max_query=None, max_group=None, max_prefix=None, max_own=None, scale=None, workspace=None,
                             stream=None):
-    """Causal attention of groups of sequences that share a cached prefix, read once for the group
+    """Causal attention of groups of sequences that share a cached prefix, read for the group and not for each sequence
     (ember_hip_shared_prefix_attn); returns out.
 
     As window_attention, and: group_start [n_groups + 1], group g being sequences group_start[g] ..

@@ -457,9 +457,11 @@ typedef struct EmberPrefixAttnArgs {
 } EmberPrefixAttnArgs;
 
 /* Causal attention (keys 0..p_i of each token) of sequences that share a
- * cached prefix: keys below prefix_len[g] are read once for the whole group,
- * through the table of the group's first sequence, those behind it through
- * each sequence's own. A token inside the prefix sees the prefix up to itself.
+ * cached prefix: keys below prefix_len[g] are read for the whole group and not
+ * for each sequence, through the table of the group's first sequence, those
+ * behind it through each sequence's own. A prefix is read once for every 128
+ * rows (a token and a query head of the kv head) of the group; for every 16 on
+ * f32 and where max_group says that a group has no more. A token inside the prefix sees the prefix up to itself.
  * Sequences of no group share nothing. With groups, two partials of every
  * (token, head) need workspace in any case: 1040 bytes * T * n_heads. */
 int ember_hip_shared_prefix_attn(const EmberPrefixAttnArgs *args, void *stream);
