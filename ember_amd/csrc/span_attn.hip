@@ -77,8 +77,8 @@ constexpr float kNoKeys = -FLT_MAX;
 
 // The exponent of a weight is one fused s * scale - max, the max rounded: what the rounding leaves of the top score,
 // half an ulp at most, moves all weights of the row alike and cancels. From 2^22 on it is not small beside f16's or f32's
-// exponents: there s * scale is rounded first, as the max was, and the top weight is 1 at any size.
-// (each row by itself: its bits do not depend on the other rows of its wave)
+// exponents: there s * scale is rounded first, as the max was, and the top weight is 1 at any size. Each row by itself, so
+// that its bits do not depend on the other rows of its wave.
 constexpr float kFar = 4194304.0f;
 
 // f16 weights are 2^(score - reference), the reference up to 15 below the max (65504 is f16's end): a long tail of weights
@@ -962,10 +962,11 @@ int tiles_for(int64_t tokens, int G, int rows) { return static_cast<int>(std::ma
 
 // `tokens` of every unit are the caller's longest run, or all of the step's: with many units most of the work-groups would
 // find no rows, at about 1 us for 300 of them. Beyond kMostGroups a unit's row tiles share its work-groups, which also
-// keeps a launch within HIP's 2^32 threads for any number of tokens. The share is odd: with an even one, 1000
-// decodes take 2 to 3 times as long, as if the few work-groups that have rows went to the same part of each XCD. Measured, us, at most
-// 2^15, 2^16, 2^17 work-groups and without a bound: 1000 decodes without max_query, window 1724, 1748, 1763 and 4870, shared
-// prefix 232, 275, 384 and 2012; 40 chunks of 512 tokens among 1000 sequences, shared prefix 1668, 1396, 1283 and 2124.
+// keeps a launch within HIP's 2^32 threads for any number of tokens. The share is odd: with an even one, 1000 decodes take
+// 2 to 3 times as long, as if the few work-groups that have rows went to the same part of each XCD.
+// Measured, us, at most 2^15, 2^16, 2^17 work-groups and without a bound: 1000 decodes without max_query, window 1724, 1748,
+// 1763 and 4870, shared prefix 232, 275, 384 and 2012; 40 chunks of 512 tokens among 1000 sequences, shared prefix 1668,
+// 1396, 1283 and 2124.
 constexpr int64_t kMostGroups = 1 << 16;
 constexpr int64_t kMostLaunch = UINT32_MAX / kTileThreads;  // work-groups of the launches that can be large: 256 threads
 
