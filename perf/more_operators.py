@@ -155,7 +155,8 @@ def _memory(case: dict) -> float:
 
 def _encode(x: torch.Tensor):
     """Codes 0..15 like x [..., n] and scale bytes [..., n / 32], in x's own precision: the scale is the lowest power
-    of two that leaves the group's largest value at 7 or less, a code the nearest of 0 .. 6, ties to the even code."""
+    of two that leaves the group's largest value at 7 or less, a code the nearest of 0 .. 6, ties to the even code.
+    Powers of two scale exactly, so 32 bits lose nothing here."""
     g = x.unflatten(-1, (-1, GROUP))
     top = g.abs().amax(-1)
     m, e = torch.frexp(top)
@@ -164,8 +165,7 @@ def _encode(x: torch.Tensor):
     y = g.abs() * torch.from_numpy(2.0 ** -np.arange(LOWEST, HIGHEST + 1.0)).to(x)[(e - LOWEST).long()][..., None]
     code = ((y > 0.25).byte() + (y >= 0.75).byte() + (y > 1.25).byte() + (y >= 1.75).byte() + (y > 2.5).byte()
             + (y >= 3.5).byte() + (y > 5.0).byte())
-    code = code + 8 * ((g < 0) & (code > 0)).byte()
-    return code.flatten(-2), (e + 127).byte()
+    return (code + 8 * torch.signbit(g).byte()).flatten(-2), (e + 127).byte()
 
 
 def _decode(code: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -294,19 +294,19 @@ def run(s: dict):
 
 
 def _plain_append(s: dict) -> dict:
-    """In 64 bits, as the codes of values next to a border need it; the angles are products in f32, as the model has them."""
+    """In 32 bits, the sums of squares and the angles' sine and cosine in 64, as the f16 cache's append computes them."""
     c, pos = s["case"], s["pos"].long()
     T, H, KV = pos.numel(), c["heads"], c["kv_heads"]
-    x = s["qkv"].double()
+    x = s["qkv"].float()
     if s["bias"] is not None:
-        x = x + s["bias"].double()
+        x = x + s["bias"]
     x = x.view(T, H + 2 * KV, D)
     qk, v = x[:, : H + KV], x[:, H + KV:]
     if s["q_norm"] is not None:
-        w = torch.cat([s["q_norm"].double().expand(H, D), s["k_norm"].double().expand(KV, D)])
-        qk = qk / torch.sqrt((qk * qk).mean(-1, keepdim=True) + 1e-6) * w
+        w = torch.cat([s["q_norm"].expand(H, D), s["k_norm"].expand(KV, D)])
+        qk = w * (qk * (1 / torch.sqrt(qk.double().square().mean(-1, keepdim=True) + 1e-6)).float())
     angle = (pos.float()[:, None] * s["inv_freq"]).double()[:, None, :]
-    cos, sin = torch.cos(angle), torch.sin(angle)
+    cos, sin = torch.cos(angle).float(), torch.sin(angle).float()
     lo, hi = qk[..., : D // 2], qk[..., D // 2:]
     qk = torch.cat([lo * cos - hi * sin, hi * cos + lo * sin], -1)
     (kc, ks), (vc, vs) = _encode(qk[:, H:]), _encode(v)
