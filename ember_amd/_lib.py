@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libember_hip.so"
 
 # Constants of include/ember_hip.h.
-ABI_VERSION = 7
+ABI_VERSION = 8
 BLOCK_SIZE = 16
 PREFILL_TILE = 64
 MAX_RUN = 8
@@ -25,6 +25,8 @@ STEP_MAX_REQUESTS = 65536
 STEP_SHORT, STEP_WIDE, STEP_LATE, STEP_INVALID = 1, 2, 4, 8
 OK = 0
 ERR_INVALID = -1
+MX_GROUP = 32
+KV4_PAGE_BYTES = 2176
 DTYPE_F16 = 0
 DTYPE_F32 = 1
 EPILOGUE_STORE_F16 = 0
@@ -173,9 +175,33 @@ class PrefixAttnArgs(ctypes.Structure):
                                        ("max_group", c_int32), ("max_prefix", c_int32), ("max_own", c_int32)]
 
 
+class Kv4AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("qkv", c_void_p), ("q_out", c_void_p), ("pool", c_void_p), ("k_out", c_void_p), ("v_out", c_void_p),
+        ("q_norm", c_void_p), ("k_norm", c_void_p), ("bias", c_void_p), ("inv_freq", c_void_p),
+        ("positions", c_void_p), ("token_seq", c_void_p), ("block_tables", c_void_p),
+        ("rows", c_int32), ("max_blocks", c_int32), ("T", c_int32), ("n_heads", c_int32), ("n_kv", c_int32),
+        ("head_dim", c_int32), ("num_blocks", c_int32), ("eps", c_float),
+    ]
+
+
+class Kv4AttnArgs(ctypes.Structure):
+    _fields_ = RaggedBatch._fields_ + [("max_context", c_int32)]
+
+
+class MxQuantizeArgs(ctypes.Structure):
+    _fields_ = [("x", c_void_p), ("ld", c_int64), ("rows", c_int32), ("cols", c_int32), ("dtype", c_int32),
+                ("codes", c_void_p), ("scales", c_void_p)]
+
+
+class Gemv4Args(ctypes.Structure):
+    _fields_ = [("A", c_void_p), ("lda", c_int64), ("W", c_void_p), ("M", c_int32), ("N", c_int32), ("K", c_int32),
+                ("C", c_void_p), ("ldc", c_int64), ("epilogue", c_int32)]
+
+
 STRUCTS = [QkvArgs, AttnArgs, PrefillArgs, CopyArgs, KvConfig, StepBatchC, LayerIo, GemvArgs, NormArgs, EmbedArgs,
            SampleParams, SampleArgs, ProbArgs, BackendOptions, ModelInfo, StepTablesArgs, RaggedBatch, WindowAttnArgs,
-           PrefixAttnArgs]
+           PrefixAttnArgs, Kv4AppendArgs, Kv4AttnArgs, MxQuantizeArgs, Gemv4Args]
 
 # name -> (restype, argtypes); every extern "C" symbol of include/ember_hip.h.
 PROTOTYPES = {
@@ -198,6 +224,13 @@ PROTOTYPES = {
     "ember_hip_window_workspace_bytes": (c_int64, [POINTER(WindowAttnArgs)]),
     "ember_hip_shared_prefix_attn": (c_int32, [POINTER(PrefixAttnArgs), c_void_p]),
     "ember_hip_shared_prefix_workspace_bytes": (c_int64, [POINTER(PrefixAttnArgs)]),
+    "ember_hip_kv4_append": (c_int32, [POINTER(Kv4AppendArgs), c_void_p]),
+    "ember_hip_kv4_attn": (c_int32, [POINTER(Kv4AttnArgs), c_void_p]),
+    "ember_hip_kv4_workspace_bytes": (c_int64, [POINTER(Kv4AttnArgs)]),
+    "ember_hip_mx_quantize": (c_int32, [POINTER(MxQuantizeArgs), c_void_p]),
+    "ember_hip_gemv4_pack": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
+    "ember_hip_gemv4_packed_bytes": (c_int64, [c_int32, c_int32]),
+    "ember_hip_gemv4": (c_int32, [POINTER(Gemv4Args), c_void_p]),
     "ember_hip_last_error": (c_char_p, []),
     "ember_hip_abi_version": (c_int32, []),
     "ember_hip_sizeof": (c_int32, [c_int32]),

@@ -32,6 +32,9 @@ SOURCES = [
     CSRC / "sampling.hip",
     CSRC / "step_tables.hip",
     CSRC / "span_attn.hip",
+    CSRC / "kv4_append.hip",
+    CSRC / "kv4_attn.hip",
+    CSRC / "linear4.hip",
     CSRC / "host" / "kvcache" / "block_manager.cpp",
     CSRC / "host" / "common" / "json.cpp",
     CSRC / "host" / "common" / "mmap_file.cpp",
@@ -89,6 +92,8 @@ EXTRA_FLAGS = {
     "gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "kv_append.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=8"],
     "span_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kv4_append.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=8"],
+    "kv4_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "prefill_attn.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=9"],
 }
 

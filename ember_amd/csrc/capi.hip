@@ -35,6 +35,10 @@ int hip_status(hipError_t e, const char *what) {
 
 namespace {
 
+constexpr int kMxGroup = EMBER_MX_GROUP;
+constexpr int kMostWeightDim = 1 << 24;   // rows or columns of a 4-bit weight
+constexpr int kMostRows4 = 1 << 21;       // rows of a product with one
+
 bool valid_dtype(int d) { return d == EMBER_DTYPE_F16 || d == EMBER_DTYPE_F32; }
 
 int check_heads(const char *who, int head_dim, int n_heads, int n_kv) {
@@ -56,7 +60,8 @@ int check_batch_sizes(const char *who, const EmberRaggedBatch &b) {
     return EMBER_OK;
 }
 
-int check_batch(const char *who, const EmberRaggedBatch &b) {
+// `pools`: K and V in one pool (k_cache) or two.
+int check_batch(const char *who, const EmberRaggedBatch &b, int pools = 2) {
     if (int e = check_batch_sizes(who, b)) return e;
     if (b.num_blocks <= 0) return set_error(EMBER_ERR_INVALID, "%s: bad sizes (num_blocks %d)", who, b.num_blocks);
     if (!(b.scale > 0.0f) || !std::isfinite(b.scale * kLog2e))  // the max is taken before scaling, in base 2
@@ -68,7 +73,7 @@ int check_batch(const char *who, const EmberRaggedBatch &b) {
     if (b.workspace_bytes < 0 || reinterpret_cast<uintptr_t>(b.workspace) % 16 != 0)
         return set_error(EMBER_ERR_INVALID, "%s: the workspace must be 16-byte aligned with a size >= 0", who);
     if (b.T == 0 || b.S == 0) return EMBER_OK;
-    if (!b.q || !b.k_cache || !b.v_cache || !b.out || !b.query_start || !b.positions || !b.block_tables)
+    if (!b.q || !b.k_cache || (pools > 1 && !b.v_cache) || !b.out || !b.query_start || !b.positions || !b.block_tables)
         return set_error(EMBER_ERR_INVALID, "%s: a required pointer is null", who);
     if ((reinterpret_cast<uintptr_t>(b.q) | reinterpret_cast<uintptr_t>(b.out) | reinterpret_cast<uintptr_t>(b.k_cache) |
          reinterpret_cast<uintptr_t>(b.v_cache)) % 16 != 0)
@@ -88,6 +93,20 @@ int check_prefix(const char *who, const EmberPrefixAttnArgs &a) {
         return set_error(EMBER_ERR_INVALID,
                          "%s: bad sizes (n_groups %d: 0..4096, max_group %d, max_prefix %d, max_own %d)", who, a.n_groups,
                          a.max_group, a.max_prefix, a.max_own);
+    return EMBER_OK;
+}
+
+// What 4-bit pages have that other batches do not.
+int check_kv4(const char *who, const EmberKv4AttnArgs &a) {
+    if (a.batch.dtype != EMBER_DTYPE_F16) return set_error(EMBER_ERR_INVALID, "%s: q and out are f16 (got dtype %d)", who, a.batch.dtype);
+    if (a.batch.v_cache) return set_error(EMBER_ERR_INVALID, "%s: v_cache must be null (K and V are in one pool, k_cache)", who);
+    if (a.max_context < 1) return set_error(EMBER_ERR_INVALID, "%s: max_context must be at least 1 (got %d)", who, a.max_context);
+    return EMBER_OK;
+}
+
+int check_weight4(const char *who, int N, int K) {
+    if (N < 1 || N > kMostWeightDim || K < kMxGroup || K > kMostWeightDim || K % kMxGroup != 0)
+        return set_error(EMBER_ERR_INVALID, "%s: N 1..2^24 and K a multiple of 32 up to 2^24 (got N %d, K %d)", who, N, K);
     return EMBER_OK;
 }
 
@@ -158,6 +177,10 @@ int32_t ember_hip_sizeof(int32_t which) {
         case 16: return sizeof(EmberRaggedBatch);
         case 17: return sizeof(EmberWindowAttnArgs);
         case 18: return sizeof(EmberPrefixAttnArgs);
+        case 19: return sizeof(EmberKv4AppendArgs);
+        case 20: return sizeof(EmberKv4AttnArgs);
+        case 21: return sizeof(EmberMxQuantizeArgs);
+        case 22: return sizeof(EmberGemv4Args);
         default: return -1;
     }
 }
@@ -439,6 +462,95 @@ int ember_hip_rmsnorm_rows(const EmberNormArgs *a, void *stream) {
     if (a->R == 0) return EMBER_OK;
     if (!a->x || !a->w || !a->out) return set_error(EMBER_ERR_INVALID, "rmsnorm_rows: a required pointer is null");
     return hip_status(launch_rmsnorm_rows(*a, static_cast<hipStream_t>(stream)), "rmsnorm_rows");
+}
+
+int ember_hip_kv4_append(const EmberKv4AppendArgs *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "kv4_append: null arguments");
+    if (int e = check_heads("kv4_append", a->head_dim, a->n_heads, a->n_kv)) return e;
+    if (a->n_heads > 64 || a->n_kv > 64)
+        return set_error(EMBER_ERR_INVALID, "kv4_append: at most 64 query and 64 kv heads (got %d, %d)", a->n_heads, a->n_kv);
+    if (a->T < 0 || a->rows <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0)
+        return set_error(EMBER_ERR_INVALID, "kv4_append: bad sizes (T %d, rows %d, max_blocks %d, num_blocks %d)", a->T, a->rows,
+                         a->max_blocks, a->num_blocks);
+    if (a->T == 0) return EMBER_OK;
+    if (!a->qkv || !a->q_out || !a->pool || !a->inv_freq || !a->positions || !a->token_seq || !a->block_tables)
+        return set_error(EMBER_ERR_INVALID, "kv4_append: a required pointer is null");
+    if ((a->q_norm == nullptr) != (a->k_norm == nullptr))
+        return set_error(EMBER_ERR_INVALID, "kv4_append: q_norm and k_norm go together");
+    if ((a->k_out == nullptr) != (a->v_out == nullptr))
+        return set_error(EMBER_ERR_INVALID, "kv4_append: k_out and v_out go together");
+    if ((reinterpret_cast<uintptr_t>(a->qkv) | reinterpret_cast<uintptr_t>(a->q_out) | reinterpret_cast<uintptr_t>(a->pool) |
+         reinterpret_cast<uintptr_t>(a->k_out) | reinterpret_cast<uintptr_t>(a->v_out)) % 16 != 0)
+        return set_error(EMBER_ERR_INVALID, "kv4_append: qkv, q_out, k_out, v_out and the pool must be 16-byte aligned");
+    return hip_status(launch_kv4_append(*a, static_cast<hipStream_t>(stream)), "kv4_append");
+}
+
+int ember_hip_kv4_attn(const EmberKv4AttnArgs *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "kv4_attn: null arguments");
+    if (int e = check_batch("kv4_attn", a->batch, 1)) return e;
+    if (int e = check_kv4("kv4_attn", *a)) return e;
+    if (a->batch.T == 0 || a->batch.S == 0) return EMBER_OK;
+    return launch_kv4_attn(*a, static_cast<hipStream_t>(stream));
+}
+
+int64_t ember_hip_kv4_workspace_bytes(const EmberKv4AttnArgs *a) {
+    g_last_error.clear();
+    if (!a || check_batch_sizes("kv4_workspace_bytes", a->batch) || check_kv4("kv4_workspace_bytes", *a) || a->batch.T == 0 ||
+        a->batch.S == 0)
+        return 0;
+    return kv4_workspace_bytes(*a);
+}
+
+int ember_hip_mx_quantize(const EmberMxQuantizeArgs *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "mx_quantize: null arguments");
+    if (!valid_dtype(a->dtype)) return set_error(EMBER_ERR_INVALID, "mx_quantize: unknown dtype %d", a->dtype);
+    if (a->rows < 0 || a->cols < 0 || a->cols % kMxGroup != 0 || a->ld < a->cols)
+        return set_error(EMBER_ERR_INVALID, "mx_quantize: cols must be a multiple of 32, ld at least cols (got rows %d, cols %d, ld %lld)",
+                         a->rows, a->cols, static_cast<long long>(a->ld));
+    if (a->rows == 0 || a->cols == 0) return EMBER_OK;
+    if (!a->x || !a->codes || !a->scales) return set_error(EMBER_ERR_INVALID, "mx_quantize: a required pointer is null");
+    if (reinterpret_cast<uintptr_t>(a->x) % (a->dtype == EMBER_DTYPE_F16 ? 2 : 4) != 0 || reinterpret_cast<uintptr_t>(a->codes) % 4 != 0)
+        return set_error(EMBER_ERR_INVALID, "mx_quantize: x must be aligned to its elements and codes to 4 bytes");
+    return hip_status(launch_mx_quantize(*a, static_cast<hipStream_t>(stream)), "mx_quantize");
+}
+
+int64_t ember_hip_gemv4_packed_bytes(int32_t N, int32_t K) {
+    g_last_error.clear();
+    return check_weight4("gemv4_packed_bytes", N, K) ? 0 : gemv4_packed_bytes(N, K);
+}
+
+int ember_hip_gemv4_pack(const uint8_t *codes, const uint8_t *scales, int32_t N, int32_t K, void *out, void *stream) {
+    g_last_error.clear();
+    if (int e = check_weight4("gemv4_pack", N, K)) return e;
+    if (!codes || !scales || !out) return set_error(EMBER_ERR_INVALID, "gemv4_pack: a required pointer is null");
+    if (reinterpret_cast<uintptr_t>(codes) % 4 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0)
+        return set_error(EMBER_ERR_INVALID, "gemv4_pack: codes must be 4-byte and out 16-byte aligned");
+    return hip_status(launch_gemv4_pack(codes, scales, N, K, out, static_cast<hipStream_t>(stream)), "gemv4_pack");
+}
+
+int ember_hip_gemv4(const EmberGemv4Args *a, void *stream) {
+    g_last_error.clear();
+    if (!a) return set_error(EMBER_ERR_INVALID, "gemv4: null arguments");
+    if (int e = check_weight4("gemv4", a->N, a->K)) return e;
+    if (a->M < 0 || a->M > kMostRows4) return set_error(EMBER_ERR_INVALID, "gemv4: M must be 0..2^21 (got %d)", a->M);
+    if (a->epilogue < EMBER_EPILOGUE_STORE_F16 || a->epilogue > EMBER_EPILOGUE_SILU_MUL)
+        return set_error(EMBER_ERR_INVALID, "gemv4: unknown epilogue %d", a->epilogue);
+    if (a->epilogue == EMBER_EPILOGUE_SILU_MUL && a->N % 2 != 0)
+        return set_error(EMBER_ERR_INVALID, "gemv4: silu_mul needs an even N (got %d)", a->N);
+    const int cols = a->epilogue == EMBER_EPILOGUE_SILU_MUL ? a->N / 2 : a->N;
+    if (a->lda < a->K || a->lda % 8 != 0 || a->ldc < cols)
+        return set_error(EMBER_ERR_INVALID, "gemv4: lda must be >= K and a multiple of 8, ldc >= %d (got %lld, %lld)", cols,
+                         static_cast<long long>(a->lda), static_cast<long long>(a->ldc));
+    if (a->M == 0) return EMBER_OK;
+    if (!a->A || !a->W || !a->C) return set_error(EMBER_ERR_INVALID, "gemv4: a required pointer is null");
+    if (reinterpret_cast<uintptr_t>(a->A) % 16 != 0 || reinterpret_cast<uintptr_t>(a->W) % 16 != 0)
+        return set_error(EMBER_ERR_INVALID, "gemv4: A and W must be 16-byte aligned");
+    const bool f32 = a->epilogue == EMBER_EPILOGUE_STORE_F32 || a->epilogue == EMBER_EPILOGUE_ADD_F32;
+    if (reinterpret_cast<uintptr_t>(a->C) % (f32 ? 4 : 2) != 0) return set_error(EMBER_ERR_INVALID, "gemv4: C must be aligned to its elements");
+    return hip_status(launch_gemv4(*a, static_cast<hipStream_t>(stream)), "gemv4");
 }
 
 }  // extern "C"

@@ -3,6 +3,8 @@
 // layouts' cross-lane steps (lane l = 16 g + c serves query column c).
 #pragma once
 
+#include <cfloat>
+
 #include "device.hpp"
 
 namespace ember::hip {
@@ -69,5 +71,26 @@ __device__ __forceinline__ f16x8 as_f16x8(const u32x4 &x) { return __builtin_bit
 // row keeps l = 0 and O = 0; the merges below treat it like -inf (weight 0
 // against any real max, and zeros when every part is empty).
 constexpr float kNoMax = -1.0e30f;
+
+// What follows is the softmax of the kernels that take scores of any size.
+
+// The running max of a row before any visible key: finite, so that a difference of two is a number, and below any score.
+constexpr float kNoKeys = -FLT_MAX;
+
+// The exponent of a weight is one fused s * scale - max, the max rounded: what the rounding leaves of the top score,
+// half an ulp at most, moves all weights of the row alike and cancels. From 2^22 on it is not small beside f16's or f32's
+// exponents: there s * scale is rounded first, as the max was, and the top weight is 1 at any size. Each row by itself, so
+// that its bits do not depend on the other rows of its wave.
+constexpr float kFar = 4194304.0f;
+
+// f16 weights are 2^(score - reference), the reference up to 15 below the max (65504 is f16's end): a long tail of weights
+// that f16 could not hold beside a largest weight of 1 counts. Sums and outputs are in the same units, so nothing else
+// changes. A far max takes no such step, which its rounding would swallow.
+constexpr float kMostExponent = 15.0f;
+__device__ __forceinline__ float below(float top, float step) { return fabsf(top) < kFar ? top - step : top; }
+
+// Whether a sum of weights holds anything: also when it is NaN (of a NaN in q, say), which a comparison would take for
+// an empty row's 0 and so turn the row into zeros.
+__device__ __forceinline__ bool filled(float l) { return __float_as_uint(l) != 0; }
 
 }  // namespace ember::hip

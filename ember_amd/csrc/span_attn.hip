@@ -30,7 +30,6 @@
 //   mixed  64 decodes behind 8000 shared tokens               55, of which the merge takes 5
 //          256 decodes in 16 groups                          110 (4.7 TB/s), of which the merge takes 5
 #include <algorithm>
-#include <cfloat>
 #include <climits>
 
 #include "capi_errors.hpp"
@@ -71,25 +70,6 @@ struct SpanParams {
 };
 
 __device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
-
-// The running max of a row before any visible key: finite, so that a difference of two is a number, and below any score.
-constexpr float kNoKeys = -FLT_MAX;
-
-// The exponent of a weight is one fused s * scale - max, the max rounded: what the rounding leaves of the top score,
-// half an ulp at most, moves all weights of the row alike and cancels. From 2^22 on it is not small beside f16's or f32's
-// exponents: there s * scale is rounded first, as the max was, and the top weight is 1 at any size. Each row by itself, so
-// that its bits do not depend on the other rows of its wave.
-constexpr float kFar = 4194304.0f;
-
-// f16 weights are 2^(score - reference), the reference up to 15 below the max (65504 is f16's end): a long tail of weights
-// that f16 could not hold beside a largest weight of 1 counts. Sums and outputs are in the same units, so nothing else
-// changes. A far max takes no such step, which its rounding would swallow.
-constexpr float kMostExponent = 15.0f;
-__device__ __forceinline__ float below(float top, float step) { return fabsf(top) < kFar ? top - step : top; }
-
-// Whether a sum of weights holds anything: also when it is NaN (of a NaN in q, say), which a comparison would take for
-// an empty row's 0 and so turn the row into zeros.
-__device__ __forceinline__ bool filled(float l) { return __float_as_uint(l) != 0; }
 
 // The rows of one work item and the bounds of the keys they see.
 struct Rows {

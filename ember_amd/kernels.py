@@ -5,7 +5,9 @@ Mirrors the reference's launcher seam (src/backend/cuda/kernels.cuh:74-120):
 (-> ember_hip_paged_decode), ``prefill_attention`` (-> ember_hip_prefill_attn),
 plus ``copy_pages`` (copy-on-write). ``step_tables``, ``window_attention`` and
 ``shared_prefix_attention`` have no counterpart there: they take a step's integers
-from the device, with no host plan. Device tensors carry activations and pools;
+from the device, with no host plan. Nor have ``kv4_append``, ``kv4_attention``,
+``mx_quantize``, ``gemv4_pack`` and ``gemv4``, for a cache and weights held in 4
+bits, which do so too. Device tensors carry activations and pools;
 the step's integer arrays are given as host arrays, checked here (every index a
 kernel will follow is in range), then uploaded. Launches go to the current torch
 stream unless ``stream`` is given.
@@ -19,7 +21,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import BLOCK_SIZE, MAX_RUN, PREFILL_TILE, AttnArgs, CopyArgs, EmberError, PrefillArgs, QkvArgs, check
+from ._lib import BLOCK_SIZE, KV4_PAGE_BYTES, MAX_RUN, PREFILL_TILE, AttnArgs, CopyArgs, EmberError, PrefillArgs, QkvArgs, check
 
 HEAD_DIM = 128
 
@@ -501,22 +503,35 @@ def step_tables(out: StepTables, request_tables, cached_len, new_len, free_block
     return out
 
 
+def _check_kv4_pool(pool, dev: int) -> None:
+    """A pool of 4-bit pages on device `dev`."""
+    if pool.dtype is not torch.uint8 or pool.get_device() != dev or not pool.is_contiguous():
+        _refuse(dict(pool=pool), dev, torch.uint8)
+    if pool.dim() != 3 or pool.shape[2] != KV4_PAGE_BYTES:
+        raise EmberError(f"pool must be [num_blocks, n_kv, {KV4_PAGE_BYTES}]")
+
+
 def _ragged_batch(q, k_pool, v_pool, out, query_start, positions, block_tables, max_query, scale, workspace):
     """Checks a ragged batch and returns its device and the fields of an EmberRaggedBatch, in order: q [T, n_heads, 128]
-    (any token stride), pools [num_blocks, n_kv, 16, 128]."""
+    (any token stride), pools [num_blocks, n_kv, 16, 128]; k_pool [num_blocks, n_kv, KV4_PAGE_BYTES] of 4-bit pages where
+    v_pool is None."""
     dev, dtype, i32 = q.get_device(), q.dtype, torch.int32
     if dev < 0 or not (dtype is torch.float16 or dtype is torch.float32):
         raise EmberError(f"q must be an f16 or f32 device tensor (got {dtype} on {q.device})")
-    for t in (k_pool, v_pool, out):
+    for t in (k_pool, v_pool, out) if v_pool is not None else (out,):
         if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
-            _refuse(dict(k_pool=k_pool, v_pool=v_pool, out=out), dev, dtype)
+            _refuse(dict(k_pool=k_pool, v_pool=v_pool, out=out) if v_pool is not None else dict(out=out), dev, dtype)
     for t in (query_start, positions, block_tables):
         if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
             _refuse(dict(query_start=query_start, positions=positions, block_tables=block_tables), dev, i32)
     shape, pool, stride = q.shape, k_pool.shape, q.stride()
     if len(shape) != 3 or shape[2] != HEAD_DIM or stride[2] != 1 or stride[1] != HEAD_DIM:
         raise EmberError("q must be [T, n_heads, 128] with each token's heads contiguous")
-    if len(pool) != 4 or pool[2] != BLOCK_SIZE or pool[3] != HEAD_DIM or v_pool.shape != pool or out.shape != shape:
+    if v_pool is None:
+        _check_kv4_pool(k_pool, dev)
+        if out.shape != shape:
+            raise EmberError("out must be shaped like q")
+    elif len(pool) != 4 or pool[2] != BLOCK_SIZE or pool[3] != HEAD_DIM or v_pool.shape != pool or out.shape != shape:
         raise EmberError("pools must be [num_blocks, n_kv, 16, 128] alike, and out shaped like q")
     T, H, _ = shape
     S = query_start.numel() - 1
@@ -528,7 +543,7 @@ def _ragged_batch(q, k_pool, v_pool, out, query_start, positions, block_tables, 
         if workspace.get_device() != dev or not workspace.is_contiguous():
             raise EmberError(f"workspace must be a contiguous tensor on cuda:{dev}")
         ws, ws_bytes = workspace.data_ptr(), workspace.nbytes
-    return dev, (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), query_start.data_ptr(),
+    return dev, (q.data_ptr(), k_pool.data_ptr(), 0 if v_pool is None else v_pool.data_ptr(), out.data_ptr(), query_start.data_ptr(),
                  positions.data_ptr(), block_tables.data_ptr(), stride[0] if T > 1 else H * HEAD_DIM, T, S, table[1], H,
                  pool[1], HEAD_DIM, pool[0], _lib.DTYPE_F16 if dtype is torch.float16 else _lib.DTYPE_F32,
                  HEAD_DIM ** -0.5 if scale is None else scale, (T or 1) if max_query is None else max_query, ws, ws_bytes)
@@ -618,3 +633,136 @@ def shared_prefix_attention(q, k_pool, v_pool, out, query_start, positions, bloc
                             *_prefix_sizes(batch[8], n_groups, max_group, max_prefix, max_own, batch[10]))
     _launch(_lib.lib().ember_hip_shared_prefix_attn, a, dev, stream, "shared_prefix_attn")
     return out
+
+
+def kv4_pool(num_blocks: int, n_kv: int, device="cuda"):
+    """A layer's pool of 4-bit pages, zeros: uint8 [num_blocks, n_kv, KV4_PAGE_BYTES], K and V together. Whole pages are
+    copied by indexing (pool[dst] = pool[src])."""
+    return torch.zeros(num_blocks, n_kv, KV4_PAGE_BYTES, dtype=torch.uint8, device=device)
+
+
+def kv4_append(qkv, q_out, pool, positions, token_seq, block_tables, *, n_heads, n_kv, inv_freq_dev, q_norm=None,
+               k_norm=None, bias=None, eps=1e-6, k_out=None, v_out=None, stream=None):
+    """QK-RMSNorm + RoPE + the write of K and V into 4-bit pages, for one layer (ember_hip_kv4_append).
+
+    qkv f16 [T, (n_heads + 2 n_kv) * 128] and q_out f16 [T, n_heads * 128] (any shape of that size); pool of kv4_pool;
+    positions [T], token_seq [T] (rows of block_tables) and block_tables [rows, max_blocks] int32 on the device, as
+    step_tables writes them. q_norm, k_norm [128], bias and inv_freq_dev [64] f32. k_out, v_out: None, or f16
+    [T, n_kv * 128], which get what the codes stand for.
+    """
+    dev, f16, f32, i32 = qkv.get_device(), torch.float16, torch.float32, torch.int32
+    if dev < 0:
+        raise EmberError(f"qkv must be a device tensor (got {qkv.device})")
+    _check_kv4_pool(pool, dev)
+    for name, t, dtype in (("qkv", qkv, f16), ("q_out", q_out, f16), ("positions", positions, i32), ("token_seq", token_seq, i32),
+                           ("block_tables", block_tables, i32), ("inv_freq_dev", inv_freq_dev, f32), ("q_norm", q_norm, f32),
+                           ("k_norm", k_norm, f32), ("bias", bias, f32), ("k_out", k_out, f16), ("v_out", v_out, f16)):
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous()):
+            _refuse({name: t}, dev, dtype)
+    width = (n_heads + 2 * n_kv) * HEAD_DIM
+    T = positions.numel()
+    if qkv.numel() != T * width or q_out.numel() != T * n_heads * HEAD_DIM or token_seq.numel() != T:
+        raise EmberError("qkv, q_out and token_seq must hold as many tokens as positions")
+    if pool.shape[1] != n_kv or block_tables.dim() != 2 or inv_freq_dev.numel() != HEAD_DIM // 2:
+        raise EmberError("pool must have n_kv heads, block_tables be [rows, max_blocks] and inv_freq_dev hold 64 frequencies")
+    for name, t, n in (("q_norm", q_norm, HEAD_DIM), ("k_norm", k_norm, HEAD_DIM), ("bias", bias, width),
+                       ("k_out", k_out, T * n_kv * HEAD_DIM), ("v_out", v_out, T * n_kv * HEAD_DIM)):
+        if t is not None and t.numel() != n:
+            raise EmberError(f"{name} must hold {n} values")
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    a = _lib.Kv4AppendArgs(qkv.data_ptr(), q_out.data_ptr(), pool.data_ptr(), p(k_out), p(v_out), p(q_norm), p(k_norm), p(bias),
+                           inv_freq_dev.data_ptr(), positions.data_ptr(), token_seq.data_ptr(), block_tables.data_ptr(),
+                           block_tables.shape[0], block_tables.shape[1], T, n_heads, n_kv, HEAD_DIM, pool.shape[0], eps)
+    _launch(_lib.lib().ember_hip_kv4_append, a, dev, stream, "kv4_append")
+
+
+def kv4_workspace(T: int, S: int, *, n_heads, n_kv, max_query=None, max_context=None, max_blocks=None, device="cuda"):
+    """A workspace (zeros) for kv4_attention of batches of these sizes and smaller ones, or None when no such call splits
+    its keys. Only kv4_attention may write to it."""
+    a = _lib.Kv4AttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, torch.float16, max_blocks),
+                         _context(max_context, 1 << 26 if max_blocks is None else max_blocks))
+    ws = _workspace(_lib.lib().ember_hip_kv4_workspace_bytes, a, torch.float16, device)
+    return None if ws is None else ws.zero_()
+
+
+def _context(max_context, max_blocks):
+    if max_context is None:
+        return max(1, min(max_blocks * BLOCK_SIZE, 0x7FFFFFFF))
+    if not 0 < max_context <= 0x7FFFFFFF:
+        raise EmberError(f"max_context must be 1 .. 2^31 - 1 (got {max_context})")
+    return max_context
+
+
+def kv4_attention(q, pool, out, query_start, positions, block_tables, *, max_query=None, max_context=None, scale=None,
+                  workspace=None, stream=None):
+    """Causal attention of a ragged batch over 4-bit pages (ember_hip_kv4_attn); returns out.
+
+    q f16 [T, n_heads, 128] (a part of wider rows is fine), out the same, contiguous; pool of kv4_pool; query_start
+    [S + 1], positions [T] and block_tables [S, max_blocks] int32 on the device, as step_tables writes them. Rows of
+    q past query_start[S] are left alone. max_query and max_context: the most tokens and keys of one sequence (None:
+    T, the tables' width); a step beyond them is computed too, only slower. workspace: of kv4_workspace, not shared
+    by calls that overlap in time (None: no splits).
+    """
+    if q.dtype is not torch.float16:
+        raise EmberError(f"q must be f16 (got {q.dtype})")
+    dev, batch = _ragged_batch(q, pool, None, out, query_start, positions, block_tables, max_query, scale, workspace)
+    _launch(_lib.lib().ember_hip_kv4_attn, _lib.Kv4AttnArgs(*batch, _context(max_context, batch[10])), dev, stream, "kv4_attn")
+    return out
+
+
+def mx_quantize(x, stream=None):
+    """Rows to 4 bits (ember_hip_mx_quantize): f16 or f32 [rows, cols], cols a multiple of 32, rows of any stride.
+    Returns codes uint8 [rows, cols / 2] (byte i: columns 2i, in the low four bits, and 2i + 1) and scales uint8
+    [rows, cols / 32]: value = (0, 0.5, 1, 1.5, 2, 3, 4, 6)[code % 8] * (-1 if code > 7) * 2^(scale - 127)."""
+    dev = x.get_device()
+    if dev < 0 or x.dim() != 2 or not (x.dtype is torch.float16 or x.dtype is torch.float32) or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise EmberError("mx_quantize: x must be an f16 or f32 device tensor [rows, cols] with contiguous rows")
+    rows, cols = x.shape
+    codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(rows, cols // _lib.MX_GROUP, dtype=torch.uint8, device=x.device)
+    a = _lib.MxQuantizeArgs(x.data_ptr(), x.stride(0) if rows > 1 else cols, rows, cols, _dtype_code(x), codes.data_ptr(),
+                            scales.data_ptr())
+    _launch(_lib.lib().ember_hip_mx_quantize, a, dev, stream, "mx_quantize")
+    return codes, scales
+
+
+def gemv4_pack(codes, scales, stream=None):
+    """A 4-bit weight [N, K] as mx_quantize returns it (or a checkpoint in that format) laid out for gemv4: a flat uint8
+    device tensor."""
+    dev = codes.get_device()
+    if dev < 0 or codes.dim() != 2 or scales.dim() != 2:
+        raise EmberError("gemv4_pack: codes [N, K / 2] and scales [N, K / 32] must be device tensors")
+    _refuse(dict(codes=codes, scales=scales), dev, torch.uint8)
+    N, K = codes.shape[0], codes.shape[1] * 2
+    if scales.shape != (N, K // _lib.MX_GROUP):
+        raise EmberError(f"gemv4_pack: scales must be [{N}, {K // _lib.MX_GROUP}]")
+    n = int(_lib.lib().ember_hip_gemv4_packed_bytes(N, K))
+    if n <= 0:
+        raise EmberError(_lib.last_error())
+    out = torch.empty(n, dtype=torch.uint8, device=codes.device)
+    fn = _lib.lib().ember_hip_gemv4_pack
+    _launch(lambda args, handle: fn(*args, handle), (codes.data_ptr(), scales.data_ptr(), N, K, out.data_ptr()), dev, stream, "gemv4_pack")
+    return out
+
+
+def gemv4(a, packed, c, epilogue: int, *, N: int, stream=None):
+    """C = epilogue(A . W^T) with W [N, K] of gemv4_pack (ember_hip_gemv4).
+
+    a: f16 [M, K] (rows of any stride that is a multiple of 8); c: as gemv's, rows of any stride. packed is known by its
+    size alone: N and K are the caller's to get right. A row's bits do not
+    depend on the other rows.
+    """
+    dev = a.get_device()
+    if dev < 0 or a.dtype is not torch.float16 or a.dim() != 2 or a.stride(1) != 1:
+        raise EmberError("gemv4: a must be an f16 device tensor [M, K] with contiguous rows")
+    M, K = a.shape
+    _refuse(dict(packed=packed), dev, torch.uint8)
+    if packed.numel() != int(_lib.lib().ember_hip_gemv4_packed_bytes(N, K)):
+        raise EmberError(f"gemv4: packed is not a weight of [{N}, {K}]")
+    cols = N // 2 if epilogue == _lib.EPILOGUE_SILU_MUL else N
+    want = torch.float32 if epilogue in (_lib.EPILOGUE_STORE_F32, _lib.EPILOGUE_ADD_F32) else torch.float16
+    if c.dtype is not want or c.get_device() != dev or tuple(c.shape) != (M, cols) or (cols > 1 and c.stride(1) != 1):
+        raise EmberError(f"gemv4: c must be {want} [{M}, {cols}] on cuda:{dev} with contiguous rows")
+    g = _lib.Gemv4Args(a.data_ptr(), a.stride(0) if M > 1 else K, packed.data_ptr(), M, N, K, c.data_ptr(),
+                       c.stride(0) if M > 1 else cols, epilogue)
+    _launch(_lib.lib().ember_hip_gemv4, g, dev, stream, "gemv4")

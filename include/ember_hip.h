@@ -9,7 +9,8 @@
  *      (src/backend/cuda/kernels.cuh:74-120) field for field, plus a few
  *      documented additions (pool size for bounds guards, element type, query
  *      runs). 1b: launchers without a counterpart there, for steps planned on
- *      the GPU, windowed attention and shared prefixes.
+ *      the GPU, windowed attention and shared prefixes; 1c: for a cache and
+ *      weights held in 4 bits.
  *   2. The KV block manager (src/kvcache/block_manager.hpp:25-67) behind an
  *      opaque handle, plus two additive calls (share, copy_on_write) that the
  *      reference does not have.
@@ -38,7 +39,7 @@
 extern "C" {
 #endif
 
-#define EMBER_ABI_VERSION 7
+#define EMBER_ABI_VERSION 8
 #define EMBER_BLOCK_SIZE 16  /* tokens per page; kBlockSize, src/backend/backend.hpp:25 */
 #define EMBER_PREFILL_TILE 64 /* query tokens per prefill tile; kPrefillTile, kernels.cuh:108 */
 #define EMBER_MAX_RUN 8      /* query tokens one decode work-group reads a page for */
@@ -467,6 +468,108 @@ typedef struct EmberPrefixAttnArgs {
 int ember_hip_shared_prefix_attn(const EmberPrefixAttnArgs *args, void *stream);
 int64_t ember_hip_shared_prefix_workspace_bytes(const EmberPrefixAttnArgs *args);
 
+/* ---- 1c. a cache and weights in 4 bits ---------------------------------------
+ * No counterpart in the reference, whose pages and weights are f16. The format
+ * is the OCP microscaling one that gfx950 converts in hardware: 4-bit codes
+ * (e2m1: a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6) in groups of 32
+ * consecutive values with one scale byte b each (e8m0: 2^(b - 127); 255 is
+ * NaN). A code and its group's scale stand for their product.
+ *
+ * What is written here takes, for a group whose largest magnitude is m, the
+ * lowest exponent e of -23 .. 13 with m <= 7 * 2^e (13 if none is enough), and
+ * for each value x the nearest of the eight magnitudes to |x| / 2^e, of two as
+ * near the one with the even code, 6 beyond 6; the sign is x's, also of a
+ * zero. Every such value is exact in f16. Other scales may be read: a value
+ * is then rounded to f16 where it is read (beyond 65504: infinite). */
+
+#define EMBER_MX_GROUP 32
+
+/* A kv head's page: 16 tokens of K and V in one piece, 17 lines of 128 bytes.
+ *   0     K codes   [token 0..15][64]: byte i of a token holds dims 2i (low
+ *                   four bits) and 2i + 1
+ *   1024  V codes   [token / 4][dim / 8][token % 4][4]: the same bytes, four
+ *                   tokens' pieces of 8 dims side by side
+ *   2048  K scales  [token][dim / 32]
+ *   2112  V scales  [dim / 32][token]
+ * A layer's pool is [num_blocks][n_kv][EMBER_KV4_PAGE_BYTES], K and V together. */
+#define EMBER_KV4_PAGE_BYTES 2176
+
+typedef struct EmberKv4AppendArgs {
+    const void *qkv;              /* f16 [T, (n_heads + 2 * n_kv) * 128]: q heads, k heads, v heads */
+    void *q_out;                  /* f16 [T, n_heads * 128] */
+    void *pool;                   /* this layer's pages, [num_blocks][n_kv][EMBER_KV4_PAGE_BYTES] */
+    void *k_out, *v_out;          /* f16 [T, n_kv * 128]: what the codes stand for, both or neither */
+    const float *q_norm, *k_norm; /* [128], or NULL: no QK-RMSNorm */
+    const float *bias;            /* [(n_heads + 2 * n_kv) * 128], or NULL */
+    const float *inv_freq;        /* [64] rotary frequencies */
+    const int32_t *positions;     /* [T] */
+    const int32_t *token_seq;     /* [T] the row of block_tables that each token belongs to */
+    const int32_t *block_tables;  /* [rows, max_blocks] */
+    int32_t rows, max_blocks, T, n_heads, n_kv, head_dim, num_blocks;
+    float eps;
+} EmberKv4AppendArgs;
+
+/* QK-RMSNorm, rotate-half RoPE and the write of K and V into 4-bit pages,
+ * fused. q_out is ember_hip_kv_append's bit for bit; K and V are its f32
+ * arithmetic's, clamped to +-65504, then as above. A token whose slot is not
+ * in the pool (a negative position or row, one past the tables, a block
+ * outside the pool) writes no page, but q_out, k_out and v_out. Tokens of one
+ * launch must have slots of their own (of padding rows that share one, any
+ * row's bytes may stay). qkv, q_out, k_out, v_out and the pool
+ * are 16-byte aligned; n_heads and n_kv at most 64. */
+int ember_hip_kv4_append(const EmberKv4AppendArgs *args, void *stream);
+
+typedef struct EmberKv4AttnArgs {
+    EmberRaggedBatch batch;       /* k_cache: the pool of 4-bit pages; v_cache: NULL; dtype (of q and out): f16 */
+    int32_t max_context;          /* keys of the longest sequence; more are computed, slower */
+} EmberKv4AttnArgs;
+
+/* Causal attention (keys 0..p_i of each token) of a ragged batch over 4-bit
+ * pages, as section 1b describes a batch. The workspace is zero-filled once
+ * after allocation; every launch leaves it reusable. */
+int ember_hip_kv4_attn(const EmberKv4AttnArgs *args, void *stream);
+/* Bytes of workspace ember_hip_kv4_attn uses for these sizes (only the sizes
+ * of args are read; 0: it would not split). Enough for smaller T, S, max_query
+ * and max_context too. */
+int64_t ember_hip_kv4_workspace_bytes(const EmberKv4AttnArgs *args);
+
+typedef struct EmberMxQuantizeArgs {
+    const void *x;                /* f16 or f32 [rows, ld] */
+    int64_t ld;                   /* elements between rows, at least cols */
+    int32_t rows, cols;           /* cols a multiple of 32 */
+    int32_t dtype;                /* EMBER_DTYPE_* of x */
+    uint8_t *codes;               /* [rows, cols / 2]: byte i holds columns 2i (low four bits) and 2i + 1 */
+    uint8_t *scales;              /* [rows, cols / 32] */
+} EmberMxQuantizeArgs;
+
+/* Rows to 4 bits, groups along the row. A group that holds a NaN gets scale
+ * 255 and codes 0; infinities are the largest value. x is aligned to its
+ * elements, codes to 4 bytes. */
+int ember_hip_mx_quantize(const EmberMxQuantizeArgs *args, void *stream);
+
+/* Lays out a weight [N, K] (K a multiple of 32) of codes and scales as
+ * ember_hip_mx_quantize writes them for ember_hip_gemv4: for each 16 rows and
+ * 128 columns a block of 1088 bytes, 1024 of codes (lane 16 g + c of a wave:
+ * row c, columns 32 g .. + 31) and 64 scales in lane order; rows past N and
+ * columns past K are zero. out is 16-byte aligned, of
+ * ember_hip_gemv4_packed_bytes(N, K); codes are 4-byte aligned. */
+int ember_hip_gemv4_pack(const uint8_t *codes, const uint8_t *scales, int32_t N, int32_t K, void *out, void *stream);
+int64_t ember_hip_gemv4_packed_bytes(int32_t N, int32_t K);
+
+typedef struct EmberGemv4Args {
+    const void *A;                /* f16 [M, lda] activations; 16-byte aligned rows */
+    int64_t lda;
+    const void *W;                /* of ember_hip_gemv4_pack */
+    int32_t M, N, K;              /* K a multiple of 32 */
+    void *C;                      /* [M, ldc], f16 or f32 by epilogue */
+    int64_t ldc;
+    int32_t epilogue;             /* EMBER_EPILOGUE_* */
+} EmberGemv4Args;
+
+/* ember_hip_gemv with 4-bit weights: C = epilogue(A . W^T), sums in f32. The
+ * bits of a row do not depend on the other rows or on M. Any M: prompts too. */
+int ember_hip_gemv4(const EmberGemv4Args *args, void *stream);
+
 /* Description of the last failure on this thread ("" if none). */
 const char *ember_hip_last_error(void);
 int ember_hip_abi_version(void);
@@ -476,7 +579,8 @@ int ember_hip_abi_version(void);
  * 8 EmberNormArgs, 9 EmberEmbedArgs, 10 EmberSampleParams, 11 EmberSampleArgs,
  * 12 EmberProbArgs, 13 EmberBackendOptions, 14 EmberModelInfo,
  * 15 EmberStepTablesArgs, 16 EmberRaggedBatch, 17 EmberWindowAttnArgs,
- * 18 EmberPrefixAttnArgs; -1 otherwise. */
+ * 18 EmberPrefixAttnArgs, 19 EmberKv4AppendArgs, 20 EmberKv4AttnArgs,
+ * 21 EmberMxQuantizeArgs, 22 EmberGemv4Args; -1 otherwise. */
 int32_t ember_hip_sizeof(int32_t which);
 
 /* ---- 2. KV block manager ------------------------------------------------- */
