@@ -32,8 +32,12 @@ __device__ __forceinline__ int mx_scale_byte(float m) {
     return min(max(e - 2, kMxLowest), kMxHighest);
 }
 
-// A scale byte in place as an f32 exponent; 255 becomes the infinity that the conversion takes for NaN.
-__device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+// Scale byte i of a word where the conversions look for it, at an f32's exponent (255 there is the scale NaN). They
+// look at the exponent alone (checked for all scales and codes), so the word's other bytes may stay in the other bits.
+// (`i` is known where loops are unrolled: one shift.)
+__device__ __forceinline__ float mx_scale(uint32_t word, int i = 0) {
+    return __uint_as_float(i < 3 ? word << (23 - 8 * i) : word >> 1);
+}
 
 // Eight values' codes, the first in the lowest four bits.
 __device__ __forceinline__ uint32_t mx_encode8(const float (&x)[8], float scale) {

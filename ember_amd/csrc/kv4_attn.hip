@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
 #pragma unroll
                     for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int v = 0; v < 4; v++) val[h][v] = mx_decode8(vc[i + h][v], mx_scale(vs[i + h] >> (8 * v) & 0xff));
+                        for (int v = 0; v < 4; v++) val[h][v] = mx_decode8(vc[i + h][v], mx_scale(vs[i + h], v));
                     auto tile = [&](auto index) {
                         constexpr int t = decltype(index)::value;
                         const f16x4 a = value_tile<t>(val[0]), b = value_tile<t>(val[1]);

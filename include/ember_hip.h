@@ -550,8 +550,8 @@ int ember_hip_mx_quantize(const EmberMxQuantizeArgs *args, void *stream);
 /* Lays out a weight [N, K] (K a multiple of 32) of codes and scales as
  * ember_hip_mx_quantize writes them for ember_hip_gemv4: for each 16 rows and
  * 128 columns a block of 1088 bytes, 1024 of codes (lane 16 g + c of a wave:
- * row c, columns 32 g .. + 31) and 64 scales in lane order; rows past N and
- * columns past K are zero. out is 16-byte aligned, of
+ * row c, columns 32 s + 8 g .. + 7 of s = 0 .. 3) and the scales [row][4];
+ * rows past N and columns past K are zero. out is 16-byte aligned, of
  * ember_hip_gemv4_packed_bytes(N, K); codes are 4-byte aligned. */
 int ember_hip_gemv4_pack(const uint8_t *codes, const uint8_t *scales, int32_t N, int32_t K, void *out, void *stream);
 int64_t ember_hip_gemv4_packed_bytes(int32_t N, int32_t K);

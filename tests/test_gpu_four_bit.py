@@ -406,7 +406,7 @@ def test_products_of_odd_feature_counts(rng, device, N):
     run_product(rng, device, rng.standard_normal((3, 256)).astype(np.float16), codes, scales, _lib.EPILOGUE_STORE_F32, wide=1)
 
 
-@pytest.mark.parametrize("N,k", [(48, 1056), (4096, 2048), (70000, 512)])
+@pytest.mark.parametrize("N,k", [(48, 1056), (4096, 2048), (70000, 512), (300, 4096), (200, 6144), (2100, 6144), (100, 8992)])
 def test_a_row_has_the_same_bits_in_every_batch(rng, device, N, k):
     codes, scales = weights(rng, N, k)
     w = K.gemv4_pack(on(codes, device), on(scales, device))
@@ -446,9 +446,10 @@ def test_pack_is_the_documented_layout(rng, device):
     want = np.zeros((2, 2, 1088), np.uint8)
     for n in range(21):
         for j in range(5):
-            lane = 16 * (j % 4) + n % 16
-            want[n // 16, j // 4, 16 * lane:16 * lane + 16] = codes[n, 16 * j:16 * j + 16]
-            want[n // 16, j // 4, 1024 + lane] = scales[n, j]
+            for g in range(4):
+                at = 16 * (16 * g + n % 16) + 4 * (j % 4)
+                want[n // 16, j // 4, at:at + 4] = codes[n, 16 * j + 4 * g:16 * j + 4 * g + 4]
+            want[n // 16, j // 4, 1024 + 4 * (n % 16) + j % 4] = scales[n, j]
     assert np.array_equal(got, want.reshape(-1))
 
 
