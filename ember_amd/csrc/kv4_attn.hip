@@ -31,8 +31,7 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kStepPages = 4;  // pages that a wave takes at a time
-constexpr int kMostRuns = 64;  // runs of pages of one row tile
-constexpr int kCounters = 4096;
+constexpr int kLeastUnits = 8;  // of a work-group's share
 constexpr int kRowPitch = kHeadDim + 4;  // floats of a row's partial in LDS
 
 struct Kv4Params {
@@ -40,23 +39,23 @@ struct Kv4Params {
     const uint8_t *pool;
     f16 *out;
     const int32_t *query_start, *positions, *tables;
-    float *part_acc, *part_ml;  // [item, run, row of the work-group][128], [...][2]; an item is a row tile of a kv head
-    uint32_t *counters;         // [item]
+    float *part_acc, *part_ml;  // [work-group, slot][row][128], [...][2]
+    uint32_t *counters;         // [work-group]
     int64_t q_stride;
     int T, S, max_blocks, n_heads, n_kv, G, num_blocks;
-    int tiles, runs, run_pages;
+    int workers;  // work-groups of a kv head
+    int tiles;    // entries of a sequence: its row tiles, those past the hint together in the last
+    int shift;    // a unit of their shares is 2^shift steps of pages
     float scale_log2;
 };
 
-// Partials are written and read with device-scope relaxed accesses, which are coherent across the XCDs' L2s; a
-// work-group waits for its stores before it counts itself, so what is counted is visible to the last to count.
-__device__ __forceinline__ void put2(float *p, float x, float y) {
-    const uint64_t v = __float_as_uint(x) | static_cast<uint64_t>(__float_as_uint(y)) << 32;
-    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float2 get2(const float *p) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+// Partials are written and read at device scope (sc1), which the XCDs' L2s do not keep from one another; a work-group
+// waits for its stores before it counts itself, so what is counted is visible to the last to count.
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+constexpr int kDeviceScope = 16;  // cache-policy bit sc1 of a gfx950 buffer access
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t partials(const float *base, int64_t at, int floats) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base) + at, 0, floats * static_cast<int>(sizeof(float)), kDescWord3);
 }
 
 __device__ __forceinline__ int clamped(int x, int most) { return min(max(x, 0), most); }
@@ -69,13 +68,484 @@ __device__ __forceinline__ void store_piece(f16 *dst, const float (&x)[8], float
     *reinterpret_cast<f16x8 *>(dst) = v;
 }
 
-template <int RT, bool KEYS>  // RT tiles of 16 rows a wave
+// The partials of a slot: ROWS rows of 128, and of (max, sum).
+template <int ROWS>
+struct Partials {
+    __amdgpu_buffer_rsrc_t acc, ml;
+    __device__ __forceinline__ Partials(const Kv4Params &p, int slot)
+        : acc(partials(p.part_acc, static_cast<int64_t>(slot) * ROWS * kHeadDim, ROWS * kHeadDim)),
+          ml(partials(p.part_ml, static_cast<int64_t>(slot) * ROWS * 2, ROWS * 2)) {}
+    __device__ __forceinline__ void put(int row, int dim, const float (&x)[8], float m, float l) const {
+        const int at = (row * kHeadDim + dim) * static_cast<int>(sizeof(float));
+        const u32x4 lo = {__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+        const u32x4 hi = {__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])};
+        __builtin_amdgcn_raw_buffer_store_b128(lo, acc, at, 0, kDeviceScope);
+        __builtin_amdgcn_raw_buffer_store_b128(hi, acc, at + 16, 0, kDeviceScope);
+        if (dim == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, ml, 8 * row, 0, kDeviceScope);
+    }
+    __device__ __forceinline__ float2 get_ml(int row) const {
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, 8 * row, 0, kDeviceScope));
+        return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
+    }
+    __device__ __forceinline__ u32x4 get4(int row, int dim) const {
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(acc, (row * kHeadDim + dim) * static_cast<int>(sizeof(float)), 0, kDeviceScope));
+    }
+};
+
+__device__ __forceinline__ float row16_max(float x) {
+    x = fmaxf(x, dpp_mov<kDppQuadXor1>(x));
+    x = fmaxf(x, dpp_mov<kDppQuadXor2>(x));
+    x = fmaxf(x, dpp_mov<kDppRowHalfMirror>(x));
+    return fmaxf(x, dpp_mov<kDppRowMirror>(x));
+}
+
+// Counts this work-group, whose partials are written, and says whether it is the last of n. Leaves the counter at 0.
+__device__ __forceinline__ bool last_of(uint32_t *counter, int n, bool &last) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<uint32_t>(n);
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return last;
+}
+
+// Joins n partials of nrows rows, slot_of(0) .. slot_of(n - 1) in that order, kMergePieces at a time. 16 lanes share a
+// row, 8 dims each; where the rows leave threads over, groups of them take every groups-th partial, and their sums are
+// added in group order.
+constexpr int kMergePieces = 32;
+constexpr int merge_floats(int rows, int threads) { return 2 * rows * kMergePieces + threads * 8; }
+
+template <int ROWS, int THREADS, typename Slot, typename At>
+__device__ __forceinline__ void merge_partials(const Kv4Params &p, int n, int nrows, float *lds, Slot slot_of, At at_of) {
+    constexpr int kPitch = kMergePieces;
+    float *const top = lds, *const sum = top + ROWS * kPitch, *const x_lds = sum + ROWS * kPitch;  // [row][partial]
+    const int tid = static_cast<int>(threadIdx.x), lanes = nrows * 16;
+    const int groups = max(1, THREADS / lanes), group = groups > 1 ? tid / lanes : 0;
+    for (int i0 = 0; i0 < lanes; i0 += THREADS) {  // (one round where there are groups)
+        const int i = i0 + (groups > 1 ? tid % lanes : tid);
+        const bool mine = i < lanes && group < groups;
+        const int row = min(i / 16, nrows - 1), dim = i % 16 * 8;
+        float M = kNoKeys, L = 0.0f, x[8] = {};
+        for (int n0 = 0; n0 < n; n0 += kMergePieces) {
+            const int some = min(kMergePieces, n - n0);
+            __syncthreads();
+            for (int k = tid; k < nrows * some; k += THREADS) {
+                const float2 ml = Partials<ROWS>(p, slot_of(n0 + k / nrows)).get_ml(k % nrows);
+                top[k % nrows * kPitch + k / nrows] = ml.x, sum[k % nrows * kPitch + k / nrows] = ml.y;
+            }
+            __syncthreads();
+            // Lane i % 16 of a row takes every 16th of its weights.
+            float now = M;
+#pragma unroll
+            for (int k = 0; k < kMergePieces; k += 16)
+                if (const int at = k + i % 16; at < some) now = fmaxf(now, top[row * kPitch + at]);
+            now = row16_max(now);
+            const float corr = exp2_hw(M - now);
+            M = now;
+            L = L * corr;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = x[e] * corr;
+            float add = 0.0f, weight[kMergePieces / 16];
+#pragma unroll
+            for (int k = 0; k < kMergePieces; k += 16) {
+                const int at = row * kPitch + min(k + i % 16, some - 1);
+                weight[k / 16] = filled(sum[at]) ? exp2_hw(top[at] - M) : 0.0f;
+                add = add + (k + i % 16 < some ? sum[at] * weight[k / 16] : 0.0f);
+            }
+            L = L + row16_sum(add);
+            __syncthreads();
+            if (mine && group == 0)
+#pragma unroll
+                for (int k = 0; k < kMergePieces; k += 16) top[row * kPitch + k + i % 16] = weight[k / 16];
+            __syncthreads();
+            constexpr int kInFlight = 4;
+            for (int k0 = group; k0 < some && mine; k0 += groups * kInFlight) {
+                u32x4 part[kInFlight][2];
+#pragma unroll
+                for (int f = 0; f < kInFlight; f++) {
+                    const Partials<ROWS> from(p, slot_of(n0 + min(k0 + f * groups, some - 1)));
+                    part[f][0] = from.get4(row, dim), part[f][1] = from.get4(row, dim + 4);
+                }
+#pragma unroll
+                for (int f = 0; f < kInFlight; f++) {
+                    if (k0 + f * groups >= some) break;
+                    const float w = top[row * kPitch + k0 + f * groups];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = x[e] + __uint_as_float(part[f][e / 4][e % 4]) * w;
+                }
+            }
+        }
+        if (groups > 1) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x_lds[e * THREADS + tid] = x[e];
+            __syncthreads();
+            if (group == 0)
+                for (int k = 1; k < groups; k++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = x[e] + x_lds[e * THREADS + k * lanes + i];
+        }
+        if (mine && group == 0) store_piece(p.out + at_of(row) * kHeadDim + dim, x, L);
+    }
+}
+
+// How U units of work are shared out: worker j of n takes units start(j) .. start(j + 1) - 1, but a start that lies
+// within `near` units of an item's border moves to the nearer one: a cut item costs its partials and a merge.
+struct Shares {
+    int each, more, near;  // `more` of the workers take one unit more than `each`
+    __device__ __forceinline__ Shares(int units, int workers)
+        : each(units / workers), more(units - each * workers), near(max(1, each / 8)) {}
+    __device__ __forceinline__ Shares(int each, int more, int near) : each(each), more(more), near(near) {}
+    __device__ __forceinline__ int start(int j) const { return j * each + min(j, more); }
+    __device__ __forceinline__ int worker_of(int unit) const {
+        const int high = more * (each + 1);
+        return unit < high ? unit / (each + 1) : more + (unit - high) / each;
+    }
+    // A start x within the item of units a .. b - 1.
+    __device__ __forceinline__ int moved(int x, int a, int b) const {
+        if (x - a <= near && x - a <= b - x) return a;
+        return b - x <= near ? b : x;
+    }
+};
+
+// Up to 16 RT rows a work-group, W waves that take turns at steps of P pages.
+//
+// A CU takes in about 27 GB/s, however many waves ask, so all of them have to
+// have the same share of the pages. A sequence's row tiles are items of as many
+// units as its context has steps; a kv head's work-groups take equal runs of
+// the units of all items, found by each wave for itself from the sequences'
+// lengths: 64 sequences a load, a scan over the lanes. An item that lies in
+// several runs is joined by the last of its work-groups.
+//
+// The pages of a wave's next step are on their way during a whole step.
+template <int RT, int W, int P>
+__global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
+    constexpr int D = kHeadDim, kRows = 16 * RT, kThreads = W * kWave;
+    constexpr int kLdsFloats = W * kRows * (kRowPitch + 2);
+    static_assert(merge_floats(kRows, kThreads) <= kLdsFloats);
+    __shared__ __align__(16) float lds[kLdsFloats];
+    __shared__ bool last;
+    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
+    const int g = lane >> 4, c = lane & 15;
+    const int kvh = static_cast<int>(blockIdx.x) % p.n_kv, worker = static_cast<int>(blockIdx.x) / p.n_kv;
+    const int table_top = p.max_blocks * kPage - 1;
+    const uint8_t *const pool = p.pool + kvh * kKv4Page;
+    const uint32_t block_bytes = static_cast<uint32_t>(p.n_kv) * kKv4Page;
+
+    __builtin_amdgcn_s_setprio(3);  // up to the first pages, which the CU's other waves would delay
+    // Lane i: entry 64 chunk + i, a row tile of a sequence (the sequence's last entry: all that are left, alike). Its
+    // sequence's first token and rows, the entry's first tile and number of them, their highest key and units each.
+    int seq_t0, seq_rows, first_tile, n_tiles, entry_top, entry_units;
+    auto load_entry = [&](int e) {
+        const int at = min(p.tiles == 1 ? e : e / p.tiles, p.S - 1), k = p.tiles == 1 ? 0 : e - at * p.tiles;
+        const int guess = p.positions[min(at, p.T - 1)];  // the last position of a sequence of a pure decode step
+        const int t0 = clamped(p.query_start[at], p.T), t1 = min(max(p.query_start[at + 1], t0), p.T);
+        int pos = guess;
+        if (__builtin_amdgcn_ballot_w64(t1 - 1 != at)) pos = p.positions[max(t1 - 1, 0)];
+        seq_t0 = t0, seq_rows = (t1 - t0) * p.G;
+        const int all = e < p.S * p.tiles ? (seq_rows + kRows - 1) / kRows : 0;
+        first_tile = k, n_tiles = k == p.tiles - 1 ? max(all - k, 0) : k < all ? 1 : 0;
+        // Positions count up: those behind the tile's last row are known from the sequence's last.
+        if (p.tiles > 1 && k < p.tiles - 1) pos = max(pos, -1) - (max(seq_rows - 1, 0) / p.G - (min((k + 1) * kRows, max(seq_rows, 1)) - 1) / p.G);
+        entry_top = min(max(pos, -1), table_top);
+        const int steps = max(1, (entry_top + P * kPage) / (P * kPage));
+        entry_units = (steps + (1 << p.shift) - 1) >> p.shift;
+        return n_tiles * entry_units;
+    };
+    auto scan = [&](int x) {  // inclusive, over the lanes
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int y = __shfl_up(x, o, kWave);
+            x += lane >= o ? y : 0;
+        }
+        return x;
+    };
+    int chunk = 0, upto, before = 0, in_chunk = 0;  // units up to this lane's entry and before the chunk; the entry's lane
+    int workers = p.workers, begin = 0, end, slots = 0;
+    int each = 0, more = 0, near = 0;
+    const int chunks = (p.S * p.tiles + kWave - 1) / kWave;
+    if (workers == 0) {  // a work-group an entry
+        upto = load_entry(worker);
+        end = upto = uniform(upto);
+        chunk = worker / kWave, in_chunk = worker % kWave;
+        near = end;
+    } else {
+        upto = scan(load_entry(lane));
+        int units = __builtin_amdgcn_readlane(upto, kWave - 1), chunk_units = units;
+        if (chunks > 1) {  // lane k: the units of chunk k
+            for (int k = 1; k < chunks; k++) {
+                const int sum = __builtin_amdgcn_readlane(scan(load_entry(k * kWave + lane)), kWave - 1);
+                chunk_units = lane == k ? sum : chunk_units;
+            }
+            chunk_units = scan(lane < chunks ? chunk_units : 0);
+            units = __builtin_amdgcn_readlane(chunk_units, kWave - 1);
+        }
+        workers = min(workers, max(1, units / kLeastUnits));
+        if (worker >= workers) return;
+        const Shares shares(units, workers);
+        each = shares.each, more = shares.more, near = shares.near;
+        begin = shares.start(worker), end = shares.start(worker + 1);
+        if (chunks > 1) {  // the chunk of the first unit
+            chunk = __popcll(__builtin_amdgcn_ballot_w64(lane < chunks && chunk_units <= begin));
+            before = chunk > 0 ? __builtin_amdgcn_readlane(chunk_units, chunk - 1) : 0;
+            upto = scan(load_entry(chunk * kWave + lane));
+        }
+        in_chunk = __popcll(__builtin_amdgcn_ballot_w64(before + upto <= begin));  // the first unit's entry
+        slots = 2 * kvh * p.workers;
+    }
+    const Shares shares(each, more, near);
+
+    for (int x = begin; x < end;) {
+        if (in_chunk == kWave) {
+            before += __builtin_amdgcn_readlane(upto, kWave - 1);
+            if (++chunk >= chunks) return;
+            upto = scan(load_entry(chunk * kWave + lane));
+            in_chunk = 0;
+        }
+        const int entry_end = before + __builtin_amdgcn_readlane(upto, in_chunk);
+        if (entry_end <= x) {
+            in_chunk++;
+            continue;
+        }
+        const int entry = chunk * kWave + in_chunk, seq = p.tiles == 1 ? entry : entry / p.tiles;
+        const int t0 = __builtin_amdgcn_readlane(seq_t0, in_chunk), rows = __builtin_amdgcn_readlane(seq_rows, in_chunk);
+        // The item is units a .. b - 1, the `left`th of the entry's from its end; this work-group's part of it x .. stop - 1.
+        const int item_units = __builtin_amdgcn_readlane(entry_units, in_chunk), tiles = __builtin_amdgcn_readlane(n_tiles, in_chunk);
+        const int left = tiles == 1 ? 1 : (entry_end - x + item_units - 1) / item_units;
+        const int tile = __builtin_amdgcn_readlane(first_tile, in_chunk) + tiles - left;
+        const int b = entry_end - (left - 1) * item_units, a = b - item_units;
+        if (x == begin) {
+            x = shares.moved(x, a, b);
+            if (x == b) continue;  // the one before takes it
+        }
+        const int stop = end >= b ? b : shares.moved(end, a, b);
+        if (stop == a) return;
+        const bool whole = x == a && stop == b;
+
+        const int row0 = tile * kRows, nrows = min(kRows, rows - row0);
+        const int32_t *const table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
+        // Step i of this wave: pages (wave + i W) P .. of the part; lane P i + j holds the id of its page j.
+        constexpr int kAhead = kWave / P;
+        const int v0 = ((x - a) << p.shift) * P;
+        const int lane_page = (wave + lane / P * W) * P + lane % P;
+        auto id_at = [&](int page) { return page < p.max_blocks ? table[page] : -1; };
+        const int first_ids = id_at(v0 + lane_page);
+        // Positions count up, so the first and last rows bound them.
+        auto top_of = [&](int row) { return min(max(p.positions[t0 + (row0 + row) / p.G], -1), table_top); };
+        const bool one_token = rows == p.G;
+        int my_top[RT];
+        u32x4 qf[RT][4];
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const int row = min(16 * r + c, nrows - 1);
+            const f16 *const qp = p.q + (t0 + (row0 + row) / p.G) * p.q_stride + (kvh * p.G + (row0 + row) % p.G) * D + 32 * g;
+#pragma unroll
+            for (int s = 0; s < 4; s++) qf[r][s] = *reinterpret_cast<const u32x4 *>(qp + 8 * s);
+        }
+        int min_top = __builtin_amdgcn_readlane(entry_top, in_chunk), max_top = min_top;
+        if (one_token) {
+#pragma unroll
+            for (int r = 0; r < RT; r++) my_top[r] = max_top;
+        } else {
+#pragma unroll
+            for (int r = 0; r < RT; r++) my_top[r] = top_of(min(16 * r + c, nrows - 1));
+            min_top = uniform(top_of(0)), max_top = uniform(top_of(nrows - 1));
+        }
+        const int pages = (max_top + kPage) / kPage;
+        const int v1 = stop == b ? pages : min(((stop - a) << p.shift) * P, pages);
+
+        float m[RT], l[RT];
+        f32x4 o[RT][8];  // o[t][v]: dim 32 g + 8 v + t of column c
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            m[r] = kNoKeys, l[r] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 8; t++) o[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const int steps = max(0, v1 - v0 + P - 1) / P;
+        for (int step0 = wave; step0 < steps; step0 += W * kAhead) {
+            const int page_base = v0 + (step0 - wave) * P;
+            const int my_page = page_base + lane_page;
+            int ids = step0 == wave ? first_ids : id_at(my_page);
+            ids = my_page < v1 ? ids : -1;
+            const int n = min(kAhead, (steps - step0 + W - 1) / W);
+            struct Step {
+                u32x4 kc[P], vc[P];
+                uint32_t ks[P], vs[P];
+            };
+            // A page that is not there, or past the part's last, has no records: its loads give zeros.
+            auto fetch = [&](Step &to, int j) {
+#pragma unroll
+                for (int i = 0; i < P; i++) {
+                    const uint32_t block = j < kAhead ? __builtin_amdgcn_readlane(ids, (j * P + i) % kWave) : ~0u;
+                    const bool ok = block < static_cast<uint32_t>(p.num_blocks);
+                    const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool) + static_cast<uint64_t>(ok ? block : 0) * block_bytes, 0,
+                                                                     ok ? kKv4Page : 0, kDescWord3);
+                    to.kc[i] = load_desc(d, 64 * c + 16 * g);
+                    to.ks[i] = __builtin_amdgcn_raw_buffer_load_b8(d, kKv4KeyScales + 4 * c + g, 0, kNonTemporal);
+                    to.vc[i] = load_desc(d, kKv4Values + 16 * lane);
+                    to.vs[i] = __builtin_amdgcn_raw_buffer_load_b32(d, kKv4ValueScales + kPage * (c / 4) + 4 * g, 0, kNonTemporal);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            // Step j, with the next one's pages on their way.
+            auto consume = [&](Step &at, Step &next, int j) {
+                fetch(next, j + 1);
+                f32x4 s[RT][P];
+                // Two pages' chains of products at a time, each of which would wait for itself.
+#pragma unroll
+                for (int i0 = 0; i0 < P; i0 += 2) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+#pragma unroll
+                        for (int i = i0; i < i0 + 2; i++) {
+                            const f16x8 kf = as_f16x8(mx_decode8(at.kc[i][w], mx_scale(at.ks[i])));
+#pragma unroll
+                            for (int r = 0; r < RT; r++)
+                                s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, as_f16x8(qf[r][w]), w == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[r][i], 0, 0, 0);
+                        }
+                }
+                const int key0 = (page_base + (wave + j * W) * P) * kPage;
+                if (key0 + P * kPage - 1 > min_top) {  // some row does not see all of these keys
+#pragma unroll
+                    for (int i = 0; i < P; i++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++) {
+                            const int key = key0 + i * kPage + 4 * g + v;
+#pragma unroll
+                            for (int r = 0; r < RT; r++) s[r][i][v] = key <= my_top[r] ? s[r][i][v] : -INFINITY;
+                            // Keys that no row sees may hold anything: their scales are taken as 2^-127, their values so as 0.
+                            if (key > max_top) at.vs[i] &= ~(0xffu << (8 * v));
+                        }
+                }
+                f16x8 wh[RT][P / 2];
+#pragma unroll
+                for (int r = 0; r < RT; r++) {
+                    float top = s[r][0][0];
+#pragma unroll
+                    for (int i = 0; i < P; i++)
+#pragma unroll
+                        for (int v = 0; v < 4; v++) top = fmaxf(top, s[r][i][v]);
+                    top = top * p.scale_log2;
+                    if (__builtin_amdgcn_ballot_w64(top - m[r] > kMostExponent)) {  // seldom: the reference moves
+                        const float row_top = groups_max(top);
+                        const bool grow = row_top - m[r] > kMostExponent;
+                        const float reference = below(row_top, kMostExponent - kLazy);
+                        const float corr = grow ? exp2_hw(m[r] - reference) : 1.0f;  // 0 from a row that had seen nothing
+                        m[r] = grow ? reference : m[r];
+                        l[r] = l[r] * corr;
+#pragma unroll
+                        for (int t = 0; t < 8; t++) o[r][t] = o[r][t] * corr;
+                    }
+                    float mul = p.scale_log2, add = -m[r];
+                    if (const bool far = fabsf(add) >= kFar; __builtin_amdgcn_ballot_w64(far)) {
+#pragma unroll
+                        for (int i = 0; i < P; i++)
+#pragma unroll
+                            for (int v = 0; v < 4; v++) s[r][i][v] = far ? s[r][i][v] * mul + add : __builtin_fmaf(s[r][i][v], mul, add);
+                        mul = 1.0f, add = 0.0f;
+                    }
+                    const f16x2 ones = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+#pragma unroll
+                    for (int i = 0; i < P; i++) {
+#pragma unroll
+                        for (int v = 0; v < 4; v++) wh[r][i / 2][i % 2 * 4 + v] = static_cast<f16>(exp2_hw(__builtin_fmaf(s[r][i][v], mul, add)));
+#pragma unroll
+                        for (int v = 0; v < 4; v += 2)
+                            l[r] = __builtin_amdgcn_fdot2(f16x2{wh[r][i / 2][i % 2 * 4 + v], wh[r][i / 2][i % 2 * 4 + v + 1]}, ones, l[r], false);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < P; i += 2) {
+                    // Dims 2 b and 2 b + 1 of the lane's eight are byte b of its keys' words.
+                    auto pair = [&](auto byte) {
+                        constexpr int b = decltype(byte)::value;
+                        uint32_t x[2][4];  // [page][key % 4]
+#pragma unroll
+                        for (int h = 0; h < 2; h++)
+#pragma unroll
+                            for (int v = 0; v < 4; v++)
+                                x[h][v] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(at.vc[i + h][v], mx_scale(at.vs[i + h], v), b));
+#pragma unroll
+                        for (int odd = 0; odd < 2; odd++) {
+                            const uint32_t sel = odd ? 0x07060302u : 0x05040100u;  // high or low halves of two keys
+                            const u32x4 vt = {__builtin_amdgcn_perm(x[0][1], x[0][0], sel), __builtin_amdgcn_perm(x[0][3], x[0][2], sel),
+                                              __builtin_amdgcn_perm(x[1][1], x[1][0], sel), __builtin_amdgcn_perm(x[1][3], x[1][2], sel)};
+#pragma unroll
+                            for (int r = 0; r < RT; r++)
+                                o[r][2 * b + odd] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(vt), wh[r][i / 2], o[r][2 * b + odd], 0, 0, 0);
+                        }
+                    };
+                    pair(std::integral_constant<int, 0>{}), pair(std::integral_constant<int, 1>{});
+                    pair(std::integral_constant<int, 2>{}), pair(std::integral_constant<int, 3>{});
+                }
+            };
+            Step one, two;
+            fetch(one, 0);
+            __builtin_amdgcn_s_setprio(0);
+            for (int j = 0; j < n; j += 2) {
+                consume(one, two, j);
+                if (j + 1 >= n) break;
+                consume(two, one, j + 1);
+            }
+        }
+        __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+        for (int r = 0; r < RT; r++) l[r] = groups_sum(l[r]);
+
+        // The row's place in out.
+        auto at_of = [&](int row) {
+            return static_cast<int64_t>(t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
+        };
+        float *const red_m = lds + W * kRows * kRowPitch, *const red_l = red_m + W * kRows;
+        __syncthreads();  // of the rows before these
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            const int row = 16 * r + c;
+            float *const dst = lds + (wave * kRows + row) * kRowPitch + 32 * g;
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                *reinterpret_cast<f32x4 *>(dst + 8 * v) = f32x4{o[r][0][v], o[r][1][v], o[r][2][v], o[r][3][v]};
+                *reinterpret_cast<f32x4 *>(dst + 8 * v + 4) = f32x4{o[r][4][v], o[r][5][v], o[r][6][v], o[r][7][v]};
+            }
+            if (g == 0) red_m[wave * kRows + row] = m[r], red_l[wave * kRows + row] = l[r];
+        }
+        __syncthreads();
+        // A work-group has two slots: for an item that it begins, and for one that began before it.
+        const Partials<kRows> mine(p, slots + 2 * worker + (x == a ? 1 : 0));
+        for (int i = tid; i < nrows * 16; i += kThreads) {
+            const int row = i / 16, dim = i % 16 * 8;
+            float M = kNoKeys, L = 0.0f, x[8] = {};
+#pragma unroll
+            for (int w = 0; w < W; w++) M = fmaxf(M, red_m[w * kRows + row]);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                const float part = red_l[w * kRows + row], f = filled(part) ? exp2_hw(red_m[w * kRows + row] - M) : 0.0f;
+                L = L + part * f;
+                const float *const src = lds + (w * kRows + row) * kRowPitch + dim;
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = x[e] + src[e] * f;
+            }
+            if (whole) store_piece(p.out + at_of(row) * D + dim, x, L);
+            else mine.put(row, dim, x, M, L);
+        }
+        if (!whole) {
+            int from = shares.worker_of(a), to = shares.worker_of(b - 1);  // the item's work-groups
+            if (from + 1 < workers && shares.start(from + 1) < b && shares.moved(shares.start(from + 1), a, b) == a) from++;
+            if (to > 0 && shares.start(to) >= a && shares.moved(shares.start(to), a, b) == b) to--;
+            if (last_of(p.counters + kvh * p.workers + from, to - from + 1, last))
+                merge_partials<kRows, kThreads>(p, to - from + 1, nrows, lds, [&](int k) { return slots + 2 * (from + k) + (k == 0 ? 1 : 0); }, at_of);
+        }
+        x = b;
+        if (stop != b) return;
+    }
+}
+
+template <int RT>
 __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
     constexpr int D = kHeadDim;
-    constexpr int kRows = 16 * RT * (KEYS ? 1 : kWaves);  // rows of a work-group
-    constexpr int kLdsFloats = KEYS ? kWaves * 16 * RT * (kRowPitch + 2) : 2 * kRows;
-    __shared__ float lds[kLdsFloats];
-    __shared__ bool last;
+    constexpr int kRows = 16 * RT * (kWaves);  // rows of a work-group
     const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
     const int g = lane >> 4, c = lane & 15;
     int rest = static_cast<int>(blockIdx.x);
@@ -83,21 +553,17 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
     rest /= p.n_kv;
     const int tile0 = rest % p.tiles;
     rest /= p.tiles;
-    const int run = rest % p.runs, seq = rest / p.runs;
-    const int64_t item = (static_cast<int64_t>(seq) * p.tiles + tile0) * p.n_kv + kvh;
+    const int seq = rest;
 
     const int t0 = clamped(uniform_load(p.query_start + seq), p.T);
     const int t1 = min(max(uniform_load(p.query_start + seq + 1), t0), p.T);
     const int rows = (t1 - t0) * p.G;
-    // More rows than the launch was shaped for: the first run's work-groups take all of them, uncut.
-    const bool cut = p.runs > 1 && rows <= p.tiles * kRows;
-    if (!cut && run > 0) return;
     const int32_t *const table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
     const int table_top = p.max_blocks * kPage - 1;
 
     for (int row0 = tile0 * kRows; row0 < rows; row0 += p.tiles * kRows) {
         const int nrows = min(kRows, rows - row0);
-        const int wave_row = KEYS ? 0 : wave * 16 * RT;
+        const int wave_row = wave * 16 * RT;
         // Positions count up, so a wave's first and last rows bound them.
         auto pos_of = [&](int r) { return p.positions[t0 + (row0 + min(r, nrows - 1)) / p.G]; };
         auto top_of = [&](int r) { return min(max(pos_of(r), -1), table_top); };
@@ -112,11 +578,8 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
             for (int s = 0; s < 4; s++) qf[r][s] = *reinterpret_cast<const u32x4 *>(qp + 8 * s);
         }
         const int min_top = uniform(top_of(wave_row)), max_top = uniform(top_of(wave_row + 16 * RT - 1));
-        const int group_pages = (uniform(top_of(kRows - 1)) + kPage) / kPage;  // of the work-group
-        const int active = cut ? max(1, (group_pages + p.run_pages - 1) / p.run_pages) : 1;
-        if (run >= active) return;
         const int pages = (max_top + kPage) / kPage;
-        const int v0 = cut ? run * p.run_pages : 0, v1 = cut ? min(v0 + p.run_pages, pages) : pages;
+        const int v0 = 0, v1 = pages;
 
         float m[RT], l[RT];
         f32x4 o[RT][8];
@@ -126,10 +589,10 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
 #pragma unroll
             for (int t = 0; t < 8; t++) o[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        constexpr int kStride = KEYS ? kWaves : 1;
+        constexpr int kStride = 1;
         constexpr int kAhead = kWave / kStepPages;  // steps whose block ids a register holds
         const int steps = max(0, v1 - v0 + kStepPages - 1) / kStepPages;
-        for (int step0 = KEYS ? wave : 0; step0 < steps; step0 += kStride * kAhead) {
+        for (int step0 = 0; step0 < steps; step0 += kStride * kAhead) {
             const int my_page = v0 + (step0 + lane / kStepPages * kStride) * kStepPages + lane % kStepPages;
             const int ids = my_page < v1 ? table[my_page] : -1;
             const int n = min(kAhead, (steps - step0 + kStride - 1) / kStride);
@@ -234,44 +697,7 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
         auto at_of = [&](int row) {
             return static_cast<int64_t>(t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
         };
-        auto emit = [&](int row, int dim, const float (&x)[8], float row_m, float row_l) {
-            if (active == 1) return store_piece(p.out + at_of(row) * D + dim, x, row_l);
-            const int64_t slot = (item * p.runs + run) * kRows + row;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) put2(p.part_acc + slot * D + dim + i, x[i], x[i + 1]);
-            if (dim == 0) put2(p.part_ml + slot * 2, row_m, row_l);
-        };
-        if constexpr (KEYS) {
-            float *const red_m = lds + kWaves * kRows * kRowPitch, *const red_l = red_m + kWaves * kRows;
-            __syncthreads();  // of the rows before these
-#pragma unroll
-            for (int r = 0; r < RT; r++) {
-                const int row = 16 * r + c;
-                float *const dst = lds + (wave * kRows + row) * kRowPitch + 32 * g;
-#pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    *reinterpret_cast<f32x4 *>(dst + 8 * v) = f32x4{o[r][0][v], o[r][1][v], o[r][2][v], o[r][3][v]};
-                    *reinterpret_cast<f32x4 *>(dst + 8 * v + 4) = f32x4{o[r][4][v], o[r][5][v], o[r][6][v], o[r][7][v]};
-                }
-                if (g == 0) red_m[wave * kRows + row] = m[r], red_l[wave * kRows + row] = l[r];
-            }
-            __syncthreads();
-            for (int i = tid; i < nrows * 16; i += kThreads) {
-                const int row = i / 16, dim = i % 16 * 8;
-                float M = kNoKeys, L = 0.0f, x[8] = {};
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) M = fmaxf(M, red_m[w * kRows + row]);
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) {
-                    const float part = red_l[w * kRows + row], f = filled(part) ? exp2_hw(red_m[w * kRows + row] - M) : 0.0f;
-                    L = L + part * f;
-                    const float *const src = lds + (w * kRows + row) * kRowPitch + dim;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = x[e] + src[e] * f;
-                }
-                emit(row, dim, x, M, L);
-            }
-        } else {
+        {
 #pragma unroll
             for (int r = 0; r < RT; r++) {
                 const int row = wave_row + 16 * r + c;
@@ -279,72 +705,47 @@ __global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
 #pragma unroll
                     for (int v = 0; v < 4; v++) {
                         const float x[8] = {o[r][0][v], o[r][1][v], o[r][2][v], o[r][3][v], o[r][4][v], o[r][5][v], o[r][6][v], o[r][7][v]};
-                        emit(row, 32 * g + 8 * v, x, m[r], l[r]);
+                        store_piece(p.out + at_of(row) * D + 32 * g + 8 * v, x, l[r]);
                     }
             }
         }
-        if (active == 1) continue;
-
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t *const counter = p.counters + item;
-            last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == static_cast<uint32_t>(active);
-            if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        __syncthreads();
-        if (!last) return;
-        for (int i = tid; i < nrows * 16; i += kThreads) {
-            const int row = i / 16, dim = i % 16 * 8;
-            const int64_t slot0 = item * p.runs * kRows + row;  // and one every kRows
-            float M = kNoKeys, L = 0.0f, x[8] = {};
-            for (int s = 0; s < active; s++) M = fmaxf(M, get2(p.part_ml + (slot0 + s * kRows) * 2).x);
-            for (int s = 0; s < active; s++) {
-                const float2 ml = get2(p.part_ml + (slot0 + s * kRows) * 2);
-                const float f = filled(ml.y) ? exp2_hw(ml.x - M) : 0.0f;
-                L = L + ml.y * f;
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const float2 a = get2(p.part_acc + (slot0 + s * kRows) * D + dim + e);
-                    x[e] = x[e] + a.x * f, x[e + 1] = x[e + 1] + a.y * f;
-                }
-            }
-            store_piece(p.out + at_of(row) * D + dim, x, L);
-        }
-        return;  // a cut step has one tile a work-group
     }
 }
 
 // ---- host ----
 
-constexpr int64_t kMostGroups = 1 << 20;                   // row tiles of a launch beyond which work-groups take several
-constexpr int64_t kMostLaunch = UINT32_MAX / kThreads;     // HIP's bound on a launch's threads
-constexpr int kWant = 1024;                                // work-groups that fill the chip
+constexpr int64_t kMostLaunch = UINT32_MAX / kThreads;  // HIP's bound on a launch's threads
+constexpr int kMostSequences = 4096;                    // of a launch: a lane for each 64 of them
+constexpr int kCus = 256;
+constexpr int kWalkGroups = 2 * kCus;  // that share out a long context
 
 struct Plan {
-    int rows = 16;  // of a work-group
-    int tiles = 1, runs = 1, run_pages = 1;
-    int most_runs = 1;  // for any number of sequences
+    int rows;       // of a work-group: 16, 32 or 128
+    int tiles;      // entries of a sequence
+    int workers;    // work-groups of a kv head that share out its items; 0: one an entry
+    int64_t bytes;  // of the workspace, with which items may be cut
 };
 
-constexpr int kForms[] = {16, 32, 128};  // rows of a work-group
+// Whether the work-groups share the items out evenly, or take one each. Sharing costs a scan of the lengths, partials
+// and their merge; not sharing, the wait for the longest item. A work-group of its own takes 64 keys a wave in 0.95 us;
+// all of them together 6.9 TB/s. Measured, us, one each and shared: 1 sequence of 4000 keys 19.1, 10.7; of 131,000 477,
+// 32; 4 of up to 3000 16.0, 13.6; 8 of 1000 9.2, 9.9; 32 of up to 4096 21.4, 24.4; 8 of up to 131,000 444, 125.
+bool share_out(int64_t items, int64_t keys) {
+    const double steps = static_cast<double>((keys + 63) / 64);
+    return steps / kWaves * 0.95 > items * steps * 0.00126 + 7.0;
+}
 
-int64_t partial_bytes(int64_t groups, int rows) { return kCounters * 4 + groups * rows * (kHeadDim + 2) * 4; }
-
-// The plan for at most `most` rows of a sequence and a kv head.
-Plan plan(const EmberKv4AttnArgs &a, int64_t most, int64_t room) {
+Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences) {
     const EmberRaggedBatch &b = a.batch;
-    Plan l;
+    Plan l{};
     l.rows = most <= 16 ? 16 : most <= 32 ? 32 : 128;
-    const int64_t units = static_cast<int64_t>(b.S) * b.n_kv;
-    l.tiles = static_cast<int>(std::clamp<int64_t>((most + l.rows - 1) / l.rows, 1, std::max<int64_t>(1, kMostGroups / units)));
-    const int pages = std::min(b.max_blocks, a.max_context / kPage + 1);
-    const int64_t items = units * l.tiles;
-    l.most_runs = std::clamp(pages / (kStepPages * 4), 1, kMostRuns);
-    int64_t runs = items > kCounters ? 1 : std::clamp<int64_t>(kWant / items, 1, l.most_runs);
-    while (runs > 1 && partial_bytes(items * runs, l.rows) > room) runs--;
-    l.run_pages = static_cast<int>((pages + runs * kStepPages - 1) / (runs * kStepPages)) * kStepPages;  // a step is of one run
-    l.runs = (pages + l.run_pages - 1) / l.run_pages;
+    l.tiles = static_cast<int>(std::clamp<int64_t>((most + l.rows - 1) / l.rows, 1, std::max(1, kMostSequences / sequences)));
+    const int64_t keys = std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage);
+    if (l.rows < 128 && share_out(static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys)) {
+        // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
+        l.workers = std::max(1, std::min(kWalkGroups / b.n_kv, 32 * sequences));
+        l.bytes = static_cast<int64_t>(l.workers) * b.n_kv * (4 + 2 * l.rows * (kHeadDim + 2) * 4);
+    }
     return l;
 }
 
@@ -352,42 +753,55 @@ int64_t most_rows(const EmberRaggedBatch &b) { return static_cast<int64_t>(std::
 
 }  // namespace
 
-// Cut launches have at most kWant work-groups, and as many as the sequences' items and runs give: the largest of what each
-// form up to this one could use.
+// Of these sizes and of smaller batches: fewer sequences may be shared out where these are not, with a form of fewer rows.
 int64_t kv4_workspace_bytes(const EmberKv4AttnArgs &a) {
     const int64_t most = most_rows(a.batch);
     int64_t bytes = 0;
-    for (int rows : kForms) {
-        const Plan l = plan(a, std::min<int64_t>(most, rows == 128 ? most : rows), 0);
-        const int64_t groups = std::min<int64_t>(kWant, static_cast<int64_t>(a.batch.S) * a.batch.n_kv * l.tiles * l.most_runs);
-        if (l.most_runs > 1 && a.batch.n_kv * 2 <= kWant) bytes = std::max(bytes, partial_bytes(groups, l.rows));
-    }
+    for (int64_t rows : {int64_t{16}, int64_t{32}})
+        for (int sequences = 1; sequences <= std::min(a.batch.S, kWalkGroups); sequences *= 2)
+            bytes = std::max(bytes, plan(a, std::min(most, rows), sequences).bytes);
     return bytes;
 }
 
 int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
     const EmberRaggedBatch &b = a.batch;
-    const Plan l = plan(a, most_rows(b), b.workspace ? b.workspace_bytes : 0);
-    const int64_t groups = static_cast<int64_t>(b.S) * b.n_kv * l.tiles * l.runs;
-    if (groups > kMostLaunch)
-        return set_error(EMBER_ERR_INVALID, "kv4_attn: too many work-groups for one launch (S %d x n_kv %d)", b.S, b.n_kv);
     Kv4Params p{};
     p.q = static_cast<const f16 *>(b.q), p.pool = static_cast<const uint8_t *>(b.k_cache), p.out = static_cast<f16 *>(b.out);
-    p.query_start = b.query_start, p.positions = b.positions, p.tables = b.block_tables;
+    p.positions = b.positions;
     p.q_stride = b.q_stride;
-    p.T = b.T, p.S = b.S, p.max_blocks = b.max_blocks, p.n_heads = b.n_heads, p.n_kv = b.n_kv, p.G = b.n_heads / b.n_kv;
+    p.T = b.T, p.max_blocks = b.max_blocks, p.n_heads = b.n_heads, p.n_kv = b.n_kv, p.G = b.n_heads / b.n_kv;
     p.num_blocks = b.num_blocks;
-    p.tiles = l.tiles, p.runs = l.runs, p.run_pages = l.run_pages;
-    if (l.runs > 1) {
-        p.counters = static_cast<uint32_t *>(b.workspace);
-        p.part_acc = reinterpret_cast<float *>(p.counters + kCounters);
-        p.part_ml = p.part_acc + groups * l.rows * kHeadDim;
-    }
     p.scale_log2 = b.scale * kLog2e;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream, p); };
-    if (l.rows == 16) go(kv4_attn_kernel<1, true>);
-    else if (l.rows == 32) go(kv4_attn_kernel<2, true>);
-    else go(kv4_attn_kernel<2, false>);
+    for (int s0 = 0; s0 < b.S; s0 += kMostSequences) {
+        p.S = std::min(kMostSequences, b.S - s0);
+        p.query_start = b.query_start + s0, p.tables = b.block_tables + static_cast<int64_t>(s0) * b.max_blocks;
+        const Plan l = plan(a, most_rows(b), p.S);
+        p.tiles = l.tiles;
+        p.workers = b.workspace && b.workspace_bytes >= l.bytes ? l.workers : 0;  // uncut, an item each is as good
+        if (p.workers > 0) {
+            const int64_t groups = static_cast<int64_t>(l.workers) * b.n_kv;
+            p.part_acc = static_cast<float *>(b.workspace);
+            p.part_ml = p.part_acc + 2 * groups * l.rows * kHeadDim;
+            p.counters = reinterpret_cast<uint32_t *>(p.part_ml + 2 * groups * l.rows * 2);
+        }
+        const int64_t items = static_cast<int64_t>(p.S) * l.tiles * b.n_kv;
+        const int64_t groups = p.workers > 0 ? static_cast<int64_t>(p.workers) * b.n_kv : items;
+        if (groups > kMostLaunch)
+            return set_error(EMBER_ERR_INVALID, "kv4_attn: too many work-groups for one launch (S %d x n_kv %d)", b.S, b.n_kv);
+        auto go = [&](auto kernel, int step_pages) {
+            // The units of all items fit 31 bits.
+            const int64_t most_items = static_cast<int64_t>(b.T) * p.G / l.rows + static_cast<int64_t>(p.S) * l.tiles;
+            for (p.shift = 0; most_items * ((b.max_blocks / step_pages >> p.shift) + 2) > INT32_MAX; p.shift++) {}
+            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream, p);
+        };
+        // Steps of two pages leave room for a third work-group on a CU; where there is one at most, four pages are fewer
+        // steps. Measured, us, two and four: 256 items of up to 4096 keys 23.2, 21.4; 512 35.7, 36.9; 2048 of up to 900
+        // 32.4, 38.9.
+        if (l.rows == 32) go(kv4_walk_kernel<2, kWaves, 2>, 2);
+        else if (l.rows == 128) go(kv4_attn_kernel<2>, kStepPages);
+        else if (p.workers == 0 && items <= kCus) go(kv4_walk_kernel<1, kWaves, 4>, 4);
+        else go(kv4_walk_kernel<1, kWaves, 2>, 2);
+    }
     return hip_status(hipGetLastError(), "kv4_attn");
 }
 

@@ -89,6 +89,12 @@ constexpr float kFar = 4194304.0f;
 constexpr float kMostExponent = 15.0f;
 __device__ __forceinline__ float below(float top, float step) { return fabsf(top) < kFar ? top - step : top; }
 
+// How far (base 2) a row's max may grow before the reference moves, so that most blocks rescale nothing: it is set
+// kMostExponent - kLazy below the max, and weights stay below 2^kMostExponent.
+// The weights are rounded to f16, the products' operand, and summed as rounded, so numerator and denominator move alike:
+// 2^-11 of each at most down to 2^-21 of the largest, 2^-32 of the largest below.
+constexpr float kLazy = 8.0f;
+
 // Whether a sum of weights holds anything: also when it is NaN (of a NaN in q, say), which a comparison would take for
 // an empty row's 0 and so turn the row into zeros.
 __device__ __forceinline__ bool filled(float l) { return __float_as_uint(l) != 0; }

@@ -546,11 +546,6 @@ constexpr int kKeyRow = kHeadDim + 8, kValueRow = kHeadDim + 32;
 typedef __fp16 tr16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
 
-// How far (base 2) a row's max may grow before the reference moves, so that most blocks rescale nothing: it is set
-// kMostExponent - kLazy below the max, and weights stay below 2^kMostExponent.
-// The weights are rounded to f16, the products' operand, and summed as rounded, so numerator and denominator move alike:
-// 2^-11 of each at most down to 2^-21 of the largest, 2^-32 of the largest below.
-constexpr float kLazy = 8.0f;
 constexpr int kAhead = 4;  // value operands in flight ahead of their products
 
 // Bound by the two waves of a SIMD taking turns: at 2000 tokens behind 12,000 (windows of 4096) the matrix unit is

@@ -114,7 +114,8 @@ def test_workspaces_refuse_sizes_that_no_call_takes(field, value, text):
 
 def test_attention_refuses_launches_that_are_too_large():
     a = _attn()
-    a.T, a.S, a.n_kv, a.n_heads = 1 << 20, 1 << 25, 2, 2
+    a.T, a.S, a.n_kv, a.n_heads, a.max_query = 1 << 12, 4096, 1 << 15, 1 << 15, 512
+    a.q_stride = 128 << 15
     assert _lib.lib().ember_hip_kv4_attn(a, None) == _lib.ERR_INVALID
     assert "work-groups" in _lib.last_error()
 
