@@ -30,7 +30,6 @@ namespace ember::hip {
 namespace {
 
 constexpr int kWaves = 4, kThreads = kWaves * kWave;
-constexpr int kStepPages = 4;  // pages that a wave takes at a time
 constexpr int kLeastUnits = 8;  // of a work-group's share
 constexpr int kRowPitch = kHeadDim + 4;  // floats of a row's partial in LDS
 
@@ -542,172 +541,230 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
     }
 }
 
-template <int RT>
-__global__ void __launch_bounds__(kThreads) kv4_attn_kernel(Kv4Params p) {
+// ---- many rows: key blocks shared in LDS ----
+
+// 128 rows a work-group; wave w owns rows 32 w .. + 31 of the tile, lane l = 32 h + c serves row c.
+//   S^T = K Q^T   v_mfma_f32_32x32x16_f16: lane l ends with row c's scores of keys 8 (i / 4) + 4 h + i % 4 of each
+//                 32-key half, so a row lives in two lanes.
+//   O^T += V^T P^T  the lane's scores, as weights, are the B operand as they stand; the A operand, the same keys of dim
+//                 c, comes from the transposing LDS read (lane r of 16 reads four dims of key r / 4).
+// A block of 64 keys is converted once for all rows: a page a wave, on its way into LDS, a block ahead. KG groups of 4
+// waves have the same rows and take the blocks in turn, each through buffers of its own; the others hand their
+// partials to group 0.
+constexpr int kTileRows = 128, kTileWaves = 4, kTileThreads = kTileWaves * kWave;
+constexpr int kBlockPages = 4, kBlockKeys = kBlockPages * kPage;
+static_assert(kBlockPages == kTileWaves);
+// LDS rows, halves: keys on 68 dwords, values on 80, for reads without bank conflicts.
+constexpr int kKeyRow = kHeadDim + 8, kValueRow = kHeadDim + 32;
+constexpr int kKeyBuffer = kBlockKeys * kKeyRow, kValueBuffer = kBlockKeys * kValueRow;
+typedef __fp16 tr16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
+typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
+constexpr int kValuesAhead = 4;  // value operands in flight ahead of their products
+
+template <int KG>
+__global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params p) {
     constexpr int D = kHeadDim;
-    constexpr int kRows = 16 * RT * (kWaves);  // rows of a work-group
-    const int tid = static_cast<int>(threadIdx.x), lane = tid % kWave, wave = uniform(tid / kWave);
-    const int g = lane >> 4, c = lane & 15;
-    int rest = static_cast<int>(blockIdx.x);
-    const int kvh = rest % p.n_kv;
-    rest /= p.n_kv;
-    const int tile0 = rest % p.tiles;
-    rest /= p.tiles;
-    const int seq = rest;
+    __shared__ __align__(16) f16 lds[KG * 2 * (kKeyBuffer + kValueBuffer)];
+    const int group = KG == 1 ? 0 : uniform(static_cast<int>(threadIdx.x) / kTileThreads);
+    const int tid = static_cast<int>(threadIdx.x) % kTileThreads, lane = tid % kWave, wave = uniform(tid / kWave);
+    f16 *const k_lds = lds + group * 2 * kKeyBuffer, *const v_lds = lds + KG * 2 * kKeyBuffer + group * 2 * kValueBuffer;
+    const int h = lane >> 5, c = lane & 31;
+    const int kvh = static_cast<int>(blockIdx.x) % p.n_kv;
+    int rest = static_cast<int>(blockIdx.x) / p.n_kv;
+    const int seq = rest % p.S, tile0 = p.tiles - 1 - rest / p.S;  // the tiles with most keys first
+    const int32_t *const table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
+    const uint8_t *const pool = p.pool + kvh * kKv4Page;
+    const uint32_t block_bytes = static_cast<uint32_t>(p.n_kv) * kKv4Page;
+    const int table_top = p.max_blocks * kPage - 1;
 
     const int t0 = clamped(uniform_load(p.query_start + seq), p.T);
     const int t1 = min(max(uniform_load(p.query_start + seq + 1), t0), p.T);
     const int rows = (t1 - t0) * p.G;
-    const int32_t *const table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
-    const int table_top = p.max_blocks * kPage - 1;
-
-    for (int row0 = tile0 * kRows; row0 < rows; row0 += p.tiles * kRows) {
-        const int nrows = min(kRows, rows - row0);
-        const int wave_row = wave * 16 * RT;
-        // Positions count up, so a wave's first and last rows bound them.
-        auto pos_of = [&](int r) { return p.positions[t0 + (row0 + min(r, nrows - 1)) / p.G]; };
-        auto top_of = [&](int r) { return min(max(pos_of(r), -1), table_top); };
-        int my_top[RT];
-        u32x4 qf[RT][4];
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-            const int row = min(wave_row + 16 * r + c, nrows - 1);
-            my_top[r] = top_of(row);
-            const f16 *const qp = p.q + (t0 + (row0 + row) / p.G) * p.q_stride + (kvh * p.G + (row0 + row) % p.G) * D + 32 * g;
-#pragma unroll
-            for (int s = 0; s < 4; s++) qf[r][s] = *reinterpret_cast<const u32x4 *>(qp + 8 * s);
-        }
-        const int min_top = uniform(top_of(wave_row)), max_top = uniform(top_of(wave_row + 16 * RT - 1));
-        const int pages = (max_top + kPage) / kPage;
-        const int v0 = 0, v1 = pages;
-
-        float m[RT], l[RT];
-        f32x4 o[RT][8];
-#pragma unroll
-        for (int r = 0; r < RT; r++) {
-            m[r] = kNoKeys, l[r] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 8; t++) o[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        constexpr int kStride = 1;
-        constexpr int kAhead = kWave / kStepPages;  // steps whose block ids a register holds
-        const int steps = max(0, v1 - v0 + kStepPages - 1) / kStepPages;
-        for (int step0 = 0; step0 < steps; step0 += kStride * kAhead) {
-            const int my_page = v0 + (step0 + lane / kStepPages * kStride) * kStepPages + lane % kStepPages;
-            const int ids = my_page < v1 ? table[my_page] : -1;
-            const int n = min(kAhead, (steps - step0 + kStride - 1) / kStride);
-            for (int j = 0; j < n; j++) {
-                const int page0 = v0 + (step0 + j * kStride) * kStepPages;
-                u32x4 kc[kStepPages], vc[kStepPages];
-                uint32_t ks[kStepPages], vs[kStepPages];
-#pragma unroll
-                for (int i = 0; i < kStepPages; i++) {
-                    const int block = __builtin_amdgcn_readlane(ids, j * kStepPages + i);
-                    const bool ok = block >= 0 && block < p.num_blocks;  // else no records: the loads give zeros
-                    const uint8_t *const base = p.pool + (static_cast<int64_t>(ok ? block : 0) * p.n_kv + kvh) * kKv4Page;
-                    const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, ok ? kKv4Page : 0, kDescWord3);
-                    kc[i] = load_desc(d, 64 * c + 16 * g);
-                    ks[i] = __builtin_amdgcn_raw_buffer_load_b8(d, kKv4KeyScales + 4 * c + g, 0, kNonTemporal);
-                    vc[i] = load_desc(d, kKv4Values + 16 * lane);
-                    vs[i] = __builtin_amdgcn_raw_buffer_load_b32(d, kKv4ValueScales + kPage * (c / 4) + 4 * g, 0, kNonTemporal);
-                }
-                f32x4 s[RT][kStepPages];
-#pragma unroll
-                for (int i = 0; i < kStepPages; i++) {
-#pragma unroll
-                    for (int r = 0; r < RT; r++) s[r][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const f16x8 kf = as_f16x8(mx_decode8(kc[i][w], mx_scale(ks[i])));
-#pragma unroll
-                        for (int r = 0; r < RT; r++) s[r][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, as_f16x8(qf[r][w]), s[r][i], 0, 0, 0);
-                    }
-                }
-                const int key0 = page0 * kPage;
-                if (key0 + kStepPages * kPage - 1 > min_top) {  // some row does not see all of these keys
-#pragma unroll
-                    for (int i = 0; i < kStepPages; i++)
-#pragma unroll
-                        for (int v = 0; v < 4; v++) {
-                            const int key = key0 + i * kPage + 4 * g + v;
-#pragma unroll
-                            for (int r = 0; r < RT; r++) s[r][i][v] = key <= my_top[r] ? s[r][i][v] : -INFINITY;
-                            // Keys that no row sees may hold anything: their scales are taken as 2^-127, their values so as 0.
-                            if (key > max_top) vs[i] &= ~(0xffu << (8 * v));
-                        }
-                }
-                f16x8 wh[RT][kStepPages / 2];
-#pragma unroll
-                for (int r = 0; r < RT; r++) {
-                    float top = s[r][0][0];
-#pragma unroll
-                    for (int i = 0; i < kStepPages; i++)
-#pragma unroll
-                        for (int v = 0; v < 4; v++) top = fmaxf(top, s[r][i][v]);
-                    top = groups_max(top) * p.scale_log2;
-                    const float mn = fmaxf(m[r], below(top, kMostExponent));
-                    const float corr = exp2_hw(m[r] - mn);
-                    m[r] = mn;
-                    float mul = p.scale_log2, add = -mn;
-                    if (const bool far = fabsf(mn) >= kFar; __builtin_amdgcn_ballot_w64(far)) {
-#pragma unroll
-                        for (int i = 0; i < kStepPages; i++)
-#pragma unroll
-                            for (int v = 0; v < 4; v++) s[r][i][v] = far ? s[r][i][v] * mul + add : __builtin_fmaf(s[r][i][v], mul, add);
-                        mul = 1.0f, add = 0.0f;
-                    }
-                    l[r] = l[r] * corr;
-                    const f16x2 ones = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
-#pragma unroll
-                    for (int i = 0; i < kStepPages; i++) {
-#pragma unroll
-                        for (int v = 0; v < 4; v++) wh[r][i / 2][i % 2 * 4 + v] = static_cast<f16>(exp2_hw(__builtin_fmaf(s[r][i][v], mul, add)));
-#pragma unroll
-                        for (int v = 0; v < 4; v += 2)
-                            l[r] = __builtin_amdgcn_fdot2(f16x2{wh[r][i / 2][i % 2 * 4 + v], wh[r][i / 2][i % 2 * 4 + v + 1]}, ones, l[r], false);
-                    }
-#pragma unroll
-                    for (int t = 0; t < 8; t++) o[r][t] = o[r][t] * corr;
-                }
-#pragma unroll
-                for (int i = 0; i < kStepPages; i += 2) {
-                    u32x4 val[2][4];  // [page][key % 4]: dims 8 c .. + 7
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int v = 0; v < 4; v++) val[h][v] = mx_decode8(vc[i + h][v], mx_scale(vs[i + h], v));
-                    auto tile = [&](auto index) {
-                        constexpr int t = decltype(index)::value;
-                        const f16x4 a = value_tile<t>(val[0]), b = value_tile<t>(val[1]);
-                        const f16x8 vt = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                        for (int r = 0; r < RT; r++) o[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vt, wh[r][i / 2], o[r][t], 0, 0, 0);
-                    };
-                    tile(std::integral_constant<int, 0>{}), tile(std::integral_constant<int, 1>{});
-                    tile(std::integral_constant<int, 2>{}), tile(std::integral_constant<int, 3>{});
-                    tile(std::integral_constant<int, 4>{}), tile(std::integral_constant<int, 5>{});
-                    tile(std::integral_constant<int, 6>{}), tile(std::integral_constant<int, 7>{});
-                }
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < RT; r++) l[r] = groups_sum(l[r]);
-
-        // The row's place in out.
-        auto at_of = [&](int row) {
-            return static_cast<int64_t>(t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
-        };
+    for (int row0 = tile0 * kTileRows; row0 < rows; row0 += p.tiles * kTileRows) {
+        // Positions count up, so first and last rows bound them. Rows past the last repeat it.
+        auto top_of = [&](int row) { return min(max(p.positions[t0 + min(row, rows - 1) / p.G], -1), table_top); };
+        const int my_row = min(row0 + 32 * wave + c, rows - 1);
+        const bool mine = row0 + 32 * wave + c < rows;
+        const int my_tok = t0 + my_row / p.G, my_head = kvh * p.G + my_row % p.G;
+        f16x8 qf[8];
         {
+            const f16 *const qp = p.q + my_tok * p.q_stride + my_head * D;
 #pragma unroll
-            for (int r = 0; r < RT; r++) {
-                const int row = wave_row + 16 * r + c;
-                if (row < nrows)
+            for (int i = 0; i < 8; i++) qf[i] = *reinterpret_cast<const f16x8 *>(qp + 16 * i + 8 * h);
+        }
+        const int my_top = top_of(my_row);
+        const int lo_top = uniform(top_of(row0 + 32 * wave)), max_top = uniform(top_of(row0 + kTileRows - 1));  // of the wave, of the tile
+        const int pages = (max_top + kPage) / kPage, blocks = (pages + kBlockPages - 1) / kBlockPages;
+
+        float m = -INFINITY, l = 0.0f;
+        f32x16 o[4];
 #pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const float x[8] = {o[r][0][v], o[r][1][v], o[r][2][v], o[r][3][v], o[r][4][v], o[r][5][v], o[r][6][v], o[r][7][v]};
-                        store_piece(p.out + at_of(row) * D + 32 * g + 8 * v, x, l[r]);
-                    }
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
+
+        // Step b of this group is block b KG + group; its page of this wave. The ids of 64 steps' pages, one a lane.
+        auto page_of = [&](int b) { return (b * KG + group) * kBlockPages + wave; };
+        auto id_of = [&](int b) {
+            const int page = page_of(b);
+            return page < pages ? table[page] : -1;
+        };
+        int ids = -1, next_ids = id_of(lane);
+        u32x4 kr, vr;
+        uint32_t ks, vs;
+        auto fetch = [&](int b) {
+            if (b % kWave == 0) {
+                ids = next_ids;
+                next_ids = id_of(b + kWave + lane);
             }
+            const uint32_t block = __builtin_amdgcn_readlane(ids, b % kWave);
+            const bool ok = block < static_cast<uint32_t>(p.num_blocks);  // else no records: the loads give zeros
+            const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool) + static_cast<uint64_t>(ok ? block : 0) * block_bytes, 0,
+                                                             ok ? kKv4Page : 0, kDescWord3);
+            kr = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, 16 * lane, 0, 0));  // key l / 4, dims 32 (l % 4) ..
+            ks = __builtin_amdgcn_raw_buffer_load_b8(d, kKv4KeyScales + lane, 0, 0);
+            vr = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, kKv4Values + 16 * lane, 0, 0));
+            vs = __builtin_amdgcn_raw_buffer_load_b32(d, kKv4ValueScales + kPage * (lane % 16 / 4) + 4 * (lane / 16), 0, 0);
+        };
+        auto stage = [&](int b) {
+            f16 *const kp = k_lds + (b & 1) * kKeyBuffer + (kPage * wave + lane / 4) * kKeyRow + 32 * (lane % 4);
+            f16 *const vp = v_lds + (b & 1) * kValueBuffer + (kPage * wave + 4 * (lane / 16)) * kValueRow + 8 * (lane % 16);
+            const int key0 = page_of(b) * kPage + 4 * (lane / 16);
+            if (page_of(b) * kPage + kPage - 1 > max_top)
+#pragma unroll
+                for (int v = 0; v < 4; v++)  // keys that no row sees may hold anything: their values are read as 0
+                    if (key0 + v > max_top) vs &= ~(0xffu << (8 * v));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                *reinterpret_cast<u32x4 *>(kp + 8 * i) = mx_decode8(kr[i], mx_scale(ks));
+                *reinterpret_cast<u32x4 *>(vp + i * kValueRow) = mx_decode8(vr[i], mx_scale(vs, i));
+            }
+        };
+        const int steps = (blocks + KG - 1) / KG;
+        if (steps > 0) {
+            fetch(0);
+            stage(0);
+        }
+        __syncthreads();
+        for (int b = 0; b < steps; b++) {
+            if (b + 1 < steps) fetch(b + 1);
+            const f16 *const kl = k_lds + (b & 1) * kKeyBuffer + c * kKeyRow + 8 * h;
+            const f16 *const vl = v_lds + (b & 1) * kValueBuffer + (4 * h + lane % 16 / 4) * kValueRow + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+            // Scores: the operands of a 32-key half are all requested before its first product, and each is
+            // replaced by the other half's as soon as its product is issued.
+            f32x16 s[2];
+            f16x8 ka[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) ka[i] = *reinterpret_cast<const f16x8 *>(kl + 16 * i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[i], qf[i], s[t], 0, 0, 0);
+                    if (t == 0) ka[i] = *reinterpret_cast<const f16x8 *>(kl + 32 * kKeyRow + 16 * i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            // The first values, in flight during the softmax: operand n = 4 j + t is dim tile t of keys 16 j .. + 15.
+            auto value = [&](int n) {
+                const f16 *const at = vl + n / 4 * 16 * kValueRow + n % 4 * 32;
+                const f16x4 lo4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)at));
+                const f16x4 hi4 = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_tr16x4 *)(at + 8 * kValueRow)));
+                return f16x8{lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
+            };
+            f16x8 va[kValuesAhead];
+#pragma unroll
+            for (int n = 0; n < kValuesAhead; n++) va[n] = value(n);
+            __builtin_amdgcn_sched_barrier(0);
+            const int key0 = (b * KG + group) * kBlockKeys;
+            if (key0 + kBlockKeys - 1 > lo_top) {  // some row of the wave does not see all of these keys
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[t][i] = key0 + 32 * t + 8 * (i / 4) + 4 * h + i % 4 <= my_top ? s[t][i] : -INFINITY;
+            }
+            float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+            for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(top, s[0][i]), s[1][i]);
+            top = top * p.scale_log2;
+            if (__builtin_amdgcn_ballot_w64(top - m > kMostExponent)) {  // seldom: the reference moves
+                const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+                const float row_top = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+                const bool grow = row_top - m > kMostExponent;
+                const float reference = below(row_top, kMostExponent - kLazy);
+                const float corr = grow ? exp2_hw(m - reference) : 1.0f;  // 0 from a row that had seen nothing
+                m = grow ? reference : m;
+                l = l * corr;
+#pragma unroll
+                for (int t = 0; t < 4; t++) o[t] = o[t] * corr;
+            }
+            float mul = p.scale_log2, neg = m == -INFINITY ? 0.0f : -m;
+            if (const bool far = fabsf(neg) >= kFar; __builtin_amdgcn_ballot_w64(far)) {
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[t][i] = far ? s[t][i] * mul + neg : __builtin_fmaf(s[t][i], mul, neg);
+                mul = 1.0f, neg = 0.0f;
+            }
+            const f16x2 ones = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+            f16x8 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[j][i] = static_cast<f16>(exp2_hw(__builtin_fmaf(s[j / 2][8 * (j % 2) + i], mul, neg)));
+#pragma unroll
+                for (int i = 0; i < 4; i++) l = __builtin_amdgcn_fdot2(f16x2{w[j][2 * i], w[j][2 * i + 1]}, ones, l, false);
+            }
+#pragma unroll
+            for (int n = 0; n < 16; n++) {
+                o[n % 4] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[n % kValuesAhead], w[n / 4], o[n % 4], 0, 0, 0);
+                if (n + kValuesAhead < 16) va[n % kValuesAhead] = value(n + kValuesAhead);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (b + 1 < steps) stage(b + 1);
+            __syncthreads();
+        }
+
+        if constexpr (KG == 2) {  // group 1's partial, through the buffers (every wave is past its last block)
+            f32x4 *const hand = reinterpret_cast<f32x4 *>(lds) + tid;
+            static_assert(17 * kTileThreads * sizeof(f32x4) <= sizeof lds);
+            if (group == 1) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    hand[i * kTileThreads] = f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+                hand[16 * kTileThreads] = f32x4{m, l, 0.0f, 0.0f};
+            }
+            __syncthreads();
+            if (group == 0) {
+                const f32x4 ml = hand[16 * kTileThreads];
+                const float top = fmaxf(m, ml[0]);
+                const float f0 = m == -INFINITY ? 0.0f : exp2_hw(m - top), f1 = ml[0] == -INFINITY ? 0.0f : exp2_hw(ml[0] - top);
+                l = l * f0 + ml[1] * f1;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const f32x4 x = hand[i * kTileThreads];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[i / 4][4 * (i % 4) + e] = o[i / 4][4 * (i % 4) + e] * f0 + x[e] * f1;
+                }
+            }
+            __syncthreads();  // the buffers are the next row tile's
+        }
+        if (group == 0) {
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+            l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+            f16 *const dst = p.out + (static_cast<int64_t>(my_tok) * p.n_heads + my_head) * D + 4 * h;
+            const float inv = filled(l) ? 1.0f / l : 0.0f;
+            if (mine)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {  // dims 32 (i / 4) + 8 (i % 4) + 4 h .. + 3
+                    f16x4 y;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) y[e] = static_cast<f16>(o[i / 4][4 * (i % 4) + e] * inv);
+                    *reinterpret_cast<f16x4 *>(dst + 8 * i) = y;
+                }
         }
     }
 }
@@ -738,10 +795,10 @@ bool share_out(int64_t items, int64_t keys) {
 Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences) {
     const EmberRaggedBatch &b = a.batch;
     Plan l{};
-    l.rows = most <= 16 ? 16 : most <= 32 ? 32 : 128;
+    l.rows = most <= 16 ? 16 : most <= 32 ? 32 : kTileRows;
     l.tiles = static_cast<int>(std::clamp<int64_t>((most + l.rows - 1) / l.rows, 1, std::max(1, kMostSequences / sequences)));
     const int64_t keys = std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage);
-    if (l.rows < 128 && share_out(static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys)) {
+    if (l.rows < kTileRows && share_out(static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys)) {
         // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
         l.workers = std::max(1, std::min(kWalkGroups / b.n_kv, 32 * sequences));
         l.bytes = static_cast<int64_t>(l.workers) * b.n_kv * (4 + 2 * l.rows * (kHeadDim + 2) * 4);
@@ -788,6 +845,14 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
         const int64_t groups = p.workers > 0 ? static_cast<int64_t>(p.workers) * b.n_kv : items;
         if (groups > kMostLaunch)
             return set_error(EMBER_ERR_INVALID, "kv4_attn: too many work-groups for one launch (S %d x n_kv %d)", b.S, b.n_kv);
+        if (l.rows == kTileRows) {
+            // A work-group of two key groups fills a CU; with more items than CUs, one each, two to a CU.
+            if (items <= kCus)
+                hipLaunchKernelGGL(kv4_tile_kernel<2>, dim3(static_cast<unsigned>(groups)), dim3(2 * kTileThreads), 0, stream, p);
+            else
+                hipLaunchKernelGGL(kv4_tile_kernel<1>, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, stream, p);
+            continue;
+        }
         auto go = [&](auto kernel, int step_pages) {
             // The units of all items fit 31 bits.
             const int64_t most_items = static_cast<int64_t>(b.T) * p.G / l.rows + static_cast<int64_t>(p.S) * l.tiles;
@@ -798,7 +863,6 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
         // steps. Measured, us, two and four: 256 items of up to 4096 keys 23.2, 21.4; 512 35.7, 36.9; 2048 of up to 900
         // 32.4, 38.9.
         if (l.rows == 32) go(kv4_walk_kernel<2, kWaves, 2>, 2);
-        else if (l.rows == 128) go(kv4_attn_kernel<2>, kStepPages);
         else if (p.workers == 0 && items <= kCus) go(kv4_walk_kernel<1, kWaves, 4>, 4);
         else go(kv4_walk_kernel<1, kWaves, 2>, 2);
     }
