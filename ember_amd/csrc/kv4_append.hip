@@ -7,6 +7,14 @@
 // lane's two pieces of 8 elements lie in one group of 32 each, whose largest
 // magnitude four neighbouring lanes find by two quad permutations; a piece's
 // codes are one 4-byte store.
+//
+// Bound by memory for many tokens, at 90% of a large copy's rate: us a call,
+// 9100 tokens of 32 + 8 + 8 heads 47 (4.2 TB/s), with k_out, v_out and a bias
+// 62; 16,384 tokens of 16 + 8 + 8 heads 51; 32 tokens 4.4, a launch and three
+// trips to memory. Waves without q or k heads take no sine and cosine, waves
+// without heads end at once (56, 68 and 59 us before). Tried: a wave for all
+// heads of a token, one sine and cosine for them all (8.0 us for 32 tokens, 55
+// for 9100: 112 registers leave half the waves).
 #include "device.hpp"
 #include "four_bit.hpp"
 #include "kernels.hpp"
@@ -37,8 +45,10 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
     constexpr int D = kHeadDim, HALF = D / 2;
     const int t = blockIdx.x;
     const int lane = static_cast<int>(threadIdx.x) % kWave;
-    const int group = static_cast<int>(blockIdx.y) * kWavesPerBlock + static_cast<int>(threadIdx.x) / kWave;
+    const int group = static_cast<int>(blockIdx.y) * kWavesPerBlock + uniform(static_cast<int>(threadIdx.x) / kWave);
     const int total = n_heads + 2 * n_kv;
+    if (group * kHeadsPerWave >= total) return;
+    const bool turns = group * kHeadsPerWave < n_heads + n_kv;  // some of the wave's heads are q or k
     const int head = group * kHeadsPerWave + lane / kLanesPerHead;
     const int piece = lane % kLanesPerHead, e0 = piece * kElems;
     const bool live = head < total;
@@ -57,13 +67,15 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
     const bool slot_ok = pos >= 0 && page < max_blocks && seq >= 0 && seq < a.rows;
     const int block = block_tables[static_cast<int64_t>(min(max(seq, 0), a.rows - 1)) * max_blocks + min(max(page, 0), max_blocks - 1)];
 
-    const float angle = static_cast<float>(pos) * freq;
-    double sd, cd;
-    sincos(static_cast<double>(angle), &sd, &cd);
-    const float s_f = static_cast<float>(sd), c_f = static_cast<float>(cd);
     float sn[kElems], cs[kElems];
+    if (turns) {
+        const float angle = static_cast<float>(pos) * freq;
+        double sd, cd;
+        sincos(static_cast<double>(angle), &sd, &cd);
+        const float s_f = static_cast<float>(sd), c_f = static_cast<float>(cd);
 #pragma unroll
-    for (int e = 0; e < kElems; e++) sn[e] = __shfl(s_f, e0 + e, kWave), cs[e] = __shfl(c_f, e0 + e, kWave);
+        for (int e = 0; e < kElems; e++) sn[e] = __shfl(s_f, e0 + e, kWave), cs[e] = __shfl(c_f, e0 + e, kWave);
+    }
 
     float x0[kElems], x1[kElems];
 #pragma unroll
@@ -74,20 +86,22 @@ __global__ void __launch_bounds__(kWavesPerBlock * kWave)
         for (int e = 0; e < kElems; e++) x0[e] = x0[e] + b[e0 + e], x1[e] = x1[e] + b[HALF + e0 + e];
     }
 
-    // Sum of squares over the head in double, in kv_append.hip's pairing order.
-    double ss[kElems];
+    double ss[kElems] = {};
+    if (turns && a.q_norm) {
+        // Sum of squares over the head in double, in kv_append.hip's pairing order.
 #pragma unroll
-    for (int e = 0; e < kElems; e++)
-        ss[e] = static_cast<double>(x0[e]) * x0[e] + static_cast<double>(x1[e]) * x1[e];
+        for (int e = 0; e < kElems; e++)
+            ss[e] = static_cast<double>(x0[e]) * x0[e] + static_cast<double>(x1[e]) * x1[e];
 #pragma unroll
-    for (int o = kLanesPerHead / 2; o > 0; o >>= 1) {
+        for (int o = kLanesPerHead / 2; o > 0; o >>= 1) {
 #pragma unroll
-        for (int e = 0; e < kElems; e++) ss[e] += __shfl_xor(ss[e], o, kLanesPerHead);
-    }
+            for (int e = 0; e < kElems; e++) ss[e] += __shfl_xor(ss[e], o, kLanesPerHead);
+        }
 #pragma unroll
-    for (int o = kElems / 2; o > 0; o >>= 1) {
+        for (int o = kElems / 2; o > 0; o >>= 1) {
 #pragma unroll
-        for (int e = 0; e < o; e++) ss[e] += ss[e + o];
+            for (int e = 0; e < o; e++) ss[e] += ss[e + o];
+        }
     }
 
     if (is_q || is_k) {

@@ -507,7 +507,8 @@ def _check_kv4_pool(pool, dev: int) -> None:
     """A pool of 4-bit pages on device `dev`."""
     if pool.dtype is not torch.uint8 or pool.get_device() != dev or not pool.is_contiguous():
         _refuse(dict(pool=pool), dev, torch.uint8)
-    if pool.dim() != 3 or pool.shape[2] != KV4_PAGE_BYTES:
+    shape = pool.shape
+    if len(shape) != 3 or shape[2] != KV4_PAGE_BYTES:
         raise EmberError(f"pool must be [num_blocks, n_kv, {KV4_PAGE_BYTES}]")
 
 
@@ -654,25 +655,39 @@ def kv4_append(qkv, q_out, pool, positions, token_seq, block_tables, *, n_heads,
     if dev < 0:
         raise EmberError(f"qkv must be a device tensor (got {qkv.device})")
     _check_kv4_pool(pool, dev)
-    for name, t, dtype in (("qkv", qkv, f16), ("q_out", q_out, f16), ("positions", positions, i32), ("token_seq", token_seq, i32),
-                           ("block_tables", block_tables, i32), ("inv_freq_dev", inv_freq_dev, f32), ("q_norm", q_norm, f32),
-                           ("k_norm", k_norm, f32), ("bias", bias, f32), ("k_out", k_out, f16), ("v_out", v_out, f16)):
-        if t is not None and (t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous()):
-            _refuse({name: t}, dev, dtype)
-    width = (n_heads + 2 * n_kv) * HEAD_DIM
-    T = positions.numel()
+    for t in (qkv, q_out):
+        if t.dtype is not f16 or t.get_device() != dev or not t.is_contiguous():
+            _refuse(dict(qkv=qkv, q_out=q_out), dev, f16)
+    for t in (positions, token_seq, block_tables):
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            _refuse(dict(positions=positions, token_seq=token_seq, block_tables=block_tables), dev, i32)
+    T, width, table, blocks = positions.numel(), (n_heads + 2 * n_kv) * HEAD_DIM, block_tables.shape, pool.shape
     if qkv.numel() != T * width or q_out.numel() != T * n_heads * HEAD_DIM or token_seq.numel() != T:
         raise EmberError("qkv, q_out and token_seq must hold as many tokens as positions")
-    if pool.shape[1] != n_kv or block_tables.dim() != 2 or inv_freq_dev.numel() != HEAD_DIM // 2:
-        raise EmberError("pool must have n_kv heads, block_tables be [rows, max_blocks] and inv_freq_dev hold 64 frequencies")
-    for name, t, n in (("q_norm", q_norm, HEAD_DIM), ("k_norm", k_norm, HEAD_DIM), ("bias", bias, width),
-                       ("k_out", k_out, T * n_kv * HEAD_DIM), ("v_out", v_out, T * n_kv * HEAD_DIM)):
-        if t is not None and t.numel() != n:
-            raise EmberError(f"{name} must hold {n} values")
-    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    a = _lib.Kv4AppendArgs(qkv.data_ptr(), q_out.data_ptr(), pool.data_ptr(), p(k_out), p(v_out), p(q_norm), p(k_norm), p(bias),
-                           inv_freq_dev.data_ptr(), positions.data_ptr(), token_seq.data_ptr(), block_tables.data_ptr(),
-                           block_tables.shape[0], block_tables.shape[1], T, n_heads, n_kv, HEAD_DIM, pool.shape[0], eps)
+    if blocks[1] != n_kv or len(table) != 2:
+        raise EmberError("pool must have n_kv heads and block_tables be [rows, max_blocks]")
+    floats = (inv_freq_dev,) if q_norm is None and k_norm is None and bias is None else (inv_freq_dev, q_norm, k_norm, bias)
+    at = [0, 0, 0, 0]
+    for i, t in enumerate(floats):
+        if t is not None:
+            if t.dtype is not f32 or t.get_device() != dev or not t.is_contiguous():
+                _refuse({("inv_freq_dev", "q_norm", "k_norm", "bias")[i]: t}, dev, f32)
+            if t.numel() != (HEAD_DIM // 2, HEAD_DIM, HEAD_DIM, width)[i]:
+                raise EmberError(f"{('inv_freq_dev', 'q_norm', 'k_norm', 'bias')[i]} must hold {(HEAD_DIM // 2, HEAD_DIM, HEAD_DIM, width)[i]} values")
+            at[i] = t.data_ptr()
+    k_at = v_at = 0
+    if k_out is not None or v_out is not None:
+        for name, t in (("k_out", k_out), ("v_out", v_out)):
+            if t is None:
+                raise EmberError("k_out and v_out go together")
+            if t.dtype is not f16 or t.get_device() != dev or not t.is_contiguous():
+                _refuse({name: t}, dev, f16)
+            if t.numel() != T * n_kv * HEAD_DIM:
+                raise EmberError(f"{name} must hold {T * n_kv * HEAD_DIM} values")
+        k_at, v_at = k_out.data_ptr(), v_out.data_ptr()
+    a = _lib.Kv4AppendArgs(qkv.data_ptr(), q_out.data_ptr(), pool.data_ptr(), k_at, v_at, at[1], at[2], at[3], at[0],
+                           positions.data_ptr(), token_seq.data_ptr(), block_tables.data_ptr(), table[0], table[1], T, n_heads, n_kv,
+                           HEAD_DIM, blocks[0], eps)
     _launch(_lib.lib().ember_hip_kv4_append, a, dev, stream, "kv4_append")
 
 
@@ -752,17 +767,18 @@ def gemv4(a, packed, c, epilogue: int, *, N: int, stream=None):
     size alone: N and K are the caller's to get right. A row's bits do not
     depend on the other rows.
     """
-    dev = a.get_device()
-    if dev < 0 or a.dtype is not torch.float16 or a.dim() != 2 or a.stride(1) != 1:
+    dev, shape, stride = a.get_device(), a.shape, a.stride()
+    if dev < 0 or a.dtype is not torch.float16 or len(shape) != 2 or stride[1] != 1:
         raise EmberError("gemv4: a must be an f16 device tensor [M, K] with contiguous rows")
-    M, K = a.shape
-    _refuse(dict(packed=packed), dev, torch.uint8)
-    if packed.numel() != int(_lib.lib().ember_hip_gemv4_packed_bytes(N, K)):
+    M, K = shape
+    if packed.dtype is not torch.uint8 or packed.get_device() != dev or not packed.is_contiguous():
+        _refuse(dict(packed=packed), dev, torch.uint8)
+    if packed.nbytes != (N + 15) // 16 * ((K + 127) // 128) * 1088 or packed.nbytes == 0:  # as ember_hip_gemv4_packed_bytes
         raise EmberError(f"gemv4: packed is not a weight of [{N}, {K}]")
     cols = N // 2 if epilogue == _lib.EPILOGUE_SILU_MUL else N
-    want = torch.float32 if epilogue in (_lib.EPILOGUE_STORE_F32, _lib.EPILOGUE_ADD_F32) else torch.float16
-    if c.dtype is not want or c.get_device() != dev or tuple(c.shape) != (M, cols) or (cols > 1 and c.stride(1) != 1):
+    want = torch.float32 if epilogue == _lib.EPILOGUE_STORE_F32 or epilogue == _lib.EPILOGUE_ADD_F32 else torch.float16
+    rows = c.stride()
+    if c.dtype is not want or c.get_device() != dev or c.shape != (M, cols) or (cols > 1 and rows[1] != 1):
         raise EmberError(f"gemv4: c must be {want} [{M}, {cols}] on cuda:{dev} with contiguous rows")
-    g = _lib.Gemv4Args(a.data_ptr(), a.stride(0) if M > 1 else K, packed.data_ptr(), M, N, K, c.data_ptr(),
-                       c.stride(0) if M > 1 else cols, epilogue)
-    _launch(_lib.lib().ember_hip_gemv4, g, dev, stream, "gemv4")
+    _launch(_lib.lib().ember_hip_gemv4, _lib.Gemv4Args(a.data_ptr(), stride[0] if M > 1 else K, packed.data_ptr(), M, N, K, c.data_ptr(),
+                                                       rows[0] if M > 1 else cols, epilogue), dev, stream, "gemv4")

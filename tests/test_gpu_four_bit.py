@@ -475,7 +475,7 @@ def test_python_refusals(device):
     a = dict(qkv=z(3, 8 * D), q_out=z(3, 4 * D), pool=pool, positions=i(3), token_seq=i(3), block_tables=i(1, 4), n_heads=4, n_kv=2, inv_freq_dev=f)
     K.kv4_append(**a)
     for name, bad, text in [("qkv", z(2, 8 * D), "as many tokens"), ("q_out", z(3, 3 * D), "as many"), ("token_seq", i(2), "as many"),
-                            ("block_tables", i(4), "block_tables"), ("inv_freq_dev", f[:32], "64 frequencies"), ("n_kv", 1, "as many"),
+                            ("block_tables", i(4), "block_tables"), ("inv_freq_dev", f[:32], "64 values"), ("n_kv", 1, "as many"),
                             ("q_norm", z(D, dtype=torch.float32), "go together"), ("k_out", z(3, 2 * D), "go together"), ("k_out", z(3, D), "k_out"),
                             ("bias", z(7, dtype=torch.float32), "bias"), ("qkv", z(3, 16 * D)[:, ::2], "qkv"), ("pool", K.kv4_pool(4, 3, device), "n_kv heads")]:
         with pytest.raises(EmberError, match=text):
