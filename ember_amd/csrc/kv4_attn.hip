@@ -74,13 +74,11 @@ struct Partials {
     __device__ __forceinline__ Partials(const Kv4Params &p, int slot)
         : acc(partials(p.part_acc, static_cast<int64_t>(slot) * ROWS * kHeadDim, ROWS * kHeadDim)),
           ml(partials(p.part_ml, static_cast<int64_t>(slot) * ROWS * 2, ROWS * 2)) {}
-    __device__ __forceinline__ void put(int row, int dim, const float (&x)[8], float m, float l) const {
-        const int at = (row * kHeadDim + dim) * static_cast<int>(sizeof(float));
-        const u32x4 lo = {__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
-        const u32x4 hi = {__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])};
-        __builtin_amdgcn_raw_buffer_store_b128(lo, acc, at, 0, kDeviceScope);
-        __builtin_amdgcn_raw_buffer_store_b128(hi, acc, at + 16, 0, kDeviceScope);
-        if (dim == 0) __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, ml, 8 * row, 0, kDeviceScope);
+    __device__ __forceinline__ void put4(int row, int dim, const f32x4 &x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), acc, (row * kHeadDim + dim) * static_cast<int>(sizeof(float)), 0, kDeviceScope);
+    }
+    __device__ __forceinline__ void put_ml(int row, float m, float l) const {
+        __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(m), __float_as_uint(l)}, ml, 8 * row, 0, kDeviceScope);
     }
     __device__ __forceinline__ float2 get_ml(int row) const {
         const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, 8 * row, 0, kDeviceScope));
@@ -208,14 +206,137 @@ struct Shares {
     }
 };
 
+// A part of an item (a row tile of a sequence for a kv head) that a work-group takes: units x .. stop - 1 of the item's
+// a .. b - 1, a unit being 2^shift steps of keys.
+struct Part {
+    int seq, t0, rows, tile;  // the sequence, its first token and its rows; the row tile
+    int a, b, x, stop;
+    int top;  // the highest key of the tile's rows (of the sequence's, for tiles past the hint)
+    __device__ __forceinline__ bool whole() const { return x == a && stop == b; }
+};
+
+// The parts of a work-group, in order. With workers, the work-groups of a kv head share the units of all items evenly,
+// found by each wave for itself from the sequences' lengths: 64 entries a load, a scan over the lanes. Without, a
+// work-group has an entry. An entry is a row tile of a sequence; the sequence's last one is all tiles that are left.
+template <int ROWS, int KEYS>  // of a tile, of a step
+struct Parts {
+    const Kv4Params &p;
+    const int lane, worker;
+    int workers;
+    // Lane i: entry 64 chunk + i. Its sequence's first token and rows, its first tile and number of them, their highest
+    // key and units each; units up to it, and before the chunk. The next part begins in lane `at`.
+    int seq_t0, seq_rows, first_tile, n_tiles, entry_top, entry_units;
+    int upto, before = 0, chunk = 0, at = 0;
+    int begin = 0, x = 0, end;
+    Shares shares{0, 0, 0};
+
+    __device__ __forceinline__ int load(int e) {
+        const int s = min(p.tiles == 1 ? e : e / p.tiles, p.S - 1), k = p.tiles == 1 ? 0 : e - s * p.tiles;
+        const int guess = p.positions[min(s, p.T - 1)];  // the last position of a sequence of a pure decode step
+        const int t0 = clamped(p.query_start[s], p.T), t1 = min(max(p.query_start[s + 1], t0), p.T);
+        int pos = guess;
+        if (__builtin_amdgcn_ballot_w64(t1 - 1 != s)) pos = p.positions[max(t1 - 1, 0)];
+        seq_t0 = t0, seq_rows = (t1 - t0) * p.G;
+        const int all = e < p.S * p.tiles ? (seq_rows + ROWS - 1) / ROWS : 0;
+        first_tile = k, n_tiles = k == p.tiles - 1 ? max(all - k, 0) : k < all ? 1 : 0;
+        // Positions count up: those behind the tile's last row are known from the sequence's last.
+        if (p.tiles > 1 && k < p.tiles - 1) pos = max(pos, -1) - (max(seq_rows - 1, 0) / p.G - (min((k + 1) * ROWS, max(seq_rows, 1)) - 1) / p.G);
+        entry_top = min(max(pos, -1), p.max_blocks * kPage - 1);
+        const int steps = max(1, (entry_top + KEYS) / KEYS);
+        entry_units = (steps + (1 << p.shift) - 1) >> p.shift;
+        return n_tiles * entry_units;
+    }
+    __device__ __forceinline__ int scan(int v) const {  // inclusive, over the lanes
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int y = __shfl_up(v, o, kWave);
+            v += lane >= o ? y : 0;
+        }
+        return v;
+    }
+    __device__ __forceinline__ int chunks() const { return (p.S * p.tiles + kWave - 1) / kWave; }
+
+    __device__ __forceinline__ Parts(const Kv4Params &params, int lane, int worker) : p(params), lane(lane), worker(worker), workers(params.workers) {
+        if (workers == 0) {
+            upto = load(worker);
+            end = upto = uniform(upto);
+            chunk = worker / kWave, at = worker % kWave;
+            return;
+        }
+        upto = scan(load(lane));
+        int units = __builtin_amdgcn_readlane(upto, kWave - 1), chunk_units = units;
+        if (chunks() > 1) {  // lane k: the units of chunk k
+            for (int k = 1; k < chunks(); k++) {
+                const int sum = __builtin_amdgcn_readlane(scan(load(k * kWave + lane)), kWave - 1);
+                chunk_units = lane == k ? sum : chunk_units;
+            }
+            chunk_units = scan(lane < chunks() ? chunk_units : 0);
+            units = __builtin_amdgcn_readlane(chunk_units, kWave - 1);
+        }
+        workers = min(workers, max(1, units / kLeastUnits));
+        if (worker >= workers) {
+            end = 0;
+            return;
+        }
+        shares = Shares(units, workers);
+        x = begin = shares.start(worker), end = shares.start(worker + 1);
+        if (chunks() > 1) {  // the chunk of the first unit
+            chunk = __popcll(__builtin_amdgcn_ballot_w64(lane < chunks() && chunk_units <= begin));
+            before = chunk > 0 ? __builtin_amdgcn_readlane(chunk_units, chunk - 1) : 0;
+            upto = scan(load(chunk * kWave + lane));
+        }
+        at = __popcll(__builtin_amdgcn_ballot_w64(before + upto <= begin));
+    }
+
+    __device__ __forceinline__ bool next(Part &part) {
+        while (x < end) {
+            if (at == kWave) {
+                before += __builtin_amdgcn_readlane(upto, kWave - 1);
+                if (++chunk >= chunks()) return false;
+                upto = scan(load(chunk * kWave + lane));
+                at = 0;
+            }
+            const int entry_end = before + __builtin_amdgcn_readlane(upto, at);
+            if (entry_end <= x) {
+                at++;
+                continue;
+            }
+            const int entry = chunk * kWave + at;
+            part.seq = p.tiles == 1 ? entry : entry / p.tiles;
+            part.t0 = __builtin_amdgcn_readlane(seq_t0, at), part.rows = __builtin_amdgcn_readlane(seq_rows, at);
+            // The item is the `left`th of its entry's from the end.
+            const int units = __builtin_amdgcn_readlane(entry_units, at), tiles = __builtin_amdgcn_readlane(n_tiles, at);
+            const int left = tiles == 1 ? 1 : (entry_end - x + units - 1) / units;
+            part.tile = __builtin_amdgcn_readlane(first_tile, at) + tiles - left;
+            part.b = entry_end - (left - 1) * units, part.a = part.b - units;
+            part.top = __builtin_amdgcn_readlane(entry_top, at);
+            if (workers > 0 && x == begin) {
+                x = shares.moved(x, part.a, part.b);
+                if (x == part.b) continue;  // the one before takes it
+            }
+            part.x = x;
+            part.stop = end >= part.b ? part.b : shares.moved(end, part.a, part.b);
+            if (part.stop == part.a) return false;
+            x = part.stop == part.b ? part.b : end;
+            return true;
+        }
+        return false;
+    }
+
+    // The work-groups that have parts of an item that is cut.
+    __device__ __forceinline__ void holders(const Part &part, int &from, int &to) const {
+        from = shares.worker_of(part.a), to = shares.worker_of(part.b - 1);
+        if (from + 1 < workers && shares.start(from + 1) < part.b && shares.moved(shares.start(from + 1), part.a, part.b) == part.a) from++;
+        if (to > 0 && shares.start(to) >= part.a && shares.moved(shares.start(to), part.a, part.b) == part.b) to--;
+    }
+    // A work-group has two slots for partials: of an item that it begins, and of one that began before it.
+    __device__ __forceinline__ int slot(int kvh, int holder, bool begins) const { return 2 * (kvh * p.workers + holder) + (begins ? 1 : 0); }
+};
+
 // Up to 16 RT rows a work-group, W waves that take turns at steps of P pages.
 //
 // A CU takes in about 27 GB/s, however many waves ask, so all of them have to
-// have the same share of the pages. A sequence's row tiles are items of as many
-// units as its context has steps; a kv head's work-groups take equal runs of
-// the units of all items, found by each wave for itself from the sequences'
-// lengths: 64 sequences a load, a scan over the lanes. An item that lies in
-// several runs is joined by the last of its work-groups.
+// have the same share of the pages where contexts are long.
 //
 // The pages of a wave's next step are on their way during a whole step.
 template <int RT, int W, int P>
@@ -233,100 +354,15 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
     const uint32_t block_bytes = static_cast<uint32_t>(p.n_kv) * kKv4Page;
 
     __builtin_amdgcn_s_setprio(3);  // up to the first pages, which the CU's other waves would delay
-    // Lane i: entry 64 chunk + i, a row tile of a sequence (the sequence's last entry: all that are left, alike). Its
-    // sequence's first token and rows, the entry's first tile and number of them, their highest key and units each.
-    int seq_t0, seq_rows, first_tile, n_tiles, entry_top, entry_units;
-    auto load_entry = [&](int e) {
-        const int at = min(p.tiles == 1 ? e : e / p.tiles, p.S - 1), k = p.tiles == 1 ? 0 : e - at * p.tiles;
-        const int guess = p.positions[min(at, p.T - 1)];  // the last position of a sequence of a pure decode step
-        const int t0 = clamped(p.query_start[at], p.T), t1 = min(max(p.query_start[at + 1], t0), p.T);
-        int pos = guess;
-        if (__builtin_amdgcn_ballot_w64(t1 - 1 != at)) pos = p.positions[max(t1 - 1, 0)];
-        seq_t0 = t0, seq_rows = (t1 - t0) * p.G;
-        const int all = e < p.S * p.tiles ? (seq_rows + kRows - 1) / kRows : 0;
-        first_tile = k, n_tiles = k == p.tiles - 1 ? max(all - k, 0) : k < all ? 1 : 0;
-        // Positions count up: those behind the tile's last row are known from the sequence's last.
-        if (p.tiles > 1 && k < p.tiles - 1) pos = max(pos, -1) - (max(seq_rows - 1, 0) / p.G - (min((k + 1) * kRows, max(seq_rows, 1)) - 1) / p.G);
-        entry_top = min(max(pos, -1), table_top);
-        const int steps = max(1, (entry_top + P * kPage) / (P * kPage));
-        entry_units = (steps + (1 << p.shift) - 1) >> p.shift;
-        return n_tiles * entry_units;
-    };
-    auto scan = [&](int x) {  // inclusive, over the lanes
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int y = __shfl_up(x, o, kWave);
-            x += lane >= o ? y : 0;
-        }
-        return x;
-    };
-    int chunk = 0, upto, before = 0, in_chunk = 0;  // units up to this lane's entry and before the chunk; the entry's lane
-    int workers = p.workers, begin = 0, end, slots = 0;
-    int each = 0, more = 0, near = 0;
-    const int chunks = (p.S * p.tiles + kWave - 1) / kWave;
-    if (workers == 0) {  // a work-group an entry
-        upto = load_entry(worker);
-        end = upto = uniform(upto);
-        chunk = worker / kWave, in_chunk = worker % kWave;
-        near = end;
-    } else {
-        upto = scan(load_entry(lane));
-        int units = __builtin_amdgcn_readlane(upto, kWave - 1), chunk_units = units;
-        if (chunks > 1) {  // lane k: the units of chunk k
-            for (int k = 1; k < chunks; k++) {
-                const int sum = __builtin_amdgcn_readlane(scan(load_entry(k * kWave + lane)), kWave - 1);
-                chunk_units = lane == k ? sum : chunk_units;
-            }
-            chunk_units = scan(lane < chunks ? chunk_units : 0);
-            units = __builtin_amdgcn_readlane(chunk_units, kWave - 1);
-        }
-        workers = min(workers, max(1, units / kLeastUnits));
-        if (worker >= workers) return;
-        const Shares shares(units, workers);
-        each = shares.each, more = shares.more, near = shares.near;
-        begin = shares.start(worker), end = shares.start(worker + 1);
-        if (chunks > 1) {  // the chunk of the first unit
-            chunk = __popcll(__builtin_amdgcn_ballot_w64(lane < chunks && chunk_units <= begin));
-            before = chunk > 0 ? __builtin_amdgcn_readlane(chunk_units, chunk - 1) : 0;
-            upto = scan(load_entry(chunk * kWave + lane));
-        }
-        in_chunk = __popcll(__builtin_amdgcn_ballot_w64(before + upto <= begin));  // the first unit's entry
-        slots = 2 * kvh * p.workers;
-    }
-    const Shares shares(each, more, near);
-
-    for (int x = begin; x < end;) {
-        if (in_chunk == kWave) {
-            before += __builtin_amdgcn_readlane(upto, kWave - 1);
-            if (++chunk >= chunks) return;
-            upto = scan(load_entry(chunk * kWave + lane));
-            in_chunk = 0;
-        }
-        const int entry_end = before + __builtin_amdgcn_readlane(upto, in_chunk);
-        if (entry_end <= x) {
-            in_chunk++;
-            continue;
-        }
-        const int entry = chunk * kWave + in_chunk, seq = p.tiles == 1 ? entry : entry / p.tiles;
-        const int t0 = __builtin_amdgcn_readlane(seq_t0, in_chunk), rows = __builtin_amdgcn_readlane(seq_rows, in_chunk);
-        // The item is units a .. b - 1, the `left`th of the entry's from its end; this work-group's part of it x .. stop - 1.
-        const int item_units = __builtin_amdgcn_readlane(entry_units, in_chunk), tiles = __builtin_amdgcn_readlane(n_tiles, in_chunk);
-        const int left = tiles == 1 ? 1 : (entry_end - x + item_units - 1) / item_units;
-        const int tile = __builtin_amdgcn_readlane(first_tile, in_chunk) + tiles - left;
-        const int b = entry_end - (left - 1) * item_units, a = b - item_units;
-        if (x == begin) {
-            x = shares.moved(x, a, b);
-            if (x == b) continue;  // the one before takes it
-        }
-        const int stop = end >= b ? b : shares.moved(end, a, b);
-        if (stop == a) return;
-        const bool whole = x == a && stop == b;
-
-        const int row0 = tile * kRows, nrows = min(kRows, rows - row0);
-        const int32_t *const table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
+    Parts<kRows, P * kPage> parts(p, lane, worker);
+    Part part;
+    while (parts.next(part)) {
+        const int t0 = part.t0, rows = part.rows;
+        const int row0 = part.tile * kRows, nrows = min(kRows, rows - row0);
+        const int32_t *const table = p.tables + static_cast<int64_t>(part.seq) * p.max_blocks;
         // Step i of this wave: pages (wave + i W) P .. of the part; lane P i + j holds the id of its page j.
         constexpr int kAhead = kWave / P;
-        const int v0 = ((x - a) << p.shift) * P;
+        const int v0 = ((part.x - part.a) << p.shift) * P;
         const int lane_page = (wave + lane / P * W) * P + lane % P;
         auto id_at = [&](int page) { return page < p.max_blocks ? table[page] : -1; };
         const int first_ids = id_at(v0 + lane_page);
@@ -342,7 +378,7 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
 #pragma unroll
             for (int s = 0; s < 4; s++) qf[r][s] = *reinterpret_cast<const u32x4 *>(qp + 8 * s);
         }
-        int min_top = __builtin_amdgcn_readlane(entry_top, in_chunk), max_top = min_top;
+        int min_top = part.top, max_top = part.top;
         if (one_token) {
 #pragma unroll
             for (int r = 0; r < RT; r++) my_top[r] = max_top;
@@ -352,7 +388,7 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
             min_top = uniform(top_of(0)), max_top = uniform(top_of(nrows - 1));
         }
         const int pages = (max_top + kPage) / kPage;
-        const int v1 = stop == b ? pages : min(((stop - a) << p.shift) * P, pages);
+        const int v1 = part.stop == part.b ? pages : min(((part.stop - part.a) << p.shift) * P, pages);
 
         float m[RT], l[RT];
         f32x4 o[RT][8];  // o[t][v]: dim 32 g + 8 v + t of column c
@@ -511,8 +547,8 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
             if (g == 0) red_m[wave * kRows + row] = m[r], red_l[wave * kRows + row] = l[r];
         }
         __syncthreads();
-        // A work-group has two slots: for an item that it begins, and for one that began before it.
-        const Partials<kRows> mine(p, slots + 2 * worker + (x == a ? 1 : 0));
+        const bool whole = part.whole();
+        const Partials<kRows> mine(p, parts.slot(kvh, worker, part.x == part.a));
         for (int i = tid; i < nrows * 16; i += kThreads) {
             const int row = i / 16, dim = i % 16 * 8;
             float M = kNoKeys, L = 0.0f, x[8] = {};
@@ -527,17 +563,18 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
                 for (int e = 0; e < 8; e++) x[e] = x[e] + src[e] * f;
             }
             if (whole) store_piece(p.out + at_of(row) * D + dim, x, L);
-            else mine.put(row, dim, x, M, L);
+            else {
+                mine.put4(row, dim, f32x4{x[0], x[1], x[2], x[3]});
+                mine.put4(row, dim + 4, f32x4{x[4], x[5], x[6], x[7]});
+                if (dim == 0) mine.put_ml(row, M, L);
+            }
         }
         if (!whole) {
-            int from = shares.worker_of(a), to = shares.worker_of(b - 1);  // the item's work-groups
-            if (from + 1 < workers && shares.start(from + 1) < b && shares.moved(shares.start(from + 1), a, b) == a) from++;
-            if (to > 0 && shares.start(to) >= a && shares.moved(shares.start(to), a, b) == b) to--;
+            int from, to;
+            parts.holders(part, from, to);
             if (last_of(p.counters + kvh * p.workers + from, to - from + 1, last))
-                merge_partials<kRows, kThreads>(p, to - from + 1, nrows, lds, [&](int k) { return slots + 2 * (from + k) + (k == 0 ? 1 : 0); }, at_of);
+                merge_partials<kRows, kThreads>(p, to - from + 1, nrows, lds, [&](int k) { return parts.slot(kvh, from + k, k == 0); }, at_of);
         }
-        x = b;
-        if (stop != b) return;
     }
 }
 
@@ -565,22 +602,24 @@ template <int KG>
 __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params p) {
     constexpr int D = kHeadDim;
     __shared__ __align__(16) f16 lds[KG * 2 * (kKeyBuffer + kValueBuffer)];
+    __shared__ bool last;
+    static_assert(merge_floats(kTileRows, KG * kTileThreads) * sizeof(float) <= sizeof lds);
     const int group = KG == 1 ? 0 : uniform(static_cast<int>(threadIdx.x) / kTileThreads);
     const int tid = static_cast<int>(threadIdx.x) % kTileThreads, lane = tid % kWave, wave = uniform(tid / kWave);
     f16 *const k_lds = lds + group * 2 * kKeyBuffer, *const v_lds = lds + KG * 2 * kKeyBuffer + group * 2 * kValueBuffer;
     const int h = lane >> 5, c = lane & 31;
     const int kvh = static_cast<int>(blockIdx.x) % p.n_kv;
-    int rest = static_cast<int>(blockIdx.x) / p.n_kv;
-    const int seq = rest % p.S, tile0 = p.tiles - 1 - rest / p.S;  // the tiles with most keys first
-    const int32_t *const table = p.tables + static_cast<int64_t>(seq) * p.max_blocks;
+    const int worker = static_cast<int>(blockIdx.x) / p.n_kv;
     const uint8_t *const pool = p.pool + kvh * kKv4Page;
     const uint32_t block_bytes = static_cast<uint32_t>(p.n_kv) * kKv4Page;
     const int table_top = p.max_blocks * kPage - 1;
 
-    const int t0 = clamped(uniform_load(p.query_start + seq), p.T);
-    const int t1 = min(max(uniform_load(p.query_start + seq + 1), t0), p.T);
-    const int rows = (t1 - t0) * p.G;
-    for (int row0 = tile0 * kTileRows; row0 < rows; row0 += p.tiles * kTileRows) {
+    // A work-group an entry: the tiles with most keys first.
+    Parts<kTileRows, kBlockKeys> parts(p, lane, p.workers > 0 ? worker : worker % p.S * p.tiles + p.tiles - 1 - worker / p.S);
+    Part part;
+    while (parts.next(part)) {
+        const int t0 = part.t0, rows = part.rows, row0 = part.tile * kTileRows;
+        const int32_t *const table = p.tables + static_cast<int64_t>(part.seq) * p.max_blocks;
         // Positions count up, so first and last rows bound them. Rows past the last repeat it.
         auto top_of = [&](int row) { return min(max(p.positions[t0 + min(row, rows - 1) / p.G], -1), table_top); };
         const int my_row = min(row0 + 32 * wave + c, rows - 1);
@@ -592,9 +631,12 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
 #pragma unroll
             for (int i = 0; i < 8; i++) qf[i] = *reinterpret_cast<const f16x8 *>(qp + 16 * i + 8 * h);
         }
-        const int my_top = top_of(my_row);
-        const int lo_top = uniform(top_of(row0 + 32 * wave)), max_top = uniform(top_of(row0 + kTileRows - 1));  // of the wave, of the tile
-        const int pages = (max_top + kPage) / kPage, blocks = (pages + kBlockPages - 1) / kBlockPages;
+        int my_top = top_of(my_row), lo_top = uniform(top_of(row0 + 32 * wave));  // of the row, of the wave
+        const int max_top = uniform(top_of(row0 + kTileRows - 1));                // of the tile
+        const int all_pages = (max_top + kPage) / kPage, all_blocks = (all_pages + kBlockPages - 1) / kBlockPages;
+        const int block0 = (part.x - part.a) << p.shift, block1 = part.stop == part.b ? all_blocks : min((part.stop - part.a) << p.shift, all_blocks);
+        const int pages = min(all_pages, block1 * kBlockPages), blocks = max(block1 - block0, 0);
+        my_top = min(my_top, block1 * kBlockKeys - 1), lo_top = min(lo_top, block1 * kBlockKeys - 1);  // a group may step past the part
 
         float m = -INFINITY, l = 0.0f;
         f32x16 o[4];
@@ -603,8 +645,8 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
 #pragma unroll
             for (int i = 0; i < 16; i++) o[t][i] = 0.0f;
 
-        // Step b of this group is block b KG + group; its page of this wave. The ids of 64 steps' pages, one a lane.
-        auto page_of = [&](int b) { return (b * KG + group) * kBlockPages + wave; };
+        // Step b of this group is block block0 + b KG + group; its page of this wave. The ids of 64 steps' pages, one a lane.
+        auto page_of = [&](int b) { return (block0 + b * KG + group) * kBlockPages + wave; };
         auto id_of = [&](int b) {
             const int page = page_of(b);
             return page < pages ? table[page] : -1;
@@ -641,6 +683,7 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
             }
         };
         const int steps = (blocks + KG - 1) / KG;
+        __syncthreads();  // the buffers' last readers, of the part before this
         if (steps > 0) {
             fetch(0);
             stage(0);
@@ -679,7 +722,7 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
 #pragma unroll
             for (int n = 0; n < kValuesAhead; n++) va[n] = value(n);
             __builtin_amdgcn_sched_barrier(0);
-            const int key0 = (b * KG + group) * kBlockKeys;
+            const int key0 = (block0 + b * KG + group) * kBlockKeys;
             if (key0 + kBlockKeys - 1 > lo_top) {  // some row of the wave does not see all of these keys
 #pragma unroll
                 for (int t = 0; t < 2; t++)
@@ -742,6 +785,7 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
                 const f32x4 ml = hand[16 * kTileThreads];
                 const float top = fmaxf(m, ml[0]);
                 const float f0 = m == -INFINITY ? 0.0f : exp2_hw(m - top), f1 = ml[0] == -INFINITY ? 0.0f : exp2_hw(ml[0] - top);
+                m = top;
                 l = l * f0 + ml[1] * f1;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
@@ -750,14 +794,13 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
                     for (int e = 0; e < 4; e++) o[i / 4][4 * (i % 4) + e] = o[i / 4][4 * (i % 4) + e] * f0 + x[e] * f1;
                 }
             }
-            __syncthreads();  // the buffers are the next row tile's
         }
         if (group == 0) {
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
             l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-            f16 *const dst = p.out + (static_cast<int64_t>(my_tok) * p.n_heads + my_head) * D + 4 * h;
-            const float inv = filled(l) ? 1.0f / l : 0.0f;
-            if (mine)
+            if (mine && part.whole()) {
+                f16 *const dst = p.out + (static_cast<int64_t>(my_tok) * p.n_heads + my_head) * D + 4 * h;
+                const float inv = filled(l) ? 1.0f / l : 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {  // dims 32 (i / 4) + 8 (i % 4) + 4 h .. + 3
                     f16x4 y;
@@ -765,6 +808,24 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
                     for (int e = 0; e < 4; e++) y[e] = static_cast<f16>(o[i / 4][4 * (i % 4) + e] * inv);
                     *reinterpret_cast<f16x4 *>(dst + 8 * i) = y;
                 }
+            } else if (mine) {
+                const Partials<kTileRows> to(p, parts.slot(kvh, worker, part.x == part.a));
+                const int row = 32 * wave + c;
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    to.put4(row, 8 * i + 4 * h, f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]});
+                if (h == 0) to.put_ml(row, filled(l) ? m : kNoKeys, l);
+            }
+        }
+        if (!part.whole()) {
+            int from, to;
+            parts.holders(part, from, to);
+            auto at_of = [&](int row) {
+                return static_cast<int64_t>(t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
+            };
+            if (last_of(p.counters + kvh * p.workers + from, to - from + 1, last))
+                merge_partials<kTileRows, KG * kTileThreads>(p, to - from + 1, min(kTileRows, rows - row0), reinterpret_cast<float *>(lds),
+                                                            [&](int k) { return parts.slot(kvh, from + k, k == 0); }, at_of);
         }
     }
 }
@@ -784,11 +845,15 @@ struct Plan {
 };
 
 // Whether the work-groups share the items out evenly, or take one each. Sharing costs a scan of the lengths, partials
-// and their merge; not sharing, the wait for the longest item. A work-group of its own takes 64 keys a wave in 0.95 us;
-// all of them together 6.9 TB/s. Measured, us, one each and shared: 1 sequence of 4000 keys 19.1, 10.7; of 131,000 477,
-// 32; 4 of up to 3000 16.0, 13.6; 8 of 1000 9.2, 9.9; 32 of up to 4096 21.4, 24.4; 8 of up to 131,000 444, 125.
-bool share_out(int64_t items, int64_t keys) {
+// and their merge; not sharing, the wait for the longest item.
+//   Few rows: a work-group of its own takes 64 keys a wave in 0.95 us, all of them together 6.9 TB/s. Measured, us, one
+//   each and shared: 1 sequence of 4000 keys 19.1, 10.7; of 131,000 477, 32; 4 of up to 3000 16.0, 13.5; 8 of 1000 9.2,
+//   9.9; 32 of up to 4096 21.4, 24.4; 8 of up to 131,000 444, 124.
+//   Tiles: 64 keys in 0.85 us; partials and merge of 128 rows 25 us. 256 tokens behind 30,000 410, 101; 2 x 128 behind
+//   4000 63.4, 55.3; 4 x 512 behind up to 3000 (as many items as CUs) 58, 74.
+bool share_out(bool tiled, int64_t items, int64_t keys) {
     const double steps = static_cast<double>((keys + 63) / 64);
+    if (tiled) return steps * 0.85 * (1.0 - static_cast<double>(items) / kCus) > 25.0;
     return steps / kWaves * 0.95 > items * steps * 0.00126 + 7.0;
 }
 
@@ -798,11 +863,11 @@ Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences) {
     l.rows = most <= 16 ? 16 : most <= 32 ? 32 : kTileRows;
     l.tiles = static_cast<int>(std::clamp<int64_t>((most + l.rows - 1) / l.rows, 1, std::max(1, kMostSequences / sequences)));
     const int64_t keys = std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage);
-    if (l.rows < kTileRows && share_out(static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys)) {
-        // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
-        l.workers = std::max(1, std::min(kWalkGroups / b.n_kv, 32 * sequences));
-        l.bytes = static_cast<int64_t>(l.workers) * b.n_kv * (4 + 2 * l.rows * (kHeadDim + 2) * 4);
-    }
+    const bool tiled = l.rows == kTileRows;
+    // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
+    if (share_out(tiled, static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys))
+        l.workers = tiled ? std::max(1, kCus / b.n_kv) : std::max(1, std::min(kWalkGroups / b.n_kv, 32 * sequences));
+    l.bytes = static_cast<int64_t>(l.workers) * b.n_kv * (4 + 2 * l.rows * (kHeadDim + 2) * 4);
     return l;
 }
 
@@ -810,12 +875,13 @@ int64_t most_rows(const EmberRaggedBatch &b) { return static_cast<int64_t>(std::
 
 }  // namespace
 
-// Of these sizes and of smaller batches: fewer sequences may be shared out where these are not, with a form of fewer rows.
+// Of these sizes and of smaller batches, which may be shared out where these are not, in any form of fewer rows. (From 16
+// sequences on a kv head has no more work-groups.)
 int64_t kv4_workspace_bytes(const EmberKv4AttnArgs &a) {
     const int64_t most = most_rows(a.batch);
     int64_t bytes = 0;
-    for (int64_t rows : {int64_t{16}, int64_t{32}})
-        for (int sequences = 1; sequences <= std::min(a.batch.S, kWalkGroups); sequences *= 2)
+    for (int64_t rows : {16, 32, 33})
+        for (int sequences = 1; sequences <= std::min(a.batch.S, 16); sequences++)
             bytes = std::max(bytes, plan(a, std::min(most, rows), sequences).bytes);
     return bytes;
 }
@@ -847,7 +913,9 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
             return set_error(EMBER_ERR_INVALID, "kv4_attn: too many work-groups for one launch (S %d x n_kv %d)", b.S, b.n_kv);
         if (l.rows == kTileRows) {
             // A work-group of two key groups fills a CU; with more items than CUs, one each, two to a CU.
-            if (items <= kCus)
+            p.shift = 0;
+            while ((static_cast<int64_t>(b.T) * p.G / kTileRows + items) * ((b.max_blocks / kBlockPages >> p.shift) + 2) > INT32_MAX) p.shift++;
+            if (p.workers > 0 || items <= kCus)
                 hipLaunchKernelGGL(kv4_tile_kernel<2>, dim3(static_cast<unsigned>(groups)), dim3(2 * kTileThreads), 0, stream, p);
             else
                 hipLaunchKernelGGL(kv4_tile_kernel<1>, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, stream, p);

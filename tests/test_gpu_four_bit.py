@@ -253,6 +253,22 @@ def test_attention_of_long_contexts(rng, device, context):
     check(b, attend(b, device))
 
 
+@pytest.mark.parametrize("H,KV", [(4, 2), (8, 1), (3, 1)])
+def test_attention_of_long_contexts_shared_out(rng, device, H, KV):
+    """Prompt tiles and decodes whose keys several work-groups share, of few sequences and of more than a wave's lanes hold."""
+    b = batch(rng, device, [(2500, 60), (0, 150), (1700, 33), (9, 0), (3100, 100)], H, KV)
+    check(b, attend(b, device))
+    check(b, attend(b, device, cut=False))
+    b = batch(rng, device, [(int(c), 1) for c in rng.integers(0, 400, 150)] + [(9000, 1), (5000, 1)], 2 * H // H, 1)
+    b["longest"] = 200000  # a hint: the sequences may be that long
+    check(b, attend(b, device))
+
+
+def test_attention_of_more_sequences_than_a_launch_takes(rng, device):
+    b = batch(rng, device, [(int(c), 1) for c in rng.integers(0, 40, 4200)], 1, 1)
+    check(b, attend(b, device, pad=1))
+
+
 def test_attention_without_hints_and_beyond_them(rng, device):
     b = batch(rng, device, [(100, 40), (700, 1)], 4, 2)
     check(b, attend(b, device, hints=False))
