@@ -470,9 +470,9 @@ int ember_hip_kv4_append(const EmberKv4AppendArgs *a, void *stream) {
     if (int e = check_heads("kv4_append", a->head_dim, a->n_heads, a->n_kv)) return e;
     if (a->n_heads > 64 || a->n_kv > 64)
         return set_error(EMBER_ERR_INVALID, "kv4_append: at most 64 query and 64 kv heads (got %d, %d)", a->n_heads, a->n_kv);
-    if (a->T < 0 || a->rows <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0)
-        return set_error(EMBER_ERR_INVALID, "kv4_append: bad sizes (T %d, rows %d, max_blocks %d, num_blocks %d)", a->T, a->rows,
-                         a->max_blocks, a->num_blocks);
+    if (a->T < 0 || a->T >= 1 << 24 || a->rows <= 0 || a->max_blocks <= 0 || a->num_blocks <= 0)  // 2^24 work-groups: HIP's bound
+        return set_error(EMBER_ERR_INVALID, "kv4_append: bad sizes (T %d: below 2^24, rows %d, max_blocks %d, num_blocks %d)", a->T,
+                         a->rows, a->max_blocks, a->num_blocks);
     if (a->T == 0) return EMBER_OK;
     if (!a->qkv || !a->q_out || !a->pool || !a->inv_freq || !a->positions || !a->token_seq || !a->block_tables)
         return set_error(EMBER_ERR_INVALID, "kv4_append: a required pointer is null");

@@ -328,6 +328,7 @@ struct Parts {
         from = shares.worker_of(part.a), to = shares.worker_of(part.b - 1);
         if (from + 1 < workers && shares.start(from + 1) < part.b && shares.moved(shares.start(from + 1), part.a, part.b) == part.a) from++;
         if (to > 0 && shares.start(to) >= part.a && shares.moved(shares.start(to), part.a, part.b) == part.b) to--;
+        from = clamped(from, workers - 1), to = clamped(to, workers - 1);  // (an invalid query_start could ask for any)
     }
     // A work-group has two slots for partials: of an item that it begins, and of one that began before it.
     __device__ __forceinline__ int slot(int kvh, int holder, bool begins) const { return 2 * (kvh * p.workers + holder) + (begins ? 1 : 0); }
@@ -695,6 +696,7 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
             const f16 *const vl = v_lds + (b & 1) * kValueBuffer + (4 * h + lane % 16 / 4) * kValueRow + 16 * (lane / 16 % 2) + 4 * (lane % 4);
             // Scores: the operands of a 32-key half are all requested before its first product, and each is
             // replaced by the other half's as soon as its product is issued.
+            __builtin_amdgcn_s_setprio(1);
             f32x16 s[2];
             f16x8 ka[8];
 #pragma unroll
@@ -722,6 +724,7 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
 #pragma unroll
             for (int n = 0; n < kValuesAhead; n++) va[n] = value(n);
             __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
             const int key0 = (block0 + b * KG + group) * kBlockKeys;
             if (key0 + kBlockKeys - 1 > lo_top) {  // some row of the wave does not see all of these keys
 #pragma unroll
@@ -761,12 +764,14 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
 #pragma unroll
                 for (int i = 0; i < 4; i++) l = __builtin_amdgcn_fdot2(f16x2{w[j][2 * i], w[j][2 * i + 1]}, ones, l, false);
             }
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int n = 0; n < 16; n++) {
                 o[n % 4] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[n % kValuesAhead], w[n / 4], o[n % 4], 0, 0, 0);
                 if (n + kValuesAhead < 16) va[n % kValuesAhead] = value(n + kValuesAhead);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_setprio(0);
             if (b + 1 < steps) stage(b + 1);
             __syncthreads();
         }
@@ -837,6 +842,10 @@ constexpr int kMostSequences = 4096;                    // of a launch: a lane f
 constexpr int kCus = 256;
 constexpr int kWalkGroups = 2 * kCus;  // that share out a long context
 
+// The workspace: the counters, at the same place whatever shape a call has, as they have to be 0 for the next one, which
+// may be of another; then its partials.
+constexpr int64_t kCounterBytes = kWalkGroups * static_cast<int64_t>(sizeof(uint32_t));
+
 struct Plan {
     int rows;       // of a work-group: 16, 32 or 128
     int tiles;      // entries of a sequence
@@ -865,9 +874,10 @@ Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences) {
     const int64_t keys = std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage);
     const bool tiled = l.rows == kTileRows;
     // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
+    const int most_workers = (tiled ? kCus : kWalkGroups) / b.n_kv;  // of kv heads that fill the chip by themselves, none
     if (share_out(tiled, static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys))
-        l.workers = tiled ? std::max(1, kCus / b.n_kv) : std::max(1, std::min(kWalkGroups / b.n_kv, 32 * sequences));
-    l.bytes = static_cast<int64_t>(l.workers) * b.n_kv * (4 + 2 * l.rows * (kHeadDim + 2) * 4);
+        l.workers = tiled ? most_workers : std::min(most_workers, 32 * sequences);
+    if (l.workers > 0) l.bytes = kCounterBytes + static_cast<int64_t>(l.workers) * b.n_kv * 2 * l.rows * (kHeadDim + 2) * 4;
     return l;
 }
 
@@ -903,9 +913,9 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
         p.workers = b.workspace && b.workspace_bytes >= l.bytes ? l.workers : 0;  // uncut, an item each is as good
         if (p.workers > 0) {
             const int64_t groups = static_cast<int64_t>(l.workers) * b.n_kv;
-            p.part_acc = static_cast<float *>(b.workspace);
+            p.counters = static_cast<uint32_t *>(b.workspace);
+            p.part_acc = reinterpret_cast<float *>(static_cast<uint8_t *>(b.workspace) + kCounterBytes);
             p.part_ml = p.part_acc + 2 * groups * l.rows * kHeadDim;
-            p.counters = reinterpret_cast<uint32_t *>(p.part_ml + 2 * groups * l.rows * 2);
         }
         const int64_t items = static_cast<int64_t>(p.S) * l.tiles * b.n_kv;
         const int64_t groups = p.workers > 0 ? static_cast<int64_t>(p.workers) * b.n_kv : items;

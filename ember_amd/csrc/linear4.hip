@@ -424,13 +424,24 @@ hipError_t launch_mx_quantize(const EmberMxQuantizeArgs &a, hipStream_t stream) 
     return hipGetLastError();
 }
 
-hipError_t launch_gemv4(const EmberGemv4Args &a, hipStream_t stream) {
-    switch (a.epilogue) {
-        case EMBER_EPILOGUE_STORE_F16: return run_gemv4<EMBER_EPILOGUE_STORE_F16>(a, stream);
-        case EMBER_EPILOGUE_STORE_F32: return run_gemv4<EMBER_EPILOGUE_STORE_F32>(a, stream);
-        case EMBER_EPILOGUE_ADD_F32: return run_gemv4<EMBER_EPILOGUE_ADD_F32>(a, stream);
-        default: return run_gemv4<EMBER_EPILOGUE_SILU_MUL>(a, stream);
+hipError_t launch_gemv4(const EmberGemv4Args &all, hipStream_t stream) {
+    constexpr int kMostRows = 1 << 20;  // of a launch, whose y counts at most 65535 tiles, of 32 rows where they are many
+    const int64_t element = all.epilogue == EMBER_EPILOGUE_STORE_F16 || all.epilogue == EMBER_EPILOGUE_SILU_MUL ? sizeof(f16) : sizeof(float);
+    for (int m0 = 0; m0 < all.M; m0 += kMostRows) {
+        EmberGemv4Args a = all;
+        a.M = std::min(all.M - m0, kMostRows);
+        a.A = static_cast<const f16 *>(all.A) + m0 * all.lda;
+        a.C = static_cast<uint8_t *>(all.C) + m0 * all.ldc * element;
+        hipError_t e;
+        switch (a.epilogue) {
+            case EMBER_EPILOGUE_STORE_F16: e = run_gemv4<EMBER_EPILOGUE_STORE_F16>(a, stream); break;
+            case EMBER_EPILOGUE_STORE_F32: e = run_gemv4<EMBER_EPILOGUE_STORE_F32>(a, stream); break;
+            case EMBER_EPILOGUE_ADD_F32: e = run_gemv4<EMBER_EPILOGUE_ADD_F32>(a, stream); break;
+            default: e = run_gemv4<EMBER_EPILOGUE_SILU_MUL>(a, stream); break;
+        }
+        if (e != hipSuccess) return e;
     }
+    return hipSuccess;
 }
 
 }  // namespace ember::hip

@@ -437,6 +437,14 @@ def _launch(fn, args, dev: int, stream, what: str) -> None:
         check(code, what)
 
 
+def _new_on(dev: int, stream, *shape):
+    """An uninitialised uint8 tensor for a launch on `stream`: its memory is not one that another stream still uses."""
+    if stream is not None and not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream), device=dev)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=torch.uint8, device=f"cuda:{dev}")
+
+
 def _refuse(tensors: dict, dev: int, dtype) -> None:
     """Names the first of these tensors that is not a contiguous `dtype` tensor on device `dev`."""
     for name, t in tensors.items():
@@ -726,15 +734,14 @@ def kv4_attention(q, pool, out, query_start, positions, block_tables, *, max_que
 
 
 def mx_quantize(x, stream=None):
-    """Rows to 4 bits (ember_hip_mx_quantize): f16 or f32 [rows, cols], cols a multiple of 32, rows of any stride.
+    """Rows to 4 bits (ember_hip_mx_quantize): f16 or f32 [rows, cols], cols a multiple of 32, rows of any stride from cols.
     Returns codes uint8 [rows, cols / 2] (byte i: columns 2i, in the low four bits, and 2i + 1) and scales uint8
     [rows, cols / 32]: value = (0, 0.5, 1, 1.5, 2, 3, 4, 6)[code % 8] * (-1 if code > 7) * 2^(scale - 127)."""
     dev = x.get_device()
     if dev < 0 or x.dim() != 2 or not (x.dtype is torch.float16 or x.dtype is torch.float32) or (x.shape[1] > 1 and x.stride(1) != 1):
         raise EmberError("mx_quantize: x must be an f16 or f32 device tensor [rows, cols] with contiguous rows")
     rows, cols = x.shape
-    codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(rows, cols // _lib.MX_GROUP, dtype=torch.uint8, device=x.device)
+    codes, scales = _new_on(dev, stream, rows, cols // 2), _new_on(dev, stream, rows, cols // _lib.MX_GROUP)
     a = _lib.MxQuantizeArgs(x.data_ptr(), x.stride(0) if rows > 1 else cols, rows, cols, _dtype_code(x), codes.data_ptr(),
                             scales.data_ptr())
     _launch(_lib.lib().ember_hip_mx_quantize, a, dev, stream, "mx_quantize")
@@ -754,7 +761,7 @@ def gemv4_pack(codes, scales, stream=None):
     n = int(_lib.lib().ember_hip_gemv4_packed_bytes(N, K))
     if n <= 0:
         raise EmberError(_lib.last_error())
-    out = torch.empty(n, dtype=torch.uint8, device=codes.device)
+    out = _new_on(dev, stream, n)
     fn = _lib.lib().ember_hip_gemv4_pack
     _launch(lambda args, handle: fn(*args, handle), (codes.data_ptr(), scales.data_ptr(), N, K, out.data_ptr()), dev, stream, "gemv4_pack")
     return out
@@ -763,9 +770,9 @@ def gemv4_pack(codes, scales, stream=None):
 def gemv4(a, packed, c, epilogue: int, *, N: int, stream=None):
     """C = epilogue(A . W^T) with W [N, K] of gemv4_pack (ember_hip_gemv4).
 
-    a: f16 [M, K] (rows of any stride that is a multiple of 8); c: as gemv's, rows of any stride. packed is known by its
-    size alone: N and K are the caller's to get right. A row's bits do not
-    depend on the other rows.
+    a: f16 [M, K] (rows of any stride from K that is a multiple of 8), up to 2^21 rows; c: as gemv's, rows of any stride
+    from its width, apart from a. packed is known by its size alone: N and K are the caller's to get right. A row's bits
+    do not depend on the other rows.
     """
     dev, shape, stride = a.get_device(), a.shape, a.stride()
     if dev < 0 or a.dtype is not torch.float16 or len(shape) != 2 or stride[1] != 1:

@@ -516,7 +516,7 @@ typedef struct EmberKv4AppendArgs {
  * outside the pool) writes no page, but q_out, k_out and v_out. Tokens of one
  * launch must have slots of their own (of padding rows that share one, any
  * row's bytes may stay). qkv, q_out, k_out, v_out and the pool
- * are 16-byte aligned; n_heads and n_kv at most 64. */
+ * are 16-byte aligned; n_heads and n_kv at most 64, T below 2^24. */
 int ember_hip_kv4_append(const EmberKv4AppendArgs *args, void *stream);
 
 typedef struct EmberKv4AttnArgs {
@@ -526,7 +526,8 @@ typedef struct EmberKv4AttnArgs {
 
 /* Causal attention (keys 0..p_i of each token) of a ragged batch over 4-bit
  * pages, as section 1b describes a batch. The workspace is zero-filled once
- * after allocation; every launch leaves it reusable. */
+ * after allocation; every launch leaves it ready for the next, of whatever
+ * sizes. Calls that overlap in time need one each. */
 int ember_hip_kv4_attn(const EmberKv4AttnArgs *args, void *stream);
 /* Bytes of workspace ember_hip_kv4_attn uses for these sizes (only the sizes
  * of args are read; 0: it would not split). Enough for smaller T, S, max_query
@@ -567,7 +568,8 @@ typedef struct EmberGemv4Args {
 } EmberGemv4Args;
 
 /* ember_hip_gemv with 4-bit weights: C = epilogue(A . W^T), sums in f32. The
- * bits of a row do not depend on the other rows or on M. Any M: prompts too. */
+ * bits of a row do not depend on the other rows or on M, which is 0 .. 2^21
+ * (prompts too). C overlaps neither A nor W. */
 int ember_hip_gemv4(const EmberGemv4Args *args, void *stream);
 
 /* Description of the last failure on this thread ("" if none). */

@@ -49,7 +49,7 @@ def _append():
 
 @pytest.mark.parametrize("field,value,text", [
     ("head_dim", 64, "head_dim"), ("n_heads", 15, "do not group"), ("n_heads", 128, "at most 64"), ("n_kv", 0, "do not group"),
-    ("T", -1, "bad sizes"), ("rows", 0, "bad sizes"), ("max_blocks", 0, "bad sizes"), ("num_blocks", 0, "bad sizes"),
+    ("T", -1, "bad sizes"), ("T", 1 << 24, "bad sizes"), ("rows", 0, "bad sizes"), ("max_blocks", 0, "bad sizes"), ("num_blocks", 0, "bad sizes"),
     ("q_norm", 4096, "go together"), ("k_norm", 4096, "go together"), ("k_out", 4096, "go together"), ("v_out", 4096, "go together"),
     ("qkv", 4104, "aligned"), ("q_out", 4104, "aligned"), ("pool", 4104, "aligned"),
     *((f, None, "null") for f in ("qkv", "q_out", "pool", "inv_freq", "positions", "token_seq", "block_tables"))])

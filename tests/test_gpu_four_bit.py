@@ -264,6 +264,22 @@ def test_attention_of_long_contexts_shared_out(rng, device, H, KV):
     check(b, attend(b, device))
 
 
+def test_a_workspace_serves_calls_of_every_shape(rng, device):
+    """Prompts, runs and decodes in turn with one workspace: each leaves it as the others, laid out otherwise, need it."""
+    ws = K.kv4_workspace(200, 6, n_heads=8, n_kv=2, max_query=100, max_context=100_000, device=device)
+    shapes = [[(6000, 100), (4500, 77)], [(9000, 1), (20, 1), (7000, 1)], [(5000, 5), (8000, 8)], [(3000, 1)] * 6]
+    calls = []
+    for seqs in shapes:
+        b = batch(rng, device, seqs, 8, 2)
+        out = torch.zeros(b["T"], 8, D, dtype=torch.float16, device=device)
+        args = (on(b["q"], device), on(b["pages"], device), out, dint(b["start"], device), dint(b["pos"], device), dint(b["table"], device))
+        calls.append((b, args))
+    for b, args in calls * 2:
+        args[2].fill_(7.0)
+        K.kv4_attention(*args, max_query=b["most"], max_context=100_000, workspace=ws)
+        check(b, args[2].double().cpu().numpy())
+
+
 def test_attention_of_more_sequences_than_a_launch_takes(rng, device):
     b = batch(rng, device, [(int(c), 1) for c in rng.integers(0, 40, 4200)], 1, 1)
     check(b, attend(b, device, pad=1))
@@ -433,6 +449,17 @@ def test_a_row_has_the_same_bits_in_every_batch(rng, device, N, k):
         c = torch.empty(rows, N, device=device)
         K.gemv4(a[:rows], w, c, _lib.EPILOGUE_STORE_F32, N=N)
         assert torch.equal(c[7], one[0]), rows
+
+
+def test_products_of_more_rows_than_a_launch_takes(rng, device):
+    codes, scales = weights(rng, 2, 32)
+    w = K.gemv4_pack(on(codes, device), on(scales, device))
+    a = torch.randn(1 << 21, 32, device=device).half()
+    c = torch.zeros(1 << 21, 2, device=device)
+    K.gemv4(a, w, c, _lib.EPILOGUE_STORE_F32, N=2)
+    for rows in (slice(0, 40), slice((1 << 20) - 20, (1 << 20) + 20), slice((1 << 21) - 40, None)):
+        want, bound = product(a[rows].double().cpu().numpy(), codes, scales, _lib.EPILOGUE_STORE_F32)
+        assert (np.abs(c[rows].double().cpu().numpy() - want) <= bound).all()
 
 
 def test_products_keep_special_values_in_their_places(rng, device):
@@ -632,3 +659,17 @@ def test_calls_on_another_stream(rng, device):
     torch.cuda.synchronize()
     for x, s, out, ws, args in calls:
         check(x, out.double().cpu().numpy())
+
+
+def test_preparation_on_another_stream(rng, device):
+    """What mx_quantize and gemv4_pack return on a stream, given as an object or a handle, is theirs from the start."""
+    x = on(rng.standard_normal((300, 256)).astype(np.float32), device)
+    codes, scales = K.mx_quantize(x)
+    packed = K.gemv4_pack(codes, scales)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for stream in (s, s.cuda_stream):
+        c, e = K.mx_quantize(x, stream=stream)
+        w = K.gemv4_pack(c, e, stream=stream)
+        s.synchronize()
+        assert torch.equal(c, codes) and torch.equal(e, scales) and torch.equal(w, packed)
