@@ -18,8 +18,8 @@
 // its own. A long context is cut into runs of pages for several work-groups;
 // the last of them to finish joins the partials, in run order.
 #include <algorithm>
-#include <cfloat>
 #include <climits>
+#include <cmath>
 #include <type_traits>
 
 #include "capi_errors.hpp"
@@ -83,6 +83,14 @@ struct Partials {
     __device__ __forceinline__ float2 get_ml(int row) const {
         const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(ml, 8 * row, 0, kDeviceScope));
         return make_float2(__uint_as_float(v[0]), __uint_as_float(v[1]));
+    }
+    // A tile's, as its lanes hold them: operand i of a lane is 16 bytes, a wave's side by side.
+    static __device__ __forceinline__ int lane_at(int wave, int i, int lane) { return ((wave * 16 + i) * kWave + lane) * 16; }
+    __device__ __forceinline__ void put_lane(int wave, int i, int lane, const f32x4 &x) const {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), acc, lane_at(wave, i, lane), 0, kDeviceScope);
+    }
+    __device__ __forceinline__ u32x4 get_lane(int wave, int i, int lane) const {
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(acc, lane_at(wave, i, lane), 0, kDeviceScope));
     }
     __device__ __forceinline__ u32x4 get4(int row, int dim) const {
         return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(acc, (row * kHeadDim + dim) * static_cast<int>(sizeof(float)), 0, kDeviceScope));
@@ -599,12 +607,51 @@ typedef __fp16 tr16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
 typedef __attribute__((address_space(3))) tr16x4 lds_tr16x4;
 constexpr int kValuesAhead = 4;  // value operands in flight ahead of their products
 
+// A row's half in a lane: element i is dims 8 i .. + 3 from dst on.
+template <int N>
+__device__ __forceinline__ void store_tile_row(f16 *dst, const f32x4 (&x)[N], float l) {
+    const float inv = filled(l) ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        f16x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = static_cast<f16>(x[i][e] * inv);
+        *reinterpret_cast<f16x4 *>(dst + 8 * i) = y;
+    }
+}
+
+// Joins n partials of a tile, slot_of(0) .. slot_of(n - 1) in that order, as the lanes that wrote them hold them; each
+// group takes its part of the dims.
+template <int KG, typename Slot>
+__device__ __forceinline__ float merge_tiles(const Kv4Params &p, int n, int wave, int lane, int group, Slot slot_of, f32x4 (&x)[16 / KG]) {
+    constexpr int N = 16 / KG;
+    const int row = 32 * wave + lane % 32;
+    float M = kNoKeys, L = 0.0f;
+    for (int k = 0; k < n; k++) M = fmaxf(M, Partials<kTileRows>(p, slot_of(k)).get_ml(row).x);
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (int k = 0; k < n; k++) {
+        const Partials<kTileRows> from(p, slot_of(k));
+        const float2 ml = from.get_ml(row);
+        u32x4 part[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) part[i] = from.get_lane(wave, group * N + i, lane);
+        const float w = filled(ml.y) ? exp2_hw(ml.x - M) : 0.0f;
+        L = L + ml.y * w;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[i][e] = x[i][e] + __uint_as_float(part[i][e]) * w;
+    }
+    return L;
+}
+
 template <int KG>
 __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params p) {
     constexpr int D = kHeadDim;
     __shared__ __align__(16) f16 lds[KG * 2 * (kKeyBuffer + kValueBuffer)];
     __shared__ bool last;
-    static_assert(merge_floats(kTileRows, KG * kTileThreads) * sizeof(float) <= sizeof lds);
     const int group = KG == 1 ? 0 : uniform(static_cast<int>(threadIdx.x) / kTileThreads);
     const int tid = static_cast<int>(threadIdx.x) % kTileThreads, lane = tid % kWave, wave = uniform(tid / kWave);
     f16 *const k_lds = lds + group * 2 * kKeyBuffer, *const v_lds = lds + KG * 2 * kKeyBuffer + group * 2 * kValueBuffer;
@@ -800,37 +847,33 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
                 }
             }
         }
+        f16 *const dst = p.out + (static_cast<int64_t>(my_tok) * p.n_heads + my_head) * D + 4 * h;
         if (group == 0) {
             const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
             l = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-            if (mine && part.whole()) {
-                f16 *const dst = p.out + (static_cast<int64_t>(my_tok) * p.n_heads + my_head) * D + 4 * h;
-                const float inv = filled(l) ? 1.0f / l : 0.0f;
+            if (mine) {
+                f32x4 x[16];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {  // dims 32 (i / 4) + 8 (i % 4) + 4 h .. + 3
-                    f16x4 y;
+                for (int i = 0; i < 16; i++) x[i] = f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]};
+                if (part.whole()) {
+                    store_tile_row(dst, x, l);
+                } else {
+                    const Partials<kTileRows> to(p, parts.slot(kvh, worker, part.x == part.a));
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[e] = static_cast<f16>(o[i / 4][4 * (i % 4) + e] * inv);
-                    *reinterpret_cast<f16x4 *>(dst + 8 * i) = y;
+                    for (int i = 0; i < 16; i++) to.put_lane(wave, i, lane, x[i]);
+                    if (h == 0) to.put_ml(32 * wave + c, filled(l) ? m : kNoKeys, l);
                 }
-            } else if (mine) {
-                const Partials<kTileRows> to(p, parts.slot(kvh, worker, part.x == part.a));
-                const int row = 32 * wave + c;
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    to.put4(row, 8 * i + 4 * h, f32x4{o[i / 4][4 * (i % 4)], o[i / 4][4 * (i % 4) + 1], o[i / 4][4 * (i % 4) + 2], o[i / 4][4 * (i % 4) + 3]});
-                if (h == 0) to.put_ml(row, filled(l) ? m : kNoKeys, l);
             }
         }
         if (!part.whole()) {
             int from, to;
             parts.holders(part, from, to);
-            auto at_of = [&](int row) {
-                return static_cast<int64_t>(t0 + (row0 + row) / p.G) * p.n_heads + kvh * p.G + (row0 + row) % p.G;
-            };
-            if (last_of(p.counters + kvh * p.workers + from, to - from + 1, last))
-                merge_partials<kTileRows, KG * kTileThreads>(p, to - from + 1, min(kTileRows, rows - row0), reinterpret_cast<float *>(lds),
-                                                            [&](int k) { return parts.slot(kvh, from + k, k == 0); }, at_of);
+            if (last_of(p.counters + kvh * p.workers + from, to - from + 1, last) && mine) {
+                constexpr int N = 16 / KG;
+                f32x4 x[N];
+                const float L = merge_tiles<KG>(p, to - from + 1, wave, lane, group, [&](int k) { return parts.slot(kvh, from + k, k == 0); }, x);
+                store_tile_row(dst + 8 * N * group, x, L);
+            }
         }
     }
 }
@@ -858,15 +901,20 @@ struct Plan {
 //   Few rows: a work-group of its own takes 64 keys a wave in 0.95 us, all of them together 6.9 TB/s. Measured, us, one
 //   each and shared: 1 sequence of 4000 keys 19.1, 10.7; of 131,000 477, 32; 4 of up to 3000 16.0, 13.5; 8 of 1000 9.2,
 //   9.9; 32 of up to 4096 21.4, 24.4; 8 of up to 131,000 444, 124.
-//   Tiles: 64 keys in 0.85 us; partials and merge of 128 rows 25 us. 256 tokens behind 30,000 410, 101; 2 x 128 behind
-//   4000 63.4, 55.3; 4 x 512 behind up to 3000 (as many items as CUs) 58, 74.
-bool share_out(bool tiled, int64_t items, int64_t keys) {
+//   Tiles: a CU takes 64 keys of one in 0.85 us; shared, 6% more, and 15 us. Of several sequences only the longest context
+//   is known: the others' are taken as half of it. Measured, us, one each and shared: 256 tokens behind 30,000 410, 76;
+//   2 x 128 behind 4000 63.4, 33.8; 8 of up to 512 behind up to 8000 209, 117; 16 of up to 512 behind up to 9000 281, 190;
+//   8 of up to 100 behind 500 to 3000 48.6, 44.5; 2 x 200 behind 1000 26.5, 27.9; 4 x 512 behind 900 to 3000 59.3, 61.6;
+//   2000 behind 12,000 (an item a CU) 218, 226; 40 x 512 (8 items a CU) 342, 355.
+bool share_out(bool tiled, bool alike, double items, int64_t keys) {
     const double steps = static_cast<double>((keys + 63) / 64);
-    if (tiled) return steps * 0.85 * (1.0 - static_cast<double>(items) / kCus) > 25.0;
-    return steps / kWaves * 0.95 > items * steps * 0.00126 + 7.0;
+    if (!tiled) return steps / kWaves * 0.95 > items * steps * 0.00126 + 7.0;
+    const double load = items / kCus;
+    const double one_each = alike ? std::max(1.0, std::ceil(load)) : std::max(1.0, 0.5 * load + 0.5);
+    return steps * 0.85 * (one_each - 1.06 * (alike ? load : 0.5 * load)) > 15.0;
 }
 
-Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences) {
+Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences, int tokens) {
     const EmberRaggedBatch &b = a.batch;
     Plan l{};
     l.rows = most <= 16 ? 16 : most <= 32 ? 32 : kTileRows;
@@ -875,7 +923,10 @@ Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences) {
     const bool tiled = l.rows == kTileRows;
     // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
     const int most_workers = (tiled ? kCus : kWalkGroups) / b.n_kv;  // of kv heads that fill the chip by themselves, none
-    if (share_out(tiled, static_cast<int64_t>(sequences) * l.tiles * b.n_kv, keys))
+    double items = static_cast<double>(sequences) * l.tiles;
+    if (tiled)  // of a tile a sequence, half is taken as empty; without tokens: the fewest items there may be
+        items = tokens == 0 ? 0.0 : std::min(items, static_cast<double>(tokens) * (b.n_heads / b.n_kv) / l.rows + 0.5 * sequences);
+    if (share_out(tiled, sequences == 1, b.n_kv * items, keys))
         l.workers = tiled ? most_workers : std::min(most_workers, 32 * sequences);
     if (l.workers > 0) l.bytes = kCounterBytes + static_cast<int64_t>(l.workers) * b.n_kv * 2 * l.rows * (kHeadDim + 2) * 4;
     return l;
@@ -885,14 +936,14 @@ int64_t most_rows(const EmberRaggedBatch &b) { return static_cast<int64_t>(std::
 
 }  // namespace
 
-// Of these sizes and of smaller batches, which may be shared out where these are not, in any form of fewer rows. (From 16
-// sequences on a kv head has no more work-groups.)
+// Of these sizes and of smaller batches, which may be shared out where these are not, in any form of fewer rows, the more so
+// the fewer their tokens. (From 16 sequences on a kv head has no more work-groups.)
 int64_t kv4_workspace_bytes(const EmberKv4AttnArgs &a) {
     const int64_t most = most_rows(a.batch);
     int64_t bytes = 0;
     for (int64_t rows : {16, 32, 33})
         for (int sequences = 1; sequences <= std::min(a.batch.S, 16); sequences++)
-            bytes = std::max(bytes, plan(a, std::min(most, rows), sequences).bytes);
+            bytes = std::max(bytes, plan(a, std::min(most, rows), sequences, 0).bytes);
     return bytes;
 }
 
@@ -908,7 +959,7 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
     for (int s0 = 0; s0 < b.S; s0 += kMostSequences) {
         p.S = std::min(kMostSequences, b.S - s0);
         p.query_start = b.query_start + s0, p.tables = b.block_tables + static_cast<int64_t>(s0) * b.max_blocks;
-        const Plan l = plan(a, most_rows(b), p.S);
+        const Plan l = plan(a, most_rows(b), p.S, b.T);
         p.tiles = l.tiles;
         p.workers = b.workspace && b.workspace_bytes >= l.bytes ? l.workers : 0;  // uncut, an item each is as good
         if (p.workers > 0) {
