@@ -11,12 +11,19 @@
 //   O^T += V^T P^T the same instruction over the keys of two pages, the
 //                  weights where the scores were; tile t holds dims 8 c + t,
 //                  two v_perm a page pair up two keys' halves.
-// Softmax online in base 2, in f32; weights are f16 and summed as rounded.
+// Softmax online in base 2: maxima and sums in f32; a weight is f16 and enters
+// the sum as rounded, so that sum and products see the same weights. A row's
+// reference is not its maximum but 7 below it, and moves only when a score
+// exceeds it by 15, short of f16's end: a weight keeps its 11 bits down to
+// 2^-21 of the largest, and the accumulators are seldom rescaled.
 //
-// Two forms. Few rows (KEYS): the waves of a work-group share the rows and
-// take turns at the pages, and meet in LDS. Many rows: each wave has rows of
-// its own. A long context is cut into runs of pages for several work-groups;
-// the last of them to finish joins the partials, in run order.
+// Two forms. Up to 32 rows of a kv head and sequence (decode, speculative
+// runs): the walk, whose four waves take turns at the pages and convert them in
+// registers. More (prompts): the tile, 128 rows on blocks of keys converted
+// once into LDS. In both, either a work-group has an item (a row tile of a
+// sequence), or the work-groups of a kv head share the keys of all items out
+// evenly; then the last to finish of an item joins its partials, in the order
+// of the keys: the bits do not depend on who that is.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -344,10 +351,13 @@ struct Parts {
 
 // Up to 16 RT rows a work-group, W waves that take turns at steps of P pages.
 //
-// A CU takes in about 27 GB/s, however many waves ask, so all of them have to
-// have the same share of the pages where contexts are long.
-//
-// The pages of a wave's next step are on their way during a whole step.
+// Bound by what a CU takes in, 27 to 43 GB/s however many waves ask: so the
+// pages of a wave's next step are on their way during a whole step, and where
+// contexts are long all CUs have the same share. With few keys, by a launch's
+// chain of trips to memory (lengths, page ids, pages, out).
+// Measured, 8 kv heads: 1 sequence of 640 keys 8.0 us, of 131,000 32 (4.4
+// TB/s); 32 of 256 to 4095 22 (4.1 TB/s); 8 of 30,000 to 131,000 124 (6.1
+// TB/s); 64 of 512 to 4096 with up to 5 tokens each 36 (4.9 TB/s).
 template <int RT, int W, int P>
 __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
     constexpr int D = kHeadDim, kRows = 16 * RT, kThreads = W * kWave;
@@ -590,6 +600,14 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
 // ---- many rows: key blocks shared in LDS ----
 
 // 128 rows a work-group; wave w owns rows 32 w .. + 31 of the tile, lane l = 32 h + c serves row c.
+//
+// Bound by the products and the softmax between them, each at half of the cycles: two waves a SIMD, with the block's
+// barrier between them, mostly do the same. (Waves at products and at arithmetic overlap all but fully where nothing
+// holds them together. Group 1 half a step behind group 0: 247 us against 233; a wave's priority raised during its
+// products 230.)
+// Measured, 16 heads on 8 kv heads: 2000 tokens behind 12,000 218 us (980 TFLOP/s), 4 of 256 to 512 behind 900 to 3000 60,
+// 512 alone 14.
+//
 //   S^T = K Q^T   v_mfma_f32_32x32x16_f16: lane l ends with row c's scores of keys 8 (i / 4) + 4 h + i % 4 of each
 //                 32-key half, so a row lives in two lanes.
 //   O^T += V^T P^T  the lane's scores, as weights, are the B operand as they stand; the A operand, the same keys of dim

@@ -643,6 +643,34 @@ def test_a_step_in_four_bits_captured_and_replayed(rng, device):
             assert torch.equal(st[n][:5], eager[n][:5]), n
 
 
+def test_long_contexts_captured_and_replayed(rng, device):
+    """A prompt's tiles and long decodes, shared out by many work-groups, in one graph with one workspace; eager calls with
+    another between its replays."""
+    shapes = [batch(rng, device, seqs, 8, 2) for seqs in ([(6000, 100), (2000, 77)], [(9000, 1), (7000, 1), (0, 0)])]
+    calls = [((on(b["q"], device), on(b["pages"], device), torch.zeros(b["T"], 8, D, dtype=torch.float16, device=device),
+               *(dint(b[n], device) for n in ("start", "pos", "table"))), dict(max_query=b["most"], max_context=b["longest"])) for b in shapes]
+    own, other = (K.kv4_workspace(200, 3, n_heads=8, n_kv=2, max_query=100, max_context=10_000, device=device) for _ in range(2))
+    eager = []
+    for b, (args, hints) in zip(shapes, calls):
+        K.kv4_attention(*args, **hints, workspace=other)
+        check(b, args[2].double().cpu().numpy())
+        eager.append(args[2].clone())
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for args, hints in calls:
+            K.kv4_attention(*args, **hints, workspace=own)
+    for _ in range(4):
+        for args, _ in calls:
+            args[2].fill_(7.0)
+        graph.replay()
+        for (args, hints), want in zip(calls, eager):
+            assert torch.equal(args[2], want)
+            K.kv4_attention(*args, **hints, workspace=other)
+            assert torch.equal(args[2], want)
+
+
 def test_calls_on_another_stream(rng, device):
     """Two streams at once, a workspace each."""
     a, b = batch(rng, device, [(900, 1), (30, 1)], 4, 2), batch(rng, device, [(500, 3)], 4, 2)
