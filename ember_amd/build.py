@@ -77,7 +77,8 @@ def common_flags() -> list[str]:
 # Per-source additions. The decode kernel rescales its MFMA accumulators on the
 # VALU every page, and the prompts' linear layers add theirs up there run by run:
 # they stay in VGPRs (the VGPR form of v_mfma) instead of being copied out of and
-# back into AGPRs around each rescale or sum; so do the span kernels'. The decode
+# back into AGPRs around each rescale or sum; so do the span kernels' and the 4-bit
+# pages'. The decode
 # kernel's first seven arguments (the work descriptors' address, n_kv, the
 # pools, the block tables, qkv and the rotary frequencies) are preloaded into
 # scalar registers at launch, so a work-group's descriptor load does not wait for a kernel-argument

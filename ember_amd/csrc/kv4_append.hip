@@ -8,7 +8,7 @@
 // magnitude four neighbouring lanes find by two quad permutations; a piece's
 // codes are one 4-byte store.
 //
-// Bound by memory for many tokens, at 90% of a large copy's rate: us a call,
+// Bound by memory for many tokens, at 90% of a large copy's rate: us a launch,
 // 9100 tokens of 32 + 8 + 8 heads 47 (4.2 TB/s), with k_out, v_out and a bias
 // 62; 16,384 tokens of 16 + 8 + 8 heads 51; 32 tokens 4.4, a launch and three
 // trips to memory. Waves without q or k heads take no sine and cosine, waves

@@ -51,6 +51,7 @@ struct Kv4Params {
     int T, S, max_blocks, n_heads, n_kv, G, num_blocks;
     int workers;  // work-groups of a kv head
     int tiles;    // entries of a sequence: its row tiles, those past the hint together in the last
+    int least, most;  // rows of the sequences that this launch is for
     int shift;    // a unit of their shares is 2^shift steps of pages
     float scale_log2;
 };
@@ -252,7 +253,7 @@ struct Parts {
         int pos = guess;
         if (__builtin_amdgcn_ballot_w64(t1 - 1 != s)) pos = p.positions[max(t1 - 1, 0)];
         seq_t0 = t0, seq_rows = (t1 - t0) * p.G;
-        const int all = e < p.S * p.tiles ? (seq_rows + ROWS - 1) / ROWS : 0;
+        const int all = e < p.S * p.tiles && seq_rows >= p.least && seq_rows <= p.most ? (seq_rows + ROWS - 1) / ROWS : 0;
         first_tile = k, n_tiles = k == p.tiles - 1 ? max(all - k, 0) : k < all ? 1 : 0;
         // Positions count up: those behind the tile's last row are known from the sequence's last.
         if (p.tiles > 1 && k < p.tiles - 1) pos = max(pos, -1) - (max(seq_rows - 1, 0) / p.G - (min((k + 1) * ROWS, max(seq_rows, 1)) - 1) / p.G);
@@ -601,10 +602,10 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
 
 // 128 rows a work-group; wave w owns rows 32 w .. + 31 of the tile, lane l = 32 h + c serves row c.
 //
-// Bound by the products and the softmax between them, each at half of the cycles: two waves a SIMD, with the block's
-// barrier between them, mostly do the same. (Waves at products and at arithmetic overlap all but fully where nothing
-// holds them together. Group 1 half a step behind group 0: 247 us against 233; a wave's priority raised during its
-// products 230.)
+// Bound by three units that are each busy about half of the cycles: the matrix unit 47%, the VALU (softmax, conversion)
+// 46%, LDS 57% (every wave reads a block's 32 KB). Tried against 233 us for 2000 tokens behind 12,000: group 1 half a step
+// behind group 0, its softmax beside the other's products, 247; work-groups of one key group, two to a CU, 237; a wave's
+// priority raised during its products 230 (kept); keys staged 16 to a quarter wave, without bank conflicts, 0.5% less (kept).
 // Measured, 16 heads on 8 kv heads: 2000 tokens behind 12,000 218 us (980 TFLOP/s), 4 of 256 to 512 behind 900 to 3000 60,
 // 512 alone 14.
 //
@@ -729,13 +730,13 @@ __global__ void __launch_bounds__(KG *kTileThreads, 2) kv4_tile_kernel(Kv4Params
             const bool ok = block < static_cast<uint32_t>(p.num_blocks);  // else no records: the loads give zeros
             const auto d = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(pool) + static_cast<uint64_t>(ok ? block : 0) * block_bytes, 0,
                                                              ok ? kKv4Page : 0, kDescWord3);
-            kr = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, 16 * lane, 0, 0));  // key l / 4, dims 32 (l % 4) ..
-            ks = __builtin_amdgcn_raw_buffer_load_b8(d, kKv4KeyScales + lane, 0, 0);
+            kr = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, kHeadDim / 2 * (lane % 16) + 16 * (lane / 16), 0, 0));  // key l % 16, dims 32 (l / 16) ..
+            ks = __builtin_amdgcn_raw_buffer_load_b8(d, kKv4KeyScales + 4 * (lane % 16) + lane / 16, 0, 0);
             vr = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(d, kKv4Values + 16 * lane, 0, 0));
             vs = __builtin_amdgcn_raw_buffer_load_b32(d, kKv4ValueScales + kPage * (lane % 16 / 4) + 4 * (lane / 16), 0, 0);
         };
         auto stage = [&](int b) {
-            f16 *const kp = k_lds + (b & 1) * kKeyBuffer + (kPage * wave + lane / 4) * kKeyRow + 32 * (lane % 4);
+            f16 *const kp = k_lds + (b & 1) * kKeyBuffer + (kPage * wave + lane % 16) * kKeyRow + 32 * (lane / 16);
             f16 *const vp = v_lds + (b & 1) * kValueBuffer + (kPage * wave + 4 * (lane / 16)) * kValueRow + 8 * (lane % 16);
             const int key0 = page_of(b) * kPage + 4 * (lane / 16);
             if (page_of(b) * kPage + kPage - 1 > max_top)
@@ -914,6 +915,10 @@ struct Plan {
     int64_t bytes;  // of the workspace, with which items may be cut
 };
 
+int64_t bytes_of(const Plan &l, int n_kv) {
+    return kCounterBytes + static_cast<int64_t>(l.workers) * n_kv * 2 * l.rows * (kHeadDim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
 // Whether the work-groups share the items out evenly, or take one each. Sharing costs a scan of the lengths, partials
 // and their merge; not sharing, the wait for the longest item.
 //   Few rows: a work-group of its own takes 64 keys a wave in 0.95 us, all of them together 6.9 TB/s. Measured, us, one
@@ -946,11 +951,71 @@ Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences, int tokens) {
         items = tokens == 0 ? 0.0 : std::min(items, static_cast<double>(tokens) * (b.n_heads / b.n_kv) / l.rows + 0.5 * sequences);
     if (share_out(tiled, sequences == 1, b.n_kv * items, keys))
         l.workers = tiled ? most_workers : std::min(most_workers, 32 * sequences);
-    if (l.workers > 0) l.bytes = kCounterBytes + static_cast<int64_t>(l.workers) * b.n_kv * 2 * l.rows * (kHeadDim + 2) * 4;
+    if (l.workers > 0) l.bytes = bytes_of(l, b.n_kv);
     return l;
 }
 
 int64_t most_rows(const EmberRaggedBatch &b) { return static_cast<int64_t>(std::min(b.max_query, b.T)) * (b.n_heads / b.n_kv); }
+
+// A step of prompt chunks and many more decodes is two launches, a form each: sequences of up to 16 rows are walked, the
+// others' tiles shared out, an entry a sequence. It is told by the mean of the rows being less than a quarter of the most,
+// and pays where the decodes as tiles, of half the longest context, would take the CUs 12.5 us. Measured, us, 8 kv heads,
+// as tiles and as two launches: 960 decodes and 40 x 512 behind up to 1000 564, 346; 196 and 4 behind up to 4000 394, 210;
+// 64 and 1 behind up to 3000 105, 66, 24 and 1 53.5, 49.0, 18 and 1 47.7, 48.5, 8 and 1 37, 43; 30 and 2 behind up to 2000
+// 84, 58; 24 and 1 behind up to 600 26, 35.
+constexpr int kFewRows = 16;
+
+bool mixed(const EmberKv4AttnArgs &a, int64_t most) {
+    const EmberRaggedBatch &b = a.batch;
+    if (most <= 32 || 4 * static_cast<int64_t>(b.T) * (b.n_heads / b.n_kv) >= b.S * most) return false;
+    const double keys = static_cast<double>(std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage));
+    return static_cast<double>(b.S) * b.n_kv * 0.5 * (keys / 64) * 0.85 / kCus > 12.5;
+}
+
+Plan shared_tiles(const EmberRaggedBatch &b) {
+    Plan l{kTileRows, 1, kCus / b.n_kv, 0};
+    if (l.workers > 0) l.bytes = bytes_of(l, b.n_kv);
+    return l;
+}
+
+// One launch of a form, for the sequences of p.
+int run(const EmberRaggedBatch &b, Kv4Params p, const Plan &l, hipStream_t stream) {
+    p.tiles = l.tiles;
+    p.workers = b.workspace && b.workspace_bytes >= l.bytes ? l.workers : 0;  // uncut, an item each is as good
+    if (p.workers > 0) {
+        const int64_t groups = static_cast<int64_t>(l.workers) * b.n_kv;
+        p.counters = static_cast<uint32_t *>(b.workspace);
+        p.part_acc = reinterpret_cast<float *>(static_cast<uint8_t *>(b.workspace) + kCounterBytes);
+        p.part_ml = p.part_acc + 2 * groups * l.rows * kHeadDim;
+    }
+    const int64_t items = static_cast<int64_t>(p.S) * l.tiles * b.n_kv;
+    const int64_t groups = p.workers > 0 ? static_cast<int64_t>(p.workers) * b.n_kv : items;
+    if (groups > kMostLaunch)
+        return set_error(EMBER_ERR_INVALID, "kv4_attn: too many work-groups for one launch (S %d x n_kv %d)", b.S, b.n_kv);
+    if (l.rows == kTileRows) {
+        // A work-group of two key groups fills a CU; with more items than CUs, one each, two to a CU.
+        p.shift = 0;
+        while ((static_cast<int64_t>(b.T) * p.G / kTileRows + items) * ((b.max_blocks / kBlockPages >> p.shift) + 2) > INT32_MAX) p.shift++;
+        if (p.workers > 0 || items <= kCus)
+            hipLaunchKernelGGL(kv4_tile_kernel<2>, dim3(static_cast<unsigned>(groups)), dim3(2 * kTileThreads), 0, stream, p);
+        else
+            hipLaunchKernelGGL(kv4_tile_kernel<1>, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, stream, p);
+        return EMBER_OK;
+    }
+    auto go = [&](auto kernel, int step_pages) {
+        // The units of all items fit 31 bits.
+        const int64_t most_items = static_cast<int64_t>(b.T) * p.G / l.rows + static_cast<int64_t>(p.S) * l.tiles;
+        for (p.shift = 0; most_items * ((b.max_blocks / step_pages >> p.shift) + 2) > INT32_MAX; p.shift++) {}
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream, p);
+    };
+    // Steps of two pages leave room for a third work-group on a CU; where there is one at most, four pages are fewer
+    // steps. Measured, us, two and four: 256 items of up to 4096 keys 23.2, 21.4; 512 35.7, 36.9; 2048 of up to 900
+    // 32.4, 38.9.
+    if (l.rows == 32) go(kv4_walk_kernel<2, kWaves, 2>, 2);
+    else if (p.workers == 0 && items <= kCus) go(kv4_walk_kernel<1, kWaves, 4>, 4);
+    else go(kv4_walk_kernel<1, kWaves, 2>, 2);
+    return EMBER_OK;
+}
 
 }  // namespace
 
@@ -958,7 +1023,7 @@ int64_t most_rows(const EmberRaggedBatch &b) { return static_cast<int64_t>(std::
 // the fewer their tokens. (From 16 sequences on a kv head has no more work-groups.)
 int64_t kv4_workspace_bytes(const EmberKv4AttnArgs &a) {
     const int64_t most = most_rows(a.batch);
-    int64_t bytes = 0;
+    int64_t bytes = a.batch.S > 1 && most > 32 ? shared_tiles(a.batch).bytes : 0;
     for (int64_t rows : {16, 32, 33})
         for (int sequences = 1; sequences <= std::min(a.batch.S, 16); sequences++)
             bytes = std::max(bytes, plan(a, std::min(most, rows), sequences, 0).bytes);
@@ -977,41 +1042,20 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
     for (int s0 = 0; s0 < b.S; s0 += kMostSequences) {
         p.S = std::min(kMostSequences, b.S - s0);
         p.query_start = b.query_start + s0, p.tables = b.block_tables + static_cast<int64_t>(s0) * b.max_blocks;
-        const Plan l = plan(a, most_rows(b), p.S, b.T);
-        p.tiles = l.tiles;
-        p.workers = b.workspace && b.workspace_bytes >= l.bytes ? l.workers : 0;  // uncut, an item each is as good
-        if (p.workers > 0) {
-            const int64_t groups = static_cast<int64_t>(l.workers) * b.n_kv;
-            p.counters = static_cast<uint32_t *>(b.workspace);
-            p.part_acc = reinterpret_cast<float *>(static_cast<uint8_t *>(b.workspace) + kCounterBytes);
-            p.part_ml = p.part_acc + 2 * groups * l.rows * kHeadDim;
+        const int64_t most = most_rows(b);
+        int e = EMBER_OK;
+        if (mixed(a, most)) {
+            p.least = 1, p.most = kFewRows;
+            e = run(b, p, plan(a, kFewRows, p.S, b.T), stream);
+            p.least = kFewRows + 1, p.most = INT_MAX;
+            const Plan shared = shared_tiles(b);
+            const bool can = shared.workers > 0 && b.workspace && b.workspace_bytes >= shared.bytes;
+            if (e == EMBER_OK) e = run(b, p, can ? shared : plan(a, most, p.S, b.T), stream);
+        } else {
+            p.least = 1, p.most = INT_MAX;
+            e = run(b, p, plan(a, most, p.S, b.T), stream);
         }
-        const int64_t items = static_cast<int64_t>(p.S) * l.tiles * b.n_kv;
-        const int64_t groups = p.workers > 0 ? static_cast<int64_t>(p.workers) * b.n_kv : items;
-        if (groups > kMostLaunch)
-            return set_error(EMBER_ERR_INVALID, "kv4_attn: too many work-groups for one launch (S %d x n_kv %d)", b.S, b.n_kv);
-        if (l.rows == kTileRows) {
-            // A work-group of two key groups fills a CU; with more items than CUs, one each, two to a CU.
-            p.shift = 0;
-            while ((static_cast<int64_t>(b.T) * p.G / kTileRows + items) * ((b.max_blocks / kBlockPages >> p.shift) + 2) > INT32_MAX) p.shift++;
-            if (p.workers > 0 || items <= kCus)
-                hipLaunchKernelGGL(kv4_tile_kernel<2>, dim3(static_cast<unsigned>(groups)), dim3(2 * kTileThreads), 0, stream, p);
-            else
-                hipLaunchKernelGGL(kv4_tile_kernel<1>, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, stream, p);
-            continue;
-        }
-        auto go = [&](auto kernel, int step_pages) {
-            // The units of all items fit 31 bits.
-            const int64_t most_items = static_cast<int64_t>(b.T) * p.G / l.rows + static_cast<int64_t>(p.S) * l.tiles;
-            for (p.shift = 0; most_items * ((b.max_blocks / step_pages >> p.shift) + 2) > INT32_MAX; p.shift++) {}
-            hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kThreads), 0, stream, p);
-        };
-        // Steps of two pages leave room for a third work-group on a CU; where there is one at most, four pages are fewer
-        // steps. Measured, us, two and four: 256 items of up to 4096 keys 23.2, 21.4; 512 35.7, 36.9; 2048 of up to 900
-        // 32.4, 38.9.
-        if (l.rows == 32) go(kv4_walk_kernel<2, kWaves, 2>, 2);
-        else if (p.workers == 0 && items <= kCus) go(kv4_walk_kernel<1, kWaves, 4>, 4);
-        else go(kv4_walk_kernel<1, kWaves, 2>, 2);
+        if (e != EMBER_OK) return e;
     }
     return hip_status(hipGetLastError(), "kv4_attn");
 }

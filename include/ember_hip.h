@@ -527,7 +527,9 @@ typedef struct EmberKv4AttnArgs {
 /* Causal attention (keys 0..p_i of each token) of a ragged batch over 4-bit
  * pages, as section 1b describes a batch. The workspace is zero-filled once
  * after allocation; every launch leaves it ready for the next, of whatever
- * sizes. Calls that overlap in time need one each. */
+ * sizes. Calls that overlap in time need one each. Without one, or with one
+ * that is too small, no keys are shared out: the same outputs up to rounding,
+ * slower where sequences are few and long. */
 int ember_hip_kv4_attn(const EmberKv4AttnArgs *args, void *stream);
 /* Bytes of workspace ember_hip_kv4_attn uses for these sizes (only the sizes
  * of args are read; 0: it would not split). Enough for smaller T, S, max_query

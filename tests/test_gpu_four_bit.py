@@ -264,6 +264,16 @@ def test_attention_of_long_contexts_shared_out(rng, device, H, KV):
     check(b, attend(b, device))
 
 
+@pytest.mark.parametrize("cut", [True, False])
+@pytest.mark.parametrize("H,KV", [(4, 2), (8, 1), (40, 2)])
+def test_attention_of_steps_of_decodes_and_prompts(rng, device, H, KV, cut):
+    """Many decodes, short runs and a few chunks in one call, told to be of long contexts."""
+    new = [1] * 60 + [5, 90, 0, 17, 130, 16, 1]
+    b = batch(rng, device, [(int(c), n) for c, n in zip(rng.integers(0, 500, len(new)), new)] + [(3000, 1), (2600, 70)], H, KV)
+    b["longest"] = 30_000
+    check(b, attend(b, device, cut=cut, pad=3))
+
+
 def test_a_workspace_serves_calls_of_every_shape(rng, device):
     """Prompts, runs and decodes in turn with one workspace: each leaves it as the others, laid out otherwise, need it."""
     ws = K.kv4_workspace(200, 6, n_heads=8, n_kv=2, max_query=100, max_context=100_000, device=device)
