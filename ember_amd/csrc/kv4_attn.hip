@@ -602,10 +602,12 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
 
 // 128 rows a work-group; wave w owns rows 32 w .. + 31 of the tile, lane l = 32 h + c serves row c.
 //
-// Bound by three units that are each busy about half of the cycles: the matrix unit 47%, the VALU (softmax, conversion)
-// 46%, LDS 57% (every wave reads a block's 32 KB). Tried against 233 us for 2000 tokens behind 12,000: group 1 half a step
-// behind group 0, its softmax beside the other's products, 247; work-groups of one key group, two to a CU, 237; a wave's
-// priority raised during its products 230 (kept); keys staged 16 to a quarter wave, without bank conflicts, 0.5% less (kept).
+// Bound by the matrix unit (48% of the cycles), the VALU (softmax, conversion: 47%) and LDS (59%) in turns: each product
+// reads a KiB of LDS, so four SIMDs at products take all of its 128 bytes a cycle, and the two waves of a SIMD mostly do
+// the same. Tried against 233 us for 2000 tokens behind 12,000: group 1 half a step behind group 0, its softmax beside the
+// other's products, 247; work-groups of one key group, two to a CU, 237; a wave's priority raised during its products 230
+// (kept); keys staged 16 to a quarter wave, without bank conflicts, 229 (kept); group 0 always before group 1, by priority,
+// 233 to 241; the two halves' chains of score products alternating 229.
 // Measured, 16 heads on 8 kv heads: 2000 tokens behind 12,000 218 us (980 TFLOP/s), 4 of 256 to 512 behind 900 to 3000 60,
 // 512 alone 14.
 //
