@@ -9,12 +9,13 @@
 // codes are one 4-byte store.
 //
 // Bound by memory for many tokens, at 90% of a large copy's rate: us a launch,
-// 9100 tokens of 32 + 8 + 8 heads 47 (4.2 TB/s), with k_out, v_out and a bias
+// 9100 tokens of 32 + 8 + 8 heads 45 (4.3 TB/s), with k_out, v_out and a bias
 // 62; 16,384 tokens of 16 + 8 + 8 heads 51; 32 tokens 4.4, a launch and three
 // trips to memory. Waves without q or k heads take no sine and cosine, waves
 // without heads end at once (56, 68 and 59 us before). Tried: a wave for all
 // heads of a token, one sine and cosine for them all (8.0 us for 32 tokens, 55
-// for 9100: 112 registers leave half the waves).
+// for 9100: 112 registers leave half the waves); sines and cosines once for 2 or
+// 4 tokens' waves, through LDS (53 and 63 for 9100).
 #include "device.hpp"
 #include "four_bit.hpp"
 #include "kernels.hpp"
