@@ -439,7 +439,9 @@ def _launch(fn, args, dev: int, stream, what: str) -> None:
 
 def _new_on(dev: int, stream, *shape):
     """An uninitialised uint8 tensor for a launch on `stream`: its memory is not one that another stream still uses."""
-    if stream is not None and not hasattr(stream, "cuda_stream"):
+    if stream is None:
+        return torch.empty(shape, dtype=torch.uint8, device=f"cuda:{dev}")
+    if not hasattr(stream, "cuda_stream"):
         stream = torch.cuda.ExternalStream(int(stream), device=dev)
     with torch.cuda.stream(stream):
         return torch.empty(shape, dtype=torch.uint8, device=f"cuda:{dev}")
