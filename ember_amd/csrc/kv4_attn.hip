@@ -40,6 +40,8 @@ constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr int kLeastUnits = 8;  // of a work-group's share
 constexpr int kRowPitch = kHeadDim + 4;  // floats of a row's partial in LDS
 
+constexpr int kMostDealt = 256;  // sequences of a launch whose items are dealt by length
+
 struct Kv4Params {
     const f16 *q;
     const uint8_t *pool;
@@ -53,6 +55,7 @@ struct Kv4Params {
     int tiles;    // entries of a sequence: its row tiles, those past the hint together in the last
     int least, most;  // rows of the sequences that this launch is for
     int shift;    // a unit of their shares is 2^shift steps of pages
+    int round;    // without sharing: sequences whose items fill the CUs once, if they are dealt by length, else 0
     float scale_log2;
 };
 
@@ -246,11 +249,19 @@ struct Parts {
     int begin = 0, x = 0, end;
     Shares shares{0, 0, 0};
 
-    __device__ __forceinline__ int load(int e) {
-        const int s = min(p.tiles == 1 ? e : e / p.tiles, p.S - 1), k = p.tiles == 1 ? 0 : e - s * p.tiles;
-        const int guess = p.positions[min(s, p.T - 1)];  // the last position of a sequence of a pure decode step
-        const int t0 = clamped(p.query_start[s], p.T), t1 = min(max(p.query_start[s + 1], t0), p.T);
-        int pos = guess;
+    struct Raw {
+        int start, stop, guess;  // the guess: the last position of a sequence of a pure decode step
+    };
+    __device__ __forceinline__ int sequence(int e) const { return min(p.tiles == 1 ? e : e / p.tiles, p.S - 1); }
+    __device__ __forceinline__ Raw fetch(int e) const {
+        const int s = sequence(e);
+        return {p.query_start[s], p.query_start[s + 1], p.positions[min(s, p.T - 1)]};
+    }
+    __device__ __forceinline__ int load(int e) { return settle(e, fetch(e)); }
+    __device__ __forceinline__ int settle(int e, const Raw &raw) {
+        const int s = sequence(e), k = p.tiles == 1 ? 0 : e - s * p.tiles;
+        const int t0 = clamped(raw.start, p.T), t1 = min(max(raw.stop, t0), p.T);
+        int pos = raw.guess;
         if (__builtin_amdgcn_ballot_w64(t1 - 1 != s)) pos = p.positions[max(t1 - 1, 0)];
         seq_t0 = t0, seq_rows = (t1 - t0) * p.G;
         const int all = e < p.S * p.tiles && seq_rows >= p.least && seq_rows <= p.most ? (seq_rows + ROWS - 1) / ROWS : 0;
@@ -270,10 +281,52 @@ struct Parts {
         }
         return v;
     }
+    // The entry of a work-group by length: the longest to the first, and the other way round in every second round, so that
+    // a CU's first item and its second are together about as long as any other's. The k-th largest, found bit by bit.
+    __device__ __forceinline__ void deal() {
+        const int turn = worker / p.round, first = turn * p.round;
+        int k = turn % 2 ? first + min(p.round, p.S - first) - 1 - (worker - first) : worker;
+        const int top = 1 << (31 - __builtin_clz(max(p.max_blocks, 1)));  // of an item; entries of several tiles count as 2 top - 1 at most
+        Raw raw[kMostDealt / kWave];
+        int units[kMostDealt / kWave];
+#pragma unroll
+        for (int c = 0; c < kMostDealt / kWave; c++)
+            if (c < chunks()) raw[c] = fetch(c * kWave + lane);
+#pragma unroll
+        for (int c = 0; c < kMostDealt / kWave; c++)
+            if (units[c] = -1; c < chunks()) {
+                upto = settle(c * kWave + lane, raw[c]);
+                units[c] = c * kWave + lane < p.S ? min(upto, 2 * top - 1) : -1;
+            }
+        auto count = [&](int least) {
+            int n = 0;
+#pragma unroll
+            for (int c = 0; c < kMostDealt / kWave; c++) n += __popcll(__builtin_amdgcn_ballot_w64(units[c] >= least));
+            return n;
+        };
+        int value = 0;
+        for (int bit = top; bit > 0; bit >>= 1) value += count(value + bit) > k ? bit : 0;
+        k -= count(value + 1);
+#pragma unroll
+        for (int c = 0; c < kMostDealt / kWave; c++) {
+            const uint64_t same = __builtin_amdgcn_ballot_w64(units[c] == value);
+            const uint64_t it = __builtin_amdgcn_ballot_w64(units[c] == value && __popcll(same & ((1ull << lane) - 1)) == k);
+            if (it) {
+                chunk = c, at = __builtin_ctzll(it);
+                if (chunks() > 1) upto = settle(c * kWave + lane, raw[c]);
+            }
+            k -= __popcll(same);
+        }
+        end = __builtin_amdgcn_readlane(upto, at);
+    }
     __device__ __forceinline__ int chunks() const { return (p.S * p.tiles + kWave - 1) / kWave; }
 
     __device__ __forceinline__ Parts(const Kv4Params &params, int lane, int worker) : p(params), lane(lane), worker(worker), workers(params.workers) {
         if (workers == 0) {
+            if (p.round > 0) {
+                deal();
+                return;
+            }
             upto = load(worker);
             end = upto = uniform(upto);
             chunk = worker / kWave, at = worker % kWave;
@@ -915,6 +968,7 @@ struct Plan {
     int tiles;      // entries of a sequence
     int workers;    // work-groups of a kv head that share out its items; 0: one an entry
     int64_t bytes;  // of the workspace, with which items may be cut
+    int64_t keys;   // of the longest context
 };
 
 int64_t bytes_of(const Plan &l, int n_kv) {
@@ -944,7 +998,7 @@ Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences, int tokens) {
     Plan l{};
     l.rows = most <= 16 ? 16 : most <= 32 ? 32 : kTileRows;
     l.tiles = static_cast<int>(std::clamp<int64_t>((most + l.rows - 1) / l.rows, 1, std::max(1, kMostSequences / sequences)));
-    const int64_t keys = std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage);
+    const int64_t keys = l.keys = std::min<int64_t>(a.max_context, static_cast<int64_t>(b.max_blocks) * kPage);
     const bool tiled = l.rows == kTileRows;
     // An item in more than 32 pieces is merged slower than it is read (131,000 keys in 64 pieces 36.6 us, in 32 32.4).
     const int most_workers = (tiled ? kCus : kWalkGroups) / b.n_kv;  // of kv heads that fill the chip by themselves, none
@@ -975,7 +1029,7 @@ bool mixed(const EmberKv4AttnArgs &a, int64_t most) {
 }
 
 Plan shared_tiles(const EmberRaggedBatch &b) {
-    Plan l{kTileRows, 1, kCus / b.n_kv, 0};
+    Plan l{kTileRows, 1, kCus / b.n_kv, 0, 0};
     if (l.workers > 0) l.bytes = bytes_of(l, b.n_kv);
     return l;
 }
@@ -1004,6 +1058,12 @@ int run(const EmberRaggedBatch &b, Kv4Params p, const Plan &l, hipStream_t strea
             hipLaunchKernelGGL(kv4_tile_kernel<1>, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, stream, p);
         return EMBER_OK;
     }
+    // More items than CUs, each with a work-group, are dealt by length, which costs each of them a look at all lengths, 1 us
+    // for 64 sequences, 3 for 256: worth it where the longest are long. Measured, us, as they come and dealt: 48 sequences
+    // of 256 to 4095 keys 34.4, 28.0; 64 37.3, 31.4; 100 55.5, 47.0; 250 of 100 to 4000 101, 94; 64 of up to 4096 with up to
+    // 5 tokens 36.5, 33.6; 200 of up to 2000 45.2, 47.4; 64 of 2000 each 27.6, 28.5; 33 of up to 4095 23.5, 25.5.
+    const int chunks = (p.S + kWave - 1) / kWave;
+    p.round = p.workers == 0 && p.S <= kMostDealt && 4 * items > 5 * kCus && l.keys > 1536 + 512 * chunks ? std::max(1, kCus / b.n_kv) : 0;
     auto go = [&](auto kernel, int step_pages) {
         // The units of all items fit 31 bits.
         const int64_t most_items = static_cast<int64_t>(b.T) * p.G / l.rows + static_cast<int64_t>(p.S) * l.tiles;

@@ -290,6 +290,27 @@ def test_a_workspace_serves_calls_of_every_shape(rng, device):
         check(b, args[2].double().cpu().numpy())
 
 
+@pytest.mark.parametrize("S,H,KV", [(64, 16, 8), (47, 8, 8), (65, 10, 5), (200, 4, 2), (256, 2, 2), (170, 12, 2)])
+def test_attention_dealt_by_length(rng, device, S, H, KV):
+    """More items than CUs of contexts that may be long: many lengths alike, empty sequences, runs of several tokens."""
+    seqs = [(int(c), int(n)) for c, n in zip(rng.choice([0, 16, 33, 150, 700], S), rng.choice([1, 1, 1, 0, 2], S))]
+    seqs[S // 2] = 4000, 1
+    b = batch(rng, device, seqs, H, KV)
+    check(b, attend(b, device, pad=2))
+    check(b, attend(b, device, cut=False))
+    b["table"][3, 1:] = -1  # missing pages
+    b["most"] = 1
+    check(b, attend(b, device))
+    # longer runs than the call was told of: entries of many tiles
+    seqs = [(int(c), 1) for c in rng.integers(0, 300, S)]
+    seqs[1] = seqs[S - 2] = 900, 300
+    b = batch(rng, device, seqs, H, KV)
+    b["most"], b["longest"] = 1, 260 * PAGE
+    b["table"] = np.pad(b["table"], ((0, 0), (0, 260 - b["table"].shape[1])), constant_values=-1)
+    b["W"] = 260
+    check(b, attend(b, device))
+
+
 def test_attention_of_more_sequences_than_a_launch_takes(rng, device):
     b = batch(rng, device, [(int(c), 1) for c in rng.integers(0, 40, 4200)], 1, 1)
     check(b, attend(b, device, pad=1))
