@@ -411,7 +411,7 @@ struct Parts {
 // chain of trips to memory (lengths, page ids, pages, out).
 // Measured, 8 kv heads: 1 sequence of 640 keys 8.0 us, of 131,000 32 (4.4
 // TB/s); 32 of 256 to 4095 22 (4.1 TB/s); 8 of 30,000 to 131,000 124 (6.1
-// TB/s); 64 of 512 to 4096 with up to 5 tokens each 36 (4.9 TB/s).
+// TB/s); 64 of 512 to 4096 with up to 5 tokens each 33 (5.4 TB/s).
 template <int RT, int W, int P>
 __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
     constexpr int D = kHeadDim, kRows = 16 * RT, kThreads = W * kWave;
