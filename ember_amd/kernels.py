@@ -437,14 +437,15 @@ def _launch(fn, args, dev: int, stream, what: str) -> None:
         check(code, what)
 
 
-def _new_on(dev: int, stream, *shape):
-    """An uninitialised uint8 tensor for a launch on `stream`: its memory is not one that another stream still uses."""
+def _new_on(device, stream, make, *shape):
+    """make(shape) in uint8 (torch.empty or torch.zeros) for a launch on `stream`: its memory is not one that another
+    stream still uses, and is written in that stream's order."""
     if stream is None:
-        return torch.empty(shape, dtype=torch.uint8, device=f"cuda:{dev}")
+        return make(shape, dtype=torch.uint8, device=device)
     if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(int(stream), device=dev)
+        stream = torch.cuda.ExternalStream(int(stream), device=device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=torch.uint8, device=f"cuda:{dev}")
+        return make(shape, dtype=torch.uint8, device=device)
 
 
 def _refuse(tensors: dict, dev: int, dtype) -> None:
@@ -567,13 +568,18 @@ def _batch_sizes(T, S, n_heads, n_kv, max_query, dtype, max_blocks):
             (T or 1) if max_query is None else max_query, 0, 0)
 
 
+def _workspace_bytes(size, args) -> int:
+    n = int(size(args))
+    if n == 0 and _lib.last_error():  # sizes that no call takes
+        raise EmberError(_lib.last_error())
+    return n
+
+
 def _workspace(size, args, dtype, device):
     """A workspace of size(args) bytes, or None for 0 of them."""
     if not (dtype is torch.float16 or dtype is torch.float32):
         raise EmberError(f"dtype must be f16 or f32 (got {dtype})")
-    n = int(size(args))
-    if n == 0 and _lib.last_error():  # sizes that no call takes
-        raise EmberError(_lib.last_error())
+    n = _workspace_bytes(size, args)
     return torch.empty(n, dtype=torch.uint8, device=device) if n > 0 else None
 
 
@@ -701,13 +707,15 @@ def kv4_append(qkv, q_out, pool, positions, token_seq, block_tables, *, n_heads,
     _launch(_lib.lib().ember_hip_kv4_append, a, dev, stream, "kv4_append")
 
 
-def kv4_workspace(T: int, S: int, *, n_heads, n_kv, max_query=None, max_context=None, max_blocks=None, device="cuda"):
+def kv4_workspace(T: int, S: int, *, n_heads, n_kv, max_query=None, max_context=None, max_blocks=None, device="cuda",
+                  stream=None):
     """A workspace (zeros) for kv4_attention of batches of these sizes and smaller ones, or None when no such call splits
-    its keys. Only kv4_attention may write to it."""
+    its keys. Only kv4_attention may write to it: not a workspace of the other attentions, which keep nothing between
+    calls. It is zeroed in the order of `stream` (None: torch's current one); calls on another stream wait for that."""
     a = _lib.Kv4AttnArgs(*_batch_sizes(T, S, n_heads, n_kv, max_query, torch.float16, max_blocks),
                          _context(max_context, 1 << 26 if max_blocks is None else max_blocks))
-    ws = _workspace(_lib.lib().ember_hip_kv4_workspace_bytes, a, torch.float16, device)
-    return None if ws is None else ws.zero_()
+    n = _workspace_bytes(_lib.lib().ember_hip_kv4_workspace_bytes, a)
+    return _new_on(device, stream, torch.zeros, n) if n > 0 else None
 
 
 def _context(max_context, max_blocks):
@@ -743,7 +751,7 @@ def mx_quantize(x, stream=None):
     if dev < 0 or x.dim() != 2 or not (x.dtype is torch.float16 or x.dtype is torch.float32) or (x.shape[1] > 1 and x.stride(1) != 1):
         raise EmberError("mx_quantize: x must be an f16 or f32 device tensor [rows, cols] with contiguous rows")
     rows, cols = x.shape
-    codes, scales = _new_on(dev, stream, rows, cols // 2), _new_on(dev, stream, rows, cols // _lib.MX_GROUP)
+    codes, scales = (_new_on(x.device, stream, torch.empty, rows, n) for n in (cols // 2, cols // _lib.MX_GROUP))
     a = _lib.MxQuantizeArgs(x.data_ptr(), x.stride(0) if rows > 1 else cols, rows, cols, _dtype_code(x), codes.data_ptr(),
                             scales.data_ptr())
     _launch(_lib.lib().ember_hip_mx_quantize, a, dev, stream, "mx_quantize")
@@ -763,7 +771,7 @@ def gemv4_pack(codes, scales, stream=None):
     n = int(_lib.lib().ember_hip_gemv4_packed_bytes(N, K))
     if n <= 0:
         raise EmberError(_lib.last_error())
-    out = _new_on(dev, stream, n)
+    out = _new_on(codes.device, stream, torch.empty, n)
     fn = _lib.lib().ember_hip_gemv4_pack
     _launch(lambda args, handle: fn(*args, handle), (codes.data_ptr(), scales.data_ptr(), N, K, out.data_ptr()), dev, stream, "gemv4_pack")
     return out

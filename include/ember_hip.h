@@ -424,9 +424,11 @@ typedef struct EmberRaggedBatch {
     float scale;                 /* positive, below 2.3e38 */
     int32_t max_query;           /* tokens of the longest sequence's run; more are computed, slower */
     /* Scratch for splitting the keys over work-groups, 16-byte aligned, no
-     * initial contents, nothing kept between launches. With NULL or fewer bytes
-     * than ember_hip_*_workspace_bytes says there are fewer splits, and the call
-     * is slower. Launches that overlap in time must not share one. */
+     * initial contents, nothing kept between launches: but ember_hip_kv4_attn
+     * (section 1c) needs one of its own, zeros at first, that no other call
+     * writes. With NULL or fewer bytes than ember_hip_*_workspace_bytes says
+     * there are fewer splits, and the call is slower. Launches that overlap in
+     * time must not share one. */
     void *workspace;
     int64_t workspace_bytes;
 } EmberRaggedBatch;
@@ -526,8 +528,10 @@ typedef struct EmberKv4AttnArgs {
 
 /* Causal attention (keys 0..p_i of each token) of a ragged batch over 4-bit
  * pages, as section 1b describes a batch. The workspace is zero-filled once
- * after allocation; every launch leaves it ready for the next, of whatever
- * sizes. Calls that overlap in time need one each. Without one, or with one
+ * after allocation, before the first launch on whatever stream; every launch
+ * leaves it ready for the next, of whatever sizes. No other call may write it:
+ * with other contents the rows of an item whose keys are shared out may never
+ * be written. Calls that overlap in time need one each. Without one, or with one
  * that is too small, no keys are shared out: the same outputs up to rounding,
  * slower where sequences are few and long. */
 int ember_hip_kv4_attn(const EmberKv4AttnArgs *args, void *stream);
