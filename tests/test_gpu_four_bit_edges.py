@@ -41,3 +41,25 @@ def test_a_workspace_is_zeroed_in_the_order_of_its_calls_stream(rng, device, han
     check(b, out.double().cpu().numpy())
     torch.cuda.synchronize()
     del busy
+
+
+def test_prepared_tensors_are_not_ones_that_the_current_stream_still_writes(rng, device):
+    """Blocks that the current stream has freed, with writes to them still queued there, are not what mx_quantize and
+    gemv4_pack return on another stream."""
+    x = on(rng.standard_normal((4096, 4096)).astype(np.float32), device)
+    codes, scales = K.mx_quantize(x)
+    packed = K.gemv4_pack(codes, scales)
+    s = torch.cuda.Stream()
+    for like, call in ((codes, lambda: K.mx_quantize(x, stream=s)[0]), (scales, lambda: K.mx_quantize(x, stream=s)[1]),
+                       (packed, lambda: K.gemv4_pack(codes, scales, stream=s))):
+        torch.cuda.synchronize()
+        busy = keep_busy()
+        freed = torch.empty_like(like)
+        at = freed.data_ptr()
+        freed.fill_(99)  # runs behind the products
+        del freed
+        assert torch.empty_like(like).data_ptr() == at  # what an allocation on the current stream would get
+        got = call()
+        torch.cuda.synchronize()
+        assert torch.equal(got, like)
+        del busy
