@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libember_hip.so"
 
 # Constants of include/ember_hip.h.
-ABI_VERSION = 8
+ABI_VERSION = 9
 BLOCK_SIZE = 16
 PREFILL_TILE = 64
 MAX_RUN = 8
@@ -189,6 +189,11 @@ class Kv4AttnArgs(ctypes.Structure):
     _fields_ = RaggedBatch._fields_ + [("max_context", c_int32)]
 
 
+class Kv4Launch(ctypes.Structure):
+    _fields_ = [("workspace", c_int64), ("rows", c_int32), ("sharers", c_int32), ("dealt", c_int32), ("least", c_int32), ("most", c_int32),
+                ("reserved", c_int32)]
+
+
 class MxQuantizeArgs(ctypes.Structure):
     _fields_ = [("x", c_void_p), ("ld", c_int64), ("rows", c_int32), ("cols", c_int32), ("dtype", c_int32),
                 ("codes", c_void_p), ("scales", c_void_p)]
@@ -201,7 +206,7 @@ class Gemv4Args(ctypes.Structure):
 
 STRUCTS = [QkvArgs, AttnArgs, PrefillArgs, CopyArgs, KvConfig, StepBatchC, LayerIo, GemvArgs, NormArgs, EmbedArgs,
            SampleParams, SampleArgs, ProbArgs, BackendOptions, ModelInfo, StepTablesArgs, RaggedBatch, WindowAttnArgs,
-           PrefixAttnArgs, Kv4AppendArgs, Kv4AttnArgs, MxQuantizeArgs, Gemv4Args]
+           PrefixAttnArgs, Kv4AppendArgs, Kv4AttnArgs, MxQuantizeArgs, Gemv4Args, Kv4Launch]
 
 # name -> (restype, argtypes); every extern "C" symbol of include/ember_hip.h.
 PROTOTYPES = {
@@ -227,6 +232,7 @@ PROTOTYPES = {
     "ember_hip_kv4_append": (c_int32, [POINTER(Kv4AppendArgs), c_void_p]),
     "ember_hip_kv4_attn": (c_int32, [POINTER(Kv4AttnArgs), c_void_p]),
     "ember_hip_kv4_workspace_bytes": (c_int64, [POINTER(Kv4AttnArgs)]),
+    "ember_hip_kv4_attn_plan": (c_int32, [POINTER(Kv4AttnArgs), POINTER(Kv4Launch)]),
     "ember_hip_mx_quantize": (c_int32, [POINTER(MxQuantizeArgs), c_void_p]),
     "ember_hip_gemv4_pack": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "ember_hip_gemv4_packed_bytes": (c_int64, [c_int32, c_int32]),

@@ -181,6 +181,7 @@ int32_t ember_hip_sizeof(int32_t which) {
         case 20: return sizeof(EmberKv4AttnArgs);
         case 21: return sizeof(EmberMxQuantizeArgs);
         case 22: return sizeof(EmberGemv4Args);
+        case 23: return sizeof(EmberKv4Launch);
         default: return -1;
     }
 }
@@ -501,6 +502,14 @@ int64_t ember_hip_kv4_workspace_bytes(const EmberKv4AttnArgs *a) {
         a->batch.S == 0)
         return 0;
     return kv4_workspace_bytes(*a);
+}
+
+int ember_hip_kv4_attn_plan(const EmberKv4AttnArgs *a, EmberKv4Launch *launches) {
+    g_last_error.clear();
+    if (!a || !launches) return set_error(EMBER_ERR_INVALID, "kv4_attn_plan: null arguments");
+    if (int e = check_batch_sizes("kv4_attn_plan", a->batch)) return e;
+    if (int e = check_kv4("kv4_attn_plan", *a)) return e;
+    return a->batch.T == 0 || a->batch.S == 0 ? 0 : kv4_attn_plan(*a, launches);
 }
 
 int ember_hip_mx_quantize(const EmberMxQuantizeArgs *a, void *stream) {

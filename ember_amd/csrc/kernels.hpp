@@ -72,6 +72,7 @@ int64_t shared_prefix_workspace_bytes(const EmberPrefixAttnArgs &a);
 hipError_t launch_kv4_append(const EmberKv4AppendArgs &a, hipStream_t stream);
 int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream);  // an EMBER_* / hipError_t code
 int64_t kv4_workspace_bytes(const EmberKv4AttnArgs &a);
+int kv4_attn_plan(const EmberKv4AttnArgs &a, EmberKv4Launch *out);  // the number of launches, 1 or 2
 hipError_t launch_mx_quantize(const EmberMxQuantizeArgs &a, hipStream_t stream);
 hipError_t launch_gemv4_pack(const uint8_t *codes, const uint8_t *scales, int N, int K, void *out, hipStream_t stream);
 int64_t gemv4_packed_bytes(int N, int K);

@@ -1034,10 +1034,46 @@ Plan shared_tiles(const EmberRaggedBatch &b) {
     return l;
 }
 
-// One launch of a form, for the sequences of p.
-int run(const EmberRaggedBatch &b, Kv4Params p, const Plan &l, hipStream_t stream) {
+// More items than CUs, each with a work-group, are dealt by length, which costs each of them a look at all lengths, 1 us
+// for 64 sequences, 3 for 256: worth it where the longest are long. Measured, us, as they come and dealt: 48 sequences
+// of 256 to 4095 keys 34.4, 28.0; 64 37.3, 31.4; 100 55.5, 47.0; 250 of 100 to 4000 101, 94; 64 of up to 4096 with up to
+// 5 tokens 36.5, 33.6; 200 of up to 2000 45.2, 47.4; 64 of 2000 each 27.6, 28.5; 33 of up to 4095 23.5, 25.5.
+bool dealt(const Plan &l, int n_kv, int sequences) {
+    const int64_t items = static_cast<int64_t>(sequences) * l.tiles * n_kv, chunks = (sequences + kWave - 1) / kWave;
+    return l.rows < kTileRows && l.workers == 0 && sequences <= kMostDealt && 4 * items > 5 * kCus && l.keys > 1536 + 512 * chunks;
+}
+
+// A launch: its form, without workers where the workspace does not let it share, and the rows that its sequences have.
+struct Launch {
+    Plan plan;
+    int least, most;
+};
+
+// The launches of a call for `sequences` of its sequences.
+int launches(const EmberKv4AttnArgs &a, int sequences, Launch (&out)[2]) {
+    const EmberRaggedBatch &b = a.batch;
+    const int64_t most = most_rows(b);
+    auto can = [&](const Plan &l) { return l.workers > 0 && b.workspace && b.workspace_bytes >= l.bytes; };
+    auto launch = [&](Plan l, int least, int rows) {
+        if (!can(l)) l.workers = 0;  // uncut, an item each is as good
+        return Launch{l, least, rows};
+    };
+    if (!mixed(a, most)) {
+        out[0] = launch(plan(a, most, sequences, b.T), 1, INT_MAX);
+        return 1;
+    }
+    const Plan shared = shared_tiles(b);
+    out[0] = launch(plan(a, kFewRows, sequences, b.T), 1, kFewRows);
+    out[1] = launch(can(shared) ? shared : plan(a, most, sequences, b.T), kFewRows + 1, INT_MAX);
+    return 2;
+}
+
+// One launch, for the sequences of p.
+int run(const EmberRaggedBatch &b, Kv4Params p, const Launch &launch, hipStream_t stream) {
+    const Plan &l = launch.plan;
+    p.least = launch.least, p.most = launch.most;
     p.tiles = l.tiles;
-    p.workers = b.workspace && b.workspace_bytes >= l.bytes ? l.workers : 0;  // uncut, an item each is as good
+    p.workers = l.workers;
     if (p.workers > 0) {
         const int64_t groups = static_cast<int64_t>(l.workers) * b.n_kv;
         p.counters = static_cast<uint32_t *>(b.workspace);
@@ -1058,12 +1094,7 @@ int run(const EmberRaggedBatch &b, Kv4Params p, const Plan &l, hipStream_t strea
             hipLaunchKernelGGL(kv4_tile_kernel<1>, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), 0, stream, p);
         return EMBER_OK;
     }
-    // More items than CUs, each with a work-group, are dealt by length, which costs each of them a look at all lengths, 1 us
-    // for 64 sequences, 3 for 256: worth it where the longest are long. Measured, us, as they come and dealt: 48 sequences
-    // of 256 to 4095 keys 34.4, 28.0; 64 37.3, 31.4; 100 55.5, 47.0; 250 of 100 to 4000 101, 94; 64 of up to 4096 with up to
-    // 5 tokens 36.5, 33.6; 200 of up to 2000 45.2, 47.4; 64 of 2000 each 27.6, 28.5; 33 of up to 4095 23.5, 25.5.
-    const int chunks = (p.S + kWave - 1) / kWave;
-    p.round = p.workers == 0 && p.S <= kMostDealt && 4 * items > 5 * kCus && l.keys > 1536 + 512 * chunks ? std::max(1, kCus / b.n_kv) : 0;
+    p.round = dealt(l, b.n_kv, p.S) ? std::max(1, kCus / b.n_kv) : 0;
     auto go = [&](auto kernel, int step_pages) {
         // The units of all items fit 31 bits.
         const int64_t most_items = static_cast<int64_t>(b.T) * p.G / l.rows + static_cast<int64_t>(p.S) * l.tiles;
@@ -1092,6 +1123,16 @@ int64_t kv4_workspace_bytes(const EmberKv4AttnArgs &a) {
     return bytes;
 }
 
+int kv4_attn_plan(const EmberKv4AttnArgs &a, EmberKv4Launch *out) {
+    Launch each[2];
+    const int sequences = std::min(kMostSequences, a.batch.S), n = launches(a, sequences, each);
+    for (int i = 0; i < n; i++) {
+        const Plan &l = each[i].plan;
+        out[i] = {l.bytes, l.rows, l.workers, dealt(l, a.batch.n_kv, sequences), each[i].least, each[i].most, 0};
+    }
+    return n;
+}
+
 int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
     const EmberRaggedBatch &b = a.batch;
     Kv4Params p{};
@@ -1104,20 +1145,10 @@ int launch_kv4_attn(const EmberKv4AttnArgs &a, hipStream_t stream) {
     for (int s0 = 0; s0 < b.S; s0 += kMostSequences) {
         p.S = std::min(kMostSequences, b.S - s0);
         p.query_start = b.query_start + s0, p.tables = b.block_tables + static_cast<int64_t>(s0) * b.max_blocks;
-        const int64_t most = most_rows(b);
-        int e = EMBER_OK;
-        if (mixed(a, most)) {
-            p.least = 1, p.most = kFewRows;
-            e = run(b, p, plan(a, kFewRows, p.S, b.T), stream);
-            p.least = kFewRows + 1, p.most = INT_MAX;
-            const Plan shared = shared_tiles(b);
-            const bool can = shared.workers > 0 && b.workspace && b.workspace_bytes >= shared.bytes;
-            if (e == EMBER_OK) e = run(b, p, can ? shared : plan(a, most, p.S, b.T), stream);
-        } else {
-            p.least = 1, p.most = INT_MAX;
-            e = run(b, p, plan(a, most, p.S, b.T), stream);
-        }
-        if (e != EMBER_OK) return e;
+        Launch each[2];
+        const int n = launches(a, p.S, each);
+        for (int i = 0; i < n; i++)
+            if (const int e = run(b, p, each[i], stream); e != EMBER_OK) return e;
     }
     return hip_status(hipGetLastError(), "kv4_attn");
 }

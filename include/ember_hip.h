@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define EMBER_ABI_VERSION 8
+#define EMBER_ABI_VERSION 9
 #define EMBER_BLOCK_SIZE 16  /* tokens per page; kBlockSize, src/backend/backend.hpp:25 */
 #define EMBER_PREFILL_TILE 64 /* query tokens per prefill tile; kPrefillTile, kernels.cuh:108 */
 #define EMBER_MAX_RUN 8      /* query tokens one decode work-group reads a page for */
@@ -540,6 +540,22 @@ int ember_hip_kv4_attn(const EmberKv4AttnArgs *args, void *stream);
  * and max_context too. */
 int64_t ember_hip_kv4_workspace_bytes(const EmberKv4AttnArgs *args);
 
+typedef struct EmberKv4Launch {
+    int64_t workspace;           /* bytes of workspace with which this launch shares out keys (0: with none) */
+    int32_t rows;                /* (token, head) rows of a work-group: 16 or 32 (pages are converted in registers), 128 (in LDS) */
+    int32_t sharers;             /* work-groups of a kv head that share out the keys of all items; 0: one an item */
+    int32_t dealt;               /* 1: the items go to the work-groups by length */
+    int32_t least, most;         /* the launch takes the sequences with this many rows of a kv head */
+    int32_t reserved;            /* 0 */
+} EmberKv4Launch;
+
+/* How ember_hip_kv4_attn launches a call of these sizes (with more than 4096
+ * sequences: each 4096 of them): fills one or two entries of `launches` (room
+ * for 2) and returns how many; 0 without tokens, negative for sizes that no
+ * call takes. Only the sizes of args and its workspace are read, the latter
+ * not followed. A diagnostic for tests and benchmarks. */
+int ember_hip_kv4_attn_plan(const EmberKv4AttnArgs *args, EmberKv4Launch *launches);
+
 typedef struct EmberMxQuantizeArgs {
     const void *x;                /* f16 or f32 [rows, ld] */
     int64_t ld;                   /* elements between rows, at least cols */
@@ -588,7 +604,7 @@ int ember_hip_abi_version(void);
  * 12 EmberProbArgs, 13 EmberBackendOptions, 14 EmberModelInfo,
  * 15 EmberStepTablesArgs, 16 EmberRaggedBatch, 17 EmberWindowAttnArgs,
  * 18 EmberPrefixAttnArgs, 19 EmberKv4AppendArgs, 20 EmberKv4AttnArgs,
- * 21 EmberMxQuantizeArgs, 22 EmberGemv4Args; -1 otherwise. */
+ * 21 EmberMxQuantizeArgs, 22 EmberGemv4Args, 23 EmberKv4Launch; -1 otherwise. */
 int32_t ember_hip_sizeof(int32_t which);
 
 /* ---- 2. KV block manager ------------------------------------------------- */

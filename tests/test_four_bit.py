@@ -219,3 +219,63 @@ def test_workspaces_are_enough_for_smaller_batches(rng):
         for _ in range(8):
             less = [max(1, int(x * rng.uniform(0, 1))) for x in (T, S, mq, ctx)]
             assert need(*less) <= most, (T, S, mq, ctx, less)
+
+
+def _plan(T, S, n_heads, n_kv, max_query, max_context, max_blocks=1 << 14, workspace_bytes=1 << 40):
+    """The launches of a call of these sizes, as a list."""
+    a = _attn()
+    a.T, a.S, a.n_heads, a.n_kv, a.max_query, a.max_context, a.max_blocks = T, S, n_heads, n_kv, max_query, max_context, max_blocks
+    a.workspace, a.workspace_bytes = (4096, workspace_bytes) if workspace_bytes else (None, 0)  # not followed
+    out = (_lib.Kv4Launch * 2)()
+    n = _lib.lib().ember_hip_kv4_attn_plan(a, out)
+    assert n >= 0, _lib.last_error()
+    return list(out[:n])
+
+
+@pytest.mark.parametrize("field,value,text", SIZES)
+def test_plans_refuse_sizes_that_no_call_takes(field, value, text):
+    a = _attn()
+    setattr(a, field, value)
+    assert _lib.lib().ember_hip_kv4_attn_plan(a, (_lib.Kv4Launch * 2)()) == _lib.ERR_INVALID
+    assert text in _lib.last_error()
+
+
+def test_plans_of_nothing():
+    lib, out = _lib.lib(), (_lib.Kv4Launch * 2)()
+    assert lib.ember_hip_kv4_attn_plan(None, out) == _lib.ERR_INVALID and "null" in _lib.last_error()
+    assert lib.ember_hip_kv4_attn_plan(_attn(), None) == _lib.ERR_INVALID and "null" in _lib.last_error()
+    assert _plan(0, 2, 16, 8, 1, 100) == _plan(4, 0, 16, 8, 1, 100) == []
+
+
+def test_plans_of_the_forms():
+    """One sequence's decode, runs of up to 32 rows, prompts, many decodes, a step of decodes and a few chunks."""
+    one = _plan(1, 1, 16, 8, 1, 640)
+    assert [(x.rows, x.sharers, x.dealt) for x in one] == [(16, 0, 0)]
+    assert [(x.rows, x.sharers > 0) for x in _plan(1, 1, 16, 8, 1, 131072)] == [(16, True)]
+    assert [x.rows for x in _plan(20, 5, 32, 8, 8, 640)] == [32] and [x.rows for x in _plan(20, 5, 32, 8, 9, 640)] == [128]
+    assert [(x.rows, x.sharers, x.dealt) for x in _plan(64, 64, 16, 8, 1, 4096)] == [(16, 0, 1)]
+    mixed = _plan(960 + 40 * 512, 1000, 16, 8, 512, 1512)
+    assert [(x.rows, x.least, x.most) for x in mixed] == [(16, 1, 16), (128, 17, 2 ** 31 - 1)]
+    # without a workspace nothing is shared, with too small a one neither
+    for size in (0, mixed[1].workspace - 1):
+        assert all(x.sharers == 0 for x in _plan(960 + 40 * 512, 1000, 16, 8, 512, 1512, workspace_bytes=size))
+
+
+def test_workspaces_are_enough_for_what_their_calls_launch(rng):
+    """The reported size, whose launches' rows are not known yet, against what every launch of a call asks for."""
+    seen = set()
+    for _ in range(3000):
+        n_kv, G = int(rng.choice([1, 2, 8])), int(rng.choice([1, 2, 3, 4, 8, 16, 20, 32, 40]))
+        S, mq, ctx, W = (int(2 ** rng.uniform(0, x)) for x in (11, 11, 17, 13))
+        T = min(int(S * mq * rng.uniform(0, 1)) + 1, 1 << 16)
+        a = _attn()
+        a.T, a.S, a.max_blocks, a.n_heads, a.n_kv, a.max_query, a.max_context = T, S, W, n_kv * G, n_kv, mq, ctx
+        size = _lib.lib().ember_hip_kv4_workspace_bytes(a)
+        less = [max(1, int(x * rng.uniform(0, 1))) for x in (T, S, mq, ctx)]
+        for t, s, q, c in ((T, S, mq, ctx), less):
+            plan = _plan(t, s, n_kv * G, n_kv, q, c, W)
+            assert all(x.workspace <= size for x in plan), (T, S, mq, ctx, W, n_kv, G, t, s, q, c)
+            seen |= {(len(plan), x.rows, x.sharers > 0, x.dealt) for x in plan}
+    # of every kind: in one launch and in two, each form, shared and not, dealt
+    assert {(1, r, cut, 0) for r in (16, 32, 128) for cut in (False, True)} <= seen
+    assert {(2, 16, True, 0), (2, 128, True, 0), (1, 16, False, 1), (1, 32, False, 1)} <= seen

@@ -3,11 +3,33 @@ import numpy as np
 import pytest
 import torch
 
+from ember_amd import _lib
 from ember_amd import kernels as K
-from four_bit_reference import D
-from test_gpu_four_bit import batch, check, dint, on
+from four_bit_reference import D, PAGE
+from test_gpu_four_bit import attend, batch, check, dint, on
 
 pytestmark = pytest.mark.gpu
+
+
+def told(b, context, most=None):
+    """The batch with tables for `context` keys a sequence, and told that it has that many (and `most` tokens a sequence)."""
+    W = context // PAGE
+    b["table"] = np.pad(b["table"], ((0, 0), (0, max(0, W - b["W"]))), constant_values=-1)
+    b["W"] = b["table"].shape[1]
+    b["longest"] = context
+    b["most"] = most or b["most"]
+    return b
+
+
+def plan(b, cut=True, pad=0):
+    """How the call that attend() makes of the batch is launched."""
+    a = _lib.Kv4AttnArgs()
+    a.T, a.S, a.max_blocks, a.n_heads, a.n_kv, a.head_dim = b["T"] + pad, len(b["start"]) - 1, b["W"], b["H"], b["KV"], D
+    a.dtype, a.max_query, a.max_context = _lib.DTYPE_F16, b["most"], b["longest"]
+    if cut:
+        a.workspace, a.workspace_bytes = 4096, _lib.lib().ember_hip_kv4_workspace_bytes(a)  # not followed
+    out = (_lib.Kv4Launch * 2)()
+    return list(out[:_lib.lib().ember_hip_kv4_attn_plan(a, out)])
 
 
 def keep_busy():
@@ -63,3 +85,105 @@ def test_prepared_tensors_are_not_ones_that_the_current_stream_still_writes(rng,
         torch.cuda.synchronize()
         assert torch.equal(got, like)
         del busy
+
+
+# ---- the forms of a launch, told by ember_hip_kv4_attn_plan ----
+
+def mixed_batch(rng, device, H, KV, context=30_000):
+    """Many decodes, short runs and a few chunks; sequences of 16 and 17 rows, and without tokens."""
+    G = H // KV
+    new = [1] * 60 + [5, 90, 0, 17, 130, 16, 1, max(1, 16 // G), 16 // G + 1, max(1, 32 // G), 32 // G + 1]
+    seqs = [(int(c), n) for c, n in zip(rng.integers(0, 500, len(new)), new)] + [(3000, 1), (2600, 70)]
+    return told(batch(rng, device, seqs, H, KV), context)
+
+
+@pytest.mark.parametrize("cut", [True, False])
+@pytest.mark.parametrize("H,KV", [(2, 2), (4, 2), (16, 8), (8, 1), (32, 2)])
+def test_steps_of_decodes_and_chunks_in_two_launches(rng, device, H, KV, cut):
+    """Short runs in the walk, dealt or shared out, the others on tiles: with one workspace, and without."""
+    b = mixed_batch(rng, device, H, KV)
+    both = plan(b, cut, pad=3)
+    assert [(x.rows, x.least) for x in both] == [(16, 1), (128, 17)]
+    assert (both[1].sharers > 0) == cut and (both[0].dealt or (both[0].sharers > 0) == cut)
+    check(b, attend(b, device, cut=cut, pad=3))
+
+
+def test_steps_in_two_launches_of_decodes_alone(rng, device):
+    """A server's fixed hints: the second launch finds no chunks."""
+    b = told(batch(rng, device, [(int(c), 1) for c in rng.integers(0, 700, 32)], 16, 8), 32_768, most=512)
+    assert len(plan(b)) == 2
+    check(b, attend(b, device))
+
+
+def test_steps_in_two_launches_of_chunks_alone(rng, device):
+    """The first launch finds no decodes."""
+    b = told(batch(rng, device, [(int(c), n) for c, n in zip(rng.integers(0, 300, 40), [0] * 36 + [20, 130, 9, 64])], 4, 2), 30_000)
+    assert len(plan(b)) == 2
+    check(b, attend(b, device))
+
+
+def test_steps_in_two_launches_of_more_sequences_than_one_takes(rng, device):
+    new = np.ones(4200, int)
+    new[[5, 4095, 4096, 4199]] = 40, 70, 33, 18
+    b = told(batch(rng, device, [(int(c), int(n)) for c, n in zip(rng.integers(0, 40, 4200), new)], 1, 1), 512)
+    assert len(plan(b)) == 2
+    check(b, attend(b, device, pad=1))
+
+
+def test_steps_in_two_launches_captured_and_replayed(rng, device):
+    b = mixed_batch(rng, device, 4, 2)
+    assert all(x.sharers > 0 for x in plan(b)) and len(plan(b)) == 2
+    out = torch.zeros(b["T"], 4, D, dtype=torch.float16, device=device)
+    args = (on(b["q"], device), on(b["pages"], device), out, dint(b["start"], device), dint(b["pos"], device), dint(b["table"], device))
+    hints = dict(max_query=b["most"], max_context=b["longest"])
+    own, other = (K.kv4_workspace(b["T"], len(b["start"]) - 1, n_heads=4, n_kv=2, device=device, **hints) for _ in range(2))
+    K.kv4_attention(*args, **hints, workspace=other)
+    check(b, out.double().cpu().numpy())
+    eager = out.clone()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        K.kv4_attention(*args, **hints, workspace=own)
+    for _ in range(4):
+        out.fill_(7.0)
+        graph.replay()
+        assert torch.equal(out, eager)
+        out.fill_(7.0)
+        K.kv4_attention(*args, **hints, workspace=other)
+        assert torch.equal(out, eager)
+
+
+HEADS = [(16, 8), (4, 2), (8, 1), (3, 1), (5, 5), (12, 1)]
+
+
+@pytest.mark.parametrize("H,KV", HEADS)
+@pytest.mark.parametrize("kind", ["decodes", "runs", "prompts"])
+def test_short_and_long_sequences_shared_out(rng, device, H, KV, kind):
+    """The edges of pages and steps where the items' keys are shared out, most of them by few work-groups or by one."""
+    seqs = dict(decodes=[(c, 1) for c in (0, 1, 15, 16, 63, 64, 65, 300, 1000)],
+                runs=[(0, 5), (14, 3), (61, 6), (200, 1), (399, 2), (777, 4)],
+                prompts=[(0, 1), (0, 70), (33, 150), (500, 97), (40, 0), (3, 2)])[kind]
+    b = told(batch(rng, device, seqs, H, KV), 40_000)
+    assert [x.sharers > 0 for x in plan(b, pad=3)] == [True]
+    check(b, attend(b, device, pad=3, strided=kind == "runs"))
+
+
+@pytest.mark.parametrize("H,KV,new", [(2, 1, 1), (3, 1, 1), (4, 1, 7), (12, 1, 3)])
+def test_more_sequences_than_lanes_shared_out(rng, device, H, KV, new):
+    """Shares are found by a scan over several loads of lengths: of decodes, of up to 32 rows and of tiles."""
+    seqs = [(int(c), int(n)) for c, n in zip(rng.integers(0, 400, 150), rng.integers(0, new + 1, 150))] + [(9000, new), (5000, 1)]
+    b = told(batch(rng, device, seqs, H, KV), 200_000)
+    form = plan(b)
+    assert len(form) == 1 and form[0].sharers > 0 and form[0].rows == (16 if new == 1 else 32 if H == 4 else 128)
+    check(b, attend(b, device))
+
+
+@pytest.mark.parametrize("S,H,KV,most", [(64, 32, 8, 8), (170, 12, 2, 5), (47, 24, 8, 10), (250, 4, 2, 16)])
+def test_runs_of_up_to_32_rows_dealt_by_length(rng, device, S, H, KV, most):
+    seqs = [(int(c), int(n)) for c, n in zip(rng.choice([0, 16, 33, 150, 500], S), rng.integers(0, most + 1, S))]
+    seqs[S // 2], seqs[0] = (2000, most), (7, 0)
+    b = told(batch(rng, device, seqs, H, KV), 4096, most=most)
+    assert [(x.rows, x.dealt) for x in plan(b, pad=2)] == [(32, 1)]
+    check(b, attend(b, device, pad=2))
+    check(b, attend(b, device, cut=False))
