@@ -1013,13 +1013,16 @@ Plan plan(const EmberKv4AttnArgs &a, int64_t most, int sequences, int tokens) {
 
 int64_t most_rows(const EmberRaggedBatch &b) { return static_cast<int64_t>(std::min(b.max_query, b.T)) * (b.n_heads / b.n_kv); }
 
-// A step of prompt chunks and many more decodes is two launches, a form each: sequences of up to 16 rows are walked, the
+// A step of prompt chunks and many more decodes is two launches, a form each: sequences of few rows are walked, the
 // others' tiles shared out, an entry a sequence. It is told by the mean of the rows being less than a quarter of the most,
 // and pays where the decodes as tiles, of half the longest context, would take the CUs 12.5 us. Measured, us, 8 kv heads,
 // as tiles and as two launches: 960 decodes and 40 x 512 behind up to 1000 564, 346; 196 and 4 behind up to 4000 394, 210;
 // 64 and 1 behind up to 3000 105, 66, 24 and 1 53.5, 49.0, 18 and 1 47.7, 48.5, 8 and 1 37, 43; 30 and 2 behind up to 2000
 // 84, 58; 24 and 1 behind up to 600 26, 35.
-constexpr int kFewRows = 16;
+// Few rows are 16, or 32 where one token has more than 16; none where a token has more than 32, whose decodes are tiles.
+// Measured with 20 heads a kv head, all as tiles behind a first launch of no rows, and so: 200 decodes and 4 x 512 behind up
+// to 4000 964, 845 (2 kv heads 272, 236), 64 and 1 behind up to 3000 226, 189, 30 and 2 behind up to 2000 188, 191.
+int few_rows(int G) { return G <= 16 ? 16 : G <= 32 ? 32 : 0; }
 
 bool mixed(const EmberKv4AttnArgs &a, int64_t most) {
     const EmberRaggedBatch &b = a.batch;
@@ -1063,9 +1066,11 @@ int launches(const EmberKv4AttnArgs &a, int sequences, Launch (&out)[2]) {
         return 1;
     }
     const Plan shared = shared_tiles(b);
-    out[0] = launch(plan(a, kFewRows, sequences, b.T), 1, kFewRows);
-    out[1] = launch(can(shared) ? shared : plan(a, most, sequences, b.T), kFewRows + 1, INT_MAX);
-    return 2;
+    const int few = few_rows(b.n_heads / b.n_kv);
+    int n = 0;
+    if (few > 0) out[n++] = launch(plan(a, few, sequences, b.T), 1, few);
+    out[n++] = launch(can(shared) ? shared : plan(a, most, sequences, b.T), few + 1, INT_MAX);
+    return n;
 }
 
 // One launch, for the sequences of p.

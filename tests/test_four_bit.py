@@ -279,3 +279,11 @@ def test_workspaces_are_enough_for_what_their_calls_launch(rng):
     # of every kind: in one launch and in two, each form, shared and not, dealt
     assert {(1, r, cut, 0) for r in (16, 32, 128) for cut in (False, True)} <= seen
     assert {(2, 16, True, 0), (2, 128, True, 0), (1, 16, False, 1), (1, 32, False, 1)} <= seen
+
+
+@pytest.mark.parametrize("G,few", [(1, 16), (16, 16), (17, 32), (20, 32), (32, 32), (33, 0), (40, 0)])
+def test_no_launch_of_a_mixed_step_is_for_rows_that_no_sequence_has(G, few):
+    """A sequence has the rows of one token at least: short ones are walked, up to 32 rows where a token has more than 16."""
+    got = [(x.rows, x.least, x.most) for x in _plan(70 + 200, 72, 2 * G, 2, 130, 30_000)]
+    tiles = (128, few + 1, 2 ** 31 - 1)
+    assert got == ([(few, 1, few), tiles] if few else [tiles])

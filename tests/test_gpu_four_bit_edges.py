@@ -187,3 +187,12 @@ def test_runs_of_up_to_32_rows_dealt_by_length(rng, device, S, H, KV, most):
     assert [(x.rows, x.dealt) for x in plan(b, pad=2)] == [(32, 1)]
     check(b, attend(b, device, pad=2))
     check(b, attend(b, device, cut=False))
+
+
+@pytest.mark.parametrize("cut", [True, False])
+@pytest.mark.parametrize("H,KV,forms", [(17, 1, [(32, 1), (128, 33)]), (40, 2, [(32, 1), (128, 33)]), (64, 2, [(32, 1), (128, 33)]), (33, 1, [(128, 1)])])
+def test_mixed_steps_of_many_heads_a_kv_head(rng, device, H, KV, forms, cut):
+    """A token has more than 16 rows: decodes are walked 32 rows at a time, or are tiles too."""
+    b = mixed_batch(rng, device, H, KV)
+    assert [(x.rows, x.least) for x in plan(b, cut, pad=3)] == forms
+    check(b, attend(b, device, cut=cut, pad=3))
