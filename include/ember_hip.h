@@ -482,7 +482,10 @@ int64_t ember_hip_shared_prefix_workspace_bytes(const EmberPrefixAttnArgs *args)
  * for each value x the nearest of the eight magnitudes to |x| / 2^e, of two as
  * near the one with the even code, 6 beyond 6; the sign is x's, also of a
  * zero. Every such value is exact in f16. Other scales may be read: a value
- * is then rounded to f16 where it is read (beyond 65504: infinite). */
+ * is then rounded to f16 where it is read (beyond 65504: infinite). In pages
+ * the values of keys that some token of the step sees must be finite, as
+ * section 1b has it, and up to scale byte 140 they are; a weight may be
+ * infinite or NaN, and its feature's outputs follow. */
 
 #define EMBER_MX_GROUP 32
 
@@ -513,12 +516,13 @@ typedef struct EmberKv4AppendArgs {
 
 /* QK-RMSNorm, rotate-half RoPE and the write of K and V into 4-bit pages,
  * fused. q_out is ember_hip_kv_append's bit for bit; K and V are its f32
- * arithmetic's, clamped to +-65504, then as above. A token whose slot is not
+ * arithmetic's, clamped to +-65504 (a NaN to -65504), then as above. A token whose slot is not
  * in the pool (a negative position or row, one past the tables, a block
  * outside the pool) writes no page, but q_out, k_out and v_out. Tokens of one
  * launch must have slots of their own (of padding rows that share one, any
- * row's bytes may stay). qkv, q_out, k_out, v_out and the pool
- * are 16-byte aligned; n_heads and n_kv at most 64, T below 2^24. */
+ * row's bytes may stay). No output may overlap an input or
+ * another output. qkv, q_out, k_out, v_out and the pool are 16-byte aligned;
+ * n_heads and n_kv at most 64, T below 2^24. */
 int ember_hip_kv4_append(const EmberKv4AppendArgs *args, void *stream);
 
 typedef struct EmberKv4AttnArgs {
@@ -533,7 +537,9 @@ typedef struct EmberKv4AttnArgs {
  * with other contents the rows of an item whose keys are shared out may never
  * be written. Calls that overlap in time need one each. Without one, or with one
  * that is too small, no keys are shared out: the same outputs up to rounding,
- * slower where sequences are few and long. */
+ * slower where sequences are few and long. The softmax's weights are rounded
+ * to f16, the products' operand, and summed as rounded; scores, maxima and sums
+ * are f32. out overlaps no input. */
 int ember_hip_kv4_attn(const EmberKv4AttnArgs *args, void *stream);
 /* Bytes of workspace ember_hip_kv4_attn uses for these sizes (only the sizes
  * of args are read; 0: it would not split). Enough for smaller T, S, max_query

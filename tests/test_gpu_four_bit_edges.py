@@ -3,9 +3,11 @@ import numpy as np
 import pytest
 import torch
 
+import four_bit_reference as ref
 from ember_amd import _lib
 from ember_amd import kernels as K
 from four_bit_reference import D, PAGE
+from span_reference import attention_reference
 from test_gpu_four_bit import attend, batch, check, dint, on
 
 pytestmark = pytest.mark.gpu
@@ -196,3 +198,92 @@ def test_mixed_steps_of_many_heads_a_kv_head(rng, device, H, KV, forms, cut):
     b = mixed_batch(rng, device, H, KV)
     assert [(x.rows, x.least) for x in plan(b, cut, pad=3)] == forms
     check(b, attend(b, device, cut=cut, pad=3))
+
+
+# ---- scales that the quantiser never writes ----
+
+def f16(x):
+    """What a value is where it is read: rounded to f16, in float64."""
+    with np.errstate(over="ignore"):
+        return x.astype(np.float16).astype(np.float64)
+
+
+LEVELS = np.concatenate([ref.LEVELS, -ref.LEVELS])  # of codes 0 .. 15
+FORMS = pytest.mark.parametrize("H", [1, 20, 40], ids=["walk of 16 rows", "walk of 32 rows", "tile"])
+
+
+def lay_out(k_code, k_scale, v_code, v_scale):
+    """Pages [n, PAGE_BYTES] of codes [n, 16, 128] and scale bytes [n, 16, 4]."""
+    n = len(k_code)
+    v = ref.pack(v_code).reshape(n, 4, 4, 16, 4).swapaxes(2, 3)
+    return np.concatenate([ref.pack(k_code).reshape(n, -1), v.reshape(n, -1), k_scale.reshape(n, -1), v_scale.swapaxes(1, 2).reshape(n, -1)], 1)
+
+
+def attend_pages(device, q, pages, scale):
+    """One token of each sequence at position 15 of its own page."""
+    S, H, _ = q.shape
+    out = torch.zeros(S, H, D, dtype=torch.float16, device=device)
+    K.kv4_attention(on(q, device), on(pages, device), out, dint(np.arange(S + 1), device), dint(np.full(S, 15), device),
+                    dint(np.arange(S)[:, None], device), max_query=1, max_context=16, scale=scale)
+    return out.double().cpu().numpy()
+
+
+@FORMS
+@pytest.mark.parametrize("key", range(4))
+def test_values_of_every_finite_scale(rng, device, H, key):
+    """V of one key, the others' weights 0: every code at every scale up to the highest that the append writes, at each of
+    the four places of a word of scales, whose other bytes are arbitrary."""
+    S = 36  # four groups of 32 dims each: 144 scales
+    at = 4 * (np.arange(S) % 4) + key
+    v_code, k_code = np.zeros((2, S, PAGE, D), np.uint8)
+    v_scale, k_scale = rng.integers(0, 255, (2, S, PAGE, 4)).astype(np.uint8)
+    s = np.arange(S)
+    code = (np.arange(D) + rng.integers(0, 16, (S, 1))).astype(np.uint8) % 16
+    byte = ((4 * s[:, None] + np.arange(4)) % 141).astype(np.uint8)
+    v_code[s, at], v_scale[s, at] = code, byte
+    k_code[s, at], k_scale[s, at] = 7, 127  # 6 in every dim: a score of 768 * 128^-1/2 = 68, the others' 0
+    q = np.ones((S, H, D), np.float16)
+    got = attend_pages(device, q, lay_out(k_code, k_scale, v_code, v_scale)[:, None], None)
+    want = f16(LEVELS[code] * np.repeat(2.0 ** (byte - 127.0), 32, -1))
+    assert np.array_equal(got, np.broadcast_to(want[:, None], got.shape))  # the one weight is 2^7 in f16, as is their sum
+
+
+@FORMS
+def test_keys_of_every_finite_scale(rng, device, H):
+    """One dim of one key against 15 keys of score 0, in every code and scale; out is that key's weight."""
+    byte, code = (x.reshape(-1) for x in np.meshgrid(np.arange(141), [c for c in range(16) if c % 8]))
+    for some, scale in ((byte <= 121, 1024.0), (byte > 121, 1.0)):
+        b, c = byte[some], code[some]
+        S = b.size
+        s, at, dim = np.arange(S), rng.integers(0, PAGE, S), rng.integers(0, D, S)
+        v_code, k_code = np.zeros((2, S, PAGE, D), np.uint8)
+        v_scale, k_scale = rng.integers(0, 255, (2, S, PAGE, 4)).astype(np.uint8)
+        k_code[s, at, dim], k_scale[s, at, dim // 32] = c, b
+        v_code[s, at], v_scale[s, at] = 2, 127
+        k = f16(LEVELS[c] * 2.0 ** (b - 127.0))
+        q = rng.standard_normal((S, 1, D)).astype(np.float16)
+        q[s, 0, dim] = np.where(k == 0, 1, 3 / np.where(k == 0, 1, k) / scale)  # a score of 3 where k is not 0
+        got = attend_pages(device, q.repeat(H, 1), lay_out(k_code, k_scale, v_code, v_scale)[:, None], scale)
+        keys, vals = np.zeros((2, S, 1, PAGE, D))
+        keys[s, 0, at, dim], vals[s, 0, at] = k, 1
+        want, bound = attention_reference(q, keys, vals, s[:, None], np.arange(S + 1), np.full(S, 15), lambda s, p, j: j <= p, True, scale)
+        assert (np.abs(got - want) <= bound).all()
+        assert (np.abs(want - 1 / 16) > 0.3)[k != 0].all()  # a key that counts is told from one that reads as 0
+
+
+@pytest.mark.parametrize("M,k", [(1, 128), (40, 1152), (64, 2304), (3, 4224), (200, 4224), (3, 8320)],
+                         ids=["rows", "two blocks a wave", "four blocks a wave", "eight blocks a wave", "prompt", "long"])
+def test_weights_of_every_scale(rng, device, M, k):
+    """Every code at every scale in a product with ones: f16's subnormals, infinities and the NaN scale among them, beside
+    arbitrary scales of groups that hold zeros."""
+    byte, code = (x.reshape(-1) for x in np.meshgrid(np.arange(256), np.arange(16)))
+    N = byte.size
+    scales = rng.integers(0, 255, (N, k // 32)).astype(np.uint8)
+    codes = np.zeros((N, k), np.uint8)
+    n, col = np.arange(N), rng.integers(0, k, N)
+    codes[n, col], scales[n, col // 32] = code, byte
+    w = K.gemv4_pack(on(ref.pack(codes), device), on(scales, device))
+    c = torch.empty(M, N, device=device)
+    K.gemv4(torch.ones(M, k, dtype=torch.float16, device=device), w, c, _lib.EPILOGUE_STORE_F32, N=N)
+    want = np.where(byte == 255, np.nan, f16(LEVELS[code] * 2.0 ** (byte - 127.0)))
+    assert np.array_equal(c.double().cpu().numpy(), np.broadcast_to(want, (M, N)), equal_nan=True)
