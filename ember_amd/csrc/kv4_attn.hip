@@ -15,7 +15,9 @@
 // the sum as rounded, so that sum and products see the same weights. A row's
 // reference is not its maximum but 7 below it, and moves only when a score
 // exceeds it by 15, short of f16's end: a weight keeps its 11 bits down to
-// 2^-21 of the largest, and the accumulators are seldom rescaled.
+// 2^-21 of the largest, and the accumulators are seldom rescaled. f16 because
+// the matrix unit takes both operands in one type at this rate; it costs 2.8e-4
+// against float64 in place of the 2.1e-4 of the outputs' rounding alone.
 //
 // Two forms. Up to 32 rows of a kv head and sequence (decode, speculative
 // runs): the walk, whose four waves take turns at the pages and convert them in
@@ -409,9 +411,9 @@ struct Parts {
 // pages of a wave's next step are on their way during a whole step, and where
 // contexts are long all CUs have the same share. With few keys, by a launch's
 // chain of trips to memory (lengths, page ids, pages, out).
-// Measured, 8 kv heads: 1 sequence of 640 keys 8.0 us, of 131,000 32 (4.4
-// TB/s); 32 of 256 to 4095 22 (4.1 TB/s); 8 of 30,000 to 131,000 124 (6.1
-// TB/s); 64 of 512 to 4096 with up to 5 tokens each 33 (5.4 TB/s).
+// Measured, 8 kv heads: 1 sequence of 640 keys 7.4 us, of 131,000 32 (4.4
+// TB/s); 32 of 256 to 4095 20.7 (4.3 TB/s); 8 of 30,000 to 131,000 135 (6.1
+// TB/s); 64 of 512 to 4096 with up to 5 tokens each 30.6 (5.3 TB/s).
 template <int RT, int W, int P>
 __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
     constexpr int D = kHeadDim, kRows = 16 * RT, kThreads = W * kWave;
@@ -661,8 +663,8 @@ __global__ void __launch_bounds__(W *kWave, 2) kv4_walk_kernel(Kv4Params p) {
 // other's products, 247; work-groups of one key group, two to a CU, 237; a wave's priority raised during its products 230
 // (kept); keys staged 16 to a quarter wave, without bank conflicts, 229 (kept); group 0 always before group 1, by priority,
 // 233 to 241; the two halves' chains of score products alternating 229.
-// Measured, 16 heads on 8 kv heads: 2000 tokens behind 12,000 218 us (980 TFLOP/s), 4 of 256 to 512 behind 900 to 3000 60,
-// 512 alone 14.
+// Measured, 16 heads on 8 kv heads: 2000 tokens behind 12,000 212 to 222 us by box (960 to 1,000 TFLOP/s), 4 of up to 512
+// behind 900 to 3000 41 (490 TFLOP/s; of 256 to 512 50), 512 alone 16.
 //
 //   S^T = K Q^T   v_mfma_f32_32x32x16_f16: lane l ends with row c's scores of keys 8 (i / 4) + 4 h + i % 4 of each
 //                 32-key half, so a row lives in two lanes.

@@ -131,9 +131,12 @@ __device__ __forceinline__ void load_rows(const Gemv4Params &p, f16 *stage, int 
 // that; each tile goes over it in rounds, rows and all.
 //
 // Bound by a launch's three trips to memory where W is small (1 row of 4096 x
-// 1024 3.0 us), by reading W where it is large (8 rows of 151936 x 1024 16 to
-// 18 us, 5 TB/s; 1 of 24576 x 4096 12.0, 4.5 TB/s), and between them by what a
-// CU takes in, A and W (32 rows of 12288 x 2048 7.7 us, 64 9.2).
+// 1024 3.0 us), by reading W where it is large (8 rows of 151936 x 1024 15.9 us,
+// 5.5 TB/s, 19 where no cache holds any of W; 1 of 24576 x 4096 12.2, 4.4 TB/s),
+// and between them by what a CU takes in, A and W (32 rows of 12288 x 2048 7.8
+// us, 64 9.6; added into f32, 32 of 2048 x 2048 4.3, of 2048 x 6144 8.0). Many
+// rows convert W once for 32 or 64 of them: 512 of 4096 x 4096 24.6 us (700
+// TFLOP/s), 2048 of 12288 x 2048 110 (940).
 template <int EP, int MT, int BPW, bool LONG>
 __global__ void __launch_bounds__(kThreads4, MT * BPW <= 2 ? 4 : 2) gemv4_kernel(Gemv4Params p) {
     constexpr int kDepth = LONG || BPW >= 4 ? 1 : 4 / BPW;
@@ -226,7 +229,8 @@ __global__ void __launch_bounds__(kThreads4, MT * BPW <= 2 ? 4 : 2) gemv4_kernel
 // next block's loads out during a block's products.
 //
 // Bound by what a CU takes in of A and W through L2, 43 GB/s: 512 rows of 2048
-// x 6144 18.4 us (700 TFLOP/s), of 4096 x 4096 24.5, 300 of 4096 x 12288 57.6.
+// x 6144 18.9 to 20.1 us (640 to 680 TFLOP/s; added into f32 the same), 2048
+// 78.5 (660), 300 of 4096 x 12288 60.7 (500).
 template <int EP, int MT, int FT>
 __global__ void __launch_bounds__(kThreads4, 2) gemm4_kernel(Gemv4Params p) {
     constexpr int kStageBytes = kWaves4 * MT * kStageTile * static_cast<int>(sizeof(f16));
@@ -373,8 +377,10 @@ hipError_t run_gemv4(const EmberGemv4Args &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// A thread per 8 columns (one word of codes), in the order of the output. Once per weight: 151936 x 1024 56 us, 24576 x
-// 4096 37 (2.9 TB/s read and written).
+// A thread per 8 columns (one word of codes), in the order of the output. Once per weight: 151936 x 1024 72 us, 24576 x
+// 4096 46 (2.3 TB/s read and written, half of a copy's rate: codes are read in
+// pieces of 4 bytes and scales one by one, which is not worth more for a layout
+// that a program does once).
 __global__ void __launch_bounds__(256) gemv4_pack_kernel(const uint8_t *codes, const uint8_t *scales, int N, int K, uint8_t *out) {
     const int blocks = blocks_of(K);
     const int64_t words = static_cast<int64_t>((N + 15) / 16) * blocks * (kBlockCodes / 4);
@@ -389,7 +395,7 @@ __global__ void __launch_bounds__(256) gemv4_pack_kernel(const uint8_t *codes, c
     }
 }
 
-// A thread per 8 columns, four lanes a group. Bound by memory: 24576 x 4096 f16 47 us (5.4 TB/s), f32 82. Rows need no
+// A thread per 8 columns, four lanes a group. Bound by memory: 24576 x 4096 f16 49 us (5.2 TB/s), f32 80. Rows need no
 // alignment, so elements are read one by one.
 template <typename T>
 __global__ void __launch_bounds__(256) mx_quantize_kernel(EmberMxQuantizeArgs a) {
