@@ -46,6 +46,12 @@ struct Gemv4Params {
 // is on a line of its own, which costs four times the cycles of the lines.
 constexpr int kStageTile = 16 * kBlockCols;  // halves of 16 rows
 
+// Holds the compiler to the order of a stage's stores and of the reads by the wave's other lanes; no instruction.
+__device__ __forceinline__ void own_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // The four features n0 .. of a row, and what ADD_F32 adds them to.
 template <int EP>
 __device__ __forceinline__ f32x4 previous(const Gemv4Params &p, int row, int n0) {
@@ -115,6 +121,7 @@ __device__ __forceinline__ void load_rows(const Gemv4Params &p, f16 *stage, int 
 #pragma unroll
         for (int i = 0; i < 4 * MT; i++)
             if (4 * i < rows) *reinterpret_cast<f16x8 *>(stage + (4 * i + g) * kBlockCols + 8 * (c ^ (4 * i + g) % 16)) = raw[u][i];
+        own_fence();
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
@@ -122,6 +129,7 @@ __device__ __forceinline__ void load_rows(const Gemv4Params &p, f16 *stage, int 
                 const int row = min(16 * m + c, rows - 1);  // rows past the last repeat it
                 x[u][m][s] = *reinterpret_cast<const f16x8 *>(stage + row * kBlockCols + 8 * ((4 * s + g) ^ row % 16));
             }
+        own_fence();
     }
 }
 
@@ -270,6 +278,7 @@ __global__ void __launch_bounds__(kThreads4, 2) gemm4_kernel(Gemv4Params p) {
 #pragma unroll
         for (int i = 0; i < 4 * MT; i++)
             if (4 * i < rows) *reinterpret_cast<f16x8 *>(stage + (4 * i + g) * kBlockCols + 8 * (c ^ (4 * i + g) % 16)) = raw[i];
+        own_fence();
         u32x4 now[FT];
         uint32_t now_scale[FT];
 #pragma unroll
@@ -290,6 +299,7 @@ __global__ void __launch_bounds__(kThreads4, 2) gemm4_kernel(Gemv4Params p) {
                 for (int m = 0; m < MT; m++) acc[f][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, x[m], acc[f][m], 0, 0, 0);
             }
         }
+        own_fence();
     }
     f32x4 *const red = reinterpret_cast<f32x4 *>(lds) + lane;
 #pragma unroll
