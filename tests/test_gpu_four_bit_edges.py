@@ -287,3 +287,43 @@ def test_weights_of_every_scale(rng, device, M, k):
     K.gemv4(torch.ones(M, k, dtype=torch.float16, device=device), w, c, _lib.EPILOGUE_STORE_F32, N=N)
     want = np.where(byte == 255, np.nan, f16(LEVELS[code] * 2.0 ** (byte - 127.0)))
     assert np.array_equal(c.double().cpu().numpy(), np.broadcast_to(want, (M, N)), equal_nan=True)
+
+
+# ---- positions ----
+
+@pytest.mark.parametrize("shared", [False, True], ids=["an item each", "shared out"])
+@pytest.mark.parametrize("n,H,KV,rows", [(1, 4, 2, 16), (6, 4, 1, 32), (70, 4, 2, 128), (1, 40, 1, 128)])
+def test_positions_at_the_ends_of_their_range(rng, device, n, H, KV, rows, shared):
+    """Negative ones see nothing, those past the table all of it, also at the end of 32 bits; runs that cross both borders."""
+    W = 40
+    full = batch(rng, device, [(W * PAGE - n, n)] * 7, H, KV, W=W)
+    firsts = [-n, -(n // 2), W * PAGE - 1, W * PAGE - n // 2, 2 ** 31 - n, 2 ** 31 - n - 16, -2 ** 31]
+    full["pos"] = np.concatenate([f + np.arange(n) for f in firsts])
+    if shared:
+        told(full, 100_000)
+    else:
+        full["longest"] = 64
+    assert [(x.rows, x.sharers > 0) for x in plan(full)] == [(rows, shared)]
+    got = attend(full, device)
+    assert (got[full["pos"] < 0] == 0).all()
+    check(full, got)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_steps_of_any_kind(seed, device):
+    """Sequences, heads, hints, strides and missing pages at random."""
+    rng = np.random.default_rng(seed)
+    KV = int(rng.choice([1, 2, 3, 8]))
+    H = KV * int(rng.choice([1, 2, 3, 5, 8, 16, 18, 33][: 5 if KV == 8 else 8]))
+    S = int(2 ** rng.uniform(0, 7))
+    new = np.where(rng.random(S) < 0.8, 1, (2 ** rng.uniform(0, 7.5, S)).astype(int) - 1)
+    seqs = [(int(c), int(m)) for c, m in zip(2 ** rng.uniform(0, 9.5, S) - 1, new)]
+    b = batch(rng, device, seqs, H, KV)
+    b["table"][rng.random(b["table"].shape) < 0.02] = int(rng.choice([-1, -7, b["pages"].shape[0], 2 ** 31 - 1]))
+    missing = (b["table"] < 0) | (b["table"] >= b["pages"].shape[0])
+    pad, strided = int(rng.integers(0, 4)), bool(rng.integers(0, 2))
+    seen = {**b, "table": np.where(missing, -1, b["table"])}
+    for context in (0, 3000, 60_000):
+        told(b, max(context, int(rng.integers(1, 1000))), most=int(rng.choice([1, 8, 200])))
+        told(seen, b["longest"])
+        check(seen, attend(b, device, cut=bool(rng.integers(0, 4)), pad=pad, strided=strided, scale=0.05), 0.05)
