@@ -16,7 +16,7 @@
 // reference is not its maximum but 7 below it, and moves only when a score
 // exceeds it by 15, short of f16's end: a weight keeps its 11 bits down to
 // 2^-21 of the largest, and the accumulators are seldom rescaled. f16 because
-// the matrix unit takes both operands in one type at this rate; it costs 2.8e-4
+// the matrix unit takes both operands in one type at this rate; it costs 2.9e-4
 // against float64 in place of the 2.1e-4 of the outputs' rounding alone.
 //
 // Two forms. Up to 32 rows of a kv head and sequence (decode, speculative
